@@ -61,6 +61,13 @@ pub const ULLM_EPI_SWIGLU: c_int = 2;
 pub const ULLM_SHARD_NO_WAIT: c_int = 1;
 pub const ULLM_SHARD_FUSED_STORES: c_int = 2;
 pub const ULLM_SHARD_SM_PUSH: c_int = 4;
+pub const ULLM_KV_FAULT_NO_PAGES: c_int = 1;
+pub const ULLM_KV_FAULT_SEQ: c_int = 2;
+pub const ULLM_KV_FAULT_LEN: c_int = 4;
+pub const ULLM_KV_FAULT_PAGE: c_int = 8;
+pub const ULLM_KV_FAULT_PATH: c_int = 16;
+pub const ULLM_KV_FAULT_SHARED: c_int = 32;
+pub const ULLM_KV_FAULT_POS: c_int = 64;
 pub const ULLM_GGUF_OK: c_int = 0;
 pub const ULLM_GGUF_ERR_UNSUPPORTED: c_int = 1;
 pub const ULLM_GGUF_ERR_FORMAT: c_int = 2;
@@ -113,6 +120,98 @@ pub struct ullm_moe_experts_input {
     pub hidden: usize,
     pub inter: usize,
     pub group: usize,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct ullm_kv_pages {
+    pub dtype: c_int,
+    pub n_layer: usize,
+    pub n_pages: usize,
+    pub page_size: usize,
+    pub n_kv_head: usize,
+    pub head_dim: usize,
+    pub d_k: *mut c_void,
+    pub d_v: *mut c_void,
+    pub layer_stride: usize,
+    pub page_stride: usize,
+    pub slot_stride: usize,
+    pub head_stride: usize,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct ullm_kv_table {
+    pub d_blocks: *mut i32,
+    pub d_len: *mut i32,
+    pub d_refs: *mut i32,
+    pub d_fault: *mut i32,
+    pub n_seq: usize,
+    pub max_blocks: usize,
+    pub d_work: *mut c_void,
+    pub work_bytes: usize,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct ullm_qk_norm_rope {
+    pub kv: *const ullm_kv_pages,
+    pub layer: usize,
+    pub x_dtype: c_int,
+    pub q_dtype: c_int,
+    pub n_rows: usize,
+    pub n_head: usize,
+    pub d_q: *const c_void,
+    pub d_k: *const c_void,
+    pub d_v: *const c_void,
+    pub q_stride: usize,
+    pub k_stride: usize,
+    pub v_stride: usize,
+    pub d_q_out: *mut c_void,
+    pub q_out_stride: usize,
+    pub d_q_norm: *const f32,
+    pub d_k_norm: *const f32,
+    pub d_q_bias: *const f32,
+    pub d_k_bias: *const f32,
+    pub d_v_bias: *const f32,
+    pub eps: f32,
+    pub d_rope: *const f32,
+    pub n_pos: usize,
+    pub rot_dim: usize,
+    pub neox: c_int,
+    pub d_row_seq: *const i32,
+    pub d_row_slot: *const i32,
+    pub d_row_pos: *const i32,
+    pub d_blocks: *const i32,
+    pub n_table: usize,
+    pub max_blocks: usize,
+    pub d_fault: *mut i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct ullm_tree_attn {
+    pub kv: *const ullm_kv_pages,
+    pub layer: usize,
+    pub dtype: c_int,
+    pub n_rows: usize,
+    pub n_seq: usize,
+    pub n_head: usize,
+    pub d_q: *const c_void,
+    pub q_stride: usize,
+    pub d_out: *mut c_void,
+    pub out_stride: usize,
+    pub d_cu: *const i32,
+    pub d_len: *const i32,
+    pub d_ids: *const i32,
+    pub d_blocks: *const i32,
+    pub n_table: usize,
+    pub max_blocks: usize,
+    pub d_mask: *const u32,
+    pub mask_words: usize,
+    pub scale: f32,
+    pub d_work: *mut c_void,
+    pub work_bytes: usize,
 }
 
 #[repr(C)]
@@ -321,6 +420,16 @@ extern "C" {
     pub fn ullm_cuda_moe_ffn(ctx: *mut ullm_cuda_ctx, e: *const ullm_cuda_experts, x: *const f32, logits: *const f32, n_tok: usize, k: usize, y: *mut f32, idx: *mut u32, wts: *mut f32) -> c_int;
     pub fn ullm_cuda_moe_ffn_dev(ctx: *mut ullm_cuda_ctx, e: *const ullm_cuda_experts, d_x: *const f32, d_logits: *const f32, n_tok: usize, k: usize, d_y: *mut f32, d_idx: *mut u32, d_wts: *mut f32, stream: *mut c_void) -> c_int;
     pub fn ullm_cuda_moe_ffn_noalloc(device: c_int, dev_experts: *const ullm_moe_experts_input, d_x: *const f32, d_logits: *const f32, n_tok: usize, k: usize, d_y: *mut f32, stream: *mut c_void, err: *mut c_char, err_cap: usize) -> c_int;
+    pub fn ullm_cuda_kv_work_bytes(n_pages: usize, n_seq: usize) -> usize;
+    pub fn ullm_cuda_kv_fork_dev(ctx: *mut ullm_cuda_ctx, kv: *const ullm_kv_pages, t: *const ullm_kv_table, d_src: *const i32, d_dst: *const i32, n: usize, stream: *mut c_void) -> c_int;
+    pub fn ullm_cuda_kv_grow_dev(ctx: *mut ullm_cuda_ctx, kv: *const ullm_kv_pages, t: *const ullm_kv_table, d_seq: *const i32, d_add: *const i32, n: usize, stream: *mut c_void) -> c_int;
+    pub fn ullm_cuda_kv_accept_dev(ctx: *mut ullm_cuda_ctx, kv: *const ullm_kv_pages, t: *const ullm_kv_table, d_seq: *const i32, d_draft: *const i32, d_path: *const i32, d_kept: *const i32, n: usize, max_path: usize, stream: *mut c_void) -> c_int;
+    pub fn ullm_cuda_kv_trim_dev(ctx: *mut ullm_cuda_ctx, kv: *const ullm_kv_pages, t: *const ullm_kv_table, d_seq: *const i32, d_new_len: *const i32, n: usize, stream: *mut c_void) -> c_int;
+    pub fn ullm_cuda_kv_copy_pages_dev(ctx: *mut ullm_cuda_ctx, kv: *const ullm_kv_pages, d_src: *const i32, d_dst: *const i32, n: usize, d_fault: *mut i32, stream: *mut c_void) -> c_int;
+    pub fn ullm_cuda_tree_plan_dev(ctx: *mut ullm_cuda_ctx, n_rows: usize, n_seq: usize, d_cu: *const i32, d_len: *const i32, d_ids: *const i32, n_table: usize, d_parent: *const i32, d_row_seq: *mut i32, d_row_slot: *mut i32, d_row_pos: *mut i32, d_mask: *mut u32, mask_words: usize, d_fault: *mut i32, stream: *mut c_void) -> c_int;
+    pub fn ullm_cuda_qk_norm_rope_dev(ctx: *mut ullm_cuda_ctx, a: *const ullm_qk_norm_rope, stream: *mut c_void) -> c_int;
+    pub fn ullm_cuda_tree_attn_work_bytes(ctx: *const ullm_cuda_ctx, kv: *const ullm_kv_pages, dtype: c_int) -> usize;
+    pub fn ullm_cuda_tree_attn_dev(ctx: *mut ullm_cuda_ctx, a: *const ullm_tree_attn, stream: *mut c_void) -> c_int;
     pub fn ullm_cuda_forward_create(ctx: *mut ullm_cuda_ctx, r#in: *const ullm_gpu_model_input, out: *mut *mut ullm_cuda_fwd) -> c_int;
     pub fn ullm_cuda_forward_create_gguf(ctx: *mut ullm_cuda_ctx, g: *const ullm_gguf, kv_f16: c_int, out: *mut *mut ullm_cuda_fwd) -> c_int;
     pub fn ullm_cuda_forward_create_st(ctx: *mut ullm_cuda_ctx, st: *const ullm_st, kv_f16: c_int, out: *mut *mut ullm_cuda_fwd) -> c_int;

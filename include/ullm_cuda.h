@@ -355,6 +355,152 @@ int ullm_cuda_moe_ffn_noalloc(int device, const ullm_moe_experts_input *dev_expe
                               const float *d_logits, size_t n_tok, size_t k, float *d_y, void *stream, char *err,
                               size_t err_cap);
 
+/* ---- paged key/value cache: pages that sequences share, drafted trees, kept rows ----
+ * No counterpart in the reference (its cache is one contiguous f32 array per layer, forward.rs:355-356, and it
+ * decodes one sequence).  A server that batches sequences and verifies drafted tokens keeps K and V in pages of
+ * `page_size` token slots and gives every sequence a row of page numbers.  All state lives in device memory that the
+ * caller owns; the calls only enqueue, read lengths and tables on the device and can be captured in a CUDA graph.
+ * A NULL stream is the context's own (cudaStreamLegacy, the handle 1, names the legacy default stream).
+ *
+ * Where K and V lie: element (layer, page, slot, head, d) is at layer * layer_stride + page * page_stride +
+ * slot * slot_stride + head * head_stride + d, counted in elements, from d_k and from d_v.  Any order of the axes
+ * may be nearest to d; head_dim values are contiguous.  d_k and d_v are 16-byte aligned and the strides multiples of
+ * 16 bytes; head_dim is a multiple of 8, at most 256.  dtype is F32, F16 or BF16. */
+typedef struct ullm_kv_pages {
+    int dtype;
+    size_t n_layer, n_pages, page_size, n_kv_head, head_dim;
+    void *d_k;
+    void *d_v;
+    size_t layer_stride, page_stride, slot_stride, head_stride;
+} ullm_kv_pages;
+/* The tables of a pool.  d_blocks [n_seq][max_blocks]: the page of every `page_size` tokens of a sequence; entries
+ * behind its last one may hold anything.  d_len [n_seq]: tokens held, 0 = the row is unused.  d_refs [n_pages]: how many
+ * rows use a page, 0 = free.  d_fault [1]: bits that the kernels set (never clear) when they refuse an entry:
+ * such an entry changes nothing, the other entries of the call are carried out.  d_work: at least
+ * ullm_cuda_kv_work_bytes(n_pages, n_seq) bytes for this table alone, contents free between calls. */
+typedef struct ullm_kv_table {
+    int32_t *d_blocks;
+    int32_t *d_len;
+    int32_t *d_refs;
+    int32_t *d_fault;
+    size_t n_seq, max_blocks;
+    void *d_work;
+    size_t work_bytes;
+} ullm_kv_table;
+enum {
+    ULLM_KV_FAULT_NO_PAGES = 1, /* not enough free pages: the whole call changed nothing */
+    ULLM_KV_FAULT_SEQ = 2,      /* a sequence index outside the table, listed twice, or a fork onto a row in use */
+    ULLM_KV_FAULT_LEN = 4,      /* a negative or too long length or count */
+    ULLM_KV_FAULT_PAGE = 8,     /* a page number outside the pool, listed twice, or freed more often than used */
+    ULLM_KV_FAULT_PATH = 16,    /* path or parent indices out of order or out of range */
+    ULLM_KV_FAULT_SHARED = 32,  /* rows would be moved into a page that another sequence uses */
+    ULLM_KV_FAULT_POS = 64      /* a position outside the rotation table */
+};
+size_t ullm_cuda_kv_work_bytes(size_t n_pages, size_t n_seq);
+/* d_dst[i] takes all pages of d_src[i] (shared, not copied) and its length.  One source may have several children; a
+ * destination is an unused row and is no source of the same call. */
+int ullm_cuda_kv_fork_dev(ullm_cuda_ctx *ctx, const ullm_kv_pages *kv, const ullm_kv_table *t, const int32_t *d_src,
+                          const int32_t *d_dst, size_t n, void *stream);
+/* Sequence d_seq[i] gets room for d_add[i] more tokens and that much more length.  New pages are the lowest-numbered
+ * free ones, handed out in list order.  A shared page into which the new tokens begin is copied first (its slots in use,
+ * every layer), so that what is written afterwards reaches no other sequence. */
+int ullm_cuda_kv_grow_dev(ullm_cuda_ctx *ctx, const ullm_kv_pages *kv, const ullm_kv_table *t, const int32_t *d_seq,
+                          const int32_t *d_add, size_t n, void *stream);
+/* The last d_draft[i] tokens of sequence d_seq[i] are drafts of which those with the (strictly increasing) indices
+ * d_path[i][0 .. d_kept[i]) are kept: their K and V rows move up behind the tokens in front of the drafts, in
+ * every layer, the length becomes that of what is kept, and pages behind it are freed.  d_path is [n][max_path]. */
+int ullm_cuda_kv_accept_dev(ullm_cuda_ctx *ctx, const ullm_kv_pages *kv, const ullm_kv_table *t, const int32_t *d_seq,
+                            const int32_t *d_draft, const int32_t *d_path, const int32_t *d_kept, size_t n, size_t max_path,
+                            void *stream);
+/* Sequence d_seq[i] keeps its first d_new_len[i] tokens (NULL: none, the row becomes unused); pages behind them are freed. */
+int ullm_cuda_kv_trim_dev(ullm_cuda_ctx *ctx, const ullm_kv_pages *kv, const ullm_kv_table *t, const int32_t *d_seq,
+                          const int32_t *d_new_len, size_t n, void *stream);
+/* Page d_src[i] is copied to page d_dst[i], all layers and slots.  An entry whose destination is also
+ * a source or another entry's destination, or whose pages are outside the pool, is skipped, with ULLM_KV_FAULT_PAGE in
+ * d_fault (may be NULL). */
+int ullm_cuda_kv_copy_pages_dev(ullm_cuda_ctx *ctx, const ullm_kv_pages *kv, const int32_t *d_src, const int32_t *d_dst,
+                                size_t n, int32_t *d_fault, void *stream);
+
+/* What the layers of a step need to know about its rows, once per step.  Sequence b (table row d_ids[b], NULL = b) owns
+ * rows d_cu[b] .. d_cu[b+1) of the step; they are its last tokens (already counted in d_len, see kv_grow) and form
+ * trees: d_parent[row] is the index among the sequence's rows of the token in front of it, smaller than its own, or -1
+ * for the last token that is no draft (d_parent NULL: a chain, every row follows the one before).  Written for each row:
+ * d_row_seq = its table row, d_row_slot = its token slot, d_row_pos = its position (slots in front of the rows + depth),
+ * d_mask [n_rows][mask_words] = the bits of itself and its ancestors (d_mask may be NULL).  Rows behind d_cu[n_seq] get
+ * d_row_seq = -1, which the other calls skip; their other entries are left alone.  With d_mask a sequence has at most
+ * 32 * mask_words rows, with d_parent at most 4096: one that has more is refused (d_fault, may be NULL) and its rows get -1. */
+int ullm_cuda_tree_plan_dev(ullm_cuda_ctx *ctx, size_t n_rows, size_t n_seq, const int32_t *d_cu, const int32_t *d_len,
+                            const int32_t *d_ids, size_t n_table, const int32_t *d_parent, int32_t *d_row_seq,
+                            int32_t *d_row_slot, int32_t *d_row_pos, uint32_t *d_mask, size_t mask_words, int32_t *d_fault,
+                            void *stream);
+
+/* Projections of a step's rows -> bias -> RMSNorm of each query and key head (math.rs:82-86) -> rotation (math.rs:116-162)
+ * -> queries to d_q_out, keys and values into their pages, in one pass.  x_dtype: type of d_q / d_k / d_v; q_dtype:
+ * type of d_q_out, F32 or the pages' type.  Row r's heads lie at r * *_stride (elements; 16-byte multiples; q, k and v may be parts of
+ * one matrix).  Norm weights [head_dim] and biases [heads * head_dim] are f32, NULL = absent (both norms or neither).
+ * d_rope [n_pos][rot_dim / 2][2] f32: cosine and sine of a position's angles; rot_dim (a multiple of 16, at most
+ * head_dim, 0 = head_dim) leading values of a head are rotated, as pairs (2i, 2i + 1) or, with neox, (i, i + rot_dim / 2).  Rows
+ * with d_row_seq < 0 are skipped.  d_q_out may be d_q when types and strides agree.  d_fault (may be NULL) tells of rows whose position or page
+ * is outside: nothing of such a row is written. */
+typedef struct ullm_qk_norm_rope {
+    const ullm_kv_pages *kv;
+    size_t layer;
+    int x_dtype, q_dtype;
+    size_t n_rows, n_head;
+    const void *d_q;
+    const void *d_k;
+    const void *d_v;
+    size_t q_stride, k_stride, v_stride;
+    void *d_q_out;
+    size_t q_out_stride;
+    const float *d_q_norm;
+    const float *d_k_norm;
+    const float *d_q_bias;
+    const float *d_k_bias;
+    const float *d_v_bias;
+    float eps;
+    const float *d_rope;
+    size_t n_pos, rot_dim;
+    int neox;
+    const int32_t *d_row_seq;
+    const int32_t *d_row_slot;
+    const int32_t *d_row_pos;
+    const int32_t *d_blocks;
+    size_t n_table, max_blocks;
+    int32_t *d_fault;
+} ullm_qk_norm_rope;
+int ullm_cuda_qk_norm_rope_dev(ullm_cuda_ctx *ctx, const ullm_qk_norm_rope *a, void *stream);
+
+/* Attention of a step's rows over their sequences' pages: out = softmax(scale * q . K) V over all tokens in front of the
+ * sequence's rows and, among the rows themselves, those whose bit is set in the row's mask (NULL: itself and those in front of it, a
+ * causal chain).  A row that sees nothing becomes zeros.  Rows, d_cu, d_len, d_ids as in ullm_cuda_tree_plan_dev; a sequence whose
+ * length is smaller than its row count gets zeros, rows behind d_cu[n_seq] are left alone.  dtype (of d_q and d_out) is
+ * the pages' type, or F32 with pages of any type.  Query head h reads key head h / (n_head / n_kv_head).  Row strides are in elements,
+ * multiples of 16 bytes, 0 = n_head * head_dim.  scale 0 = 1 / sqrt(head_dim).  A page number outside the pool reads as zeros.  d_work: ullm_cuda_tree_attn_work_bytes
+ * bytes, not shared by calls that may run at the same time. */
+typedef struct ullm_tree_attn {
+    const ullm_kv_pages *kv;
+    size_t layer;
+    int dtype;
+    size_t n_rows, n_seq, n_head;
+    const void *d_q;
+    size_t q_stride;
+    void *d_out;
+    size_t out_stride;
+    const int32_t *d_cu;
+    const int32_t *d_len;
+    const int32_t *d_ids;
+    const int32_t *d_blocks;
+    size_t n_table, max_blocks;
+    const uint32_t *d_mask;
+    size_t mask_words;
+    float scale;
+    void *d_work;
+    size_t work_bytes;
+} ullm_tree_attn;
+size_t ullm_cuda_tree_attn_work_bytes(const ullm_cuda_ctx *ctx, const ullm_kv_pages *kv, int dtype);
+int ullm_cuda_tree_attn_dev(ullm_cuda_ctx *ctx, const ullm_tree_attn *a, void *stream);
+
 /* ---- full decode step: GpuForward (forward.rs:162-757) ---- */
 typedef struct { /* GpuParams, forward.rs:24-51 */
     size_t n_embd, n_layer, n_head, n_kv_head, head_dim, n_ff, n_ctx, vocab;

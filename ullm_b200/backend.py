@@ -109,6 +109,16 @@ SIGNATURES = {
     "ullm_cuda_moe_ffn": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp]),
     "ullm_cuda_moe_ffn_dev": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp]),
     "ullm_cuda_moe_ffn_noalloc": (_i, [_i, _vp, _vp, _vp, _sz, _sz, _vp, _vp, C.c_char_p, _sz]),
+    "ullm_cuda_kv_work_bytes": (_sz, [_sz, _sz]),
+    "ullm_cuda_kv_fork_dev": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ullm_cuda_kv_grow_dev": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ullm_cuda_kv_accept_dev": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _vp]),
+    "ullm_cuda_kv_trim_dev": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ullm_cuda_kv_copy_pages_dev": (_i, [_vp, _vp, _vp, _vp, _sz, _vp, _vp]),
+    "ullm_cuda_tree_plan_dev": (_i, [_vp, _sz, _sz, _vp, _vp, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp]),
+    "ullm_cuda_qk_norm_rope_dev": (_i, [_vp, _vp, _vp]),
+    "ullm_cuda_tree_attn_work_bytes": (_sz, [_vp, _vp, _i]),
+    "ullm_cuda_tree_attn_dev": (_i, [_vp, _vp, _vp]),
     "ullm_cuda_forward_create": (_i, [_vp, _vp, C.POINTER(_vp)]),
     "ullm_cuda_forward_create_gguf": (_i, [_vp, _vp, _i, C.POINTER(_vp)]),
     "ullm_cuda_forward_create_st": (_i, [_vp, _vp, _i, C.POINTER(_vp)]),
@@ -299,6 +309,12 @@ class CudaContext:
         self._check(
             self._lib.ullm_cuda_matmul_dev(self._h, dtype, d_w, d_scales, d_biases, table_dtype, group, d_x, d_y, out_dim, in_dim, s, stream)
         )
+
+    def tree_plan_dev(self, n_rows, n_seq, d_cu, d_len, d_parent, d_row_seq, d_row_slot, d_row_pos, d_mask=None, mask_words=0, d_fault=None,
+                      d_ids=None, n_table=None, stream=None):
+        """Rows of a step of drafted trees -> their sequence, slot, position and ancestor bits (``ullm_cuda_tree_plan_dev``)."""
+        self._check(self._lib.ullm_cuda_tree_plan_dev(self._h, n_rows, n_seq, d_cu, d_len, d_ids, n_seq if n_table is None else n_table, d_parent,
+                                                      d_row_seq, d_row_slot, d_row_pos, d_mask, mask_words, d_fault, stream))
 
     def set_option(self, option: int, value: int):
         """``ullm_cuda_ctx_set_option``: ``OPT_PDL`` or ``OPT_SHARD_TIMEOUT_MS``."""
@@ -649,6 +665,126 @@ class Experts:
             self.free()
         except Exception:
             pass
+
+
+# ---- paged key/value cache: the tables, norm + rotation + cache write, attention of drafted trees ----
+KV_FAULT_NO_PAGES, KV_FAULT_SEQ, KV_FAULT_LEN, KV_FAULT_PAGE, KV_FAULT_PATH, KV_FAULT_SHARED, KV_FAULT_POS = (1 << i for i in range(7))
+
+
+class KvPages(C.Structure):
+    """``ullm_kv_pages``: a pool of pages in the caller's device memory.  ``strides`` are (layer, page, slot, head) in
+    elements; by default pages lie as ``[layer][page][slot][head][head_dim]``."""
+
+    _fields_ = [("dtype", _i)] + [(n, _sz) for n in ("n_layer", "n_pages", "page_size", "n_kv_head", "head_dim")] + [
+        ("d_k", _vp), ("d_v", _vp)] + [(n, _sz) for n in ("layer_stride", "page_stride", "slot_stride", "head_stride")]
+
+    def __init__(self, dtype: int, n_layer: int, n_pages: int, page_size: int, n_kv_head: int, head_dim: int, d_k: int, d_v: int, strides=None):
+        if strides is None:
+            slot = n_kv_head * head_dim
+            strides = (n_pages * page_size * slot, page_size * slot, slot, head_dim)
+        super().__init__(dtype, n_layer, n_pages, page_size, n_kv_head, head_dim, d_k, d_v, *strides)
+
+
+class KvTableC(C.Structure):
+    _fields_ = [(n, _vp) for n in ("d_blocks", "d_len", "d_refs", "d_fault")] + [("n_seq", _sz), ("max_blocks", _sz), ("d_work", _vp), ("work_bytes", _sz)]
+
+
+class KvTable:
+    """The tables of a :class:`KvPages` pool (``ullm_kv_table``; the arrays are the caller's int32 device memory) and what is
+    done with them.  Every call only enqueues on ``stream``; refused entries show as bits in ``d_fault``."""
+
+    def __init__(self, ctx: CudaContext, pages: KvPages, d_blocks: int, d_len: int, d_refs: int, d_fault: int, n_seq: int, max_blocks: int):
+        self._ctx, self.pages = ctx, pages
+        nbytes = ctx._lib.ullm_cuda_kv_work_bytes(pages.n_pages, n_seq)
+        self._work = ctx.alloc(nbytes)
+        self._c = KvTableC(d_blocks, d_len, d_refs, d_fault, n_seq, max_blocks, self._work.ptr, nbytes)
+        self._p, self._t = C.byref(self.pages), C.byref(self._c)
+
+    def fork_dev(self, d_src: int, d_dst: int, n: int, stream=None):
+        """Row ``dst[i]`` shares all pages of row ``src[i]``."""
+        c = self._ctx
+        c._check(c._lib.ullm_cuda_kv_fork_dev(c._h, self._p, self._t, d_src, d_dst, n, stream))
+
+    def grow_dev(self, d_seq: int, d_add: int, n: int, stream=None):
+        """Room for ``add[i]`` more tokens in row ``seq[i]``; a shared page that will be written is copied."""
+        c = self._ctx
+        c._check(c._lib.ullm_cuda_kv_grow_dev(c._h, self._p, self._t, d_seq, d_add, n, stream))
+
+    def accept_dev(self, d_seq: int, d_draft: int, d_path: int, d_kept: int, n: int, max_path: int, stream=None):
+        """Of the last ``draft[i]`` tokens of row ``seq[i]`` those at ``path[i][:kept[i]]`` stay."""
+        c = self._ctx
+        c._check(c._lib.ullm_cuda_kv_accept_dev(c._h, self._p, self._t, d_seq, d_draft, d_path, d_kept, n, max_path, stream))
+
+    def trim_dev(self, d_seq: int, d_new_len: int | None, n: int, stream=None):
+        """Row ``seq[i]`` keeps its first ``new_len[i]`` tokens (``None``: none)."""
+        c = self._ctx
+        c._check(c._lib.ullm_cuda_kv_trim_dev(c._h, self._p, self._t, d_seq, d_new_len, n, stream))
+
+    def copy_pages_dev(self, d_src: int, d_dst: int, n: int, stream=None):
+        """Page ``src[i]`` is copied to page ``dst[i]`` in every layer."""
+        c = self._ctx
+        c._check(c._lib.ullm_cuda_kv_copy_pages_dev(c._h, self._p, d_src, d_dst, n, self._c.d_fault, stream))
+
+
+class QkNormRopeC(C.Structure):
+    _fields_ = [("kv", _vp), ("layer", _sz), ("x_dtype", _i), ("q_dtype", _i), ("n_rows", _sz), ("n_head", _sz), ("d_q", _vp), ("d_k", _vp), ("d_v", _vp),
+                ("q_stride", _sz), ("k_stride", _sz), ("v_stride", _sz), ("d_q_out", _vp), ("q_out_stride", _sz), ("d_q_norm", _vp), ("d_k_norm", _vp),
+                ("d_q_bias", _vp), ("d_k_bias", _vp), ("d_v_bias", _vp), ("eps", C.c_float), ("d_rope", _vp), ("n_pos", _sz), ("rot_dim", _sz), ("neox", _i),
+                ("d_row_seq", _vp), ("d_row_slot", _vp), ("d_row_pos", _vp), ("d_blocks", _vp), ("n_table", _sz), ("max_blocks", _sz), ("d_fault", _vp)]
+
+
+class QkNormRope:
+    """Bias, per-head norm and rotation of a step's projections, K and V into their pages (``ullm_cuda_qk_norm_rope_dev``).
+    What the layers share is given once; weights of one layer may be given again with every call."""
+
+    def __init__(self, ctx: CudaContext, pages: KvPages, n_head: int, x_dtype: int, d_rope: int, n_pos: int, q_dtype: int | None = None, rot_dim: int = 0,
+                 neox: bool = False, d_q_norm: int | None = None, d_k_norm: int | None = None, eps: float = 1e-6, d_q_bias: int | None = None,
+                 d_k_bias: int | None = None, d_v_bias: int | None = None):
+        self._ctx, self.pages = ctx, pages
+        a = self._a = QkNormRopeC()
+        a.kv, a.x_dtype, a.q_dtype, a.n_head = C.addressof(pages), x_dtype, pages.dtype if q_dtype is None else q_dtype, n_head
+        a.d_rope, a.n_pos, a.rot_dim, a.neox, a.eps = d_rope, n_pos, rot_dim, 1 if neox else 0, eps
+        a.d_q_norm, a.d_k_norm, a.d_q_bias, a.d_k_bias, a.d_v_bias = d_q_norm, d_k_norm, d_q_bias, d_k_bias, d_v_bias
+        self._ref = C.byref(a)
+
+    def run_dev(self, layer: int, d_q: int, d_k: int, d_v: int, d_q_out: int, n_rows: int, d_row_pos: int, d_row_seq: int, d_row_slot: int, d_blocks: int,
+                n_table: int, max_blocks: int, x_stride: int = 0, q_out_stride: int = 0, d_fault: int | None = None, stream=None):
+        """``x_stride``: elements between two rows of q, of k and of v (0: each packed)."""
+        a, c = self._a, self._ctx
+        a.layer, a.n_rows, a.d_q, a.d_k, a.d_v, a.d_q_out, a.q_out_stride = layer, n_rows, d_q, d_k, d_v, d_q_out, q_out_stride
+        a.q_stride = a.k_stride = a.v_stride = x_stride
+        a.d_row_pos, a.d_row_seq, a.d_row_slot, a.d_blocks = d_row_pos, d_row_seq, d_row_slot, d_blocks
+        a.n_table, a.max_blocks, a.d_fault = n_table, max_blocks, d_fault
+        c._check(c._lib.ullm_cuda_qk_norm_rope_dev(c._h, self._ref, stream))
+
+
+class TreeAttnC(C.Structure):
+    _fields_ = [("kv", _vp), ("layer", _sz), ("dtype", _i), ("n_rows", _sz), ("n_seq", _sz), ("n_head", _sz), ("d_q", _vp), ("q_stride", _sz), ("d_out", _vp),
+                ("out_stride", _sz), ("d_cu", _vp), ("d_len", _vp), ("d_ids", _vp), ("d_blocks", _vp), ("n_table", _sz), ("max_blocks", _sz), ("d_mask", _vp),
+                ("mask_words", _sz), ("scale", C.c_float), ("d_work", _vp), ("work_bytes", _sz)]
+
+
+class TreeAttention:
+    """Attention of a step's rows over a paged cache (``ullm_cuda_tree_attn_dev``) with a work area of its own: calls through
+    one object do not run at the same time (two streams: two objects)."""
+
+    def __init__(self, ctx: CudaContext, pages: KvPages, n_head: int, dtype: int | None = None, scale: float = 0.0):
+        self._ctx, self.pages = ctx, pages
+        a = self._a = TreeAttnC()
+        a.kv, a.n_head, a.dtype, a.scale = C.addressof(pages), n_head, pages.dtype if dtype is None else dtype, scale
+        a.work_bytes = ctx._lib.ullm_cuda_tree_attn_work_bytes(ctx._h, a.kv, a.dtype)
+        self._work = ctx.alloc(a.work_bytes)
+        a.d_work = self._work.ptr
+        self._ref = C.byref(a)
+
+    def run_dev(self, layer: int, d_q: int, d_out: int, n_rows: int, n_seq: int, d_cu: int, d_len: int, d_blocks: int, max_blocks: int,
+                d_mask: int | None = None, mask_words: int = 0, d_ids: int | None = None, n_table: int | None = None, q_stride: int = 0, out_stride: int = 0,
+                stream=None):
+        a, c = self._a, self._ctx
+        a.layer, a.n_rows, a.n_seq, a.d_q, a.q_stride, a.d_out, a.out_stride = layer, n_rows, n_seq, d_q, q_stride, d_out, out_stride
+        a.d_cu, a.d_len, a.d_ids, a.d_blocks, a.n_table, a.max_blocks = d_cu, d_len, d_ids, d_blocks, n_seq if n_table is None else n_table, max_blocks
+        a.d_mask, a.mask_words = d_mask, mask_words
+        c._check(c._lib.ullm_cuda_tree_attn_dev(c._h, self._ref, stream))
 
 
 # ---- full decode step: GpuForward (crates/ullm-metal/src/forward.rs:162-757) ----

@@ -58,10 +58,10 @@ template <typename Q, typename KV> __global__ void __launch_bounds__(FT) tree_at
     const bool pv = part < split;
     for (Walk<FM, FK> w(p, share); w.more(); w.next()) {
         const SeqView v = w.v;
-        const int rows = (int)min((long long)FM, (long long)v.n * p.group - (long long)w.t * FM);
+        const int rows = min(FM, v.n * p.group - w.t * FM);
         const int key_end = Tiles<FM, FK>::key_end(p, v, w.t);
-        auto token_of = [&](int r) { return (int)(((long long)w.t * FM + r) / p.group); };
-        auto head_of = [&](int r) { return w.h * p.group + (int)(((long long)w.t * FM + r) % p.group); };
+        auto token_of = [&](int r) { return (w.t * FM + r) / p.group; };
+        auto head_of = [&](int r) { return w.h * p.group + (w.t * FM + r) % p.group; };
         __syncthreads();
         for (int i = tid; i < FM * D / 8; i += FT) {
             const int r = i / (D / 8), d = i % (D / 8) * 8;
@@ -80,7 +80,6 @@ template <typename Q, typename KV> __global__ void __launch_bounds__(FT) tree_at
         const int *const table = p.blocks + (size_t)v.id * p.max_blocks;
         for (int blk = w.blk; blk < w.end; ++blk) {
             const int k0 = blk * FK;
-            const bool tail = k0 + FK > v.ctx; // holds some of the rows' own tokens, or keys behind the last
             __syncthreads();
             for (int i = tid; i < FK * D / 8; i += FT) {
                 const int j = i / (D / 8), d = i % (D / 8) * 8, token = k0 + j;
@@ -151,7 +150,6 @@ template <typename Q, typename KV> __global__ void __launch_bounds__(FT) tree_at
                         for (int e = 0; e < 4; ++e) acc[a][e] += qq[a] * xs[e];
                 }
             }
-            (void)tail;
         }
         __syncthreads();
         // sum the key parts in order, in the keys' memory
@@ -209,16 +207,16 @@ template <typename Q, typename KV> static cudaError_t launch_fma(const DeviceInf
 
 using namespace ullm;
 
-static size_t tree_work_bytes(int sm_count, int dim) {
+static size_t tree_work_bytes(int sm_count, int dim, bool tc) {
     const int ctas = fma_ctas(sm_count, dim);
-    return meta_bytes(ctas) + sizeof(float) * (size_t)ctas * 2 * FM * (dim + 2);
+    const size_t fma = sizeof(float) * (size_t)ctas * 2 * FM * (dim + 2);
+    return meta_bytes(ctas) + (tc ? std::max(fma, tree_attn_tc_work(sm_count, dim)) : fma);
 }
 
 size_t ullm_cuda_tree_attn_work_bytes(const ullm_cuda_ctx *c, const ullm_kv_pages *kv, int dtype) {
     PoolDev pool;
-    (void)dtype;
     if (!c || !kv || pool_check(kv, &pool)) return 0;
-    return tree_work_bytes(c->dev.sm_count, pool.head_dim);
+    return tree_work_bytes(c->dev.sm_count, pool.head_dim, tree_attn_tc_supported(pool, dtype));
 }
 
 int ullm_cuda_tree_attn_dev(ullm_cuda_ctx *c, const ullm_tree_attn *a, void *stream) {
@@ -233,7 +231,8 @@ int ullm_cuda_tree_attn_dev(ullm_cuda_ctx *c, const ullm_tree_attn *a, void *str
     if (a->layer >= a->kv->n_layer) return ctx_fail(c, ULLM_ERR_FORMAT, "layer %zu of a pool of %zu", a->layer, a->kv->n_layer);
     if (!a->n_head || a->n_head > 65535 || a->n_head % a->kv->n_kv_head)
         return ctx_fail(c, ULLM_ERR_FORMAT, "%zu query heads over %zu key heads", a->n_head, a->kv->n_kv_head);
-    if (a->n_rows > INT32_MAX / 2 || a->n_seq > INT32_MAX / 2) return ctx_fail(c, ULLM_ERR_FORMAT, "too many rows or sequences");
+    if (a->n_rows > INT32_MAX / 2 || a->n_seq > INT32_MAX / 2 || a->n_rows * a->n_head > INT32_MAX / 2)
+        return ctx_fail(c, ULLM_ERR_FORMAT, "too many rows or sequences for one call");
     if (!a->n_table || a->n_table > INT32_MAX / 2 || !a->max_blocks || a->max_blocks > (size_t)(INT32_MAX / 2) / a->kv->page_size)
         return ctx_fail(c, ULLM_ERR_FORMAT, "bad size of the page table");
     if (!a->d_ids && a->n_seq > a->n_table) return ctx_fail(c, ULLM_ERR_FORMAT, "%zu sequences in a table of %zu rows", a->n_seq, a->n_table);
@@ -243,7 +242,8 @@ int ullm_cuda_tree_attn_dev(ullm_cuda_ctx *c, const ullm_tree_attn *a, void *str
     if (qs < qd || os < qd) return ctx_fail(c, ULLM_ERR_FORMAT, "row strides must cover all heads");
     if (qs * qb % 16 || os * qb % 16 || (uintptr_t)a->d_q % 16 || (uintptr_t)a->d_out % 16)
         return ctx_fail(c, ULLM_ERR_FORMAT, "rows must start on 16-byte boundaries");
-    if (!std::isfinite(a->scale) || a->scale < 0.f) return ctx_fail(c, ULLM_ERR_FORMAT, "scale must be finite and not negative");
+    if (!std::isfinite(a->scale) || a->scale < 0.f || (a->scale > 0.f && a->scale < 1e-30f))
+        return ctx_fail(c, ULLM_ERR_FORMAT, "scale must be finite, at least 1e-30 or 0 for the default");
     if (!a->n_rows || !a->n_seq) return ULLM_OK;
     const size_t need = ullm_cuda_tree_attn_work_bytes(c, a->kv, a->dtype);
     if (a->work_bytes < need) return ctx_fail(c, ULLM_ERR_FORMAT, "the work area has %zu bytes, %zu are needed", a->work_bytes, need);
@@ -261,7 +261,12 @@ int ullm_cuda_tree_attn_dev(ullm_cuda_ctx *c, const ullm_tree_attn *a, void *str
     DeviceGuard guard(c->device);
     const cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
     t.meta = (int4 *)a->d_work, t.part = (float *)((uint8_t *)a->d_work + meta_bytes(fma_ctas(c->dev.sm_count, t.dim)));
-    cudaError_t e;
+    cudaError_t e = cudaErrorNotSupported;
+    if (tree_attn_tc_supported(pool, a->dtype)) e = launch_tree_attn_tc(c->dev, pool, a->dtype, t, c->d_status, c->use_pdl, st);
+    if (e != cudaErrorNotSupported) { // (strides that a tensor map cannot describe go to the f32 kernel)
+        ULLM_CUDA_TRY(c, e);
+        return ULLM_OK;
+    }
     if (a->dtype == ULLM_DTYPE_F16) e = launch_fma<__half, __half>(c->dev, t, c->use_pdl, st);
     else if (a->dtype == ULLM_DTYPE_BF16) e = launch_fma<__nv_bfloat16, __nv_bfloat16>(c->dev, t, c->use_pdl, st);
     else if (a->kv->dtype == ULLM_DTYPE_F32) e = launch_fma<float, float>(c->dev, t, c->use_pdl, st);

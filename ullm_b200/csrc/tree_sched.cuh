@@ -39,12 +39,11 @@ __device__ __forceinline__ bool sees(const TreeDev &p, const SeqView &v, int i, 
 }
 
 template <int M, int KB> struct Tiles {
-    static __device__ __forceinline__ int count(const TreeDev &p, const SeqView &v) { return (int)(((long long)v.n * p.group + M - 1) / M); }
+    static __device__ __forceinline__ int count(const TreeDev &p, const SeqView &v) { return (v.n * p.group + M - 1) / M; }
     // one behind the last key that a tile's rows can see
     static __device__ __forceinline__ int key_end(const TreeDev &p, const SeqView &v, int t) {
         if (p.mask || !v.kv) return v.kv;
-        const long long last = (((long long)t + 1) * M - 1) / p.group;
-        return v.ctx + (int)min(last, (long long)v.n - 1) + 1;
+        return v.ctx + min((int)(((t + 1u) * M - 1u) / (unsigned)p.group), v.n - 1) + 1;
     }
     static __device__ __forceinline__ int blocks(const TreeDev &p, const SeqView &v, int t) { return max(1, (key_end(p, v, t) + KB - 1) / KB); }
     // blocks of all tiles of one key head

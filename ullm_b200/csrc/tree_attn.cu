@@ -16,6 +16,7 @@
 namespace ullm {
 
 constexpr int FM = 16, FK = 64, FT = 256; // rows, keys of a block, threads
+constexpr int F_COST = 1, F_MIN = 2;       // places that a unit costs beside its blocks; places that a CTA takes at least
 
 template <typename T> __device__ __forceinline__ void load8(const T *p, float (&o)[8]);
 template <> __device__ __forceinline__ void load8<float>(const float *p, float (&o)[8]) {
@@ -47,22 +48,36 @@ template <typename Q, typename KV> __global__ void __launch_bounds__(FT) tree_at
     const int D = p.dim, KP = fma_kp(D), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     float *const qs = sm, *const ks = qs + FM * D, *const vs = ks + FK * KP, *const sc = vs + FK * D, *const ms = sc + FK * FSP, *const ls = ms + FM,
                 *const cs = ls + FM;
-    __shared__ int odd; // a value that is not finite lies among the rows' own tokens
+    __shared__ Seg seg;
     pdl_wait_prior();
     pdl_launch_dependents();
-    const Share share = cta_share<FM, FK, FT, 1>(p);
-    if (tid == 0) p.meta[blockIdx.x * TREE_META] = make_int4(-1, 0, 0, 0);
+    Sched<FM, FK, F_COST, F_MIN> sched(p);
+    bool some = false;
+    if (warp == 0) {
+        if (lane == 0) p.meta[blockIdx.x * TREE_META] = make_int4(-1, 0, 0, 0);
+        __syncwarp();
+        some = sched.init();
+    }
     // weighted sum of values: thread (key part, four rows, four values)
     const int quads = D / 4, per = 4 * quads, split = per <= 64 ? 4 : (per <= 128 ? 2 : 1);
     const int part = tid / per, item = tid % per, rg = item / quads, dq = item % quads;
     const bool pv = part < split;
-    for (Walk<FM, FK> w(p, share); w.more(); w.next()) {
-        const SeqView v = w.v;
-        const int rows = min(FM, v.n * p.group - w.t * FM);
-        const int key_end = Tiles<FM, FK>::key_end(p, v, w.t);
-        auto token_of = [&](int r) { return (w.t * FM + r) / p.group; };
-        auto head_of = [&](int r) { return w.h * p.group + (w.t * FM + r) % p.group; };
+    for (;;) {
         __syncthreads();
+        if (warp == 0) {
+            Seg next;
+            next.count = 0;
+            if (some) next = sched.next(p.meta + blockIdx.x * TREE_META);
+            if (lane == 0) seg = next;
+        }
+        __syncthreads();
+        const Seg w = seg;
+        if (!w.count) break;
+        SeqView v;
+        v.r0 = w.r0, v.n = w.n, v.id = w.id, v.ctx = w.ctx, v.kv = w.kv;
+        const int rows = w.rows, key_end = w.key_end, blk_end = w.blk + w.count;
+        auto token_of = [&](int r) { return (w.row0 + r) / p.group; };
+        auto head_of = [&](int r) { return w.h * p.group + (w.row0 + r) % p.group; };
         for (int i = tid; i < FM * D / 8; i += FT) {
             const int r = i / (D / 8), d = i % (D / 8) * 8;
             float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -71,14 +86,13 @@ template <typename Q, typename KV> __global__ void __launch_bounds__(FT) tree_at
             for (int e = 0; e < 8; ++e) qs[r * D + d + e] = x[e];
         }
         if (tid < FM) ms[tid] = -INFINITY, ls[tid] = 0.f;
-        if (tid == 0) odd = 0;
         float acc[4][4];
 #pragma unroll
         for (int a = 0; a < 4; ++a)
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[a][e] = 0.f;
         const int *const table = p.blocks + (size_t)v.id * p.max_blocks;
-        for (int blk = w.blk; blk < w.end; ++blk) {
+        for (int blk = w.blk; blk < blk_end; ++blk) {
             const int k0 = blk * FK;
             __syncthreads();
             for (int i = tid; i < FK * D / 8; i += FT) {
@@ -94,7 +108,7 @@ template <typename Q, typename KV> __global__ void __launch_bounds__(FT) tree_at
                     if (token >= v.ctx) { // some rows may not see it: 0 * inf must not reach them
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            if (!isfinite(vv[e])) vv[e] = 0.f, odd = 1;
+                            if (!isfinite(vv[e])) vv[e] = 0.f, seg.odd = 1;
                     }
                 }
 #pragma unroll
@@ -159,14 +173,14 @@ template <typename Q, typename KV> __global__ void __launch_bounds__(FT) tree_at
             for (int a = 0; a < 4; ++a)
                 if (rg * 4 + a < rows) *(float4 *)(red + ((size_t)part * FM + rg * 4 + a) * D + dq * 4) = make_float4(acc[a][0], acc[a][1], acc[a][2], acc[a][3]);
         __syncthreads();
-        const bool whole = w.whole();
-        float *const mine = whole ? nullptr : part_of<FM>(p, blockIdx.x, w.slot());
+        const bool whole = w.flags & 1, odd = seg.odd;
+        float *const mine = whole ? nullptr : part_of<FM>(p, blockIdx.x, w.flags >> 1);
         for (int i = tid; i < rows * D; i += FT) {
             const int r = i / D, d = i % D;
             float o = 0.f;
             for (int s = 0; s < split; ++s) o += red[((size_t)s * FM + r) * D + d];
             if (odd) { // infinities and NaN of the tokens that the row does see
-                const int first = max(v.ctx, w.blk * FK), last = min(key_end, w.end * FK), me = token_of(r);
+                const int first = max(v.ctx, w.blk * FK), last = min(key_end, blk_end * FK), me = token_of(r);
                 for (int token = first; token < last; ++token) {
                     const int page = table[token / p.page_size];
                     if ((unsigned)page >= (unsigned)p.n_pages || !sees(p, v, me, token - v.ctx)) continue;
@@ -182,10 +196,7 @@ template <typename Q, typename KV> __global__ void __launch_bounds__(FT) tree_at
                 mine[i] = o;
             }
         }
-        if (!whole) {
-            if (tid < rows) *(float2 *)(mine + (size_t)FM * D + 2 * tid) = make_float2(ms[tid], ls[tid]);
-            if (tid == 0 && w.first()) w.record(p.meta + blockIdx.x * TREE_META);
-        }
+        if (!whole && tid < rows) *(float2 *)(mine + (size_t)FM * D + 2 * tid) = make_float2(ms[tid], ls[tid]);
     }
 }
 
@@ -200,7 +211,7 @@ template <typename Q, typename KV> static cudaError_t launch_fma(const DeviceInf
     const int ctas = fma_ctas(dev.sm_count, t.dim);
     e = launch_kernel(tree_attn_fma_kernel<Q, KV>, dim3(ctas), dim3(FT), smem, st, pdl, t);
     if (e != cudaSuccess) return e;
-    return launch_kernel(tree_join_kernel<Q, FM>, dim3(ctas, FM / 8), dim3(256), 0, st, pdl, t);
+    return launch_kernel(tree_join_kernel<Q, FM>, dim3(dev.sm_count * 2), dim3(32 * JOIN_WARPS), 0, st, pdl, t, ctas);
 }
 
 } // namespace ullm
@@ -244,6 +255,11 @@ int ullm_cuda_tree_attn_dev(ullm_cuda_ctx *c, const ullm_tree_attn *a, void *str
         return ctx_fail(c, ULLM_ERR_FORMAT, "rows must start on 16-byte boundaries");
     if (!std::isfinite(a->scale) || a->scale < 0.f || (a->scale > 0.f && a->scale < 1e-30f))
         return ctx_fail(c, ULLM_ERR_FORMAT, "scale must be finite, at least 1e-30 or 0 for the default");
+    { // the line of all blocks is counted in 32 bits (with what the smaller tiles of the f32 kernel would need)
+        const double units = ((double)a->n_rows * (a->n_head / a->kv->n_kv_head) / 16 + (double)a->n_seq) * a->kv->n_kv_head;
+        if (units * ((double)a->max_blocks * a->kv->page_size / 64 + 4) > 2147483000.0)
+            return ctx_fail(c, ULLM_ERR_FORMAT, "rows times table size too large for one call: split the rows");
+    }
     if (!a->n_rows || !a->n_seq) return ULLM_OK;
     const size_t need = ullm_cuda_tree_attn_work_bytes(c, a->kv, a->dtype);
     if (a->work_bytes < need) return ctx_fail(c, ULLM_ERR_FORMAT, "the work area has %zu bytes, %zu are needed", a->work_bytes, need);

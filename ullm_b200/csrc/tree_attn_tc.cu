@@ -14,7 +14,9 @@
 // result is the same quotient).  Sums, references and accumulators are f32; the weights are rounded once, to the type
 // the tensor cores take.
 //
-// Warps: 0 TMA (every lane a box: a page's keys, 64 values of the head), 1 MMA issue, 2 tensor memory, 4-7 and 8-11 the streams.
+// Warps: 0 TMA (every lane a box: a page's keys, 64 values of the head), 1 MMA issue, 2 the next segment's queries into the
+// other query buffer, 3 the division of the work (Sched), 4-7 and 8-11 the streams.  Segments pass through a ring, so that loads and
+// score products of the next one begin while the last one's results are stored.  Warps of a stream whose rows are all padding only keep step.
 // Blocks that hold the rows' own tokens, or keys behind the last one, are masked, and their values in shared memory are cleaned
 // first: rows behind the last key become zeros and values that are not finite are set aside (0 * inf would reach
 // rows that do not see the token); the epilogue adds them for the rows that do.
@@ -30,11 +32,13 @@ namespace ullm {
 namespace {
 
 constexpr int TM = 128, TK = 128, TT = 384;
+constexpr int T_COST = 2, T_MIN = 4; // places that a unit costs beside its blocks; places that a CTA takes at least
+constexpr int SEGS = 4;
 template <int D> struct Cfg {
     static constexpr int ATOMS = D / 64;            // 64 values of a head: one 128-byte swizzle row
-    static constexpr int TILE = ATOMS * TK * 128;   // bytes of 128 keys
-    static constexpr int STAGES = D == 128 ? 6 : 10;
-    static constexpr int SMEM = ATOMS * TM * 128 + STAGES * TILE + 1024;
+    static constexpr int TILE = ATOMS * TK * 128;   // bytes of 128 keys, and of 128 queries
+    static constexpr int STAGES = D == 128 ? 5 : 10;
+    static constexpr int SMEM = (2 + STAGES) * TILE + 1024;
     static constexpr uint32_t O_COL = 256;          // columns: scores 0 / 128, accumulators 256 / 256 + D
 };
 
@@ -48,15 +52,16 @@ struct TcMaps {
     CUtensorMap k, v;
 };
 
+// A converged warp waits; every lane gets the same answer, so that no lane leaves alone.
 __device__ __forceinline__ bool wait_bounded(uint64_t *bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity)) return true;
+    bool done = mbar_try_wait(bar, parity);
     const long long t0 = clock64();
-    for (;;) {
+    while (!__all_sync(0xffffffffu, done)) {
 #pragma unroll 1
-        for (int i = 0; i < 256; ++i)
-            if (mbar_try_wait(bar, parity)) return true;
-        if (clock64() - t0 > (1ll << 31)) return false;
+        for (int i = 0; i < 64 && !done; ++i) done = mbar_try_wait(bar, parity);
+        if (__any_sync(0xffffffffu, clock64() - t0 > (1ll << 31))) return __all_sync(0xffffffffu, done);
     }
+    return true;
 }
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap *map, int x, int c1, int c2, int page, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
@@ -76,16 +81,37 @@ template <typename T> constexpr uint32_t idesc(int n, bool b_mn) {
     constexpr uint32_t ty = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
     return (1u << 4) | (ty << 7) | (ty << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc)
+// Four MMAs (K = 16 each) by one elected lane of a converged warp, as one instruction sequence: issued one by one under a branch on the
+// lane they took 100 cycles each.  A, B: descriptors that advance by `da`, `db` per step; `acc`: whether the first one adds to D.
+__device__ __forceinline__ void mma4_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile("{\n.reg .pred pe, pf, pt;\n.reg .b64 a1, a2, a3, b1, b2, b3;\n"
+                 "setp.ne.b32 pf, %4, 0;\nsetp.eq.b32 pt, 0, 0;\nelect.sync _|pe, 0xffffffff;\n"
+                 "add.u64 a1, %1, 2;\nadd.u64 a2, %1, 4;\nadd.u64 a3, %1, 6;\nadd.u64 b1, %2, 2;\nadd.u64 b2, %2, 4;\nadd.u64 b3, %2, 6;\n"
+                 "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, pf;\n"
+                 "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, pt;\n"
+                 "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, pt;\n"
+                 "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, pt;\n}" ::"r"(d),
+                 "l"(a), "l"(b), "r"(id), "r"(acc)
                  : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc)
+__device__ __forceinline__ void mma4_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile("{\n.reg .pred pe, pf, pt;\n.reg .b32 a1, a2, a3;\n.reg .b64 b1, b2, b3;\n"
+                 "setp.ne.b32 pf, %4, 0;\nsetp.eq.b32 pt, 0, 0;\nelect.sync _|pe, 0xffffffff;\n"
+                 "add.u32 a1, %1, 8;\nadd.u32 a2, %1, 16;\nadd.u32 a3, %1, 24;\nadd.u64 b1, %2, 128;\nadd.u64 b2, %2, 256;\nadd.u64 b3, %2, 384;\n"
+                 "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, pf;\n"
+                 "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, pt;\n"
+                 "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, pt;\n"
+                 "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, pt;\n}" ::"r"(d),
+                 "r"(a), "l"(b), "r"(id), "r"(acc)
                  : "memory");
 }
-__device__ __forceinline__ void mma_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+// Arrives on both barriers once the MMAs issued so far are complete.
+__device__ __forceinline__ void commit2(uint64_t *x, uint64_t *y) {
+    asm volatile("{\n.reg .pred pe;\nelect.sync _|pe, 0xffffffff;\n"
+                 "@pe tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
+                 "@pe tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n}" ::"r"(smem_u32(x)),
+                 "r"(smem_u32(y))
+                 : "memory");
 }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -115,18 +141,25 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *v) {
                  "r"(v[14]), "r"(v[15])
                  : "memory");
 }
-__device__ __forceinline__ void tmem_st2(uint32_t addr, float a, float b) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1,%2};" ::"r"(addr), "r"(__float_as_uint(a)), "r"(__float_as_uint(b)) : "memory");
-}
-__device__ __forceinline__ float2 tmem_ld2(uint32_t addr) {
-    uint32_t a, b;
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0,%1}, [%2];" : "=r"(a), "=r"(b) : "r"(addr));
-    return make_float2(__uint_as_float(a), __uint_as_float(b));
-}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { // two multiply-adds in one instruction
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b), "l"(*(unsigned long long *)&c));
+    return *(float2 *)&r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b));
+    return *(float2 *)&r;
 }
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
@@ -167,62 +200,113 @@ __device__ __forceinline__ uint32_t view_bits(const TreeDev &p, const SeqView &v
 __device__ __forceinline__ uint32_t k_tile(uint32_t j) { return j ? 2 * j - 1 : 0; }
 __device__ __forceinline__ uint32_t v_tile(uint32_t j, uint32_t n) { return j + 1 == n ? 2 * n - 1 : 2 * j + 2; }
 
+// Infinities and NaN among the values [c, c + 32) of tokens [first, last) that row `me` sees, added to the row's sums.  Rare, and out of the way.
+template <typename T> __device__ __noinline__ void add_odd_at(const TreeDev &p, const SeqView &v, int head, int me, int first, int last, int c, float *o) {
+    const int *const table = p.blocks + (size_t)v.id * p.max_blocks;
+    for (int token = first; token < last; ++token) {
+        const int page = table[token / p.page_size];
+        if ((unsigned)page >= (unsigned)p.n_pages || !sees(p, v, me, token - v.ctx)) continue;
+        const T *const at = (const T *)p.v + page * p.page_stride + token % p.page_size * p.slot_stride + head * p.head_stride + c;
+        for (int e = 0; e < 32; ++e) {
+            const float y = (float)at[e];
+            if (!isfinite(y)) o[e] += y;
+        }
+    }
+}
+template <typename T> __device__ __forceinline__ void add_odd(const TreeDev &p, const SeqView &v, int head, int me, int first, int last, int c, float (&o)[32]) {
+    float copy[32]; // (a register array cannot be indexed by the loop above)
+#pragma unroll
+    for (int e = 0; e < 32; ++e) copy[e] = o[e];
+    add_odd_at<T>(p, v, head, me, first, last, c, copy);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) o[e] = copy[e];
+}
+
 template <typename T, int D> __global__ void __launch_bounds__(TT, 1) tree_attn_tc_kernel(const __grid_constant__ TcParams prm, const __grid_constant__ TcMaps maps) {
     using C = Cfg<D>;
-    using W = Walk<TM, TK>;
     constexpr int NST = C::STAGES;
     extern __shared__ __align__(1024) uint8_t gsm[];
-    uint8_t *const q_sm = (uint8_t *)(((uintptr_t)gsm + 1023) & ~(uintptr_t)1023), *const ring = q_sm + C::ATOMS * TM * 128;
-    __shared__ uint64_t full[NST], empty[NST], s_full[2], p_full[2], o_done[2], q_full, x_full, epi_done;
-    __shared__ uint32_t tmem_s, odd_sm; // odd_sm: number of the last segment with values set aside
+    uint8_t *const q_sm = (uint8_t *)(((uintptr_t)gsm + 1023) & ~(uintptr_t)1023), *const ring = q_sm + 2 * C::TILE;
+    __shared__ uint64_t full[NST], empty[NST], s_full[2], p_full[2], o_done[2], q_full[2], q_empty[2], seg_full[SEGS], seg_empty[SEGS], x_full, epi_done;
+    __shared__ Seg segs[SEGS];
+    __shared__ uint32_t tmem_s;
     const TreeDev &p = prm.t;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < NST; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-        for (int s = 0; s < 2; ++s) mbar_init(&s_full[s], 1), mbar_init(&p_full[s], 4), mbar_init(&o_done[s], 1);
-        mbar_init(&q_full, 8), mbar_init(&x_full, 8), mbar_init(&epi_done, 8);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&s_full[s], 1), mbar_init(&p_full[s], 4), mbar_init(&o_done[s], 1);
+            mbar_init(&q_full[s], 1), mbar_init(&q_empty[s], 8);
+        }
+        for (int i = 0; i < SEGS; ++i) mbar_init(&seg_full[i], 1), mbar_init(&seg_empty[i], 11);
+        mbar_init(&x_full, 8), mbar_init(&epi_done, 8);
         mbar_fence_init();
-        odd_sm = 0;
     }
     if (warp == 2) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     fence_before();
-    pdl_wait_prior();
-    pdl_launch_dependents();
-    const Share share = cta_share<TM, TK, TT, 1>(p); // (its barriers also publish the set-up above)
     __syncthreads();
     fence_after();
-    const uint32_t tmem = tmem_s;
-    if (tid == 0) p.meta[blockIdx.x * TREE_META] = make_int4(-1, 0, 0, 0);
-    __syncthreads(); // ordered before the record of the CTA's cut unit
+    pdl_wait_prior();
+    pdl_launch_dependents();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_s, 0);
     bool ok = true;
+    // the next segment of the ring; count 0: no more
+    uint32_t seg = 0;
+    auto take = [&]() -> int {
+        ok = wait_bounded(&seg_full[seg % SEGS], seg / SEGS & 1);
+        return ok ? __shfl_sync(0xffffffffu, segs[seg % SEGS].count, 0) : 0;
+    };
+    auto give = [&]() { // this warp is done with the segment
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&seg_empty[seg % SEGS]);
+        ++seg;
+    };
 
-    if (warp == 0) {
+    if (warp == 3) {
+        // ---- division of the work ----
+        if (lane == 0) p.meta[blockIdx.x * TREE_META] = make_int4(-1, 0, 0, 0);
+        __syncwarp();
+        Sched<TM, TK, T_COST, T_MIN> sched(p);
+        const bool some = sched.init();
+        for (;; ++seg) {
+            Seg next;
+            next.count = 0;
+            if (some) next = sched.next(p.meta + blockIdx.x * TREE_META);
+            if (seg >= SEGS && !(ok = wait_bounded(&seg_empty[seg % SEGS], (seg / SEGS - 1) & 1))) break;
+            if (lane == 0) {
+                segs[seg % SEGS] = next;
+                mbar_arrive(&seg_full[seg % SEGS]);
+            }
+            if (!next.count) break;
+        }
+    } else if (warp == 0) {
         // ---- TMA: lane -> (64 values, box of keys) ----
         const int atom = lane % C::ATOMS, part = lane / C::ATOMS, box = prm.box, parts = TK / box;
         const bool mine = part < parts;
         uint32_t tile0 = 0;
-        for (W w(p, share); w.more() && ok; w.next()) {
-            const int key_end = Tiles<TM, TK>::key_end(p, w.v, w.t), n = w.end - w.blk;
-            const int *const table = p.blocks + (size_t)w.v.id * p.max_blocks;
+        for (int n; (n = take()) != 0 && ok; give()) {
+            const Seg &w = segs[seg % SEGS];
+            const int key_end = w.key_end, h = w.h, first = w.blk * TK + part * box;
+            const int *const table = p.blocks + (size_t)w.id * p.max_blocks;
             auto page_of = [&](int j) { // page of this lane's box in block j of the segment
-                const int token = (w.blk + j) * TK + part * box;
+                const int token = first + j * TK;
                 return mine && j < n && token < key_end ? table[token / p.page_size] : 0;
             };
             auto load = [&](const CUtensorMap *map, int j, uint32_t tile, int page) {
                 const uint32_t st = tile % NST;
                 if (tile >= NST && !wait_bounded(&empty[st], (tile / NST - 1) & 1)) return false;
-                const int token = (w.blk + j) * TK + part * box;
+                const int token = first + j * TK;
                 const bool go = mine && token < key_end;
                 const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, go));
                 if (lane == 0) mbar_arrive_expect_tx(&full[st], boxes * box * 128);
                 __syncwarp();
                 if (go) {
                     const int slot = token % p.page_size;
-                    tma_box(smem_u32(ring) + st * C::TILE + atom * (TK * 128) + part * box * 128, map, atom * 64, prm.slot_dim == 1 ? slot : w.h,
-                            prm.slot_dim == 1 ? w.h : slot, page, smem_u32(&full[st]));
+                    tma_box(smem_u32(ring) + st * C::TILE + atom * (TK * 128) + part * box * 128, map, atom * 64, prm.slot_dim == 1 ? slot : h,
+                            prm.slot_dim == 1 ? h : slot, page, smem_u32(&full[st]));
                 }
                 return true;
             };
@@ -233,92 +317,100 @@ template <typename T, int D> __global__ void __launch_bounds__(TT, 1) tree_attn_
                 if (i > 0 && ok) ok = load(&maps.v, i - 1, tile0 + v_tile(i - 1, n), prev);
                 prev = cur, cur = next;
             }
+            if (!ok) break;
             tile0 += 2 * n;
         }
+    } else if (warp == 2) {
+        // ---- queries: 16-byte pieces into swizzled rows, padding as zeros ----
+        constexpr int PIECES = D / 8;
+        const int piece = lane % PIECES, step = 32 / PIECES;
+        for (int n; (n = take()) != 0 && ok; give()) {
+            const uint32_t b = seg & 1;
+            if (seg >= 2 && !(ok = wait_bounded(&q_empty[b], (seg / 2 - 1) & 1))) break;
+            const Seg &w = segs[seg % SEGS];
+            const int rows = w.rows, group = p.group;
+            int r = lane / PIECES, token = (w.row0 + r) / group, g = (w.row0 + r) % group;
+            const T *const src = (const T *)p.q + w.r0 * p.q_stride + (long long)w.h * group * D + piece * 8;
+            const uint32_t dst = smem_u32(q_sm) + b * C::TILE + (piece / 8) * (TM * 128);
+#pragma unroll 8
+            for (; r < TM; r += step) {
+                const bool on = r < rows;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + r * 128 + (((piece % 8) ^ (r & 7)) << 4)),
+                             "l"(on ? src + token * p.q_stride + g * D : src), "r"(on ? 16 : 0)
+                             : "memory");
+                for (g += step; g >= group; g -= group) ++token;
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full[b]);
+        }
     } else if (warp == 1) {
-        // ---- MMA issue ----
-        uint32_t tile0 = 0, seg = 0, done[2] = {0, 0};
+        // ---- MMA issue: the whole warp with uniform control flow, one elected lane issues ----
+        uint32_t tile0 = 0, done[2] = {0, 0};
         const uint32_t q0 = smem_u32(q_sm), r0 = smem_u32(ring);
-        for (W w(p, share); w.more() && ok; w.next(), ++seg) {
-            const uint32_t n = w.end - w.blk;
-            ok = wait_bounded(&q_full, seg & 1);
-            if (ok && seg) ok = wait_bounded(&epi_done, (seg - 1) & 1); // the accumulators have been read
+        for (uint32_t n; (n = (uint32_t)take()) != 0 && ok; give()) {
+            const uint64_t qd = desc_k_major(q0 + (seg & 1) * C::TILE);
+            if (!(ok = wait_bounded(&q_full[seg & 1], seg / 2 & 1))) break;
             for (uint32_t i = 0; i <= n && ok; ++i) {
                 if (i < n) {
                     const uint32_t tile = tile0 + k_tile(i), st = tile % NST;
                     if (!(ok = wait_bounded(&full[st], tile / NST & 1))) break;
                     fence_after();
-                    if (lane == 0) {
-                        // the score tile's last user, P V of the block before last, was issued earlier and runs before
+                    // (the score tile's last user, P V of the block before last, was issued earlier and runs before)
+                    const uint64_t kd = desc_k_major(r0 + st * C::TILE);
 #pragma unroll
-                        for (int kk = 0; kk < D / 16; ++kk) {
-                            const uint32_t off = (kk / 4) * (TK * 128) + (kk % 4) * 32;
-                            mma_ss(tmem + (i & 1) * 128, desc_k_major(q0 + off), desc_k_major(r0 + st * C::TILE + off), idesc<T>(TK, false), kk > 0);
-                        }
-                        mma_commit(&empty[st]);
-                        mma_commit(&s_full[i & 1]);
-                    }
-                    __syncwarp();
+                    for (int a = 0; a < C::ATOMS; ++a) mma4_ss(tmem + (i & 1) * 128, qd + a * (TM * 128 >> 4), kd + a * (TK * 128 >> 4), idesc<T>(TK, false), a > 0);
+                    commit2(&empty[st], &s_full[i & 1]);
                 }
                 if (i > 0) {
                     const uint32_t j = i - 1, s = j & 1, tile = tile0 + v_tile(j, n), st = tile % NST;
-                    if (!(ok = wait_bounded(&full[st], tile / NST & 1) && wait_bounded(&p_full[s], done[s] & 1))) break;
+                    if (!(ok = wait_bounded(&full[st], tile / NST & 1))) break;
+                    if (j == 0 && seg && !(ok = wait_bounded(&epi_done, (seg - 1) & 1))) break; // the accumulators have been read
+                    if (!(ok = wait_bounded(&p_full[s], done[s] & 1))) break;
                     fence_after();
-                    if (lane == 0) {
-#pragma unroll
-                        for (int kk = 0; kk < TK / 16; ++kk)
-                            mma_ts(tmem + C::O_COL + s * D, tmem + s * 128 + kk * 8, desc_mn_major(r0 + st * C::TILE + kk * 16 * 128), idesc<T>(D, true), j >= 2 || kk > 0);
-                        mma_commit(&empty[st]);
-                        mma_commit(&o_done[s]);
-                    }
-                    __syncwarp();
+                    const uint64_t vd = desc_mn_major(r0 + st * C::TILE);
+                    mma4_ts(tmem + C::O_COL + s * D, tmem + s * 128, vd, idesc<T>(D, true), j >= 2);
+                    mma4_ts(tmem + C::O_COL + s * D, tmem + s * 128 + 32, vd + 4 * 128, idesc<T>(D, true), 1);
+                    commit2(&empty[st], &o_done[s]);
                     ++done[s];
                 }
             }
+            if (!ok) break;
             tile0 += 2 * n;
         }
-    } else if (warp >= 4) {
+    } else {
         // ---- the streams ----
         const uint32_t s = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t t_lane = tmem + (quarter * 32u << 16), t_s = t_lane + s * 128, t_o = t_lane + C::O_COL + s * D;
-        uint32_t tile0 = 0, seg = 0, done[2] = {0, 0};
-        for (W w(p, share); w.more() && ok; w.next(), ++seg) {
-            const SeqView v = w.v;
-            const uint32_t n = w.end - w.blk;
-            const int row0 = w.t * TM, rows = min(TM, v.n * p.group - row0);
-            const int key_end = Tiles<TM, TK>::key_end(p, v, w.t);
-            { // queries: 16-byte pieces into the swizzled rows
-                constexpr int PIECES = D / 8;
-                for (int c = tid - 128; c < TM * PIECES; c += 256) {
-                    const int r = c / PIECES, d = c % PIECES;
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (r < rows)
-                        x = *(const uint4 *)((const T *)p.q + (v.r0 + (row0 + r) / p.group) * p.q_stride + (w.h * p.group + (row0 + r) % p.group) * D + d * 8);
-                    *(uint4 *)(q_sm + (d / 8) * (TM * 128) + r * 128 + (((d % 8) ^ (r & 7)) << 4)) = x;
-                }
-                fence_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full);
-            }
-            const int me = (row0 + min((int)row, rows - 1)) / p.group; // this row's index in the sequence
+        uint32_t tile0 = 0, done[2] = {0, 0};
+        const float scale = p.scale_log2;
+        for (uint32_t n; (n = (uint32_t)take()) != 0 && ok; give()) {
+            Seg &w = segs[seg % SEGS];
+            SeqView v;
+            v.r0 = w.r0, v.n = w.n, v.id = w.id, v.ctx = w.ctx, v.kv = w.kv;
+            const int rows = w.rows, key_end = w.key_end, blk = w.blk;
+            const bool idle = (int)(quarter * 32) >= rows; // rows of padding: what they hold reaches no other row
+            const int me = (w.row0 + min((int)row, rows - 1)) / p.group; // this row's index in the sequence
             float m = -INFINITY, l = 0.f; // reference (a power of two), sum of weights
             for (uint32_t j = s; j < n && ok; j += 2) {
-                const int key0 = (w.blk + j) * TK;
+                const int key0 = (blk + j) * TK;
                 const bool tail = key0 + TK > v.ctx;
-                if (!(ok = wait_bounded(&s_full[s], done[s] & 1))) break;
-                fence_after();
-                if (tail) { // clean the values of this block: thread = key
-                    const uint32_t tile = tile0 + v_tile(j, n), st = tile % NST;
-                    if (!(ok = wait_bounded(&full[st], tile / NST & 1))) break;
-                    const int token = key0 + (int)(tid & 127);
-                    if (token >= v.ctx) {
-                        const uint32_t kr = tid & 127;
-                        bool odd = false;
+                uint32_t bits[4];
+                if (tail) {
 #pragma unroll
+                    for (int c = 0; c < 4; ++c) bits[c] = view_bits(p, v, me, key0 + 32 * c);
+                    // clean the values of this block: thread = key
+                    const uint32_t tile = tile0 + v_tile(j, n), st = tile % NST, kr = tid & 127;
+                    if (!(ok = wait_bounded(&full[st], tile / NST & 1))) break;
+                    const int token = key0 + (int)kr;
+                    if (token >= v.ctx) {
+                        bool odd = false;
+#pragma unroll 1
                         for (int a = 0; a < C::ATOMS; ++a)
 #pragma unroll
-                            for (int c = 0; c < 8; ++c) {
-                                uint4 *const at = (uint4 *)(ring + st * C::TILE + a * (TK * 128) + kr * 128 + c * 16);
+                            for (int c = 0; c < 8; ++c) { // (the lanes of a row group on different banks)
+                                uint4 *const at = (uint4 *)(ring + st * C::TILE + a * (TK * 128) + kr * 128 + ((c ^ (kr & 7)) << 4));
                                 if (token >= key_end) {
                                     *at = make_uint4(0, 0, 0, 0);
                                 } else {
@@ -331,73 +423,85 @@ template <typename T, int D> __global__ void __launch_bounds__(TT, 1) tree_attn_
                                     }
                                 }
                             }
-                        if (odd) odd_sm = seg + 1;
+                        if (odd) w.odd = 1;
+                        fence_async();
                     }
-                    fence_async();
                 }
-                // two passes over the scores, 64 columns in registers at a time: reading tensor memory twice costs less
-                // than what 128 live values spill
-                uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
-                if (tail)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) bits[c] = view_bits(p, v, me, key0 + 32 * c);
-                auto scores = [&](int half, uint32_t(&x)[64]) {
-                    tmem_ld32(t_s + 64 * half, x);
-                    tmem_ld32(t_s + 64 * half + 32, x + 32);
-                    wait_ld();
-                    if (tail)
-#pragma unroll
-                        for (int e = 0; e < 64; ++e)
-                            if (!(bits[2 * half + e / 32] >> (e % 32) & 1u)) x[e] = 0xff800000u;
-                };
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t x[64];
-                    scores(half, x);
-#pragma unroll
-                    for (int e = 0; e < 64; ++e) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(x[e]));
-                }
-                const float block_max = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2 - lift<T>();
-                if (__any_sync(0xffffffffu, block_max > m + 8.f)) {
-                    const float to = block_max > m + 8.f ? block_max : m;
-                    const float corr = m == to ? 1.f : ex2(m - to);
-                    if (j >= 2) {
-                        if (!(ok = wait_bounded(&o_done[s], (done[s] - 1) & 1))) break; // P V of the stream's block before
-                        fence_after();
-#pragma unroll
-                        for (int c = 0; c < D; c += 32) {
-                            uint32_t o[32];
-                            tmem_ld32(t_o + c, o);
+                if (!(ok = wait_bounded(&s_full[s], done[s] & 1))) break;
+                fence_after();
+                if (!idle) {
+                    if (tail) { // what a row does not see is masked where the scores lie
+#pragma unroll 1
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t x[32];
+                            const uint32_t see = c == 0 ? bits[0] : (c == 1 ? bits[1] : (c == 2 ? bits[2] : bits[3]));
+                            tmem_ld32(t_s + 32 * c, x);
                             wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-                            tmem_st32(t_o + c, o);
+                            for (int e = 0; e < 32; ++e)
+                                if (!(see >> e & 1u)) x[e] = 0xff800000u;
+                            tmem_st32(t_s + 32 * c, x);
+                        }
+                        wait_st();
+                    }
+                    // two passes over the scores, 64 columns in registers at a time: reading tensor memory twice costs less than
+                    // what 128 live values spill, and loops keep the code of a block small (a CTA runs it a few times only)
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t x[64];
+                        tmem_ld32(t_s + 64 * half, x);
+                        tmem_ld32(t_s + 64 * half + 32, x + 32);
+                        wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 64; e += 8)
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) top[u] = max3(top[u], __uint_as_float(x[e + u]), __uint_as_float(x[e + 4 + u]));
+                    }
+                    const float block_max = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale - lift<T>();
+                    if (__any_sync(0xffffffffu, block_max > m + 8.f)) {
+                        const float to = block_max > m + 8.f ? block_max : m;
+                        const float corr = m == to ? 1.f : ex2(m - to);
+                        if (j >= 2) {
+                            if (!(ok = wait_bounded(&o_done[s], (done[s] - 1) & 1))) break; // P V of the stream's block before
+                            fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 32) {
+                                uint32_t o[32];
+                                tmem_ld32(t_o + c, o);
+                                wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                                tmem_st32(t_o + c, o);
+                            }
+                        }
+                        l *= corr, m = to;
+                    }
+                    const float sub = m == -INFINITY ? 0.f : m; // nothing seen yet: every weight is 2^-inf
+                    float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+                    const float2 scale2 = {scale, scale}, sub2 = {-sub, -sub};
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t x[64];
+                        tmem_ld32(t_s + 64 * half, x);
+                        tmem_ld32(t_s + 64 * half + 32, x + 32);
+                        wait_ld();
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            uint32_t w16[16];
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                float2 a = fma2(make_float2(__uint_as_float(x[32 * c + 2 * e]), __uint_as_float(x[32 * c + 2 * e + 1])), scale2, sub2);
+                                a.x = ex2(a.x), a.y = ex2(a.y);
+                                sum[e & 1] = add2(sum[e & 1], a);
+                                w16[e] = pack2<T>(a.x, a.y);
+                            }
+                            tmem_st16(t_s + 32 * half + 16 * c, w16);
                         }
                     }
-                    l *= corr, m = to;
+                    l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                    wait_st();
                 }
-                const float sub = m == -INFINITY ? 0.f : m; // nothing seen yet: every weight is 2^-inf
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t x[64];
-                    scores(half, x);
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t w16[16];
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const float a = ex2(fmaf(__uint_as_float(x[32 * c + 2 * e]), p.scale_log2, -sub));
-                            const float b = ex2(fmaf(__uint_as_float(x[32 * c + 2 * e + 1]), p.scale_log2, -sub));
-                            sum[e & 1] += a, sum[2 + (e & 1)] += b;
-                            w16[e] = pack2<T>(a, b);
-                        }
-                        tmem_st16(t_s + 32 * half + 16 * c, w16);
-                    }
-                }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                wait_st();
                 fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[s]);
@@ -406,67 +510,53 @@ template <typename T, int D> __global__ void __launch_bounds__(TT, 1) tree_attn_
             if (!ok) break;
             // ---- join the streams' parts, store ----
             done[1 - s] += s == 0 ? n / 2 : (n + 1) / 2;
-            tmem_st2(t_s + 64, m, l); // behind the weights, in columns that only scores use
-            wait_st();
-            fence_before();
+            // all products of this segment that this stream waits for here were issued after the last use of the queries,
+            // whose memory carries the references and sums from one stream to the other
+            ok = wait_bounded(&o_done[0], (done[0] - 1) & 1) && (n < 2 || wait_bounded(&o_done[1], (done[1] - 1) & 1));
+            if (!ok) break;
+            float2 *const ml = (float2 *)(q_sm + (seg & 1) * C::TILE);
+            ml[s * TM + row] = make_float2(m, l);
             __syncwarp();
             if (lane == 0) mbar_arrive(&x_full);
-            ok = wait_bounded(&x_full, seg & 1) && wait_bounded(&o_done[0], (done[0] - 1) & 1) && (n < 2 || wait_bounded(&o_done[1], (done[1] - 1) & 1));
-            if (!ok) break;
+            if (!(ok = wait_bounded(&x_full, seg & 1))) break;
             fence_after();
-            const float2 a = tmem_ld2(t_lane + 64), b1 = tmem_ld2(t_lane + 128 + 64);
-            wait_ld();
-            const float2 b = n < 2 ? make_float2(-INFINITY, 0.f) : b1;
-            const float mm = fmaxf(a.x, b.x);
-            const float wa = a.x == -INFINITY ? 0.f : exp2f(a.x - mm), wb = b.x == -INFINITY ? 0.f : exp2f(b.x - mm);
-            const float ll = a.y * wa + b.y * wb;
-            const bool whole = w.whole(), live = (int)row < rows, odd = odd_sm == seg + 1;
-            float *const mine = part_of<TM>(p, blockIdx.x, w.slot());
-            const float inv = ll == 0.f ? 0.f : 1.0f / ll;
-            T *const out = (T *)p.out + (v.r0 + (row0 + row) / p.group) * p.out_stride + (w.h * p.group + (row0 + row) % p.group) * (long long)D;
-#pragma unroll
-            for (int c = (int)s * (D / 2), u = 0; u < D / 2; u += 32) {
-                uint32_t o0[32], o1[32];
-                tmem_ld32(t_lane + C::O_COL + c + u, o0);
-                tmem_ld32(t_lane + C::O_COL + D + c + u, o1);
-                wait_ld();
-                float o[32];
-#pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(o0[e]) * wa + (n < 2 ? 0.f : __uint_as_float(o1[e]) * wb);
-                if (odd && live) { // infinities and NaN of the tokens that the row sees
-                    const int *const table = p.blocks + (size_t)v.id * p.max_blocks;
-                    for (int token = max(v.ctx, w.blk * TK); token < min(key_end, w.end * TK); ++token) {
-                        const int page = table[token / p.page_size];
-                        if ((unsigned)page >= (unsigned)p.n_pages || !sees(p, v, me, token - v.ctx)) continue;
-                        const T *const at = (const T *)p.v + page * p.page_stride + token % p.page_size * p.slot_stride + w.h * p.head_stride + c + u;
+            const float2 a = ml[row], b = n < 2 ? make_float2(-INFINITY, 0.f) : ml[TM + row];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_empty[seg & 1]);
+            if (!idle) {
+                const float mm = fmaxf(a.x, b.x);
+                const float wa = a.x == -INFINITY ? 0.f : ex2(a.x - mm), wb = b.x == -INFINITY ? 0.f : ex2(b.x - mm);
+                const float ll = a.y * wa + b.y * wb;
+                const bool whole = w.flags & 1, live = (int)row < rows, odd = w.odd;
+                const int head = w.h;
+                float *const mine = part_of<TM>(p, blockIdx.x, w.flags >> 1);
+                const float inv = ll == 0.f ? 0.f : 1.0f / ll;
+                T *const out = (T *)p.out + (v.r0 + me) * p.out_stride + (head * p.group + (w.row0 + row) % p.group) * (long long)D;
 #pragma unroll 1
-                        for (int e4 = 0; e4 < 32; e4 += 4) {
+                for (int c = (int)s * (D / 2); c < (int)(s + 1) * (D / 2); c += 32) {
+                    uint32_t o0[32], o1[32];
+                    tmem_ld32(t_lane + C::O_COL + c, o0);
+                    tmem_ld32(t_lane + C::O_COL + D + c, o1);
+                    wait_ld();
+                    float o[32];
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) // (a register array wants constant indices)
-                                if ((e & ~3) == e4) {
-                                    const float y = (float)at[e];
-                                    if (!isfinite(y)) o[e] += y;
-                                }
+                    for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(o0[e]) * wa + (n < 2 ? 0.f : __uint_as_float(o1[e]) * wb);
+                    if (odd && live) add_odd<T>(p, v, head, me, max(v.ctx, blk * TK), min(key_end, (int)(blk + n) * TK), c, o);
+                    if (!live) continue;
+                    if (whole) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            uint32_t y[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) y[k] = pack2<T>(ll == 0.f ? 0.f : o[e + 2 * k] * inv, ll == 0.f ? 0.f : o[e + 2 * k + 1] * inv);
+                            *(uint4 *)(out + c + e) = make_uint4(y[0], y[1], y[2], y[3]);
                         }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) *(float4 *)(mine + (size_t)row * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                     }
                 }
-                if (!live) continue;
-                if (whole) {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        uint32_t y[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) y[k] = pack2<T>(ll == 0.f ? 0.f : o[e + 2 * k] * inv, ll == 0.f ? 0.f : o[e + 2 * k + 1] * inv);
-                        *(uint4 *)(out + c + u + e) = make_uint4(y[0], y[1], y[2], y[3]);
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4) *(float4 *)(mine + (size_t)row * D + c + u + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                }
-            }
-            if (!whole) {
-                if (s == 0 && live) *(float2 *)(mine + (size_t)TM * D + 2 * row) = make_float2(mm, ll);
-                if (tid == 128 && w.first()) w.record(p.meta + blockIdx.x * TREE_META);
+                if (!whole && s == 0 && live) *(float2 *)(mine + (size_t)TM * D + 2 * row) = make_float2(mm, ll);
             }
             fence_before();
             __syncwarp();
@@ -512,7 +602,7 @@ template <typename T, int D> cudaError_t launch(const DeviceInfo &dev, const TcP
     cudaError_t e = cudaFuncSetAttribute(tree_attn_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
     if (e != cudaSuccess) return e;
     if ((e = launch_kernel(tree_attn_tc_kernel<T, D>, dim3(dev.sm_count), dim3(TT), Cfg<D>::SMEM, st, pdl, prm, maps)) != cudaSuccess) return e;
-    return launch_kernel(tree_join_kernel<T, TM>, dim3(dev.sm_count, TM / 8), dim3(256), 0, st, pdl, prm.t);
+    return launch_kernel(tree_join_kernel<T, TM>, dim3(dev.sm_count * 2), dim3(32 * JOIN_WARPS), 0, st, pdl, prm.t, dev.sm_count);
 }
 
 } // namespace

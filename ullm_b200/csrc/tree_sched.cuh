@@ -2,11 +2,13 @@
 //
 // A unit of work is (sequence, key head, tile of M query rows); a query row is (row of the step, query head of the
 // group), so that a group's heads share every key that is loaded.  A unit takes its key blocks in order.  All units'
-// blocks are laid end to end and every CTA takes an equal contiguous part of that line, whatever the
-// lengths are: one long sequence fills the machine as well as a thousand short ones.  A unit that is cut leaves unnormalised
-// partial results (running maximum, sum and weighted values of each row) in the work area; a CTA has at most two of
-// them, its first and its last, and the CTA in which a cut unit ends records what the joining kernel needs.
-// Lengths are read on the device, so a captured call serves every later state of the tables.
+// blocks are laid end to end, each unit led in by COST places for what it costs to begin and to end one, and every CTA
+// takes an equal contiguous part of that line, whatever the lengths are: one long sequence fills the machine as well as a
+// thousand short ones.  A unit that is cut leaves unnormalised partial results (running maximum, sum and
+// weighted values of each row) in the work area; a CTA has at most two of them, its first and its last, and the CTA in
+// which a cut unit ends records what the joining kernel needs.  Lengths are read on the device, so a captured call serves
+// every later state of the tables.  One warp of a CTA works the division out (Sched) and hands the segments to the others:
+// done by every thread, with 64-bit divisions, it took 6,000 of the 13,800 cycles of a one-token call.
 #pragma once
 
 #include "paged.h"
@@ -46,143 +48,169 @@ template <int M, int KB> struct Tiles {
         return v.ctx + min((int)(((t + 1u) * M - 1u) / (unsigned)p.group), v.n - 1) + 1;
     }
     static __device__ __forceinline__ int blocks(const TreeDev &p, const SeqView &v, int t) { return max(1, (key_end(p, v, t) + KB - 1) / KB); }
-    // blocks of all tiles of one key head
-    static __device__ __forceinline__ long long per_head(const TreeDev &p, const SeqView &v) {
-        const int T = count(p, v);
-        if (!T) return 0;
-        if (p.mask || T == 1) return (long long)T * blocks(p, v, 0);
-        long long s = 0;
-        for (int t = 0; t < T; ++t) s += blocks(p, v, t);
+};
+
+// The part of one unit that lies in a CTA's share.
+struct __align__(16) Seg {
+    int r0, n, id, ctx, kv;       // the sequence (SeqView)
+    int key_end;                  // one behind the last key that the tile's rows see
+    int h, row0, rows;            // key head; first row of the tile among the sequence's query rows, and how many there are
+    int blk, count;               // first key block, blocks (0: no more segments)
+    int flags;                    // 1: the whole unit; 2: its partial result goes to slot 1
+    int odd;                      // set by who finds values that are not finite among the rows' own tokens
+    int pad[3];
+};
+
+template <int M, int KB, int COST, int MINS> struct Sched {
+    using T = Tiles<M, KB>;
+    static constexpr unsigned ALL = 0xffffffffu;
+    const TreeDev &p;
+    const int lane;
+    unsigned total, active, each, more, lo, hi, cur; // share c begins at c * each + min(c, more)
+    int b, h, t, nt;
+    unsigned off; // place of `cur` in its unit
+    SeqView win;  // view of sequence wb + lane
+    int wb;
+    SeqView v;
+    bool first;
+
+    __device__ __forceinline__ explicit Sched(const TreeDev &p_) : p(p_), lane((int)(threadIdx.x & 31)) {}
+
+    __device__ __forceinline__ unsigned share_at(unsigned c) const { return c * each + min(c, more); }
+    __device__ __forceinline__ unsigned share_of(unsigned x) const { // the share that holds place x
+        const unsigned big = more * (each + 1);
+        return x < big ? x / (each + 1) : more + (x - big) / each;
+    }
+    // places of one key head of the sequence that lane `who` views (`mine`: this lane's); every lane calls it
+    __device__ __forceinline__ unsigned head_places(const SeqView &mine) const {
+        const int T_ = T::count(p, mine);
+        const bool simple = p.mask || T_ <= 8;
+        unsigned s = 0;
+        if (p.mask) {
+            s = T_ ? (unsigned)T_ * (T::blocks(p, mine, 0) + COST) : 0u;
+        } else if (simple) {
+            for (int i = 0; i < T_; ++i) s += T::blocks(p, mine, i) + COST;
+        }
+        for (unsigned long_ones = __ballot_sync(ALL, !simple); long_ones; long_ones &= long_ones - 1) { // prompts: all lanes together
+            const int who = __ffs(long_ones) - 1;
+            const SeqView u = view_of(mine, who);
+            const int n = T::count(p, u);
+            unsigned x = 0;
+            for (int i = lane; i < n; i += 32) x += T::blocks(p, u, i) + COST;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(ALL, x, o);
+            if (lane == who) s = x;
+        }
         return s;
     }
-};
-
-struct Share { // of one CTA
-    long long total, lo, hi;
-    int active; // CTAs that have a share
-    int b;      // sequence in which it begins
-    long long base; // blocks in front of that sequence
-};
-__device__ __forceinline__ long long share_at(long long total, int active, long long c) { return total * c / active; }
-
-// Sum over the CTA and exclusive prefix, NT threads (a multiple of 32).
-template <int NT> __device__ __forceinline__ long long cta_scan64(long long v, long long *excl, long long *warp_sums) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long x = v;
+    __device__ __forceinline__ SeqView view_of(const SeqView &mine, int who) const {
+        SeqView u;
+        u.r0 = __shfl_sync(ALL, mine.r0, who), u.n = __shfl_sync(ALL, mine.n, who), u.id = __shfl_sync(ALL, mine.id, who);
+        u.ctx = __shfl_sync(ALL, mine.ctx, who), u.kv = __shfl_sync(ALL, mine.kv, who);
+        return u;
+    }
+    __device__ __forceinline__ SeqView lane_view(int b0) const {
+        SeqView u;
+        u.r0 = u.n = u.id = u.ctx = u.kv = 0;
+        if (b0 + lane < p.n_seq) u = seq_view(p, b0 + lane);
+        return u;
+    }
+    // Works out the CTA's share; false: it has none.
+    __device__ __forceinline__ bool init() {
+        total = 0;
+        unsigned places = 0;
+        for (int b0 = 0; b0 < p.n_seq; b0 += 32) {
+            win = lane_view(b0), wb = b0;
+            places = head_places(win) * (unsigned)p.n_kv;
+            unsigned x = places;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-    }
-    __syncthreads();
-    if (lane == 31) warp_sums[warp] = x;
-    __syncthreads();
-    long long before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < NT / 32; ++w) {
-        const long long s = warp_sums[w];
-        if (w < warp) before += s;
-        all += s;
-    }
-    *excl = before + x - v;
-    return all;
-}
-
-// Every thread of the CTA calls it; MINB: a CTA takes at least so many blocks where there are few.
-template <int M, int KB, int NT, int MINB> __device__ __forceinline__ Share cta_share(const TreeDev &p) {
-    __shared__ long long sums[NT / 32];
-    __shared__ long long s_base;
-    __shared__ int s_b;
-    Share s;
-    s.total = 0;
-    long long work = 0, excl = 0;
-    for (int b0 = 0; b0 < p.n_seq; b0 += NT) {
-        const int b = b0 + threadIdx.x;
-        work = b < p.n_seq ? Tiles<M, KB>::per_head(p, seq_view(p, b)) * p.n_kv : 0;
-        s.total += cta_scan64<NT>(work, &excl, sums);
-    }
-    const long long wanted = (s.total + MINB - 1) / MINB;
-    s.active = (int)max(1ll, min((long long)gridDim.x, wanted));
-    s.b = 0, s.base = 0, s.lo = s.hi = 0;
-    if ((int)blockIdx.x >= s.active || s.total == 0) return s;
-    s.lo = share_at(s.total, s.active, blockIdx.x), s.hi = share_at(s.total, s.active, blockIdx.x + 1);
-    long long run = 0;
-    for (int b0 = 0; b0 < p.n_seq; b0 += NT) {
-        const int b = b0 + threadIdx.x;
-        long long sum;
-        if (p.n_seq > NT) {
-            work = b < p.n_seq ? Tiles<M, KB>::per_head(p, seq_view(p, b)) * p.n_kv : 0;
-            sum = cta_scan64<NT>(work, &excl, sums);
-        } else {
-            sum = s.total;
+            for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(ALL, x, o);
+            total += x;
         }
-        if (s.lo >= run + excl && s.lo < run + excl + work) s_b = b, s_base = run + excl;
-        run += sum;
-        if (run > s.lo) break;
-    }
-    __syncthreads();
-    s.b = s_b, s.base = s_base;
-    return s;
-}
-
-// Steps through a CTA's share, one segment (the part of one unit that lies in it) at a time.
-template <int M, int KB> struct Walk {
-    using T = Tiles<M, KB>;
-    const TreeDev &p;
-    const Share &s;
-    long long cur;
-    SeqView v;
-    int b, h, t, nt, blk; // the segment: key head, tile, first block ...
-    int nb, end;          // ... blocks of its unit, one behind its last block
-    __device__ Walk(const TreeDev &p_, const Share &s_) : p(p_), s(s_), cur(s_.lo), b(s_.b) {
-        if (cur >= s.hi) return;
-        v = seq_view(p, b);
-        nt = T::count(p, v);
-        const long long per = T::per_head(p, v);
-        long long o = cur - s.base;
-        h = (int)(o / per);
-        o -= h * per;
-        t = 0;
+        active = max(1u, min(gridDim.x, (total + MINS - 1) / MINS));
+        each = total / active, more = total - each * active;
+        if (blockIdx.x >= active || total == 0) return false;
+        lo = share_at(blockIdx.x), hi = share_at(blockIdx.x + 1), cur = lo, first = true;
+        unsigned run = 0; // places in front of the window
+        for (int b0 = 0; b0 < p.n_seq; b0 += 32) {
+            if (p.n_seq > 32) win = lane_view(b0), wb = b0, places = head_places(win) * (unsigned)p.n_kv;
+            unsigned incl = places;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned y = __shfl_up_sync(ALL, incl, o);
+                if (lane >= o) incl += y;
+            }
+            const unsigned here = __ballot_sync(ALL, lo < run + incl && lo >= run + incl - places);
+            if (here) {
+                const int who = __ffs(here) - 1;
+                off = lo - (run + __shfl_sync(ALL, incl - places, who));
+                b = b0 + who;
+                break;
+            }
+            run += __shfl_sync(ALL, incl, 31);
+        }
+        v = view_of(win, b - wb), nt = T::count(p, v);
+        const unsigned per = __shfl_sync(ALL, places / (unsigned)p.n_kv, b - wb);
+        h = (int)(off / per), off -= h * per, t = 0;
         if (p.mask) {
-            nb = T::blocks(p, v, 0);
-            t = (int)(o / nb), blk = (int)(o % nb);
+            const unsigned u = T::blocks(p, v, 0) + COST;
+            t = (int)(off / u), off -= t * u;
         } else {
-            for (nb = T::blocks(p, v, 0); o >= nb; nb = T::blocks(p, v, ++t)) o -= nb;
-            blk = (int)o;
-        }
-        end = blk + (int)min((long long)(nb - blk), s.hi - cur);
-    }
-    __device__ bool more() const { return cur < s.hi; }
-    __device__ bool first() const { return cur == s.lo; }
-    __device__ bool whole() const { return blk == 0 && end == nb; }
-    // where a cut unit's partial result goes
-    __device__ int slot() const { return first() ? 0 : 1; }
-    __device__ void next() {
-        cur += end - blk;
-        if (cur >= s.hi) return;
-        blk = 0;
-        if (++t == nt) {
-            t = 0;
-            if (++h == p.n_kv) {
-                h = 0;
-                do {
-                    v = seq_view(p, ++b);
-                    nt = T::count(p, v);
-                } while (nt == 0);
+            for (int t0 = 0;; t0 += 32) { // the tile, 32 at a time
+                const unsigned mine = t0 + lane < nt ? T::blocks(p, v, t0 + lane) + COST : 0u;
+                unsigned incl = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const unsigned y = __shfl_up_sync(ALL, incl, o);
+                    if (lane >= o) incl += y;
+                }
+                const unsigned here = __ballot_sync(ALL, off < incl && off >= incl - mine);
+                if (here) {
+                    t = t0 + __ffs(here) - 1, off -= __shfl_sync(ALL, incl - mine, t - t0);
+                    break;
+                }
+                off -= __shfl_sync(ALL, incl, 31);
             }
         }
-        nb = T::blocks(p, v, t);
-        end = (int)min((long long)nb, s.hi - cur);
+        return true;
     }
-    // What the joining kernel needs of the CTA in which a cut unit ends: the CTA and slot in which it begins.
-    __device__ void record(int4 *meta) const {
-        if (blk == 0 || end != nb) return;
-        const long long start = cur - blk;
-        long long c0 = start * s.active / s.total;
-        while (share_at(s.total, s.active, c0 + 1) <= start) ++c0;
-        while (share_at(s.total, s.active, c0) > start) --c0;
-        meta[0] = make_int4((int)c0, share_at(s.total, s.active, c0) == start ? 0 : 1, v.r0, v.n);
-        meta[1] = make_int4(t, h, 0, 0);
+    // The next segment; count 0 when the share is used up.  meta: where the joining kernel's record goes.
+    __device__ __forceinline__ Seg next(int4 *meta) {
+        Seg s;
+        s.count = 0, s.odd = 0;
+        while (cur < hi) {
+            const int nb = T::blocks(p, v, t);
+            const unsigned len = nb + COST, take = min(len - off, hi - cur);
+            const int b0 = max((int)off - COST, 0), b1 = (int)(off + take) - COST;
+            if (b1 > b0) {
+                s.r0 = v.r0, s.n = v.n, s.id = v.id, s.ctx = v.ctx, s.kv = v.kv, s.key_end = T::key_end(p, v, t);
+                s.h = h, s.row0 = t * M, s.rows = min(M, v.n * p.group - t * M);
+                s.blk = b0, s.count = b1 - b0;
+                const bool whole = b0 == 0 && b1 == nb;
+                s.flags = (whole ? 1 : 0) | (first ? 0 : 2);
+                if (!whole && b1 == nb && lane == 0) {
+                    // the unit begins in the CTA that holds its first block; it is that CTA's first segment unless
+                    // the CTA's share begins before the unit
+                    const unsigned unit = cur - off, c0 = share_of(unit + COST);
+                    meta[0] = make_int4((int)c0, share_at(c0) >= unit ? 0 : 1, v.r0, v.n);
+                    meta[1] = make_int4(t, h, 0, 0);
+                }
+                first = false;
+            }
+            cur += take, off = 0;
+            if (cur < hi && ++t == nt) {
+                t = 0;
+                if (++h == p.n_kv) {
+                    h = 0;
+                    do {
+                        if (++b - wb == 32) win = lane_view(b), wb = b;
+                        v = view_of(win, b - wb), nt = T::count(p, v);
+                    } while (nt == 0);
+                }
+            }
+            if (s.count) break;
+        }
+        return s;
     }
 };
 
@@ -196,46 +224,121 @@ template <> __device__ __forceinline__ float out_from<float>(float v) { return v
 template <> __device__ __forceinline__ __half out_from<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 out_from<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Joins the parts of the unit that ends in CTA blockIdx.x, in the order of the CTAs: a row per warp.
-// out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c.
-template <typename O, int M> __global__ void __launch_bounds__(256) tree_join_kernel(const TreeDev p) {
+// Joins the parts of the units that were cut, in the order of the CTAs:
+//   out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c.
+// A fixed number of CTAs share the rows of all cut units: every CTA reads the records, SPLIT warps take a row together (each
+// a part of the parts, eight loads in flight), because a long context of one sequence is cut into as many parts as there are CTAs.
+constexpr int JOIN_WARPS = 8;
+template <typename O, int M> __global__ void __launch_bounds__(32 * JOIN_WARPS) tree_join_kernel(const TreeDev p, int ctas) {
+    __shared__ int2 duty[1024]; // {CTA, rows in front}
+    __shared__ int n_duty, n_rows, most;
+    __shared__ float red[JOIN_WARPS][256], red_l[JOIN_WARPS];
     pdl_wait_prior();
     pdl_launch_dependents();
-    const int c = blockIdx.x, lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
-    const int4 a = p.meta[c * TREE_META], b = p.meta[c * TREE_META + 1];
-    if (a.x < 0) return;
-    const long long row = (long long)b.x * M + r;
-    if (row >= (long long)a.w * p.group) return;
-    const int parts = c - a.x + 1;
-    auto part = [&](int k) { return part_of<M>(p, a.x + k, k == 0 ? a.y : 0); };
-    float m = -INFINITY;
-    for (int k = lane; k < parts; k += 32) m = fmaxf(m, part(k)[(size_t)M * p.dim + 2 * r]);
-    m = warp_max(m);
-    float l = 0.f, acc[8];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (warp == 0) {
+        int found = 0, rows = 0, parts = 0;
+        for (int c0 = 0; c0 < ctas; c0 += 32) {
+            const int c = c0 + lane;
+            int4 a = make_int4(-1, 0, 0, 0);
+            int r = 0;
+            if (c < ctas) a = p.meta[c * TREE_META];
+            if (a.x >= 0) r = min(M, a.w * p.group - p.meta[c * TREE_META + 1].x * M), parts = max(parts, c - a.x + 1);
+            const unsigned has = __ballot_sync(0xffffffffu, a.x >= 0);
+            int incl = r;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-    for (int k0 = 0; k0 < parts; k0 += 32) {
-        float w = 0.f;
-        if (k0 + lane < parts) {
-            const float2 ml = *(const float2 *)(part(k0 + lane) + (size_t)M * p.dim + 2 * r);
-            w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
-            l += ml.y * w;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += y;
+            }
+            if (a.x >= 0) duty[found + __popc(has & ((1u << lane) - 1u))] = make_int2(c, rows + incl - r);
+            found += __popc(has), rows += __shfl_sync(0xffffffffu, incl, 31);
         }
-        for (int k = 0; k < min(32, parts - k0); ++k) {
-            const float wk = __shfl_sync(0xffffffffu, w, k);
-            if (wk == 0.f) continue; // an empty part's values were never written
-            const float *o = part(k0 + k) + (size_t)r * p.dim;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (lane + 32 * e < p.dim) acc[e] += wk * o[lane + 32 * e];
-        }
+        for (int o = 16; o > 0; o >>= 1) parts = max(parts, __shfl_xor_sync(0xffffffffu, parts, o));
+        if (lane == 0) n_duty = found, n_rows = rows, most = parts;
     }
-    l = warp_sum(l);
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    O *out = (O *)p.out + (a.z + row / p.group) * p.out_stride + ((long long)b.y * p.group + row % p.group) * p.dim;
+    __syncthreads();
+    const int split = most > 8 ? 4 : 1, per = JOIN_WARPS / split, sub = warp % split;
+    for (int i0 = blockIdx.x * per; i0 < n_rows; i0 += gridDim.x * per) {
+        const int i = i0 + warp / split;
+        float m = -INFINITY, l = 0.f, acc[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (lane + 32 * e < p.dim) out[lane + 32 * e] = out_from<O>(l == 0.f ? 0.f : acc[e] * inv);
+        for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+        int4 a, b;
+        int r = 0;
+        if (i < n_rows) {
+            int lo = 0, hi = n_duty; // the unit of row i
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (duty[mid].y <= i) lo = mid;
+                else hi = mid;
+            }
+            const int c = duty[lo].x;
+            r = i - duty[lo].y;
+            a = p.meta[c * TREE_META], b = p.meta[c * TREE_META + 1];
+            const int parts = c - a.x + 1;
+            auto part = [&](int k) { return part_of<M>(p, a.x + k, k == 0 ? a.y : 0); };
+            for (int k = lane; k < parts; k += 32) m = fmaxf(m, part(k)[(size_t)M * p.dim + 2 * r]);
+            m = warp_max(m);
+            // this warp's parts: sub, sub + split, ...; 32 weights at a time, one per lane
+            for (int k0 = sub; k0 < parts; k0 += 32 * split) {
+                float w = 0.f;
+                if (k0 + lane * split < parts) {
+                    const float2 ml = *(const float2 *)(part(k0 + lane * split) + (size_t)M * p.dim + 2 * r);
+                    w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
+                    l += ml.y * w;
+                }
+                const int n = min(32, (parts - k0 + split - 1) / split);
+                for (int u0 = 0; u0 < n; u0 += 8) {
+                    if (p.dim <= 128) { // four values per lane
+                        float4 x[8];
+                        const bool on = lane * 4 < p.dim;
+#pragma unroll
+                        for (int u = 0; u < 8; ++u)
+                            if (u0 + u < n && on) x[u] = *(const float4 *)(part(k0 + (u0 + u) * split) + (size_t)r * p.dim + lane * 4);
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {
+                            const float wk = __shfl_sync(0xffffffffu, w, (u0 + u) & 31);
+                            if (u0 + u < n && on && wk != 0.f) acc[0] += wk * x[u].x, acc[1] += wk * x[u].y, acc[2] += wk * x[u].z, acc[3] += wk * x[u].w;
+                        }
+                    } else {
+                        for (int u = 0; u < 8 && u0 + u < n; ++u) {
+                            const float wk = __shfl_sync(0xffffffffu, w, u0 + u);
+                            if (wk == 0.f) continue;
+                            const float *o = part(k0 + (u0 + u) * split) + (size_t)r * p.dim;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (lane * 8 + e < p.dim) acc[e] += wk * o[lane * 8 + e];
+                        }
+                    }
+                }
+            }
+            l = warp_sum(l);
+        }
+        const int wide = p.dim <= 128 ? 4 : 8;
+        if (split > 1) { // the row's warps in order
+            __syncthreads();
+            if (lane * wide < p.dim)
+                for (int e = 0; e < wide; ++e) red[warp][lane * wide + e] = e < 4 ? acc[e & 3] : acc[4 + (e & 3)];
+            if (lane == 0) red_l[warp] = l;
+            __syncthreads();
+        }
+        if (i >= n_rows || sub) continue;
+        if (split > 1)
+            for (int s = 1; s < split; ++s) {
+                l += red_l[warp + s];
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e < wide && lane * wide < p.dim) acc[e] += red[warp + s][lane * wide + e];
+            }
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        const int row = b.x * M + r;
+        O *out = (O *)p.out + (a.z + row / p.group) * p.out_stride + ((long long)b.y * p.group + row % p.group) * p.dim;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < wide && lane * wide < p.dim) out[lane * wide + e] = out_from<O>(l == 0.f ? 0.f : acc[e] * inv);
+    }
 }
 
 } // namespace ullm

@@ -1,15 +1,16 @@
 // Attention of drafted rows over a paged cache on the 5th-generation tensor cores: f16 / bf16 queries and pages,
 // head_dim 64 or 128, pages of 8, 16, 32, 64 or a multiple of 128 slots.
 //
-// A CTA takes 128 query rows (rows of the step x query heads of a group; what is missing is padding, which costs no
-// memory traffic) and walks blocks of 128 keys.  Two streams of four warps take the blocks in turn, each with a score
-// tile and an accumulator of its own in tensor memory, so that one stream's exponentials run while the tensor cores work for the other:
+// A CTA walks blocks of 128 keys for a tile of query rows (rows of the step x query heads of a group; what is missing is padding, which
+// costs no memory traffic).  Two streams of four warps each have 128 rows, a score tile and an accumulator in tensor memory, so
+// that one stream's exponentials run while the tensor cores work for the other.  Where sequences have few rows the streams share a tile of
+// 128 and take its key blocks in turn; where they have more (TWO) each has a tile of its own and both use every block:
 //
 //   S_s = Q K_j^T          tcgen05.mma, operands in shared memory (TMA, 128-byte swizzle), f32 scores in tensor memory
 //   P_s = 2^(S_s - m_s)    one thread per row; rounded to the pages' type, written over the scores in tensor memory
 //   O_s += P_s V_j         tcgen05.mma, P from tensor memory, V from shared memory as it lies there (keys are the rows)
 //
-// and the two accumulators are joined when the CTA leaves the unit.  A row's reference m_s follows its running maximum
+// and, where they shared the rows, the two accumulators are joined when the CTA leaves the unit.  A row's reference m_s follows its running maximum
 // only when that has grown by more than 2^8 (weights then stay below 2^8 and the accumulator is rarely rescaled: the
 // result is the same quotient).  Sums, references and accumulators are f32; the weights are rounded once, to the type
 // the tensor cores take.
@@ -47,9 +48,11 @@ struct TcParams {
     int *status;
     int box;       // keys of a TMA box
     int slot_dim;  // coordinate (1 or 2) of the slot; the other one is the head
+    int q_box;     // rows of the step in a TMA box of queries; 0: queries through cp.async
+    int lanes;     // CTAs of a team (Sched)
 };
 struct TcMaps {
-    CUtensorMap k, v;
+    CUtensorMap k, v, q;
 };
 
 // A converged warp waits; every lane gets the same answer, so that no lane leaves alone.
@@ -111,6 +114,11 @@ __device__ __forceinline__ void commit2(uint64_t *x, uint64_t *y) {
                  "@pe tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
                  "@pe tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n}" ::"r"(smem_u32(x)),
                  "r"(smem_u32(y))
+                 : "memory");
+}
+__device__ __forceinline__ void commit1(uint64_t *x) {
+    asm volatile("{\n.reg .pred pe;\nelect.sync _|pe, 0xffffffff;\n"
+                 "@pe tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_u32(x))
                  : "memory");
 }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -196,9 +204,11 @@ __device__ __forceinline__ uint32_t view_bits(const TreeDev &p, const SeqView &v
     return limit >= 32 ? r : (limit <= 0 ? 0u : r & ((1u << limit) - 1u));
 }
 
-// Tiles reach shared memory in the order in which the tensor cores take them: K0 K1 V0 K2 V1 ... K(n-1) V(n-2) V(n-1)
-__device__ __forceinline__ uint32_t k_tile(uint32_t j) { return j ? 2 * j - 1 : 0; }
-__device__ __forceinline__ uint32_t v_tile(uint32_t j, uint32_t n) { return j + 1 == n ? 2 * n - 1 : 2 * j + 2; }
+// Place of the tile with the keys / values of block j of a segment of n blocks in the order in which tiles reach shared memory, which is
+// that in which the tensor cores take them: K0 K1 V0 K2 V1 ... K(n-1) V(n-2) V(n-1) where blocks alternate between the
+// streams, K0 V0 K1 V1 ... where both streams take each.
+template <bool TWO> __device__ __forceinline__ uint32_t k_tile(uint32_t j) { return TWO ? 2 * j : (j ? 2 * j - 1 : 0); }
+template <bool TWO> __device__ __forceinline__ uint32_t v_tile(uint32_t j, uint32_t n) { return TWO ? 2 * j + 1 : (j + 1 == n ? 2 * n - 1 : 2 * j + 2); }
 
 // Infinities and NaN among the values [c, c + 32) of tokens [first, last) that row `me` sees, added to the row's sums.  Rare, and out of the way.
 template <typename T> __device__ __noinline__ void add_odd_at(const TreeDev &p, const SeqView &v, int head, int me, int first, int last, int c, float *o) {
@@ -222,9 +232,9 @@ template <typename T> __device__ __forceinline__ void add_odd(const TreeDev &p, 
     for (int e = 0; e < 32; ++e) o[e] = copy[e];
 }
 
-template <typename T, int D> __global__ void __launch_bounds__(TT, 1) tree_attn_tc_kernel(const __grid_constant__ TcParams prm, const __grid_constant__ TcMaps maps) {
+template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) tree_attn_tc_kernel(const __grid_constant__ TcParams prm, const __grid_constant__ TcMaps maps) {
     using C = Cfg<D>;
-    constexpr int NST = C::STAGES;
+    constexpr int NST = C::STAGES, ROWS = TWO ? 2 * TM : TM, STEP = TWO ? 1 : 2; // STEP: a stream takes every so many blocks
     extern __shared__ __align__(1024) uint8_t gsm[];
     uint8_t *const q_sm = (uint8_t *)(((uintptr_t)gsm + 1023) & ~(uintptr_t)1023), *const ring = q_sm + 2 * C::TILE;
     __shared__ uint64_t full[NST], empty[NST], s_full[2], p_full[2], o_done[2], q_full[2], q_empty[2], seg_full[SEGS], seg_empty[SEGS], x_full, epi_done;
@@ -232,6 +242,7 @@ template <typename T, int D> __global__ void __launch_bounds__(TT, 1) tree_attn_
     __shared__ uint32_t tmem_s;
     const TreeDev &p = prm.t;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (warp == 0 && lane < 3) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &maps.k : (lane == 1 ? &maps.v : &maps.q)) : "memory");
     if (tid == 0) {
         for (int i = 0; i < NST; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
         for (int s = 0; s < 2; ++s) {
@@ -269,7 +280,7 @@ template <typename T, int D> __global__ void __launch_bounds__(TT, 1) tree_attn_
         // ---- division of the work ----
         if (lane == 0) p.meta[blockIdx.x * TREE_META] = make_int4(-1, 0, 0, 0);
         __syncwarp();
-        Sched<TM, TK, T_COST, T_MIN> sched(p);
+        Sched<ROWS, TK, T_COST, T_MIN> sched(p, prm.lanes);
         const bool some = sched.init();
         for (;; ++seg) {
             Seg next;
@@ -290,10 +301,16 @@ template <typename T, int D> __global__ void __launch_bounds__(TT, 1) tree_attn_
         for (int n; (n = take()) != 0 && ok; give()) {
             const Seg &w = segs[seg % SEGS];
             const int key_end = w.key_end, h = w.h, first = w.blk * TK + part * box;
+            // entries of the page table, 32 at a time and one such load ahead: a block has 1 to 16 of them
+            const int per = p.page_size < TK ? parts : 1, e0 = p.page_size < TK ? w.blk * parts : w.blk * TK / p.page_size, e_end = (key_end + p.page_size - 1) / p.page_size;
             const int *const table = p.blocks + (size_t)w.id * p.max_blocks;
+            auto entries = [&](int e) { return e + (int)lane < e_end ? table[e + lane] : 0; };
+            int win = e0, now = entries(e0), ahead = entries(e0 + 32);
             auto page_of = [&](int j) { // page of this lane's box in block j of the segment
-                const int token = first + j * TK;
-                return mine && j < n && token < key_end ? table[token / p.page_size] : 0;
+                const int block_e = p.page_size < TK ? e0 + j * per : max(min((w.blk + j) * TK, key_end - 1), 0) / p.page_size; // the same in every lane
+                const int e = p.page_size < TK ? block_e + part : block_e;
+                if (block_e >= win + 32) win += 32, now = ahead, ahead = entries(win + 32);
+                return __shfl_sync(0xffffffffu, now, (e - win) & 31);
             };
             auto load = [&](const CUtensorMap *map, int j, uint32_t tile, int page) {
                 const uint32_t st = tile % NST;
@@ -304,76 +321,119 @@ template <typename T, int D> __global__ void __launch_bounds__(TT, 1) tree_attn_
                 if (lane == 0) mbar_arrive_expect_tx(&full[st], boxes * box * 128);
                 __syncwarp();
                 if (go) {
-                    const int slot = token % p.page_size;
+                    const int slot = p.page_size <= TK ? 0 : token % p.page_size;
                     tma_box(smem_u32(ring) + st * C::TILE + atom * (TK * 128) + part * box * 128, map, atom * 64, prm.slot_dim == 1 ? slot : h,
                             prm.slot_dim == 1 ? h : slot, page, smem_u32(&full[st]));
                 }
                 return true;
             };
-            int prev = 0, cur = page_of(0);
-            for (int i = 0; i <= n && ok; ++i) {
-                const int next = page_of(i + 1);
-                if (i < n) ok = load(&maps.k, i, tile0 + k_tile(i), cur);
-                if (i > 0 && ok) ok = load(&maps.v, i - 1, tile0 + v_tile(i - 1, n), prev);
-                prev = cur, cur = next;
+            if (TWO) {
+                for (int i = 0; i < n && ok; ++i) {
+                    const int page = page_of(i);
+                    ok = load(&maps.k, i, tile0 + k_tile<TWO>(i), page) && load(&maps.v, i, tile0 + v_tile<TWO>(i, n), page);
+                }
+            } else {
+                int prev = 0;
+                for (int i = 0; i <= n && ok; ++i) {
+                    const int cur = i < n ? page_of(i) : 0;
+                    if (i < n) ok = load(&maps.k, i, tile0 + k_tile<TWO>(i), cur);
+                    if (i > 0 && ok) ok = load(&maps.v, i - 1, tile0 + v_tile<TWO>(i - 1, n), prev);
+                    prev = cur;
+                }
             }
             if (!ok) break;
             tile0 += 2 * n;
         }
     } else if (warp == 2) {
-        // ---- queries: 16-byte pieces into swizzled rows, padding as zeros ----
-        constexpr int PIECES = D / 8;
-        const int piece = lane % PIECES, step = 32 / PIECES;
+        // ---- queries, as rows of the swizzled tile(s): a stream's 128 rows, or those that the streams share ----
         for (int n; (n = take()) != 0 && ok; give()) {
-            const uint32_t b = seg & 1;
-            if (seg >= 2 && !(ok = wait_bounded(&q_empty[b], (seg / 2 - 1) & 1))) break;
+            const uint32_t b = TWO ? 0 : seg & 1, use = TWO ? seg : seg / 2; // TWO: both buffers in one go
+            if (use && !(ok = wait_bounded(&q_empty[b], (use - 1) & 1))) break;
             const Seg &w = segs[seg % SEGS];
-            const int rows = w.rows, group = p.group;
-            int r = lane / PIECES, token = (w.row0 + r) / group, g = (w.row0 + r) % group;
-            const T *const src = (const T *)p.q + w.r0 * p.q_stride + (long long)w.h * group * D + piece * 8;
-            const uint32_t dst = smem_u32(q_sm) + b * C::TILE + (piece / 8) * (TM * 128);
-#pragma unroll 8
-            for (; r < TM; r += step) {
-                const bool on = r < rows;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + r * 128 + (((piece % 8) ^ (r & 7)) << 4)),
-                             "l"(on ? src + token * p.q_stride + g * D : src), "r"(on ? 16 : 0)
-                             : "memory");
-                for (g += step; g >= group; g -= group) ++token;
+            const int rows = w.rows, group = p.group, token0 = w.r0 + w.row0 / group;
+            if (prm.q_box) { // a box: q_box rows of the step x the group's heads x 64 values (rows behind the sequence's last are padding too)
+                const int box_rows = prm.q_box * group, parts = (rows + box_rows - 1) / box_rows, boxes = parts * C::ATOMS;
+                if (lane == 0) mbar_arrive_expect_tx(&q_full[b], boxes * box_rows * 128);
+                __syncwarp();
+                for (int i = lane; i < boxes; i += 32) {
+                    const int atom = i % C::ATOMS, part = i / C::ATOMS, r = part * box_rows;
+                    tma_box(smem_u32(q_sm) + (b + r / TM) * C::TILE + atom * (TM * 128) + r % TM * 128, &maps.q, atom * 64, 0, w.h, token0 + part * prm.q_box,
+                            smem_u32(&q_full[b]));
+                }
+            } else {
+                constexpr int PIECES = D / 8, STRIDE = 32 / PIECES;
+                const int piece = lane % PIECES, jump = STRIDE / group, left = STRIDE % group;
+                int r = lane / PIECES, g = (w.row0 + r) % group;
+                const T *src = (const T *)p.q + (w.r0 + (w.row0 + r) / group) * p.q_stride + ((long long)w.h * group + g) * D + piece * 8;
+                const long long step = jump * p.q_stride + left * D, wrap = p.q_stride - (long long)group * D;
+                const uint32_t dst = smem_u32(q_sm) + b * C::TILE + (piece / 8) * (TM * 128);
+#pragma unroll 4
+                for (; r < rows; r += STRIDE) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + r / TM * C::TILE + r % TM * 128 + (((piece % 8) ^ (r & 7)) << 4)), "l"(src) : "memory");
+                    src += step, g += left;
+                    if (g >= group) g -= group, src += wrap;
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                fence_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[b]);
             }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            fence_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&q_full[b]);
         }
     } else if (warp == 1) {
         // ---- MMA issue: the whole warp with uniform control flow, one elected lane issues ----
         uint32_t tile0 = 0, done[2] = {0, 0};
         const uint32_t q0 = smem_u32(q_sm), r0 = smem_u32(ring);
         for (uint32_t n; (n = (uint32_t)take()) != 0 && ok; give()) {
-            const uint64_t qd = desc_k_major(q0 + (seg & 1) * C::TILE);
-            if (!(ok = wait_bounded(&q_full[seg & 1], seg / 2 & 1))) break;
-            for (uint32_t i = 0; i <= n && ok; ++i) {
-                if (i < n) {
-                    const uint32_t tile = tile0 + k_tile(i), st = tile % NST;
-                    if (!(ok = wait_bounded(&full[st], tile / NST & 1))) break;
-                    fence_after();
-                    // (the score tile's last user, P V of the block before last, was issued earlier and runs before)
-                    const uint64_t kd = desc_k_major(r0 + st * C::TILE);
+            const uint64_t qd = desc_k_major(q0 + (TWO ? 0 : seg & 1) * C::TILE);
+            if (!(ok = TWO ? wait_bounded(&q_full[0], seg & 1) : wait_bounded(&q_full[seg & 1], seg / 2 & 1))) break;
+            // scores of block i for stream s; (the score tile's last user, P V of the stream's block before, was issued earlier and runs before)
+            auto scores = [&](uint32_t s, uint32_t st) {
+                const uint64_t kd = desc_k_major(r0 + st * C::TILE), q = qd + (TWO ? s : 0) * (C::TILE >> 4);
 #pragma unroll
-                    for (int a = 0; a < C::ATOMS; ++a) mma4_ss(tmem + (i & 1) * 128, qd + a * (TM * 128 >> 4), kd + a * (TK * 128 >> 4), idesc<T>(TK, false), a > 0);
-                    commit2(&empty[st], &s_full[i & 1]);
-                }
-                if (i > 0) {
-                    const uint32_t j = i - 1, s = j & 1, tile = tile0 + v_tile(j, n), st = tile % NST;
-                    if (!(ok = wait_bounded(&full[st], tile / NST & 1))) break;
-                    if (j == 0 && seg && !(ok = wait_bounded(&epi_done, (seg - 1) & 1))) break; // the accumulators have been read
-                    if (!(ok = wait_bounded(&p_full[s], done[s] & 1))) break;
-                    fence_after();
-                    const uint64_t vd = desc_mn_major(r0 + st * C::TILE);
-                    mma4_ts(tmem + C::O_COL + s * D, tmem + s * 128, vd, idesc<T>(D, true), j >= 2);
-                    mma4_ts(tmem + C::O_COL + s * D, tmem + s * 128 + 32, vd + 4 * 128, idesc<T>(D, true), 1);
-                    commit2(&empty[st], &o_done[s]);
-                    ++done[s];
+                for (int a = 0; a < C::ATOMS; ++a) mma4_ss(tmem + s * 128, q + a * (TM * 128 >> 4), kd + a * (TK * 128 >> 4), idesc<T>(TK, false), a > 0);
+            };
+            auto values = [&](uint32_t s, uint32_t st, bool add) {
+                const uint64_t vd = desc_mn_major(r0 + st * C::TILE);
+                mma4_ts(tmem + C::O_COL + s * D, tmem + s * 128, vd, idesc<T>(D, true), add);
+                mma4_ts(tmem + C::O_COL + s * D, tmem + s * 128 + 32, vd + 4 * 128, idesc<T>(D, true), 1);
+            };
+            for (uint32_t i = 0; i <= n && ok; ++i) {
+                const uint32_t kt = tile0 + k_tile<TWO>(i), ks = kt % NST, vt = tile0 + v_tile<TWO>(i - 1, n), vs = vt % NST; // (values of the block before)
+                if (i == 1 && seg && !(ok = wait_bounded(&epi_done, (seg - 1) & 1))) break; // the accumulators have been read
+                if (TWO) {
+                    if (i > 0 && !(ok = wait_bounded(&full[vs], vt / NST & 1))) break;
+#pragma unroll
+                    for (uint32_t s = 0; s < 2; ++s) {
+                        if (i > 0) {
+                            if (!(ok = wait_bounded(&p_full[s], done[s]++ & 1))) break;
+                            fence_after();
+                            values(s, vs, i > 1);
+                            if (s == 1) commit2(&empty[vs], &o_done[s]);
+                            else commit1(&o_done[s]);
+                        }
+                        if (i < n) {
+                            if (s == 0 && !(ok = wait_bounded(&full[ks], kt / NST & 1))) break;
+                            fence_after();
+                            scores(s, ks);
+                            if (s == 1) commit2(&empty[ks], &s_full[s]);
+                            else commit1(&s_full[s]);
+                        }
+                    }
+                } else {
+                    if (i < n) {
+                        if (!(ok = wait_bounded(&full[ks], kt / NST & 1))) break;
+                        fence_after();
+                        scores(i & 1, ks);
+                        commit2(&empty[ks], &s_full[i & 1]);
+                    }
+                    if (i > 0) {
+                        const uint32_t s = (i - 1) & 1;
+                        if (!(ok = wait_bounded(&full[vs], vt / NST & 1) && wait_bounded(&p_full[s], done[s] & 1))) break;
+                        fence_after();
+                        values(s, vs, i > 2);
+                        commit2(&empty[vs], &o_done[s]);
+                        ++done[s];
+                    }
                 }
             }
             if (!ok) break;
@@ -389,11 +449,11 @@ template <typename T, int D> __global__ void __launch_bounds__(TT, 1) tree_attn_
             Seg &w = segs[seg % SEGS];
             SeqView v;
             v.r0 = w.r0, v.n = w.n, v.id = w.id, v.ctx = w.ctx, v.kv = w.kv;
-            const int rows = w.rows, key_end = w.key_end, blk = w.blk;
+            const int row0 = w.row0 + (TWO ? (int)s * TM : 0), rows = w.rows - (TWO ? (int)s * TM : 0), key_end = w.key_end, blk = w.blk; // this stream's
             const bool idle = (int)(quarter * 32) >= rows; // rows of padding: what they hold reaches no other row
-            const int me = (w.row0 + min((int)row, rows - 1)) / p.group; // this row's index in the sequence
+            const int me = min((row0 + max(min((int)row, rows - 1), 0)) / p.group, v.n - 1); // this row's index in the sequence
             float m = -INFINITY, l = 0.f; // reference (a power of two), sum of weights
-            for (uint32_t j = s; j < n && ok; j += 2) {
+            for (uint32_t j = TWO ? 0 : s; j < n && ok; j += STEP) {
                 const int key0 = (blk + j) * TK;
                 const bool tail = key0 + TK > v.ctx;
                 uint32_t bits[4];
@@ -401,7 +461,7 @@ template <typename T, int D> __global__ void __launch_bounds__(TT, 1) tree_attn_
 #pragma unroll
                     for (int c = 0; c < 4; ++c) bits[c] = view_bits(p, v, me, key0 + 32 * c);
                     // clean the values of this block: thread = key
-                    const uint32_t tile = tile0 + v_tile(j, n), st = tile % NST, kr = tid & 127;
+                    const uint32_t tile = tile0 + v_tile<TWO>(j, n), st = tile % NST, kr = tid & 127;
                     if (!(ok = wait_bounded(&full[st], tile / NST & 1))) break;
                     const int token = key0 + (int)kr;
                     if (token >= v.ctx) {
@@ -462,7 +522,7 @@ template <typename T, int D> __global__ void __launch_bounds__(TT, 1) tree_attn_
                     if (__any_sync(0xffffffffu, block_max > m + 8.f)) {
                         const float to = block_max > m + 8.f ? block_max : m;
                         const float corr = m == to ? 1.f : ex2(m - to);
-                        if (j >= 2) {
+                        if (j >= STEP) {
                             if (!(ok = wait_bounded(&o_done[s], (done[s] - 1) & 1))) break; // P V of the stream's block before
                             fence_after();
 #pragma unroll 1
@@ -509,38 +569,47 @@ template <typename T, int D> __global__ void __launch_bounds__(TT, 1) tree_attn_
             }
             if (!ok) break;
             // ---- join the streams' parts, store ----
-            done[1 - s] += s == 0 ? n / 2 : (n + 1) / 2;
-            // all products of this segment that this stream waits for here were issued after the last use of the queries,
-            // whose memory carries the references and sums from one stream to the other
-            ok = wait_bounded(&o_done[0], (done[0] - 1) & 1) && (n < 2 || wait_bounded(&o_done[1], (done[1] - 1) & 1));
-            if (!ok) break;
-            float2 *const ml = (float2 *)(q_sm + (seg & 1) * C::TILE);
-            ml[s * TM + row] = make_float2(m, l);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&x_full);
-            if (!(ok = wait_bounded(&x_full, seg & 1))) break;
-            fence_after();
-            const float2 a = ml[row], b = n < 2 ? make_float2(-INFINITY, 0.f) : ml[TM + row];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&q_empty[seg & 1]);
+            float2 a = make_float2(m, l), b = make_float2(-INFINITY, 0.f);
+            if (TWO) {
+                if (!(ok = wait_bounded(&o_done[s], (done[s] - 1) & 1))) break;
+                fence_after();
+            } else {
+                done[1 - s] += s == 0 ? n / 2 : (n + 1) / 2;
+                // all products of this segment that this stream waits for here were issued after the last use of the queries,
+                // whose memory carries the references and sums from one stream to the other
+                ok = wait_bounded(&o_done[0], (done[0] - 1) & 1) && (n < 2 || wait_bounded(&o_done[1], (done[1] - 1) & 1));
+                if (!ok) break;
+                float2 *const ml = (float2 *)(q_sm + (seg & 1) * C::TILE);
+                ml[s * TM + row] = a;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&x_full);
+                if (!(ok = wait_bounded(&x_full, seg & 1))) break;
+                fence_after();
+                a = ml[row];
+                if (n >= 2) b = ml[TM + row];
+                __syncwarp();
+            }
+            if (lane == 0) mbar_arrive(&q_empty[TWO ? 0 : seg & 1]);
             if (!idle) {
                 const float mm = fmaxf(a.x, b.x);
-                const float wa = a.x == -INFINITY ? 0.f : ex2(a.x - mm), wb = b.x == -INFINITY ? 0.f : ex2(b.x - mm);
+                const float wa = TWO ? 1.f : a.x == -INFINITY ? 0.f : ex2(a.x - mm), wb = b.x == -INFINITY ? 0.f : ex2(b.x - mm);
                 const float ll = a.y * wa + b.y * wb;
                 const bool whole = w.flags & 1, live = (int)row < rows, odd = w.odd;
                 const int head = w.h;
-                float *const mine = part_of<TM>(p, blockIdx.x, w.flags >> 1);
+                const int part_row = (TWO ? (int)s * TM : 0) + (int)row;
+                float *const mine = part_of<ROWS>(p, blockIdx.x, w.flags >> 1);
                 const float inv = ll == 0.f ? 0.f : 1.0f / ll;
-                T *const out = (T *)p.out + (v.r0 + me) * p.out_stride + (head * p.group + (w.row0 + row) % p.group) * (long long)D;
+                T *const out = (T *)p.out + (v.r0 + me) * p.out_stride + (head * p.group + (row0 + row) % p.group) * (long long)D;
+                // the streams share a tile's columns, or each stores its own rows
 #pragma unroll 1
-                for (int c = (int)s * (D / 2); c < (int)(s + 1) * (D / 2); c += 32) {
+                for (int c = TWO ? 0 : (int)s * (D / 2); c < (TWO ? D : (int)(s + 1) * (D / 2)); c += 32) {
                     uint32_t o0[32], o1[32];
-                    tmem_ld32(t_lane + C::O_COL + c, o0);
-                    tmem_ld32(t_lane + C::O_COL + D + c, o1);
+                    tmem_ld32(TWO ? t_o + c : t_lane + C::O_COL + c, o0);
+                    if (!TWO) tmem_ld32(t_lane + C::O_COL + D + c, o1);
                     wait_ld();
                     float o[32];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(o0[e]) * wa + (n < 2 ? 0.f : __uint_as_float(o1[e]) * wb);
+                    for (int e = 0; e < 32; ++e) o[e] = TWO ? __uint_as_float(o0[e]) : __uint_as_float(o0[e]) * wa + (n < 2 ? 0.f : __uint_as_float(o1[e]) * wb);
                     if (odd && live) add_odd<T>(p, v, head, me, max(v.ctx, blk * TK), min(key_end, (int)(blk + n) * TK), c, o);
                     if (!live) continue;
                     if (whole) {
@@ -553,10 +622,10 @@ template <typename T, int D> __global__ void __launch_bounds__(TT, 1) tree_attn_
                         }
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) *(float4 *)(mine + (size_t)row * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        for (int e = 0; e < 32; e += 4) *(float4 *)(mine + (size_t)part_row * D + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                     }
                 }
-                if (!whole && s == 0 && live) *(float2 *)(mine + (size_t)TM * D + 2 * row) = make_float2(mm, ll);
+                if (!whole && (TWO || s == 0) && live) *(float2 *)(mine + (size_t)ROWS * D + 2 * part_row) = make_float2(mm, ll);
             }
             fence_before();
             __syncwarp();
@@ -598,11 +667,28 @@ bool encode_pool(const PoolDev &pool, int dtype, const uint8_t *base, int box, i
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int D> cudaError_t launch(const DeviceInfo &dev, const TcParams &prm, const TcMaps &maps, bool pdl, cudaStream_t st) {
-    cudaError_t e = cudaFuncSetAttribute(tree_attn_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
+// [values, head of the group, group, row of the step]; boxes of q_box rows x all heads of a group x 64 values.  Such a box is a run of
+// query rows in the tile's order when a tile holds whole rows of the step, and starts on a swizzle group.
+bool encode_queries(const TreeDev &t, int dtype, int q_box, CUtensorMap *map) {
+    const EncodeTiled enc = encoder();
+    if (!enc) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)t.dim, (cuuint64_t)t.group, (cuuint64_t)t.n_kv, (cuuint64_t)t.n_rows};
+    const cuuint64_t strides[3] = {(cuuint64_t)t.dim * 2, (cuuint64_t)t.group * t.dim * 2, (cuuint64_t)t.q_stride * 2};
+    const cuuint32_t boxes[4] = {64, (cuuint32_t)t.group, 1, (cuuint32_t)q_box}, one[4] = {1, 1, 1, 1};
+    return t.q_stride < (1ll << 38) &&
+           enc(map, dtype == ULLM_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<uint8_t *>(t.q), dims, strides, boxes, one,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D, bool TWO> cudaError_t launch(const DeviceInfo &dev, const TcParams &prm, const TcMaps &maps, bool pdl, cudaStream_t st) {
+    cudaError_t e = cudaFuncSetAttribute(tree_attn_tc_kernel<T, D, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
     if (e != cudaSuccess) return e;
-    if ((e = launch_kernel(tree_attn_tc_kernel<T, D>, dim3(dev.sm_count), dim3(TT), Cfg<D>::SMEM, st, pdl, prm, maps)) != cudaSuccess) return e;
-    return launch_kernel(tree_join_kernel<T, TM>, dim3(dev.sm_count * 2), dim3(32 * JOIN_WARPS), 0, st, pdl, prm.t, dev.sm_count);
+    if ((e = launch_kernel(tree_attn_tc_kernel<T, D, TWO>, dim3(dev.sm_count), dim3(TT), Cfg<D>::SMEM, st, pdl, prm, maps)) != cudaSuccess) return e;
+    return launch_kernel(tree_join_kernel<T, TWO ? 2 * TM : TM>, dim3(dev.sm_count * 2), dim3(32 * JOIN_WARPS), 0, st, pdl, prm.t, dev.sm_count);
+}
+template <typename T> cudaError_t launch_any(const DeviceInfo &dev, int dim, bool two, const TcParams &prm, const TcMaps &maps, bool pdl, cudaStream_t st) {
+    if (dim == 64) return two ? launch<T, 64, true>(dev, prm, maps, pdl, st) : launch<T, 64, false>(dev, prm, maps, pdl, st);
+    return two ? launch<T, 128, true>(dev, prm, maps, pdl, st) : launch<T, 128, false>(dev, prm, maps, pdl, st);
 }
 
 } // namespace
@@ -612,7 +698,7 @@ bool tree_attn_tc_supported(const PoolDev &pool, int dtype) {
     const int ps = pool.page_size; // a box of keys starts on a swizzle group of eight rows and lies in one page
     return ps % 128 == 0 || ps == 8 || ps == 16 || ps == 32 || ps == 64;
 }
-size_t tree_attn_tc_work(int sm_count, int dim) { return sizeof(float) * (size_t)sm_count * 2 * TM * (dim + 2); }
+size_t tree_attn_tc_work(int sm_count, int dim) { return sizeof(float) * (size_t)sm_count * 2 * (2 * TM) * (dim + 2); }
 
 cudaError_t launch_tree_attn_tc(const DeviceInfo &dev, const PoolDev &pool, int dtype, const TreeDev &t, int *d_status, bool pdl, cudaStream_t st) {
     TcParams prm;
@@ -620,8 +706,21 @@ cudaError_t launch_tree_attn_tc(const DeviceInfo &dev, const PoolDev &pool, int 
     prm.t = t, prm.status = d_status, prm.box = pool.page_size < TK ? pool.page_size : TK, prm.slot_dim = 1;
     if (!encode_pool(pool, dtype, t.k, prm.box, &prm.slot_dim, &maps.k) || !encode_pool(pool, dtype, t.v, prm.box, &prm.slot_dim, &maps.v))
         return cudaErrorNotSupported;
-    if (dtype == ULLM_DTYPE_F16) return pool.head_dim == 64 ? launch<__half, 64>(dev, prm, maps, pdl, st) : launch<__half, 128>(dev, prm, maps, pdl, st);
-    return pool.head_dim == 64 ? launch<__nv_bfloat16, 64>(dev, prm, maps, pdl, st) : launch<__nv_bfloat16, 128>(dev, prm, maps, pdl, st);
+    // Rows per sequence and key head on average (the lengths themselves are on the device; either way is right for any of them).
+    const long long rows = ((long long)t.n_rows * t.group + t.n_seq - 1) / t.n_seq;
+    const bool two = rows > TM;
+    prm.lanes = 1;
+    while (two && prm.lanes < 4 && prm.lanes * 4 * TM < rows + TM && dev.sm_count / (prm.lanes * 2) > 0) prm.lanes *= 2;
+    // query boxes of about a sequence's rows
+    prm.q_box = 0;
+    if (TM % t.group == 0) {
+        int box = 1;
+        while (box < t.n_rows / t.n_seq && box * t.group < TM) box *= 2;
+        while (box * t.group % 8) box *= 2;
+        if (encode_queries(t, dtype, box, &maps.q)) prm.q_box = box;
+    }
+    if (!prm.q_box) maps.q = maps.k; // (never used)
+    return dtype == ULLM_DTYPE_F16 ? launch_any<__half>(dev, pool.head_dim, two, prm, maps, pdl, st) : launch_any<__nv_bfloat16>(dev, pool.head_dim, two, prm, maps, pdl, st);
 }
 
 } // namespace ullm

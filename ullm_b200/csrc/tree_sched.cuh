@@ -7,7 +7,9 @@
 // thousand short ones.  A unit that is cut leaves unnormalised partial results (running maximum, sum and
 // weighted values of each row) in the work area; a CTA has at most two of them, its first and its last, and the CTA in
 // which a cut unit ends records what the joining kernel needs.  Lengths are read on the device, so a captured call serves
-// every later state of the tables.  One warp of a CTA works the division out (Sched) and hands the segments to the others:
+// every later state of the tables.  Where sequences have many rows, `lanes` CTAs form a team that shares one line: its
+// members take neighbouring tiles of a unit over the same keys at about the same time, so that the keys come from DRAM once and
+// from the L2 afterwards (each tile at a time of its own: 437 MB of keys and values were read four times).  One warp of a CTA works the division out (Sched) and hands the segments to the others:
 // done by every thread, with 64-bit divisions, it took 6,000 of the 13,800 cycles of a one-token call.
 #pragma once
 
@@ -66,15 +68,19 @@ template <int M, int KB, int COST, int MINS> struct Sched {
     static constexpr unsigned ALL = 0xffffffffu;
     const TreeDev &p;
     const int lane;
+    const int lanes, member, team; // CTAs of a team, this one's place in it, the team
     unsigned total, active, each, more, lo, hi, cur; // share c begins at c * each + min(c, more)
     int b, h, t, nt;
     unsigned off; // place of `cur` in its unit
     SeqView win;  // view of sequence wb + lane
     int wb;
     SeqView v;
-    bool first;
 
-    __device__ __forceinline__ explicit Sched(const TreeDev &p_) : p(p_), lane((int)(threadIdx.x & 31)) {}
+    __device__ __forceinline__ explicit Sched(const TreeDev &p_, int lanes_ = 1)
+        : p(p_), lane((int)(threadIdx.x & 31)), lanes(lanes_), member((int)blockIdx.x % lanes_), team((int)blockIdx.x / lanes_) {}
+    // tiles that a team takes together, and their places: those of the one that sees most
+    __device__ __forceinline__ int groups(const SeqView &u) const { return (T::count(p, u) + lanes - 1) / lanes; }
+    __device__ __forceinline__ int group_blocks(const SeqView &u, int g) const { return T::blocks(p, u, min((g + 1) * lanes, T::count(p, u)) - 1); }
 
     __device__ __forceinline__ unsigned share_at(unsigned c) const { return c * each + min(c, more); }
     __device__ __forceinline__ unsigned share_of(unsigned x) const { // the share that holds place x
@@ -83,20 +89,20 @@ template <int M, int KB, int COST, int MINS> struct Sched {
     }
     // places of one key head of the sequence that lane `who` views (`mine`: this lane's); every lane calls it
     __device__ __forceinline__ unsigned head_places(const SeqView &mine) const {
-        const int T_ = T::count(p, mine);
+        const int T_ = groups(mine);
         const bool simple = p.mask || T_ <= 8;
         unsigned s = 0;
         if (p.mask) {
             s = T_ ? (unsigned)T_ * (T::blocks(p, mine, 0) + COST) : 0u;
         } else if (simple) {
-            for (int i = 0; i < T_; ++i) s += T::blocks(p, mine, i) + COST;
+            for (int i = 0; i < T_; ++i) s += group_blocks(mine, i) + COST;
         }
         for (unsigned long_ones = __ballot_sync(ALL, !simple); long_ones; long_ones &= long_ones - 1) { // prompts: all lanes together
             const int who = __ffs(long_ones) - 1;
             const SeqView u = view_of(mine, who);
-            const int n = T::count(p, u);
+            const int n = groups(u);
             unsigned x = 0;
-            for (int i = lane; i < n; i += 32) x += T::blocks(p, u, i) + COST;
+            for (int i = lane; i < n; i += 32) x += group_blocks(u, i) + COST;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(ALL, x, o);
             if (lane == who) s = x;
@@ -127,10 +133,10 @@ template <int M, int KB, int COST, int MINS> struct Sched {
             for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(ALL, x, o);
             total += x;
         }
-        active = max(1u, min(gridDim.x, (total + MINS - 1) / MINS));
+        active = max(1u, min(gridDim.x / lanes, (total + MINS - 1) / MINS));
         each = total / active, more = total - each * active;
-        if (blockIdx.x >= active || total == 0) return false;
-        lo = share_at(blockIdx.x), hi = share_at(blockIdx.x + 1), cur = lo, first = true;
+        if ((unsigned)team >= active || total == 0) return false;
+        lo = share_at(team), hi = share_at(team + 1), cur = lo;
         unsigned run = 0; // places in front of the window
         for (int b0 = 0; b0 < p.n_seq; b0 += 32) {
             if (p.n_seq > 32) win = lane_view(b0), wb = b0, places = head_places(win) * (unsigned)p.n_kv;
@@ -149,7 +155,7 @@ template <int M, int KB, int COST, int MINS> struct Sched {
             }
             run += __shfl_sync(ALL, incl, 31);
         }
-        v = view_of(win, b - wb), nt = T::count(p, v);
+        v = view_of(win, b - wb), nt = groups(v);
         const unsigned per = __shfl_sync(ALL, places / (unsigned)p.n_kv, b - wb);
         h = (int)(off / per), off -= h * per, t = 0;
         if (p.mask) {
@@ -157,7 +163,7 @@ template <int M, int KB, int COST, int MINS> struct Sched {
             t = (int)(off / u), off -= t * u;
         } else {
             for (int t0 = 0;; t0 += 32) { // the tile, 32 at a time
-                const unsigned mine = t0 + lane < nt ? T::blocks(p, v, t0 + lane) + COST : 0u;
+                const unsigned mine = t0 + lane < nt ? group_blocks(v, t0 + lane) + COST : 0u;
                 unsigned incl = mine;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -179,23 +185,22 @@ template <int M, int KB, int COST, int MINS> struct Sched {
         Seg s;
         s.count = 0, s.odd = 0;
         while (cur < hi) {
-            const int nb = T::blocks(p, v, t);
+            const int nb = group_blocks(v, t), tile = t * lanes + member;
             const unsigned len = nb + COST, take = min(len - off, hi - cur);
-            const int b0 = max((int)off - COST, 0), b1 = (int)(off + take) - COST;
+            // this member's tile: it may be missing, or see fewer keys than the group's last
+            const int mine = tile * M < v.n * p.group ? T::blocks(p, v, tile) : 0;
+            const int b0 = max((int)off - COST, 0), b1 = min((int)(off + take) - COST, mine);
             if (b1 > b0) {
-                s.r0 = v.r0, s.n = v.n, s.id = v.id, s.ctx = v.ctx, s.kv = v.kv, s.key_end = T::key_end(p, v, t);
-                s.h = h, s.row0 = t * M, s.rows = min(M, v.n * p.group - t * M);
+                s.r0 = v.r0, s.n = v.n, s.id = v.id, s.ctx = v.ctx, s.kv = v.kv, s.key_end = T::key_end(p, v, tile);
+                s.h = h, s.row0 = tile * M, s.rows = min(M, v.n * p.group - tile * M);
                 s.blk = b0, s.count = b1 - b0;
-                const bool whole = b0 == 0 && b1 == nb;
-                s.flags = (whole ? 1 : 0) | (first ? 0 : 2);
-                if (!whole && b1 == nb && lane == 0) {
-                    // the unit begins in the CTA that holds its first block; it is that CTA's first segment unless
-                    // the CTA's share begins before the unit
-                    const unsigned unit = cur - off, c0 = share_of(unit + COST);
-                    meta[0] = make_int4((int)c0, share_at(c0) >= unit ? 0 : 1, v.r0, v.n);
-                    meta[1] = make_int4(t, h, 0, 0);
+                const bool whole = b0 == 0 && b1 == mine;
+                s.flags = (whole ? 1 : 0) | (cur == lo ? 0 : 2); // slot 0: the unit with which the share begins
+                if (!whole && b1 == mine && lane == 0) {
+                    const unsigned unit = cur - off, c0 = share_of(unit + COST); // the team that holds its first block
+                    meta[0] = make_int4((int)c0 * lanes + member, (share_at(c0) >= unit ? 0 : 1) | lanes << 1, v.r0, v.n);
+                    meta[1] = make_int4(tile, h, 0, 0);
                 }
-                first = false;
             }
             cur += take, off = 0;
             if (cur < hi && ++t == nt) {
@@ -204,7 +209,7 @@ template <int M, int KB, int COST, int MINS> struct Sched {
                     h = 0;
                     do {
                         if (++b - wb == 32) win = lane_view(b), wb = b;
-                        v = view_of(win, b - wb), nt = T::count(p, v);
+                        v = view_of(win, b - wb), nt = groups(v);
                     } while (nt == 0);
                 }
             }
@@ -228,35 +233,45 @@ template <> __device__ __forceinline__ __nv_bfloat16 out_from<__nv_bfloat16>(flo
 //   out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c.
 // A fixed number of CTAs share the rows of all cut units: every CTA reads the records, SPLIT warps take a row together (each
 // a part of the parts, eight loads in flight), because a long context of one sequence is cut into as many parts as there are CTAs.
-constexpr int JOIN_WARPS = 8;
+constexpr int JOIN_WARPS = 8, JOIN_MAX = 1024; // CTAs of the attention kernel at most
 template <typename O, int M> __global__ void __launch_bounds__(32 * JOIN_WARPS) tree_join_kernel(const TreeDev p, int ctas) {
-    __shared__ int2 duty[1024]; // {CTA, rows in front}
-    __shared__ int n_duty, n_rows, most;
+    struct Duty {
+        int c, front, c0, slot, lanes, r0, t, h; // the CTA in which it ends, rows of the units in front of it, ...
+    };
+    __shared__ Duty duty[JOIN_MAX];
+    __shared__ int s_found[JOIN_WARPS], s_rows[JOIN_WARPS], s_most[JOIN_WARPS];
     __shared__ float red[JOIN_WARPS][256], red_l[JOIN_WARPS];
     pdl_wait_prior();
     pdl_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (warp == 0) {
-        int found = 0, rows = 0, parts = 0;
-        for (int c0 = 0; c0 < ctas; c0 += 32) {
-            const int c = c0 + lane;
-            int4 a = make_int4(-1, 0, 0, 0);
-            int r = 0;
-            if (c < ctas) a = p.meta[c * TREE_META];
-            if (a.x >= 0) r = min(M, a.w * p.group - p.meta[c * TREE_META + 1].x * M), parts = max(parts, c - a.x + 1);
-            const unsigned has = __ballot_sync(0xffffffffu, a.x >= 0);
-            int incl = r;
+    int n_duty = 0, n_rows = 0, most = 0;
+    for (int c0 = 0; c0 < ctas; c0 += 32 * JOIN_WARPS) {
+        const int c = c0 + tid;
+        int4 a = make_int4(-1, 0, 0, 0), b = a;
+        if (c < ctas) a = p.meta[c * TREE_META], b = p.meta[c * TREE_META + 1];
+        const bool has = a.x >= 0;
+        const int r = has ? min(M, a.w * p.group - b.x * M) : 0;
+        int incl = r, parts = has ? (c - a.x) / (a.y >> 1) + 1 : 0;
+        const unsigned who = __ballot_sync(0xffffffffu, has);
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += y;
-            }
-            if (a.x >= 0) duty[found + __popc(has & ((1u << lane) - 1u))] = make_int2(c, rows + incl - r);
-            found += __popc(has), rows += __shfl_sync(0xffffffffu, incl, 31);
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+            parts = max(parts, __shfl_xor_sync(0xffffffffu, parts, o));
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) parts = max(parts, __shfl_xor_sync(0xffffffffu, parts, o));
-        if (lane == 0) n_duty = found, n_rows = rows, most = parts;
+        __syncthreads();
+        if (lane == 31) s_found[warp] = __popc(who), s_rows[warp] = incl, s_most[warp] = parts;
+        __syncthreads();
+        int at = n_duty + __popc(who & ((1u << lane) - 1u)), front = n_rows + incl - r;
+        for (int k = 0; k < JOIN_WARPS; ++k) {
+            if (k < warp) at += s_found[k], front += s_rows[k];
+            n_duty += s_found[k], n_rows += s_rows[k], most = max(most, s_most[k]);
+        }
+        if (has) {
+            Duty d;
+            d.c = c, d.front = front, d.c0 = a.x, d.slot = a.y & 1, d.lanes = a.y >> 1, d.r0 = a.z, d.t = b.x, d.h = b.y;
+            duty[at] = d;
+        }
     }
     __syncthreads();
     const int split = most > 8 ? 4 : 1, per = JOIN_WARPS / split, sub = warp % split;
@@ -265,20 +280,19 @@ template <typename O, int M> __global__ void __launch_bounds__(32 * JOIN_WARPS) 
         float m = -INFINITY, l = 0.f, acc[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-        int4 a, b;
+        Duty u;
         int r = 0;
         if (i < n_rows) {
             int lo = 0, hi = n_duty; // the unit of row i
             while (hi - lo > 1) {
                 const int mid = (lo + hi) / 2;
-                if (duty[mid].y <= i) lo = mid;
+                if (duty[mid].front <= i) lo = mid;
                 else hi = mid;
             }
-            const int c = duty[lo].x;
-            r = i - duty[lo].y;
-            a = p.meta[c * TREE_META], b = p.meta[c * TREE_META + 1];
-            const int parts = c - a.x + 1;
-            auto part = [&](int k) { return part_of<M>(p, a.x + k, k == 0 ? a.y : 0); };
+            u = duty[lo];
+            r = i - u.front;
+            const int parts = (u.c - u.c0) / u.lanes + 1;
+            auto part = [&](int k) { return part_of<M>(p, u.c0 + k * u.lanes, k == 0 ? u.slot : 0); };
             for (int k = lane; k < parts; k += 32) m = fmaxf(m, part(k)[(size_t)M * p.dim + 2 * r]);
             m = warp_max(m);
             // this warp's parts: sub, sub + split, ...; 32 weights at a time, one per lane
@@ -290,23 +304,23 @@ template <typename O, int M> __global__ void __launch_bounds__(32 * JOIN_WARPS) 
                     l += ml.y * w;
                 }
                 const int n = min(32, (parts - k0 + split - 1) / split);
-                for (int u0 = 0; u0 < n; u0 += 8) {
+                for (int j0 = 0; j0 < n; j0 += 8) {
                     if (p.dim <= 128) { // four values per lane
                         float4 x[8];
                         const bool on = lane * 4 < p.dim;
 #pragma unroll
-                        for (int u = 0; u < 8; ++u)
-                            if (u0 + u < n && on) x[u] = *(const float4 *)(part(k0 + (u0 + u) * split) + (size_t)r * p.dim + lane * 4);
+                        for (int j = 0; j < 8; ++j)
+                            if (j0 + j < n && on) x[j] = *(const float4 *)(part(k0 + (j0 + j) * split) + (size_t)r * p.dim + lane * 4);
 #pragma unroll
-                        for (int u = 0; u < 8; ++u) {
-                            const float wk = __shfl_sync(0xffffffffu, w, (u0 + u) & 31);
-                            if (u0 + u < n && on && wk != 0.f) acc[0] += wk * x[u].x, acc[1] += wk * x[u].y, acc[2] += wk * x[u].z, acc[3] += wk * x[u].w;
+                        for (int j = 0; j < 8; ++j) {
+                            const float wk = __shfl_sync(0xffffffffu, w, (j0 + j) & 31);
+                            if (j0 + j < n && on && wk != 0.f) acc[0] += wk * x[j].x, acc[1] += wk * x[j].y, acc[2] += wk * x[j].z, acc[3] += wk * x[j].w;
                         }
                     } else {
-                        for (int u = 0; u < 8 && u0 + u < n; ++u) {
-                            const float wk = __shfl_sync(0xffffffffu, w, u0 + u);
+                        for (int j = 0; j < 8 && j0 + j < n; ++j) {
+                            const float wk = __shfl_sync(0xffffffffu, w, j0 + j);
                             if (wk == 0.f) continue;
-                            const float *o = part(k0 + (u0 + u) * split) + (size_t)r * p.dim;
+                            const float *o = part(k0 + (j0 + j) * split) + (size_t)r * p.dim;
 #pragma unroll
                             for (int e = 0; e < 8; ++e)
                                 if (lane * 8 + e < p.dim) acc[e] += wk * o[lane * 8 + e];
@@ -333,8 +347,8 @@ template <typename O, int M> __global__ void __launch_bounds__(32 * JOIN_WARPS) 
                     if (e < wide && lane * wide < p.dim) acc[e] += red[warp + s][lane * wide + e];
             }
         const float inv = l == 0.f ? 0.f : 1.0f / l;
-        const int row = b.x * M + r;
-        O *out = (O *)p.out + (a.z + row / p.group) * p.out_stride + ((long long)b.y * p.group + row % p.group) * p.dim;
+        const int row = u.t * M + r;
+        O *out = (O *)p.out + (u.r0 + row / p.group) * p.out_stride + ((long long)u.h * p.group + row % p.group) * p.dim;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
             if (e < wide && lane * wide < p.dim) out[lane * wide + e] = out_from<O>(l == 0.f ? 0.f : acc[e] * inv);

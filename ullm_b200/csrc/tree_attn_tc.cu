@@ -124,7 +124,11 @@ __device__ __forceinline__ void commit1(uint64_t *x) {
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Waits for a load of 32 values; their uses stay behind it.
+__device__ __forceinline__ void wait_ld32(uint32_t *v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
+}
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t *v) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -237,7 +241,7 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
     constexpr int NST = C::STAGES, ROWS = TWO ? 2 * TM : TM, STEP = TWO ? 1 : 2; // STEP: a stream takes every so many blocks
     extern __shared__ __align__(1024) uint8_t gsm[];
     uint8_t *const q_sm = (uint8_t *)(((uintptr_t)gsm + 1023) & ~(uintptr_t)1023), *const ring = q_sm + 2 * C::TILE;
-    __shared__ uint64_t full[NST], empty[NST], s_full[2], p_full[2], o_done[2], q_full[2], q_empty[2], seg_full[SEGS], seg_empty[SEGS], x_full, epi_done;
+    __shared__ uint64_t full[NST], empty[NST], s_full[2], p_full[2], o_done[2], h_full[2], q_full[2], q_empty[2], seg_full[SEGS], seg_empty[SEGS], x_full, epi_done;
     __shared__ Seg segs[SEGS];
     __shared__ uint32_t tmem_s;
     const TreeDev &p = prm.t;
@@ -246,7 +250,7 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
     if (tid == 0) {
         for (int i = 0; i < NST; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
         for (int s = 0; s < 2; ++s) {
-            mbar_init(&s_full[s], 1), mbar_init(&p_full[s], 4), mbar_init(&o_done[s], 1);
+            mbar_init(&s_full[s], 1), mbar_init(&h_full[s], 4), mbar_init(&p_full[s], 4), mbar_init(&o_done[s], 1);
             mbar_init(&q_full[s], 1), mbar_init(&q_empty[s], 8);
         }
         for (int i = 0; i < SEGS; ++i) mbar_init(&seg_full[i], 1), mbar_init(&seg_empty[i], 11);
@@ -256,6 +260,16 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
     if (warp == 2) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    Sched<ROWS, TK, T_COST, T_MIN> sched(p, prm.lanes);
+    Seg first;
+    first.count = 0;
+    if (warp == 3) { // (while the others set up)
+        pdl_wait_prior();
+        if (lane == 0) p.meta[blockIdx.x * TREE_META] = make_int4(-1, 0, 0, 0);
+        __syncwarp();
+        if (sched.init()) first = sched.next(p.meta + blockIdx.x * TREE_META);
+        if (lane == 0) segs[0] = first;
     }
     fence_before();
     __syncthreads();
@@ -277,21 +291,15 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
     };
 
     if (warp == 3) {
-        // ---- division of the work ----
-        if (lane == 0) p.meta[blockIdx.x * TREE_META] = make_int4(-1, 0, 0, 0);
-        __syncwarp();
-        Sched<ROWS, TK, T_COST, T_MIN> sched(p, prm.lanes);
-        const bool some = sched.init();
-        for (;; ++seg) {
-            Seg next;
-            next.count = 0;
-            if (some) next = sched.next(p.meta + blockIdx.x * TREE_META);
+        // ---- division of the work: the first segment lies in the ring already ----
+        if (lane == 0) mbar_arrive(&seg_full[0]);
+        for (seg = 1; first.count; ++seg) {
+            first = sched.next(p.meta + blockIdx.x * TREE_META);
             if (seg >= SEGS && !(ok = wait_bounded(&seg_empty[seg % SEGS], (seg / SEGS - 1) & 1))) break;
             if (lane == 0) {
-                segs[seg % SEGS] = next;
+                segs[seg % SEGS] = first;
                 mbar_arrive(&seg_full[seg % SEGS]);
             }
-            if (!next.count) break;
         }
     } else if (warp == 0) {
         // ---- TMA: lane -> (64 values, box of keys) ----
@@ -392,10 +400,16 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
 #pragma unroll
                 for (int a = 0; a < C::ATOMS; ++a) mma4_ss(tmem + s * 128, q + a * (TM * 128 >> 4), kd + a * (TK * 128 >> 4), idesc<T>(TK, false), a > 0);
             };
-            auto values = [&](uint32_t s, uint32_t st, bool add) {
+            auto values = [&](uint32_t s, uint32_t st, bool add) { // P V as the halves of P arrive
                 const uint64_t vd = desc_mn_major(r0 + st * C::TILE);
+                if (!wait_bounded(&h_full[s], done[s] & 1)) return false;
+                fence_after();
                 mma4_ts(tmem + C::O_COL + s * D, tmem + s * 128, vd, idesc<T>(D, true), add);
+                if (!wait_bounded(&p_full[s], done[s] & 1)) return false;
+                ++done[s];
+                fence_after();
                 mma4_ts(tmem + C::O_COL + s * D, tmem + s * 128 + 32, vd + 4 * 128, idesc<T>(D, true), 1);
+                return true;
             };
             for (uint32_t i = 0; i <= n && ok; ++i) {
                 const uint32_t kt = tile0 + k_tile<TWO>(i), ks = kt % NST, vt = tile0 + v_tile<TWO>(i - 1, n), vs = vt % NST; // (values of the block before)
@@ -405,9 +419,7 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
 #pragma unroll
                     for (uint32_t s = 0; s < 2; ++s) {
                         if (i > 0) {
-                            if (!(ok = wait_bounded(&p_full[s], done[s]++ & 1))) break;
-                            fence_after();
-                            values(s, vs, i > 1);
+                            if (!(ok = values(s, vs, i > 1))) break;
                             if (s == 1) commit2(&empty[vs], &o_done[s]);
                             else commit1(&o_done[s]);
                         }
@@ -428,11 +440,8 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
                     }
                     if (i > 0) {
                         const uint32_t s = (i - 1) & 1;
-                        if (!(ok = wait_bounded(&full[vs], vt / NST & 1) && wait_bounded(&p_full[s], done[s] & 1))) break;
-                        fence_after();
-                        values(s, vs, i > 2);
+                        if (!(ok = wait_bounded(&full[vs], vt / NST & 1) && values(s, vs, i > 2))) break;
                         commit2(&empty[vs], &o_done[s]);
-                        ++done[s];
                     }
                 }
             }
@@ -457,10 +466,86 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
                 const int key0 = (blk + j) * TK;
                 const bool tail = key0 + TK > v.ctx;
                 uint32_t bits[4];
-                if (tail) {
+                if (tail && !idle)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) bits[c] = view_bits(p, v, me, key0 + 32 * c);
-                    // clean the values of this block: thread = key
+                if (!(ok = wait_bounded(&s_full[s], done[s] & 1))) break;
+                fence_after();
+                if (!idle) {
+                    if (tail) { // what a row does not see is masked where the scores lie
+#pragma unroll 1
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t x[32];
+                            const uint32_t see = c == 0 ? bits[0] : (c == 1 ? bits[1] : (c == 2 ? bits[2] : bits[3]));
+                            tmem_ld32(t_s + 32 * c, x);
+                            wait_ld32(x);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (!(see >> e & 1u)) x[e] = 0xff800000u;
+                            tmem_st32(t_s + 32 * c, x);
+                        }
+                        wait_st();
+                    }
+                    // Two passes over the scores: the maximum, then the weights.  Reading tensor memory twice costs less than what 128 live values
+                    // spill; the next 32 scores are on their way while 32 are worked on, and the tensor cores take the weights of
+                    // the first 64 keys while those of the others are made.
+                    float top[2] = {-INFINITY, -INFINITY};
+                    uint32_t x[2][32];
+                    tmem_ld32(t_s, x[0]);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        wait_ld32(x[c & 1]);
+                        if (c < 3) tmem_ld32(t_s + 32 * (c + 1), x[(c + 1) & 1]);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) top[e >> 1 & 1] = max3(top[e >> 1 & 1], __uint_as_float(x[c & 1][e]), __uint_as_float(x[c & 1][e + 1]));
+                    }
+                    tmem_ld32(t_s, x[0]);
+                    const float block_max = fmaxf(top[0], top[1]) * scale - lift<T>();
+                    if (__any_sync(0xffffffffu, block_max > m + 8.f)) {
+                        const float to = block_max > m + 8.f ? block_max : m;
+                        const float corr = m == to ? 1.f : ex2(m - to);
+                        if (j >= STEP) {
+                            if (!(ok = wait_bounded(&o_done[s], (done[s] - 1) & 1))) break; // P V of the stream's block before
+                            fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 32) {
+                                uint32_t o[32];
+                                tmem_ld32(t_o + c, o);
+                                wait_ld32(o);
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                                tmem_st32(t_o + c, o);
+                            }
+                        }
+                        l *= corr, m = to;
+                    }
+                    const float sub = m == -INFINITY ? 0.f : m; // nothing seen yet: every weight is 2^-inf
+                    const float2 scale2 = {scale, scale}, sub2 = {-sub, -sub};
+                    float2 acc[2] = {{0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        wait_ld32(x[c & 1]);
+                        if (c < 3) tmem_ld32(t_s + 32 * (c + 1), x[(c + 1) & 1]);
+                        uint32_t w16[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            float2 a = fma2(make_float2(__uint_as_float(x[c & 1][2 * e]), __uint_as_float(x[c & 1][2 * e + 1])), scale2, sub2);
+                            a.x = ex2(a.x), a.y = ex2(a.y);
+                            acc[e & 1] = add2(acc[e & 1], a);
+                            w16[e] = pack2<T>(a.x, a.y);
+                        }
+                        tmem_st16(t_s + 16 * c, w16); // over scores that have been read
+                        if (c == 1 && !tail) {
+                            wait_st();
+                            fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&h_full[s]);
+                        }
+                    }
+                    l += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
+                    wait_st();
+                }
+                if (tail) { // clean the values of this block: thread = key
                     const uint32_t tile = tile0 + v_tile<TWO>(j, n), st = tile % NST, kr = tid & 127;
                     if (!(ok = wait_bounded(&full[st], tile / NST & 1))) break;
                     const int token = key0 + (int)kr;
@@ -487,84 +572,12 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
                         fence_async();
                     }
                 }
-                if (!(ok = wait_bounded(&s_full[s], done[s] & 1))) break;
-                fence_after();
-                if (!idle) {
-                    if (tail) { // what a row does not see is masked where the scores lie
-#pragma unroll 1
-                        for (int c = 0; c < 4; ++c) {
-                            uint32_t x[32];
-                            const uint32_t see = c == 0 ? bits[0] : (c == 1 ? bits[1] : (c == 2 ? bits[2] : bits[3]));
-                            tmem_ld32(t_s + 32 * c, x);
-                            wait_ld();
-#pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                if (!(see >> e & 1u)) x[e] = 0xff800000u;
-                            tmem_st32(t_s + 32 * c, x);
-                        }
-                        wait_st();
-                    }
-                    // two passes over the scores, 64 columns in registers at a time: reading tensor memory twice costs less than
-                    // what 128 live values spill, and loops keep the code of a block small (a CTA runs it a few times only)
-                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-                    for (int half = 0; half < 2; ++half) {
-                        uint32_t x[64];
-                        tmem_ld32(t_s + 64 * half, x);
-                        tmem_ld32(t_s + 64 * half + 32, x + 32);
-                        wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 64; e += 8)
-#pragma unroll
-                            for (int u = 0; u < 4; ++u) top[u] = max3(top[u], __uint_as_float(x[e + u]), __uint_as_float(x[e + 4 + u]));
-                    }
-                    const float block_max = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale - lift<T>();
-                    if (__any_sync(0xffffffffu, block_max > m + 8.f)) {
-                        const float to = block_max > m + 8.f ? block_max : m;
-                        const float corr = m == to ? 1.f : ex2(m - to);
-                        if (j >= STEP) {
-                            if (!(ok = wait_bounded(&o_done[s], (done[s] - 1) & 1))) break; // P V of the stream's block before
-                            fence_after();
-#pragma unroll 1
-                            for (int c = 0; c < D; c += 32) {
-                                uint32_t o[32];
-                                tmem_ld32(t_o + c, o);
-                                wait_ld();
-#pragma unroll
-                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-                                tmem_st32(t_o + c, o);
-                            }
-                        }
-                        l *= corr, m = to;
-                    }
-                    const float sub = m == -INFINITY ? 0.f : m; // nothing seen yet: every weight is 2^-inf
-                    float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
-                    const float2 scale2 = {scale, scale}, sub2 = {-sub, -sub};
-#pragma unroll 1
-                    for (int half = 0; half < 2; ++half) {
-                        uint32_t x[64];
-                        tmem_ld32(t_s + 64 * half, x);
-                        tmem_ld32(t_s + 64 * half + 32, x + 32);
-                        wait_ld();
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            uint32_t w16[16];
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                float2 a = fma2(make_float2(__uint_as_float(x[32 * c + 2 * e]), __uint_as_float(x[32 * c + 2 * e + 1])), scale2, sub2);
-                                a.x = ex2(a.x), a.y = ex2(a.y);
-                                sum[e & 1] = add2(sum[e & 1], a);
-                                w16[e] = pack2<T>(a.x, a.y);
-                            }
-                            tmem_st16(t_s + 32 * half + 16 * c, w16);
-                        }
-                    }
-                    l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-                    wait_st();
-                }
                 fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[s]);
+                if (lane == 0) {
+                    if (idle || tail) mbar_arrive(&h_full[s]); // (a tail's values are clean only now)
+                    mbar_arrive(&p_full[s]);
+                }
                 ++done[s];
             }
             if (!ok) break;
@@ -606,7 +619,8 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
                     uint32_t o0[32], o1[32];
                     tmem_ld32(TWO ? t_o + c : t_lane + C::O_COL + c, o0);
                     if (!TWO) tmem_ld32(t_lane + C::O_COL + D + c, o1);
-                    wait_ld();
+                    wait_ld32(o0);
+                    if (!TWO) wait_ld32(o1);
                     float o[32];
 #pragma unroll
                     for (int e = 0; e < 32; ++e) o[e] = TWO ? __uint_as_float(o0[e]) : __uint_as_float(o0[e]) * wa + (n < 2 ? 0.f : __uint_as_float(o1[e]) * wb);
@@ -710,7 +724,7 @@ cudaError_t launch_tree_attn_tc(const DeviceInfo &dev, const PoolDev &pool, int 
     const long long rows = ((long long)t.n_rows * t.group + t.n_seq - 1) / t.n_seq;
     const bool two = rows > TM;
     prm.lanes = 1;
-    while (two && prm.lanes < 4 && prm.lanes * 4 * TM < rows + TM && dev.sm_count / (prm.lanes * 2) > 0) prm.lanes *= 2;
+    while (two && prm.lanes < 4 && rows > prm.lanes * 2 * TM * 5 / 4 && dev.sm_count / (prm.lanes * 2) > 0) prm.lanes *= 2;
     // query boxes of about a sequence's rows
     prm.q_box = 0;
     if (TM % t.group == 0) {

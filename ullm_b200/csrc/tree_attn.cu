@@ -211,7 +211,7 @@ template <typename Q, typename KV> static cudaError_t launch_fma(const DeviceInf
     const int ctas = fma_ctas(dev.sm_count, t.dim);
     e = launch_kernel(tree_attn_fma_kernel<Q, KV>, dim3(ctas), dim3(FT), smem, st, pdl, t);
     if (e != cudaSuccess) return e;
-    return launch_kernel(tree_join_kernel<Q, FM>, dim3(dev.sm_count * 2), dim3(32 * JOIN_WARPS), 0, st, pdl, t, ctas);
+    return launch_kernel(tree_join_kernel<Q, FM>, dim3(dev.sm_count * JOIN_PER_SM), dim3(32 * JOIN_WARPS), 0, st, pdl, t, ctas);
 }
 
 } // namespace ullm

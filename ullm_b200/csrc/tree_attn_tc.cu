@@ -246,39 +246,35 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
     __shared__ uint32_t tmem_s;
     const TreeDev &p = prm.t;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (warp == 0 && lane < 3) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &maps.k : (lane == 1 ? &maps.v : &maps.q)) : "memory");
-    if (tid == 0) {
-        for (int i = 0; i < NST; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-        for (int s = 0; s < 2; ++s) {
-            mbar_init(&s_full[s], 1), mbar_init(&h_full[s], 4), mbar_init(&p_full[s], 4), mbar_init(&o_done[s], 1);
-            mbar_init(&q_full[s], 1), mbar_init(&q_empty[s], 8);
+    // Set-up: warp 3 makes the barriers, tells the others and goes on to its part; they wait for it and the tensor memory.
+    if (warp == 3) {
+        if (lane == 0) {
+            for (int i = 0; i < NST; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+            for (int s = 0; s < 2; ++s) {
+                mbar_init(&s_full[s], 1), mbar_init(&h_full[s], 4), mbar_init(&p_full[s], 4), mbar_init(&o_done[s], 1);
+                mbar_init(&q_full[s], 1), mbar_init(&q_empty[s], 8);
+            }
+            for (int i = 0; i < SEGS; ++i) mbar_init(&seg_full[i], 1), mbar_init(&seg_empty[i], 11);
+            mbar_init(&x_full, 8), mbar_init(&epi_done, 8);
+            mbar_fence_init();
         }
-        for (int i = 0; i < SEGS; ++i) mbar_init(&seg_full[i], 1), mbar_init(&seg_empty[i], 11);
-        mbar_init(&x_full, 8), mbar_init(&epi_done, 8);
-        mbar_fence_init();
-    }
-    if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "r"(512u) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    Sched<ROWS, TK, T_COST, T_MIN> sched(p, prm.lanes);
-    Seg first;
-    first.count = 0;
-    if (warp == 3) { // (while the others set up)
-        pdl_wait_prior();
-        if (lane == 0) p.meta[blockIdx.x * TREE_META] = make_int4(-1, 0, 0, 0);
         __syncwarp();
-        if (sched.init()) first = sched.next(p.meta + blockIdx.x * TREE_META);
-        if (lane == 0) segs[0] = first;
+        asm volatile("barrier.cta.arrive 1, %0;" ::"n"(TT) : "memory");
+    } else {
+        if (warp == 0 && lane < 3) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &maps.k : (lane == 1 ? &maps.v : &maps.q)) : "memory");
+        if (warp == 2) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+        fence_before();
+        asm volatile("barrier.cta.sync 1, %0;" ::"n"(TT) : "memory");
+        fence_after();
     }
-    fence_before();
-    __syncthreads();
-    fence_after();
     pdl_wait_prior();
     pdl_launch_dependents();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_s, 0);
+    const uint32_t tmem = warp == 3 ? 0 : __shfl_sync(0xffffffffu, tmem_s, 0);
     bool ok = true;
-    // the next segment of the ring; count 0: no more
+    // the next segment of the ring; 0: no more
     uint32_t seg = 0;
     auto take = [&]() -> int {
         ok = wait_bounded(&seg_full[seg % SEGS], seg / SEGS & 1);
@@ -291,15 +287,21 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
     };
 
     if (warp == 3) {
-        // ---- division of the work: the first segment lies in the ring already ----
-        if (lane == 0) mbar_arrive(&seg_full[0]);
-        for (seg = 1; first.count; ++seg) {
-            first = sched.next(p.meta + blockIdx.x * TREE_META);
+        // ---- division of the work ----
+        if (lane == 0) p.meta[blockIdx.x * TREE_META] = make_int4(-1, 0, 0, 0);
+        __syncwarp();
+        Sched<ROWS, TK, T_COST, T_MIN> sched(p, prm.lanes);
+        const bool some = sched.init();
+        for (;; ++seg) {
+            Seg next;
+            next.count = 0;
+            if (some) next = sched.next(p.meta + blockIdx.x * TREE_META);
             if (seg >= SEGS && !(ok = wait_bounded(&seg_empty[seg % SEGS], (seg / SEGS - 1) & 1))) break;
             if (lane == 0) {
-                segs[seg % SEGS] = first;
+                segs[seg % SEGS] = next;
                 mbar_arrive(&seg_full[seg % SEGS]);
             }
+            if (!next.count) break;
         }
     } else if (warp == 0) {
         // ---- TMA: lane -> (64 values, box of keys) ----
@@ -400,14 +402,18 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
 #pragma unroll
                 for (int a = 0; a < C::ATOMS; ++a) mma4_ss(tmem + s * 128, q + a * (TM * 128 >> 4), kd + a * (TK * 128 >> 4), idesc<T>(TK, false), a > 0);
             };
-            auto values = [&](uint32_t s, uint32_t st, bool add) { // P V as the halves of P arrive
+            // P V.  Where both streams take every block the tensor cores set the pace and P comes in halves (262 -> 250 us for 12 x 64 drafted rows over
+            // 4,000-16,000 tokens); where they alternate the second barrier costs more than it saves (64 decoded tokens: 125 -> 130 us).
+            auto values = [&](uint32_t s, uint32_t st, bool add) {
                 const uint64_t vd = desc_mn_major(r0 + st * C::TILE);
-                if (!wait_bounded(&h_full[s], done[s] & 1)) return false;
+                if (!wait_bounded(TWO ? &h_full[s] : &p_full[s], done[s] & 1)) return false;
                 fence_after();
                 mma4_ts(tmem + C::O_COL + s * D, tmem + s * 128, vd, idesc<T>(D, true), add);
-                if (!wait_bounded(&p_full[s], done[s] & 1)) return false;
+                if (TWO) {
+                    if (!wait_bounded(&p_full[s], done[s] & 1)) return false;
+                    fence_after();
+                }
                 ++done[s];
-                fence_after();
                 mma4_ts(tmem + C::O_COL + s * D, tmem + s * 128 + 32, vd + 4 * 128, idesc<T>(D, true), 1);
                 return true;
             };
@@ -492,14 +498,17 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
                     float top[2] = {-INFINITY, -INFINITY};
                     uint32_t x[2][32];
                     tmem_ld32(t_s, x[0]);
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
+                        wait_ld32(x[0]);
+                        tmem_ld32(t_s + 64 * half + 32, x[1]);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        wait_ld32(x[c & 1]);
-                        if (c < 3) tmem_ld32(t_s + 32 * (c + 1), x[(c + 1) & 1]);
+                        for (int e = 0; e < 32; e += 2) top[e >> 1 & 1] = max3(top[e >> 1 & 1], __uint_as_float(x[0][e]), __uint_as_float(x[0][e + 1]));
+                        wait_ld32(x[1]);
+                        tmem_ld32(t_s + 64 - 64 * half, x[0]); // (the second time: the first ones again)
 #pragma unroll
-                        for (int e = 0; e < 32; e += 2) top[e >> 1 & 1] = max3(top[e >> 1 & 1], __uint_as_float(x[c & 1][e]), __uint_as_float(x[c & 1][e + 1]));
+                        for (int e = 0; e < 32; e += 2) top[e >> 1 & 1] = max3(top[e >> 1 & 1], __uint_as_float(x[1][e]), __uint_as_float(x[1][e + 1]));
                     }
-                    tmem_ld32(t_s, x[0]);
                     const float block_max = fmaxf(top[0], top[1]) * scale - lift<T>();
                     if (__any_sync(0xffffffffu, block_max > m + 8.f)) {
                         const float to = block_max > m + 8.f ? block_max : m;
@@ -522,20 +531,24 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
                     const float sub = m == -INFINITY ? 0.f : m; // nothing seen yet: every weight is 2^-inf
                     const float2 scale2 = {scale, scale}, sub2 = {-sub, -sub};
                     float2 acc[2] = {{0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        wait_ld32(x[c & 1]);
-                        if (c < 3) tmem_ld32(t_s + 32 * (c + 1), x[(c + 1) & 1]);
-                        uint32_t w16[16];
+                        for (int c = 0; c < 2; ++c) {
+                            wait_ld32(x[c]);
+                            if (c == 0) tmem_ld32(t_s + 64 * half + 32, x[1]);
+                            else if (half == 0) tmem_ld32(t_s + 64, x[0]);
+                            uint32_t w16[16];
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            float2 a = fma2(make_float2(__uint_as_float(x[c & 1][2 * e]), __uint_as_float(x[c & 1][2 * e + 1])), scale2, sub2);
-                            a.x = ex2(a.x), a.y = ex2(a.y);
-                            acc[e & 1] = add2(acc[e & 1], a);
-                            w16[e] = pack2<T>(a.x, a.y);
+                            for (int e = 0; e < 16; ++e) {
+                                float2 a = fma2(make_float2(__uint_as_float(x[c][2 * e]), __uint_as_float(x[c][2 * e + 1])), scale2, sub2);
+                                a.x = ex2(a.x), a.y = ex2(a.y);
+                                acc[e & 1] = add2(acc[e & 1], a);
+                                w16[e] = pack2<T>(a.x, a.y);
+                            }
+                            tmem_st16(t_s + 32 * half + 16 * c, w16); // over scores that have been read
                         }
-                        tmem_st16(t_s + 16 * c, w16); // over scores that have been read
-                        if (c == 1 && !tail) {
+                        if (TWO && half == 0 && !tail) {
                             wait_st();
                             fence_before();
                             __syncwarp();
@@ -575,7 +588,7 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
                 fence_before();
                 __syncwarp();
                 if (lane == 0) {
-                    if (idle || tail) mbar_arrive(&h_full[s]); // (a tail's values are clean only now)
+                    if (TWO && (idle || tail)) mbar_arrive(&h_full[s]); // (a tail's values are clean only now)
                     mbar_arrive(&p_full[s]);
                 }
                 ++done[s];
@@ -648,6 +661,7 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
         }
     }
     if (!ok) *(volatile int *)prm.status = DEV_TIMEOUT;
+    __syncwarp();
     fence_before();
     __syncthreads();
     fence_after();
@@ -698,7 +712,7 @@ template <typename T, int D, bool TWO> cudaError_t launch(const DeviceInfo &dev,
     cudaError_t e = cudaFuncSetAttribute(tree_attn_tc_kernel<T, D, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
     if (e != cudaSuccess) return e;
     if ((e = launch_kernel(tree_attn_tc_kernel<T, D, TWO>, dim3(dev.sm_count), dim3(TT), Cfg<D>::SMEM, st, pdl, prm, maps)) != cudaSuccess) return e;
-    return launch_kernel(tree_join_kernel<T, TWO ? 2 * TM : TM>, dim3(dev.sm_count * 2), dim3(32 * JOIN_WARPS), 0, st, pdl, prm.t, dev.sm_count);
+    return launch_kernel(tree_join_kernel<T, TWO ? 2 * TM : TM>, dim3(dev.sm_count * JOIN_PER_SM), dim3(32 * JOIN_WARPS), 0, st, pdl, prm.t, dev.sm_count);
 }
 template <typename T> cudaError_t launch_any(const DeviceInfo &dev, int dim, bool two, const TcParams &prm, const TcMaps &maps, bool pdl, cudaStream_t st) {
     if (dim == 64) return two ? launch<T, 64, true>(dev, prm, maps, pdl, st) : launch<T, 64, false>(dev, prm, maps, pdl, st);

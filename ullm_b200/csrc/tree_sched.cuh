@@ -231,19 +231,23 @@ template <> __device__ __forceinline__ __nv_bfloat16 out_from<__nv_bfloat16>(flo
 
 // Joins the parts of the units that were cut, in the order of the CTAs:
 //   out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c.
-// A fixed number of CTAs share the rows of all cut units: every CTA reads the records, SPLIT warps take a row together (each
-// a part of the parts, eight loads in flight), because a long context of one sequence is cut into as many parts as there are CTAs.
-constexpr int JOIN_WARPS = 8, JOIN_MAX = 1024; // CTAs of the attention kernel at most
+// A fixed number of CTAs share the rows of all cut units; every CTA reads the records.  Four warps take a row together (or one, where units have few
+// parts), each every fourth part, up to eight at a time; a row's values, references and sums are all on their way at once, because
+// the kernel is bound by round trips to memory: with weights first and values after them a row took 6,500 cycles.
+constexpr int JOIN_WARPS = 8, JOIN_MAX = 1024, JOIN_PER_SM = 4; // JOIN_MAX: CTAs of the attention kernel at most
 template <typename O, int M> __global__ void __launch_bounds__(32 * JOIN_WARPS) tree_join_kernel(const TreeDev p, int ctas) {
     struct Duty {
-        int c, front, c0, slot, lanes, r0, t, h; // the CTA in which it ends, rows of the units in front of it, ...
+        int front;                // rows of the units in front of it
+        short c, c0;              // the CTAs in which it ends and begins ...
+        int r0, t;
+        unsigned short h, how;    // how: slot | lanes << 1
     };
     __shared__ Duty duty[JOIN_MAX];
     __shared__ int s_found[JOIN_WARPS], s_rows[JOIN_WARPS], s_most[JOIN_WARPS];
     __shared__ float red[JOIN_WARPS][256], red_l[JOIN_WARPS];
     pdl_wait_prior();
     pdl_launch_dependents();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = p.dim;
     int n_duty = 0, n_rows = 0, most = 0;
     for (int c0 = 0; c0 < ctas; c0 += 32 * JOIN_WARPS) {
         const int c = c0 + tid;
@@ -269,12 +273,13 @@ template <typename O, int M> __global__ void __launch_bounds__(32 * JOIN_WARPS) 
         }
         if (has) {
             Duty d;
-            d.c = c, d.front = front, d.c0 = a.x, d.slot = a.y & 1, d.lanes = a.y >> 1, d.r0 = a.z, d.t = b.x, d.h = b.y;
+            d.front = front, d.c = (short)c, d.c0 = (short)a.x, d.r0 = a.z, d.t = b.x, d.h = (unsigned short)b.y, d.how = (unsigned short)a.y;
             duty[at] = d;
         }
     }
     __syncthreads();
-    const int split = most > 8 ? 4 : 1, per = JOIN_WARPS / split, sub = warp % split;
+    const int split = most > 8 ? 4 : 1, per = JOIN_WARPS / split, sub = warp % split, wide = D <= 128 ? 4 : 8;
+    const bool on = lane * wide < D;
     for (int i0 = blockIdx.x * per; i0 < n_rows; i0 += gridDim.x * per) {
         const int i = i0 + warp / split;
         float m = -INFINITY, l = 0.f, acc[8];
@@ -291,50 +296,49 @@ template <typename O, int M> __global__ void __launch_bounds__(32 * JOIN_WARPS) 
             }
             u = duty[lo];
             r = i - u.front;
-            const int parts = (u.c - u.c0) / u.lanes + 1;
-            auto part = [&](int k) { return part_of<M>(p, u.c0 + k * u.lanes, k == 0 ? u.slot : 0); };
-            for (int k = lane; k < parts; k += 32) m = fmaxf(m, part(k)[(size_t)M * p.dim + 2 * r]);
-            m = warp_max(m);
-            // this warp's parts: sub, sub + split, ...; 32 weights at a time, one per lane
-            for (int k0 = sub; k0 < parts; k0 += 32 * split) {
-                float w = 0.f;
-                if (k0 + lane * split < parts) {
-                    const float2 ml = *(const float2 *)(part(k0 + lane * split) + (size_t)M * p.dim + 2 * r);
+            const int lanes = u.how >> 1, parts = (u.c - u.c0) / lanes + 1;
+            auto part = [&](int k) { return part_of<M>(p, u.c0 + k * lanes, k == 0 ? u.how & 1 : 0); };
+            auto pair = [&](int k) { return k < parts ? *(const float2 *)(part(k) + (size_t)M * D + 2 * r) : make_float2(-INFINITY, 0.f); };
+            for (int j0 = sub; j0 < parts; j0 += 8 * split) { // this warp's parts j0, j0 + split, ...
+                const int n = min(8, (parts - j0 + split - 1) / split);
+                float4 x[8];
+                if (wide == 4) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (j < n && on) x[j] = *(const float4 *)(part(j0 + j * split) + (size_t)r * D + lane * 4);
+                }
+                if (j0 == sub) { // the row's reference, over all parts
+                    for (int k = lane; k < parts; k += 32) m = fmaxf(m, pair(k).x);
+                    m = warp_max(m);
+                }
+                float w = 0.f; // weight of this warp's part number `lane` of the eight
+                if (lane < n) {
+                    const float2 ml = pair(j0 + lane * split);
                     w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
                     l += ml.y * w;
                 }
-                const int n = min(32, (parts - k0 + split - 1) / split);
-                for (int j0 = 0; j0 < n; j0 += 8) {
-                    if (p.dim <= 128) { // four values per lane
-                        float4 x[8];
-                        const bool on = lane * 4 < p.dim;
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (j0 + j < n && on) x[j] = *(const float4 *)(part(k0 + (j0 + j) * split) + (size_t)r * p.dim + lane * 4);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float wk = __shfl_sync(0xffffffffu, w, (j0 + j) & 31);
-                            if (j0 + j < n && on && wk != 0.f) acc[0] += wk * x[j].x, acc[1] += wk * x[j].y, acc[2] += wk * x[j].z, acc[3] += wk * x[j].w;
-                        }
+                for (int j = 0; j < 8; ++j) {
+                    const float wk = __shfl_sync(0xffffffffu, w, j);
+                    if (j >= n || !on || wk == 0.f) continue; // (an empty part's values were never written)
+                    if (wide == 4) {
+                        acc[0] += wk * x[j].x, acc[1] += wk * x[j].y, acc[2] += wk * x[j].z, acc[3] += wk * x[j].w;
                     } else {
-                        for (int j = 0; j < 8 && j0 + j < n; ++j) {
-                            const float wk = __shfl_sync(0xffffffffu, w, j0 + j);
-                            if (wk == 0.f) continue;
-                            const float *o = part(k0 + (j0 + j) * split) + (size_t)r * p.dim;
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                if (lane * 8 + e < p.dim) acc[e] += wk * o[lane * 8 + e];
-                        }
+                        const float *o = part(j0 + j * split) + (size_t)r * D + lane * 8;
+                        const float4 y0 = *(const float4 *)o, y1 = *(const float4 *)(o + 4);
+                        acc[0] += wk * y0.x, acc[1] += wk * y0.y, acc[2] += wk * y0.z, acc[3] += wk * y0.w;
+                        acc[4] += wk * y1.x, acc[5] += wk * y1.y, acc[6] += wk * y1.z, acc[7] += wk * y1.w;
                     }
                 }
             }
             l = warp_sum(l);
         }
-        const int wide = p.dim <= 128 ? 4 : 8;
         if (split > 1) { // the row's warps in order
             __syncthreads();
-            if (lane * wide < p.dim)
-                for (int e = 0; e < wide; ++e) red[warp][lane * wide + e] = e < 4 ? acc[e & 3] : acc[4 + (e & 3)];
+            if (on)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e < wide) red[warp][lane * wide + e] = acc[e];
             if (lane == 0) red_l[warp] = l;
             __syncthreads();
         }
@@ -344,14 +348,14 @@ template <typename O, int M> __global__ void __launch_bounds__(32 * JOIN_WARPS) 
                 l += red_l[warp + s];
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (e < wide && lane * wide < p.dim) acc[e] += red[warp + s][lane * wide + e];
+                    if (e < wide && on) acc[e] += red[warp + s][lane * wide + e];
             }
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         const int row = u.t * M + r;
-        O *out = (O *)p.out + (u.r0 + row / p.group) * p.out_stride + ((long long)u.h * p.group + row % p.group) * p.dim;
+        O *out = (O *)p.out + (u.r0 + row / p.group) * p.out_stride + ((long long)u.h * p.group + row % p.group) * D + lane * wide;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-            if (e < wide && lane * wide < p.dim) out[lane * wide + e] = out_from<O>(l == 0.f ? 0.f : acc[e] * inv);
+            if (e < wide && on) out[e] = out_from<O>(l == 0.f ? 0.f : acc[e] * inv);
     }
 }
 

@@ -8,7 +8,9 @@
 #include "paged.h"
 #include "engine.h"
 
+#include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 namespace ullm {
 
@@ -119,19 +121,23 @@ __global__ void __launch_bounds__(128) kv_trim_kernel(const TableDev t, int page
 }
 
 // ---- accept ---------------------------------------------------------------------------------------------------------
-// grid (sequences, 2 * layers): CTA (i, y) moves the kept rows of layer y / 2, K or V.  A thread owns 16-byte pieces of
-// a row and takes up to eight rows into registers before it stores them: kept indices increase, so a row is never
-// moved onto one that a later batch still reads (destination j <= path[j] < path[j + 1]), and pieces of different threads never meet.
-// The verdict on the entry is the same in every CTA (the tables do not change until kv_accept_end_kernel); the first
-// one leaves it in t.work[i].
-constexpr int MOVE_BATCH = 8;
+// grid (sequences, Y): CTA (i, y) moves the kept rows of its share of the layers' K and V.  A thread owns 16-byte pieces of a row and
+// takes up to eight rows into registers before it stores them: kept indices increase, so a row is never moved onto one that a
+// later batch still reads (destination j <= path[j] < path[j + 1]), and pieces of different threads never meet.  The
+// verdict on the entry is the same in every CTA (the tables do not change until kv_accept_end_kernel); the first one leaves it
+// in t.work[i].  What costs time is the chain of loads in front of the first move (entry, length, path, page numbers,
+// counts): Y is chosen so that all CTAs run at once and pay it once (192 entries, 24 matrices: 21 us with a CTA for each matrix).
+constexpr int MOVE_BATCH = 8, MOVE_KEEP = 64; // MOVE_KEEP: rows whose places a CTA keeps in shared memory
 __global__ void __launch_bounds__(128) kv_accept_move_kernel(const TableDev t, const PoolDev pool, const int *seq, const int *draft, const int *path,
                                                             const int *kept, int n, int max_path) {
+    __shared__ long long s_from[MOVE_KEEP], s_to[MOVE_KEEP]; // bytes from a matrix' start
+    __shared__ int s_first;                                  // rows of the path that stay where they are
     pdl_wait_prior();
     pdl_launch_dependents();
     const int i = blockIdx.x, s = seq[i], nd = draft[i], nk = kept[i], ps = pool.page_size;
     const int *p = path + (size_t)i * max_path;
     int bad = s < 0 || s >= t.n_seq ? ULLM_KV_FAULT_SEQ : 0;
+    if (threadIdx.x == 0) s_first = INT32_MAX;
     if (cta_listed_elsewhere(seq, n, s, i)) bad |= ULLM_KV_FAULT_SEQ;
     int len = 0;
     if (!bad) {
@@ -140,6 +146,7 @@ __global__ void __launch_bounds__(128) kv_accept_move_kernel(const TableDev t, c
     }
     const int base = len - nd;
     const int *row = t.blocks + (size_t)(bad ? 0 : s) * t.max_blocks;
+    auto at = [&](int token, int page) { return (page * pool.page_stride + (token % ps) * pool.slot_stride) * pool.elem_bytes; };
     int seen = 0;
     if (!bad)
         for (int j = threadIdx.x; j < nk; j += blockDim.x) {
@@ -150,6 +157,8 @@ __global__ void __launch_bounds__(128) kv_accept_move_kernel(const TableDev t, c
                 const int a = row[(base + from) / ps], b = row[(base + j) / ps];
                 if ((unsigned)a >= (unsigned)pool.n_pages || (unsigned)b >= (unsigned)pool.n_pages) seen |= ULLM_KV_FAULT_PAGE;
                 else if (t.refs[b] != 1) seen |= ULLM_KV_FAULT_SHARED;
+                if (j < MOVE_KEEP) s_from[j] = at(base + from, a), s_to[j] = at(base + j, b);
+                atomicMin(&s_first, j);
             }
         }
     if (__syncthreads_or(seen)) {
@@ -159,23 +168,24 @@ __global__ void __launch_bounds__(128) kv_accept_move_kernel(const TableDev t, c
         set_fault(t.fault, bad);
     }
     if (blockIdx.y == 0 && threadIdx.x == 0) t.work[i] = bad;
-    if (bad || nk == 0) return;
-    const int layer = blockIdx.y >> 1;
-    uint8_t *const mem = (blockIdx.y & 1 ? pool.v : pool.k) + layer * pool.layer_stride * pool.elem_bytes;
-    const int pieces = pool.head_dim * pool.elem_bytes / 16, total = pieces * pool.n_kv_head;
-    auto at = [&](int token) { return (row[token / ps] * pool.page_stride + (token % ps) * pool.slot_stride) * pool.elem_bytes; };
-    for (int c = threadIdx.x; c < total; c += blockDim.x) {
-        uint8_t *const col = mem + (long long)(c / pieces) * pool.head_stride * pool.elem_bytes + (c % pieces) * 16;
-        int j = 0;
-        while (j < nk && p[j] == j) ++j; // a kept prefix stays where it is
-        for (; j < nk; j += MOVE_BATCH) {
+    const int first = s_first;
+    if (bad || first >= nk) return;
+    auto from_at = [&](int j) { return j < MOVE_KEEP ? s_from[j] : at(base + p[j], row[(base + p[j]) / ps]); };
+    auto to_at = [&](int j) { return j < MOVE_KEEP ? s_to[j] : at(base + j, row[(base + j) / ps]); };
+    const int pieces = pool.head_dim * pool.elem_bytes / 16, per = pieces * pool.n_kv_head, mats = 2 * pool.n_layer;
+    const int m0 = (int)((long long)mats * blockIdx.y / gridDim.y), m1 = (int)((long long)mats * (blockIdx.y + 1) / gridDim.y);
+    for (int c = threadIdx.x; c < per * (m1 - m0); c += blockDim.x) {
+        const int mat = m0 + c / per, r = c % per;
+        uint8_t *const col = (mat & 1 ? pool.v : pool.k) +
+                             ((mat >> 1) * pool.layer_stride + (long long)(r / pieces) * pool.head_stride) * pool.elem_bytes + (r % pieces) * 16;
+        for (int j = first; j < nk; j += MOVE_BATCH) { // from the first row that moves on, every one does
             uint4 v[MOVE_BATCH];
 #pragma unroll
             for (int u = 0; u < MOVE_BATCH; ++u)
-                if (j + u < nk) v[u] = *(const uint4 *)(col + at(base + p[j + u]));
+                if (j + u < nk) v[u] = *(const uint4 *)(col + from_at(j + u));
 #pragma unroll
             for (int u = 0; u < MOVE_BATCH; ++u)
-                if (j + u < nk) *(uint4 *)(col + at(base + j + u)) = v[u];
+                if (j + u < nk) *(uint4 *)(col + to_at(j + u)) = v[u];
         }
     }
 }
@@ -429,6 +439,7 @@ __global__ void __launch_bounds__(128) tree_plan_kernel(int n_rows, int n_seq, c
 }
 
 // ---- norm, rotation, cache write ------------------------------------------------------------------------------------
+constexpr int ROPE_HPG = 4; // 2: 184 us, 4: 146, 6: 145, 8 with spills: 255 for the long prompt below
 struct RopeDev {
     const uint8_t *q, *k, *v;
     long long q_stride, k_stride, v_stride, q_out_stride;
@@ -443,157 +454,166 @@ struct RopeDev {
     int n_rows, n_head, n_kv, dim, n_pos, rot, n_table, max_blocks, n_pages, page_size;
 };
 
+// Four neighbouring values: as they lie in memory, and as two pairs of f32
 template <typename T> struct Io;
 template <> struct Io<float> {
-    static __device__ __forceinline__ void load(const float *p, float (&o)[8]) {
-        const float4 a = *(const float4 *)p, b = *(const float4 *)(p + 4);
-        o[0] = a.x, o[1] = a.y, o[2] = a.z, o[3] = a.w, o[4] = b.x, o[5] = b.y, o[6] = b.z, o[7] = b.w;
-    }
-    static __device__ __forceinline__ void store(float *p, const float (&o)[8]) {
-        *(float4 *)p = make_float4(o[0], o[1], o[2], o[3]);
-        *(float4 *)(p + 4) = make_float4(o[4], o[5], o[6], o[7]);
-    }
+    using Raw = float4;
+    static __device__ __forceinline__ void widen(const Raw &v, float2 *o) { o[0] = make_float2(v.x, v.y), o[1] = make_float2(v.z, v.w); }
+    static __device__ __forceinline__ Raw narrow(const float2 *o) { return make_float4(o[0].x, o[0].y, o[1].x, o[1].y); }
 };
 template <> struct Io<__half> {
-    static __device__ __forceinline__ void load(const __half *p, float (&o)[8]) {
-        const uint4 v = *(const uint4 *)p;
-        const __half2 *h = (const __half2 *)&v;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(h[i]);
-            o[2 * i] = f.x, o[2 * i + 1] = f.y;
-        }
-    }
-    static __device__ __forceinline__ void store(__half *p, const float (&o)[8]) {
-        uint4 v;
-        __half2 *h = (__half2 *)&v;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(o[2 * i], o[2 * i + 1]);
-        *(uint4 *)p = v;
+    using Raw = uint2;
+    static __device__ __forceinline__ void widen(const Raw &v, float2 *o) { o[0] = __half22float2(*(const __half2 *)&v.x), o[1] = __half22float2(*(const __half2 *)&v.y); }
+    static __device__ __forceinline__ Raw narrow(const float2 *o) {
+        Raw v;
+        *(__half2 *)&v.x = __floats2half2_rn(o[0].x, o[0].y), *(__half2 *)&v.y = __floats2half2_rn(o[1].x, o[1].y);
+        return v;
     }
 };
 template <> struct Io<__nv_bfloat16> {
-    static __device__ __forceinline__ void load(const __nv_bfloat16 *p, float (&o)[8]) {
-        const uint4 v = *(const uint4 *)p;
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[2 * i] = __uint_as_float(w[i] << 16), o[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    using Raw = uint2;
+    static __device__ __forceinline__ void widen(const Raw &v, float2 *o) {
+        o[0] = make_float2(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u)), o[1] = make_float2(__uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
     }
-    static __device__ __forceinline__ void store(__nv_bfloat16 *p, const float (&o)[8]) {
-        uint4 v;
-        __nv_bfloat162 *h = (__nv_bfloat162 *)&v;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
-        *(uint4 *)p = v;
+    static __device__ __forceinline__ Raw narrow(const float2 *o) {
+        Raw v;
+        *(__nv_bfloat162 *)&v.x = __floats2bfloat162_rn(o[0].x, o[0].y), *(__nv_bfloat162 *)&v.y = __floats2bfloat162_rn(o[1].x, o[1].y);
+        return v;
     }
 };
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { // two products in one instruction
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b));
+    return *(float2 *)&r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b), "l"(*(unsigned long long *)&c));
+    return *(float2 *)&r;
+}
+template <typename T> __device__ __forceinline__ typename Io<T>::Raw raw4(const T *p) { return *(const typename Io<T>::Raw *)p; }
+template <typename T> __device__ __forceinline__ void put4(T *p, const float2 *o) { *(typename Io<T>::Raw *)p = Io<T>::narrow(o); }
 
-// A group of L lanes (8, 16 or 32: as many as cover head_dim / 8) owns one head of one row, eight values per lane: one
-// 16-byte load of a 16-bit type, the sum of squares over the group by shuffles, the rotation's partner either in the
-// same lane (interleaved) or rot / 16 lanes away (rotate-half).  One pass, bound by memory.
-template <typename X, typename Q, typename KV, int L>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const RopeDev p, int neox) {
+// A group of L lanes (8, 16 or 32: as many as cover head_dim / 8) owns HPG heads of one kind (q, k or v) of one row.  A lane holds eight values of
+// a head as two runs of four: with rotate-half one of each half, so that both values of a pair lie in the lane
+// (fetched from a neighbour they cost eight shuffles a head), with interleaved pairs and in the part that is not rotated
+// neighbouring runs.  Row, page and angles are worked out once for the group's heads.  One pass over the data; for many rows the
+// instructions per head count as much as the bytes (16,000 rows of 80 heads of 128 bf16 values, 664 MB: 298 us with eight
+// shuffles, a division, scalar arithmetic and addresses for each head; 146 us = 4.5 TB/s as it is, 0.69 of the copy bandwidth).
+template <typename X, typename Q, typename KV, int L, int HPG, bool NEOX>
+__global__ void __launch_bounds__(256, HPG > 1 ? 4 : 1) qk_norm_rope_kernel(const RopeDev p) {
     pdl_wait_prior();
     pdl_launch_dependents();
     constexpr int GROUPS = 256 / L;
-    const int g = threadIdx.x / L, gl = threadIdx.x % L, heads = p.n_head + 2 * p.n_kv;
-    const long long item = (long long)blockIdx.x * GROUPS + g;
-    const int row = (int)(item / heads), head = (int)(item % heads);
-    const bool live = row < p.n_rows;
-    const int d0 = gl * 8;
-    const bool mine = live && d0 < p.dim; // lanes behind head_dim only take part in the shuffles
-    const bool is_q = head < p.n_head, is_v = head >= p.n_head + p.n_kv;
-    const int hk = is_q ? head : (is_v ? head - p.n_head - p.n_kv : head - p.n_head);
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const int gl = threadIdx.x % L, gq = (p.n_head + HPG - 1) / HPG, gk = (p.n_kv + HPG - 1) / HPG, per_row = gq + 2 * gk;
+    const unsigned item = blockIdx.x * (unsigned)GROUPS + threadIdx.x / L;
+    const int row = (int)(item / (unsigned)per_row), g = (int)(item % (unsigned)per_row);
+    const int kind = g < gq ? 0 : (g < gq + gk ? 1 : 2), head0 = (g - (kind == 0 ? 0 : (kind == 1 ? gq : gq + gk))) * HPG;
+    const int heads = min(HPG, (kind == 0 ? p.n_head : p.n_kv) - head0); // of this group
+    const unsigned group_lanes = L == 32 ? 0xffffffffu : ((1u << L % 32) - 1u) << (threadIdx.x & 31 & ~(L - 1)); // (a warp's groups may be of different kinds)
+    const bool live = row < p.n_rows, mine = live && gl * 8 < p.dim; // lanes behind head_dim only take part in the shuffles
     int seq = -1, slot = 0, pos = 0;
-    if (live) {
-        seq = p.row_seq[row], slot = p.row_slot[row], pos = p.row_pos[row];
-    }
-    if (mine) {
-        const uint8_t *const base = is_q ? p.q : (is_v ? p.v : p.k);
-        const long long stride = is_q ? p.q_stride : (is_v ? p.v_stride : p.k_stride);
-        Io<X>::load((const X *)base + row * stride + (long long)hk * p.dim + d0, x);
+    if (live) seq = p.row_seq[row], slot = p.row_slot[row], pos = p.row_pos[row];
+    const bool rotated = gl * 8 < p.rot;
+    const int a0 = !NEOX || !rotated ? gl * 8 : gl * 4, b0 = !NEOX || !rotated ? a0 + 4 : p.rot / 2 + gl * 4; // the lane's two runs
+    using Raw = typename Io<X>::Raw;
+    Raw ra[HPG], rb[HPG];
+    {
+        const X *src = (const X *)(kind == 0 ? p.q : (kind == 1 ? p.k : p.v)) + row * (kind == 0 ? p.q_stride : (kind == 1 ? p.k_stride : p.v_stride)) + head0 * p.dim;
+#pragma unroll
+        for (int u = 0; u < HPG; ++u) {
+            ra[u] = rb[u] = Raw();
+            if (mine && u < heads) ra[u] = raw4(src + u * p.dim + a0), rb[u] = raw4(src + u * p.dim + b0);
+        }
     }
     // where the row goes; a row with a position or page outside is left out as a whole
-    int page = 0;
+    int page = 0, at = 0;
     if (seq >= 0) {
         const bool ok = seq < p.n_table && slot >= 0 && slot < (long long)p.max_blocks * p.page_size;
-        if (ok) page = p.blocks[(size_t)seq * p.max_blocks + slot / p.page_size];
+        if (ok) {
+            const int block = slot / p.page_size;
+            page = p.blocks[(size_t)seq * p.max_blocks + block], at = slot - block * p.page_size;
+        }
         int bad = !ok ? ULLM_KV_FAULT_LEN : ((unsigned)page >= (unsigned)p.n_pages ? ULLM_KV_FAULT_PAGE : 0);
         if ((unsigned)pos >= (unsigned)p.n_pos) bad |= ULLM_KV_FAULT_POS;
         if (bad) {
-            if (head == 0 && gl == 0) set_fault(p.fault, bad);
+            if (g == 0 && gl == 0) set_fault(p.fault, bad);
             seq = -1;
         }
     }
     const bool write = mine && seq >= 0;
-    const float *const bias = is_q ? p.q_bias : (is_v ? p.v_bias : p.k_bias);
-    if (bias && mine) {
-        float b[8];
-        Io<float>::load(bias + (long long)hk * p.dim + d0, b);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] += b[e];
+    // the lane's four pairs' angles, as (first two, last two)
+    float2 c[2] = {{1.f, 1.f}, {1.f, 1.f}}, sn[2] = {{0.f, 0.f}, {0.f, 0.f}};
+    if (kind < 2 && write && rotated) {
+        const float4 *const t = (const float4 *)(p.rope + (size_t)pos * (p.rot / 2) + gl * 4);
+        const float4 u = t[0], v = t[1];
+        c[0] = make_float2(u.x, u.z), sn[0] = make_float2(u.y, u.w), c[1] = make_float2(v.x, v.z), sn[1] = make_float2(v.y, v.w);
     }
-    const float *const norm = is_q ? p.q_norm : p.k_norm;
-    float ss = 0.f;
+    const float *const norm = kind == 0 ? p.q_norm : (kind == 1 ? p.k_norm : nullptr);
+    const float *const bias = kind == 0 ? p.q_bias : (kind == 1 ? p.k_bias : p.v_bias);
+    float2 w[4] = {};
+    if (norm && mine) Io<float>::widen(raw4(norm + a0), w), Io<float>::widen(raw4(norm + b0), w + 2);
+    const float share = 1.0f / (float)p.dim;
+    Q *const q_dst = (Q *)p.q_out + row * p.q_out_stride + head0 * p.dim;
+    KV *const kv_dst = (KV *)(kind == 2 ? p.pv : p.pk) + page * p.page_stride + at * p.slot_stride + head0 * p.head_stride;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+    for (int u = 0; u < HPG; ++u) {
+        float2 x[4];
+        Io<X>::widen(ra[u], x), Io<X>::widen(rb[u], x + 2);
+        if (bias && mine && u < heads) {
+            float2 b[4];
+            Io<float>::widen(raw4(bias + (size_t)(head0 + u) * p.dim + a0), b), Io<float>::widen(raw4(bias + (size_t)(head0 + u) * p.dim + b0), b + 2);
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (norm && !is_v && mine) {
-        const float inv = 1.0f / sqrtf(ss / (float)p.dim + p.eps);
-        float w[8];
-        Io<float>::load(norm + d0, w);
+            for (int e = 0; e < 4; ++e) x[e].x += b[e].x, x[e].y += b[e].y;
+        }
+        if (norm) {
+            float2 sq = mul2(x[0], x[0]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * w[e];
-    }
-    const int half = p.rot / 2;
-    const float2 *const cs = p.rope + (size_t)(write ? pos : 0) * half;
-    const bool turn = write && !is_v && d0 < p.rot;
-    if (neox) {
-        const int hl = half / 8;                     // lanes per half
-        const bool first = gl < hl;
-        const int from = (threadIdx.x & 31) - gl + (first ? gl + hl : (gl < 2 * hl ? gl - hl : gl));
-        float y[8];
+            for (int e = 1; e < 4; ++e) sq = fma2(x[e], x[e], sq);
+            float ss = sq.x + sq.y;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], from);
-        if (turn) {
-            const int i0 = first ? d0 : d0 - half;
+            for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(group_lanes, ss, o);
+            const float inv = rsqrtf(ss * share + p.eps);
+            const float2 inv2 = make_float2(inv, inv);
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                const float4 c = *(const float4 *)(cs + i0 + e);
-                x[e] = first ? x[e] * c.x - y[e] * c.y : y[e] * c.y + x[e] * c.x;
-                x[e + 1] = first ? x[e + 1] * c.z - y[e + 1] * c.w : y[e + 1] * c.w + x[e + 1] * c.z;
+            for (int e = 0; e < 4; ++e) x[e] = mul2(mul2(x[e], inv2), w[e]);
+        }
+        if (kind < 2 && rotated) {
+            if (NEOX) { // x[0..1] and x[2..3] are the pairs' first and second values
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float2 a = x[e], b = x[2 + e], minus = make_float2(-sn[e].x, -sn[e].y);
+                    x[e] = fma2(b, minus, mul2(a, c[e])), x[2 + e] = fma2(b, c[e], mul2(a, sn[e]));
+                }
+            } else { // each x is a pair
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float ce = e & 1 ? c[e / 2].y : c[e / 2].x, se = e & 1 ? sn[e / 2].y : sn[e / 2].x;
+                    x[e] = make_float2(x[e].x * ce - x[e].y * se, x[e].x * se + x[e].y * ce);
+                }
             }
         }
-    } else if (turn) {
-#pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-            const float4 c = *(const float4 *)(cs + (d0 + e) / 2);
-            const float a0 = x[e], b0 = x[e + 1], a1 = x[e + 2], b1 = x[e + 3];
-            x[e] = a0 * c.x - b0 * c.y, x[e + 1] = a0 * c.y + b0 * c.x;
-            x[e + 2] = a1 * c.z - b1 * c.w, x[e + 3] = a1 * c.w + b1 * c.z;
-        }
-    }
-    if (!write) return;
-    if (is_q) {
-        Io<Q>::store((Q *)p.q_out + row * p.q_out_stride + (long long)hk * p.dim + d0, x);
-    } else {
-        KV *const pool = (KV *)(is_v ? p.pv : p.pk);
-        Io<KV>::store(pool + page * p.page_stride + (slot % p.page_size) * p.slot_stride + hk * p.head_stride + d0, x);
+        if (!write || u >= heads) continue;
+        if (kind == 0) put4(q_dst + u * p.dim + a0, x), put4(q_dst + u * p.dim + b0, x + 2);
+        else put4(kv_dst + u * p.head_stride + a0, x), put4(kv_dst + u * p.head_stride + b0, x + 2);
     }
 }
 
 template <typename X, typename Q, typename KV>
 cudaError_t launch_rope_l(const RopeDev &p, int neox, bool pdl, cudaStream_t st) {
-    const long long items = (long long)p.n_rows * (p.n_head + 2 * p.n_kv);
-    auto go = [&](auto kernel, int l) {
-        const int per = 256 / l;
-        return launch_kernel(kernel, dim3((unsigned)((items + per - 1) / per)), dim3(256), 0, st, pdl, p, neox);
+    const bool many = p.n_rows >= 256; // several waves of CTAs either way
+    auto go = [&](auto kernel, int l, int hpg) {
+        const long long items = (long long)p.n_rows * ((p.n_head + hpg - 1) / hpg + 2 * ((p.n_kv + hpg - 1) / hpg)), per = 256 / l;
+        return launch_kernel(kernel, dim3((unsigned)((items + per - 1) / per)), dim3(256), 0, st, pdl, p);
     };
-    if (p.dim <= 64) return go(qk_norm_rope_kernel<X, Q, KV, 8>, 8);
-    if (p.dim <= 128) return go(qk_norm_rope_kernel<X, Q, KV, 16>, 16);
-    return go(qk_norm_rope_kernel<X, Q, KV, 32>, 32);
+    auto with = [&](auto lanes) {
+        constexpr int L = decltype(lanes)::value, H = ROPE_HPG;
+        if (neox) return many ? go(qk_norm_rope_kernel<X, Q, KV, L, H, true>, L, H) : go(qk_norm_rope_kernel<X, Q, KV, L, 1, true>, L, 1);
+        return many ? go(qk_norm_rope_kernel<X, Q, KV, L, H, false>, L, H) : go(qk_norm_rope_kernel<X, Q, KV, L, 1, false>, L, 1);
+    };
+    if (p.dim <= 64) return with(std::integral_constant<int, 8>());
+    if (p.dim <= 128) return with(std::integral_constant<int, 16>());
+    return with(std::integral_constant<int, 32>());
 }
 // queries leave as the pages' type (for the tensor-core attention) or as f32
 template <typename X>
@@ -621,6 +641,12 @@ int table_check(ullm_cuda_ctx *c, const ullm_kv_pages *kv, const ullm_kv_table *
     out->blocks = t->d_blocks, out->len = t->d_len, out->refs = t->d_refs, out->fault = t->d_fault;
     out->n_seq = (int)t->n_seq, out->max_blocks = (int)t->max_blocks, out->work = (int *)t->d_work;
     return ULLM_OK;
+}
+
+// CTAs per entry for work on all matrices of a pool, so that about twelve CTAs of 128 threads fall on an SM
+unsigned mats_per_wave(const ullm_cuda_ctx *c, const PoolDev &pool, size_t n) {
+    const size_t mats = (size_t)pool.n_layer * 2, all = 12 * (size_t)c->dev.sm_count;
+    return (unsigned)std::min(mats, std::max((size_t)1, all / n));
 }
 
 } // namespace
@@ -667,7 +693,7 @@ int ullm_cuda_kv_accept_dev(ullm_cuda_ctx *c, const ullm_kv_pages *kv, const ull
     if (!n) return ULLM_OK;
     DeviceGuard guard(c->device);
     const cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
-    ULLM_CUDA_TRY(c, launch_kernel(kv_accept_move_kernel, dim3((unsigned)n, (unsigned)pool.n_layer * 2), dim3(128), 0, st, c->use_pdl, td, pool, d_seq, d_draft,
+    ULLM_CUDA_TRY(c, launch_kernel(kv_accept_move_kernel, dim3((unsigned)n, mats_per_wave(c, pool, n)), dim3(128), 0, st, c->use_pdl, td, pool, d_seq, d_draft,
                                    d_path, d_kept, (int)n, (int)max_path));
     ULLM_CUDA_TRY(c, launch_kernel(kv_accept_end_kernel, dim3((unsigned)n), dim3(128), 0, st, c->use_pdl, td, pool.page_size, pool.n_pages, d_seq, d_draft, d_kept));
     return ULLM_OK;
@@ -740,7 +766,7 @@ int ullm_cuda_qk_norm_rope_dev(ullm_cuda_ctx *c, const ullm_qk_norm_rope *a, voi
     for (const void *p : aligned)
         if ((uintptr_t)p % 16) return ctx_fail(c, ULLM_ERR_FORMAT, "norm weights, biases and the rotation table must be 16-byte aligned");
     const size_t items = a->n_rows * (a->n_head + 2 * a->kv->n_kv_head);
-    if (items / 8 >= (size_t)INT32_MAX) return ctx_fail(c, ULLM_ERR_FORMAT, "too many rows for one call");
+    if (items >= (size_t)INT32_MAX) return ctx_fail(c, ULLM_ERR_FORMAT, "too many rows for one call");
     if (!a->n_rows) return ULLM_OK;
     RopeDev p;
     p.q = (const uint8_t *)a->d_q, p.k = (const uint8_t *)a->d_k, p.v = (const uint8_t *)a->d_v, p.q_out = (uint8_t *)a->d_q_out;

@@ -4,9 +4,10 @@
 //
 // over the keys that row i sees, in one pass with a running maximum m, sum l and weighted sum of values, all f32.
 //
-// tree_attn_fma_kernel: f32 arithmetic on the CUDA cores, for f32 queries and for whatever the tensor-core kernel
-// (tree_attn_tc.cu) does not take.  A CTA of 256 threads holds 16 query rows and walks blocks of 64 keys that it has
-// widened to f32 in shared memory.
+// tree_attn_fma_kernel: f32 arithmetic on the CUDA cores, for f32 queries and for whatever the tensor-core kernel (tree_attn_tc.cu) does not take.
+// A CTA of 256 threads holds 16 or 32 query rows in shared memory and walks blocks of keys; the next block's keys and values arrive by cp.async, as they lie
+// in the pages, while one is worked on.  A warp's scores form a tile of 16 keys x 16 (or 8) rows, a thread's one of two keys x four (two) rows, so that
+// lanes share what they read from shared memory: with a key per lane these reads took three times as long as the multiply-adds.
 #include "engine.h"
 #include "tree_sched.cuh"
 
@@ -15,53 +16,55 @@
 
 namespace ullm {
 
-constexpr int FM = 16, FK = 64, FT = 256; // rows, keys of a block, threads
-constexpr int F_COST = 1, F_MIN = 2;       // places that a unit costs beside its blocks; places that a CTA takes at least
+constexpr int FT = 256;              // threads
+constexpr int F_COST = 1, F_MIN = 2; // places that a unit costs beside its blocks; places that a CTA takes at least
+constexpr int F_PER_SM = 2;          // CTAs on an SM at most: 128 registers a thread
+constexpr int FSP = 4;               // floats behind a row of queries and of scores, for the same
+constexpr int F_PAD = 16;            // bytes behind a key's row: 128-bit reads one row apart hit distinct banks
+// keys of a block, by the bytes of a row
+__host__ __device__ constexpr int fma_keys(int row_bytes) { return row_bytes <= 512 ? 64 : 32; }
 
-template <typename T> __device__ __forceinline__ void load8(const T *p, float (&o)[8]);
-template <> __device__ __forceinline__ void load8<float>(const float *p, float (&o)[8]) {
-    const float4 a = *(const float4 *)p, b = *(const float4 *)(p + 4);
-    o[0] = a.x, o[1] = a.y, o[2] = a.z, o[3] = a.w, o[4] = b.x, o[5] = b.y, o[6] = b.z, o[7] = b.w;
+// Four neighbouring values as f32
+__device__ __forceinline__ float4 widen4(const float *p) { return *(const float4 *)p; }
+__device__ __forceinline__ float4 widen4(const __half *p) {
+    const uint2 v = *(const uint2 *)p;
+    const float2 a = __half22float2(*(const __half2 *)&v.x), b = __half22float2(*(const __half2 *)&v.y);
+    return make_float4(a.x, a.y, b.x, b.y);
 }
-template <> __device__ __forceinline__ void load8<__half>(const __half *p, float (&o)[8]) {
-    const uint4 v = *(const uint4 *)p;
-    const __half2 *h = (const __half2 *)&v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(h[i]);
-        o[2 * i] = f.x, o[2 * i + 1] = f.y;
-    }
+__device__ __forceinline__ float4 widen4(const __nv_bfloat16 *p) {
+    const uint2 v = *(const uint2 *)p;
+    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
 }
-template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16 *p, float (&o)[8]) {
-    const uint4 v = *(const uint4 *)p;
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[2 * i] = __uint_as_float(w[i] << 16), o[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+__device__ __forceinline__ void copy16(void *dst, const void *src, bool on) { // zeros where it is off
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
 
-constexpr int fma_kp(int dim) { return dim + 4; } // padded key row: 128-bit reads one row apart hit distinct banks
-constexpr int FSP = FM + 4;                        // padded row of the transposed scores
-inline size_t fma_smem(int dim) { return sizeof(float) * ((size_t)FM * dim + (size_t)FK * fma_kp(dim) + (size_t)FK * dim + FK * FSP + 3 * FM); }
+// bytes of shared memory: queries, two stages of keys (padded) and values, scores, three numbers per row
+inline size_t fma_smem(int dim, int kv_bytes, int rows) {
+    const int keys = fma_keys(dim * kv_bytes);
+    return sizeof(float) * ((size_t)rows * (dim + FSP) + (size_t)rows * (keys + FSP) + 3 * rows) + 2 * (size_t)keys * (2 * dim * kv_bytes + F_PAD);
+}
 
-template <typename Q, typename KV> __global__ void __launch_bounds__(FT) tree_attn_fma_kernel(const TreeDev p) {
-    extern __shared__ __align__(16) float sm[];
-    const int D = p.dim, KP = fma_kp(D), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    float *const qs = sm, *const ks = qs + FM * D, *const vs = ks + FK * KP, *const sc = vs + FK * D, *const ms = sc + FK * FSP, *const ls = ms + FM,
-                *const cs = ls + FM;
+template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bounds__(FT, F_PER_SM) tree_attn_fma_kernel(const TreeDev p) {
+    extern __shared__ __align__(16) uint8_t fsm[];
+    constexpr int SP = KEYS + FSP, KS = KEYS / 32, RG = M / 4; // RG: groups of four rows
+    const int D = p.dim, QP = D + FSP, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row_b = D * (int)sizeof(KV), key_b = row_b + F_PAD;
+    float *const qs = (float *)fsm, *const sc = qs + M * QP, *const ms = sc + M * SP, *const ls = ms + M, *const cs = ls + M;
+    uint8_t *const stage0 = (uint8_t *)(cs + M);
+    const int stage_b = KEYS * (key_b + row_b);
     __shared__ Seg seg;
     pdl_wait_prior();
     pdl_launch_dependents();
-    Sched<FM, FK, F_COST, F_MIN> sched(p);
+    Sched<M, KEYS, F_COST, F_MIN> sched(p);
     bool some = false;
     if (warp == 0) {
         if (lane == 0) p.meta[blockIdx.x * TREE_META] = make_int4(-1, 0, 0, 0);
         __syncwarp();
         some = sched.init();
     }
-    // weighted sum of values: thread (key part, four rows, four values)
-    const int quads = D / 4, per = 4 * quads, split = per <= 64 ? 4 : (per <= 128 ? 2 : 1);
-    const int part = tid / per, item = tid % per, rg = item / quads, dq = item % quads;
-    const bool pv = part < split;
+    // weighted sums of values: items (four rows, four values), spread over the threads, each for a part of the keys
+    const int quads = D / 4, items = RG * quads, split = items <= FT / 4 ? 4 : (items <= FT / 2 ? 2 : 1), per = (items + FT - 1) / FT;
+    const int part = split > 1 ? tid / items : 0;
     for (;;) {
         __syncthreads();
         if (warp == 0) {
@@ -78,156 +81,222 @@ template <typename Q, typename KV> __global__ void __launch_bounds__(FT) tree_at
         const int rows = w.rows, key_end = w.key_end, blk_end = w.blk + w.count;
         auto token_of = [&](int r) { return (w.row0 + r) / p.group; };
         auto head_of = [&](int r) { return w.h * p.group + (w.row0 + r) % p.group; };
-        for (int i = tid; i < FM * D / 8; i += FT) {
-            const int r = i / (D / 8), d = i % (D / 8) * 8;
-            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (r < rows) load8<Q>((const Q *)p.q + (v.r0 + token_of(r)) * p.q_stride + (long long)head_of(r) * D + d, x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) qs[r * D + d + e] = x[e];
-        }
-        if (tid < FM) ms[tid] = -INFINITY, ls[tid] = 0.f;
-        float acc[4][4];
-#pragma unroll
-        for (int a = 0; a < 4; ++a)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[a][e] = 0.f;
         const int *const table = p.blocks + (size_t)v.id * p.max_blocks;
-        for (int blk = w.blk; blk < blk_end; ++blk) {
-            const int k0 = blk * FK;
-            __syncthreads();
-            for (int i = tid; i < FK * D / 8; i += FT) {
-                const int j = i / (D / 8), d = i % (D / 8) * 8, token = k0 + j;
-                float kk[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, vv[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (token < key_end) {
-                    const int page = table[token / p.page_size];
-                    if ((unsigned)page < (unsigned)p.n_pages) {
-                        const long long at = page * p.page_stride + token % p.page_size * p.slot_stride + w.h * p.head_stride + d;
-                        load8<KV>((const KV *)p.k + at, kk);
-                        load8<KV>((const KV *)p.v + at, vv);
-                    }
-                    if (token >= v.ctx) { // some rows may not see it: 0 * inf must not reach them
+        // 16-byte pieces of a block's keys and values; keys behind the last, and pages outside the pool, as zeros
+        const int pieces = row_b / 16, total = KEYS * pieces;
+        auto fetch = [&](int blk, uint8_t *stage) {
+            for (int i0 = tid; i0 < total; i0 += 4 * FT) { // four page numbers on their way at once
+                int page[4];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (!isfinite(vv[e])) vv[e] = 0.f, seg.odd = 1;
-                    }
+                for (int u = 0; u < 4; ++u) {
+                    const int token = blk * KEYS + (i0 + u * FT) / pieces;
+                    page[u] = i0 + u * FT < total && token < key_end ? table[token / p.page_size] : -1;
                 }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) ks[j * KP + d + e] = kk[e], vs[j * D + d + e] = vv[e];
+                for (int u = 0; u < 4; ++u) {
+                    const int i = i0 + u * FT, j = i / pieces, c = (i - j * pieces) * 16, token = blk * KEYS + j;
+                    if (i >= total) break;
+                    const bool on = (unsigned)page[u] < (unsigned)p.n_pages;
+                    const long long at = on ? (page[u] * p.page_stride + token % p.page_size * p.slot_stride + w.h * p.head_stride) * (long long)sizeof(KV) + c : 0;
+                    copy16(stage + j * key_b + c, p.k + at, on);
+                    copy16(stage + KEYS * key_b + j * row_b + c, p.v + at, on);
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        fetch(w.blk, stage0);
+        for (int i = tid; i < M * quads; i += FT) {
+            const int r = i / quads, d = i % quads * 4;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < rows) x = widen4((const Q *)p.q + (v.r0 + token_of(r)) * p.q_stride + (long long)head_of(r) * D + d);
+            *(float4 *)(qs + r * QP + d) = x;
+        }
+        if (tid < M) ms[tid] = -INFINITY, ls[tid] = 0.f;
+        float acc[2][4][4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int a = 0; a < 4; ++a)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[u][a][e] = 0.f;
+        for (int blk = w.blk; blk < blk_end; ++blk) {
+            uint8_t *const stage = stage0 + ((blk - w.blk) & 1) * stage_b;
+            const KV *const vs = (const KV *)(stage + KEYS * key_b);
+            const int k0 = blk * KEYS;
+            if (blk + 1 < blk_end) {
+                fetch(blk + 1, stage0 + ((blk + 1 - w.blk) & 1) * stage_b);
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+            } else {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
             }
             __syncthreads();
-            { // scores: thread (key, four rows)
-                const int j = tid % FK, r0 = tid / FK * 4;
-                if (r0 < rows) {
-                    float s[4] = {0.f, 0.f, 0.f, 0.f};
-                    for (int d = 0; d < D; d += 4) {
-                        const float4 k = *(const float4 *)(ks + j * KP + d);
+            if (k0 + KEYS > v.ctx) { // the rows' own tokens: some rows may not see them, and 0 * inf must not reach those
+                for (int i = tid; i < KEYS * D; i += FT) {
+                    KV *const at = (KV *)(stage + KEYS * key_b) + i;
+                    if (k0 + i / D >= v.ctx && !isfinite((float)*at)) *at = (KV)0.f, seg.odd = 1;
+                }
+            }
+            { // scores: warps (tile of 16 keys, tile of rows), lanes 8 x 4, a thread two keys eight apart and every fourth of its rows
+                constexpr int TILES = KEYS / 16, GROUPS = FT / 32 / TILES, R = M / GROUPS / 4;
+                const int j0 = warp % TILES * 16 + lane % 8, r0 = warp / TILES * (4 * R) + lane / 8;
+                if (warp / TILES * (4 * R) < rows) {
+                    float s[2][R];
 #pragma unroll
-                        for (int a = 0; a < 4; ++a) {
-                            const float4 q = *(const float4 *)(qs + (r0 + a) * D + d);
-                            s[a] += q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w;
+                    for (int a = 0; a < R; ++a) s[0][a] = s[1][a] = 0.f;
+                    const KV *const key0 = (const KV *)(stage + j0 * key_b), *const key1 = (const KV *)(stage + (j0 + 8) * key_b);
+#pragma unroll 4
+                    for (int d = 0; d < D; d += 4) {
+                        const float4 k0 = widen4(key0 + d), k1 = widen4(key1 + d);
+#pragma unroll
+                        for (int a = 0; a < R; ++a) {
+                            const float4 q = *(const float4 *)(qs + (r0 + 4 * a) * QP + d);
+                            s[0][a] += q.x * k0.x + q.y * k0.y + q.z * k0.z + q.w * k0.w;
+                            s[1][a] += q.x * k1.x + q.y * k1.y + q.z * k1.z + q.w * k1.w;
                         }
                     }
 #pragma unroll
-                    for (int a = 0; a < 4; ++a) {
-                        bool see = k0 + j < key_end && r0 + a < rows;
-                        if (see && k0 + j >= v.ctx) see = sees(p, v, token_of(r0 + a), k0 + j - v.ctx);
-                        sc[j * FSP + r0 + a] = see ? s[a] * p.scale_log2 : -INFINITY;
-                    }
+                    for (int a = 0; a < R; ++a)
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            const int r = r0 + 4 * a, j = j0 + 8 * b;
+                            bool see = k0 + j < key_end && r < rows;
+                            if (see && k0 + j >= v.ctx) see = sees(p, v, token_of(r), k0 + j - v.ctx);
+                            sc[r * SP + j] = see ? s[b][a] * p.scale_log2 : -INFINITY;
+                        }
                 }
             }
             __syncthreads();
             for (int r = warp; r < rows; r += FT / 32) {
-                const float s0 = sc[lane * FSP + r], s1 = sc[(lane + 32) * FSP + r], m = ms[r];
-                const float mn = fmaxf(m, warp_max(fmaxf(s0, s1)));
+                float s[KS], mn = -INFINITY, sum = 0.f;
+                const float m = ms[r];
+#pragma unroll
+                for (int k = 0; k < KS; ++k) s[k] = sc[r * SP + lane + 32 * k], mn = fmaxf(mn, s[k]);
+                mn = fmaxf(m, warp_max(mn));
                 // nothing seen so far: all weights are zero.  (A score of +inf or NaN gives NaN, as the formula does.)
-                const float p0 = s0 == -INFINITY ? 0.f : exp2f(s0 - mn), p1 = s1 == -INFINITY ? 0.f : exp2f(s1 - mn);
-                const float corr = m == -INFINITY ? 0.f : exp2f(m - mn), sum = warp_sum(p0 + p1);
-                sc[lane * FSP + r] = p0, sc[(lane + 32) * FSP + r] = p1;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    s[k] = s[k] == -INFINITY ? 0.f : exp2f(s[k] - mn);
+                    sum += s[k];
+                    sc[r * SP + lane + 32 * k] = s[k];
+                }
+                const float corr = m == -INFINITY ? 0.f : exp2f(m - mn);
+                sum = warp_sum(sum);
                 __syncwarp();
                 if (lane == 0) ms[r] = mn, ls[r] = ls[r] * corr + sum, cs[r] = corr;
             }
             __syncthreads();
-            if (pv && rg * 4 < rows) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int item = split > 1 ? tid % items : tid + u * FT, rg = item / quads, dq = item % quads;
+                if (u >= per || part >= split || item >= items || rg * 4 >= rows) continue;
 #pragma unroll
                 for (int a = 0; a < 4; ++a) {
                     const float corr = rg * 4 + a < rows ? cs[rg * 4 + a] : 0.f;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[a][e] *= corr;
+                    for (int e = 0; e < 4; ++e) acc[u][a][e] *= corr;
                 }
-                const int j0 = part * (FK / split), j1 = j0 + FK / split;
-                for (int j = j0; j < j1; ++j) {
-                    const float4 x = *(const float4 *)(vs + j * D + dq * 4), q = *(const float4 *)(sc + j * FSP + rg * 4);
-                    const float xs[4] = {x.x, x.y, x.z, x.w}, qq[4] = {q.x, q.y, q.z, q.w};
+                const int j0 = part * (KEYS / split), j1 = j0 + KEYS / split;
+#pragma unroll 2
+                for (int j = j0; j < j1; j += 4) {
+                    float4 q[4];
 #pragma unroll
-                    for (int a = 0; a < 4; ++a)
+                    for (int a = 0; a < 4; ++a) q[a] = *(const float4 *)(sc + (rg * 4 + a) * SP + j);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[a][e] += qq[a] * xs[e];
+                    for (int k = 0; k < 4; ++k) {
+                        const float4 x = widen4(vs + (j + k) * D + dq * 4);
+#pragma unroll
+                        for (int a = 0; a < 4; ++a) {
+                            const float wa = k == 0 ? q[a].x : (k == 1 ? q[a].y : (k == 2 ? q[a].z : q[a].w));
+                            acc[u][a][0] += wa * x.x, acc[u][a][1] += wa * x.y, acc[u][a][2] += wa * x.z, acc[u][a][3] += wa * x.w;
+                        }
+                    }
                 }
             }
+            __syncthreads(); // the stage and the scores are free
         }
-        __syncthreads();
-        // sum the key parts in order, in the keys' memory
-        float *const red = ks;
-        if (pv)
+        // sum the key parts in order, in the stages' memory
+        float *const red = (float *)stage0;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int item = split > 1 ? tid % items : tid + u * FT, rg = item / quads, dq = item % quads;
+            if (u >= per || part >= split || item >= items) continue;
 #pragma unroll
             for (int a = 0; a < 4; ++a)
-                if (rg * 4 + a < rows) *(float4 *)(red + ((size_t)part * FM + rg * 4 + a) * D + dq * 4) = make_float4(acc[a][0], acc[a][1], acc[a][2], acc[a][3]);
+                if (rg * 4 + a < rows) *(float4 *)(red + ((size_t)part * M + rg * 4 + a) * D + dq * 4) = make_float4(acc[u][a][0], acc[u][a][1], acc[u][a][2], acc[u][a][3]);
+        }
         __syncthreads();
         const bool whole = w.flags & 1, odd = seg.odd;
-        float *const mine = whole ? nullptr : part_of<FM>(p, blockIdx.x, w.flags >> 1);
-        for (int i = tid; i < rows * D; i += FT) {
-            const int r = i / D, d = i % D;
-            float o = 0.f;
-            for (int s = 0; s < split; ++s) o += red[((size_t)s * FM + r) * D + d];
+        float *const mine = whole ? nullptr : part_of<M>(p, blockIdx.x, w.flags >> 1);
+        for (int i = tid; i < rows * quads; i += FT) {
+            const int r = i / quads, d = (i - r * quads) * 4;
+            float4 o = *(const float4 *)(red + r * D + d);
+            for (int s = 1; s < split; ++s) {
+                const float4 x = *(const float4 *)(red + ((size_t)s * M + r) * D + d);
+                o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+            }
             if (odd) { // infinities and NaN of the tokens that the row does see
-                const int first = max(v.ctx, w.blk * FK), last = min(key_end, blk_end * FK), me = token_of(r);
+                const int first = max(v.ctx, w.blk * KEYS), last = min(key_end, blk_end * KEYS), me = token_of(r);
                 for (int token = first; token < last; ++token) {
                     const int page = table[token / p.page_size];
                     if ((unsigned)page >= (unsigned)p.n_pages || !sees(p, v, me, token - v.ctx)) continue;
-                    const long long at = page * p.page_stride + token % p.page_size * p.slot_stride + w.h * p.head_stride + d;
-                    const float x = (float)((const KV *)p.v)[at];
-                    if (!isfinite(x)) o += x;
+                    const float4 x = widen4((const KV *)p.v + page * p.page_stride + token % p.page_size * p.slot_stride + w.h * p.head_stride + d);
+                    if (!isfinite(x.x)) o.x += x.x;
+                    if (!isfinite(x.y)) o.y += x.y;
+                    if (!isfinite(x.z)) o.z += x.z;
+                    if (!isfinite(x.w)) o.w += x.w;
                 }
             }
             if (whole) {
-                const float l = ls[r];
-                ((Q *)p.out)[(v.r0 + token_of(r)) * p.out_stride + (long long)head_of(r) * D + d] = out_from<Q>(l == 0.f ? 0.f : o / l);
+                const float l = ls[r], inv = l == 0.f ? 0.f : 1.0f / l;
+                Q *const out = (Q *)p.out + (v.r0 + token_of(r)) * p.out_stride + (long long)head_of(r) * D + d;
+                const float y[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) out[e] = out_from<Q>(l == 0.f ? 0.f : y[e] * inv);
             } else {
-                mine[i] = o;
+                *(float4 *)(mine + (size_t)r * D + d) = o;
             }
         }
-        if (!whole && tid < rows) *(float2 *)(mine + (size_t)FM * D + 2 * tid) = make_float2(ms[tid], ls[tid]);
+        if (!whole && tid < rows) *(float2 *)(mine + (size_t)M * D + 2 * tid) = make_float2(ms[tid], ls[tid]);
     }
 }
 
 // CTAs of the f32 kernel: as many as the SMs hold at once
-static int fma_ctas(int sm_count, int dim) { return sm_count * (dim <= 64 ? 4 : (dim <= 128 ? 2 : 1)); }
+static int fma_ctas(const DeviceInfo &dev, int dim, int kv_bytes, int rows) {
+    const size_t one = fma_smem(dim, kv_bytes, rows) + 1024 + 256; // what the system and the static variables take
+    return dev.sm_count * (int)std::max((size_t)1, std::min((size_t)F_PER_SM, (size_t)dev.max_smem_sm / one));
+}
 static size_t meta_bytes(int ctas) { return ((size_t)ctas * TREE_META * sizeof(int4) + 255) / 256 * 256; }
+constexpr int F_ROWS = 32; // rows of the larger tile
 
+template <typename Q, typename KV, int M, int KEYS> static cudaError_t launch_fma_as(const DeviceInfo &dev, const TreeDev &t, bool pdl, cudaStream_t st) {
+    const size_t smem = fma_smem(t.dim, sizeof(KV), M);
+    cudaError_t e = cudaFuncSetAttribute(tree_attn_fma_kernel<Q, KV, M, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, dev.max_smem_optin - 1024);
+    if (e != cudaSuccess) return e;
+    const int ctas = fma_ctas(dev, t.dim, sizeof(KV), M);
+    e = launch_kernel(tree_attn_fma_kernel<Q, KV, M, KEYS>, dim3(ctas), dim3(FT), smem, st, pdl, t);
+    if (e != cudaSuccess) return e;
+    return launch_kernel(tree_join_kernel<Q, M>, dim3(dev.sm_count * JOIN_PER_SM), dim3(32 * JOIN_WARPS), 0, st, pdl, t, ctas);
+}
 template <typename Q, typename KV> static cudaError_t launch_fma(const DeviceInfo &dev, const TreeDev &t, bool pdl, cudaStream_t st) {
-    const size_t smem = fma_smem(t.dim);
-    cudaError_t e = cudaFuncSetAttribute(tree_attn_fma_kernel<Q, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)fma_smem(256));
-    if (e != cudaSuccess) return e;
-    const int ctas = fma_ctas(dev.sm_count, t.dim);
-    e = launch_kernel(tree_attn_fma_kernel<Q, KV>, dim3(ctas), dim3(FT), smem, st, pdl, t);
-    if (e != cudaSuccess) return e;
-    return launch_kernel(tree_join_kernel<Q, FM>, dim3(dev.sm_count * JOIN_PER_SM), dim3(32 * JOIN_WARPS), 0, st, pdl, t, ctas);
+    const bool wide = ((long long)t.n_rows * t.group + t.n_seq - 1) / t.n_seq > 16; // rows per sequence and key head, on average
+    if (fma_keys(t.dim * (int)sizeof(KV)) == 64) return wide ? launch_fma_as<Q, KV, F_ROWS, 64>(dev, t, pdl, st) : launch_fma_as<Q, KV, 16, 64>(dev, t, pdl, st);
+    return wide ? launch_fma_as<Q, KV, F_ROWS, 32>(dev, t, pdl, st) : launch_fma_as<Q, KV, 16, 32>(dev, t, pdl, st);
 }
 
 } // namespace ullm
 
 using namespace ullm;
 
-static size_t tree_work_bytes(int sm_count, int dim, bool tc) {
-    const int ctas = fma_ctas(sm_count, dim);
-    const size_t fma = sizeof(float) * (size_t)ctas * 2 * FM * (dim + 2);
-    return meta_bytes(ctas) + (tc ? std::max(fma, tree_attn_tc_work(sm_count, dim)) : fma);
+// The work area begins with the CTAs' records (for the most CTAs of any kernel), then the partial results.
+static size_t tree_work_bytes(const DeviceInfo &dev, int dim, bool tc) {
+    const size_t fma = sizeof(float) * (size_t)dev.sm_count * F_PER_SM * 2 * F_ROWS * (dim + 2);
+    return meta_bytes(dev.sm_count * F_PER_SM) + (tc ? std::max(fma, tree_attn_tc_work(dev.sm_count, dim)) : fma);
 }
 
 size_t ullm_cuda_tree_attn_work_bytes(const ullm_cuda_ctx *c, const ullm_kv_pages *kv, int dtype) {
     PoolDev pool;
     if (!c || !kv || pool_check(kv, &pool)) return 0;
-    return tree_work_bytes(c->dev.sm_count, pool.head_dim, tree_attn_tc_supported(pool, dtype));
+    return tree_work_bytes(c->dev, pool.head_dim, tree_attn_tc_supported(pool, dtype));
 }
 
 int ullm_cuda_tree_attn_dev(ullm_cuda_ctx *c, const ullm_tree_attn *a, void *stream) {
@@ -257,7 +326,7 @@ int ullm_cuda_tree_attn_dev(ullm_cuda_ctx *c, const ullm_tree_attn *a, void *str
         return ctx_fail(c, ULLM_ERR_FORMAT, "scale must be finite, at least 1e-30 or 0 for the default");
     { // the line of all blocks is counted in 32 bits (with what the smaller tiles of the f32 kernel would need)
         const double units = ((double)a->n_rows * (a->n_head / a->kv->n_kv_head) / 16 + (double)a->n_seq) * a->kv->n_kv_head;
-        if (units * ((double)a->max_blocks * a->kv->page_size / 64 + 4) > 2147483000.0)
+        if (units * ((double)a->max_blocks * a->kv->page_size / 32 + 4) > 2147483000.0)
             return ctx_fail(c, ULLM_ERR_FORMAT, "rows times table size too large for one call: split the rows");
     }
     if (!a->n_rows || !a->n_seq) return ULLM_OK;
@@ -276,7 +345,7 @@ int ullm_cuda_tree_attn_dev(ullm_cuda_ctx *c, const ullm_tree_attn *a, void *str
     t.scale_log2 = (float)((a->scale == 0.f ? 1.0 / std::sqrt((double)dim) : (double)a->scale) * 1.4426950408889634);
     DeviceGuard guard(c->device);
     const cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
-    t.meta = (int4 *)a->d_work, t.part = (float *)((uint8_t *)a->d_work + meta_bytes(fma_ctas(c->dev.sm_count, t.dim)));
+    t.meta = (int4 *)a->d_work, t.part = (float *)((uint8_t *)a->d_work + meta_bytes(c->dev.sm_count * F_PER_SM));
     cudaError_t e = cudaErrorNotSupported;
     if (tree_attn_tc_supported(pool, a->dtype)) e = launch_tree_attn_tc(c->dev, pool, a->dtype, t, c->d_status, c->use_pdl, st);
     if (e != cudaErrorNotSupported) { // (strides that a tensor map cannot describe go to the f32 kernel)

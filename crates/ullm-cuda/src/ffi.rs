@@ -40,6 +40,7 @@ pub const ULLM_SHARD_HANDLE_BYTES: usize = 64;
 pub const ULLM_SHARD_MAX_RANKS: usize = 8;
 pub const ULLM_SHARD_NCCL_ID_BYTES: usize = 128;
 pub const ULLM_CUDA_MOE_NOALLOC_SCRATCH_BYTES: usize = 4194304;
+pub const ULLM_FORWARD_VERIFY_MAX: c_int = 64;
 pub const ULLM_OK: c_int = 0;
 pub const ULLM_ERR_UNSUPPORTED: c_int = 1;
 pub const ULLM_ERR_FORMAT: c_int = 2;
@@ -439,6 +440,8 @@ extern "C" {
     pub fn ullm_cuda_forward_set_kv(f: *mut ullm_cuda_fwd, pos0: usize, n: usize, k: *const f32, v: *const f32) -> c_int;
     pub fn ullm_cuda_forward_supports_batched_prefill(f: *const ullm_cuda_fwd) -> c_int;
     pub fn ullm_cuda_forward_batch(f: *mut ullm_cuda_fwd, embeds: *const f32, s: usize, logits: *mut f32) -> c_int;
+    pub fn ullm_cuda_forward_verify(f: *mut ullm_cuda_fwd, embeds: *const f32, parents: *const i32, n: usize, pos: usize, logits: *mut f32) -> c_int;
+    pub fn ullm_cuda_forward_accept(f: *mut ullm_cuda_fwd, pos: usize, n: usize, path: *const i32, kept: usize) -> c_int;
     pub fn ullm_cuda_forward_greedy(f: *mut ullm_cuda_fwd, embd_table: *const ullm_cuda_buf, embd_dtype: c_int, first_token: u32, pos: usize, n: usize, tokens_out: *mut u32) -> c_int;
     pub fn ullm_cuda_forward_greedy_weight(f: *mut ullm_cuda_fwd, embd_table: *const ullm_cuda_weight, first_token: u32, pos: usize, n: usize, tokens_out: *mut u32) -> c_int;
     pub fn ullm_gguf_open(path: *const c_char, out: *mut *mut ullm_gguf, err: *mut c_char, err_cap: usize) -> c_int;

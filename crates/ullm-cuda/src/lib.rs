@@ -392,6 +392,25 @@ impl GpuForward {
         check(rc, self.ctx.raw).map(|_| logits)
     }
 
+    /// A tree of drafted tokens in one pass (speculative decoding; no counterpart in the reference): `embeds` is `[n, n_embd]`,
+    /// `parents[i]` the index of the token that token `i` follows, -1 for the one at `pos - 1`; `None` is a chain.  Returns `[n, vocab]`.
+    pub fn verify(&self, embeds: &[f32], parents: Option<&[i32]>, pos: usize) -> Result<Vec<f32>> {
+        let n = embeds.len() / self.n_embd;
+        assert_eq!(embeds.len(), n * self.n_embd);
+        if let Some(p) = parents {
+            assert_eq!(p.len(), n);
+        }
+        let mut logits = vec![0.0f32; n * self.vocab];
+        let par = parents.map_or(ptr::null(), |p| p.as_ptr());
+        let rc = unsafe { ffi::ullm_cuda_forward_verify(self.raw, embeds.as_ptr(), par, n, pos, logits.as_mut_ptr()) };
+        check(rc, self.ctx.raw).map(|_| logits)
+    }
+
+    /// Of the `n` tokens of the last `verify` at `pos` those at the increasing indices `path` stay, as positions `pos..pos + path.len()`.
+    pub fn accept(&self, pos: usize, n: usize, path: &[i32]) -> Result<()> {
+        check(unsafe { ffi::ullm_cuda_forward_accept(self.raw, pos, n, path.as_ptr(), path.len()) }, self.ctx.raw)
+    }
+
     /// The numbers behind `forward_debug`: layer 0 one op at a time.
     pub fn forward_debug_stats(&self, x_init: &[f32], pos: usize) -> Result<Vec<DebugStat>> {
         let mut raw = vec![ffi::ullm_debug_stat { label: [0; 16], nan: 0, inf: 0, maxabs: 0.0 }; 32];

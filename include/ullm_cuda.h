@@ -589,6 +589,16 @@ int ullm_cuda_forward_supports_batched_prefill(const ullm_cuda_fwd *f);
  * LAST token's logits [vocab].  The projections run as bf16 tensor-core GEMMs, so logits
  * agree with s calls of ullm_cuda_forward to the bf16 tolerance (2e-2), not to 1e-3. */
 int ullm_cuda_forward_batch(ullm_cuda_fwd *f, const float *embeds, size_t s, float *logits);
+/* Speculative decoding over the resident model (no counterpart in the reference): a tree of `n` drafted tokens (at most
+ * ULLM_FORWARD_VERIFY_MAX) through every layer in one pass.  Token i has the embedding embeds[i] ([n, n_embd]) and follows token parents[i]
+ * of the tree, an earlier one, or -1 = the token at pos - 1 (parents NULL: a chain); it sees positions 0 .. pos - 1,
+ * its ancestors and itself.  logits [n, vocab].  The tokens' K and V are left at cache slots pos .. pos + n - 1 in the
+ * order given; _accept keeps those with the (increasing) indices path[0 .. kept) as positions pos .. pos + kept - 1, after which
+ * ullm_cuda_forward, _verify and _greedy go on at pos + kept.  From eight tokens on, the projections of models that support the batched prefill run
+ * as bf16 tensor-core GEMMs (tolerance 2e-2, as in ullm_cuda_forward_batch); otherwise they are the decode step's matvecs (1e-3). */
+#define ULLM_FORWARD_VERIFY_MAX 64
+int ullm_cuda_forward_verify(ullm_cuda_fwd *f, const float *embeds, const int32_t *parents, size_t n, size_t pos, float *logits);
+int ullm_cuda_forward_accept(ullm_cuda_fwd *f, size_t pos, size_t n, const int32_t *path, size_t kept);
 /* Greedy continuation kept on the device: runs `n` decode steps starting from
  * token embedding lookups of `embd_table` (dtype rows, resident) — argmax
  * (sample.rs:125-133, first index wins) feeds the next step without a host

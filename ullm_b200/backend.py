@@ -128,6 +128,8 @@ SIGNATURES = {
     "ullm_cuda_forward_set_kv": (_i, [_vp, _sz, _sz, _vp, _vp]),
     "ullm_cuda_forward_debug": (_i, [_vp, _vp, _sz, _vp, _sz, C.POINTER(_sz)]),
     "ullm_cuda_forward_supports_batched_prefill": (_i, [_vp]),
+    "ullm_cuda_forward_verify": (_i, [_vp, _vp, _vp, _sz, _sz, _vp]),
+    "ullm_cuda_forward_accept": (_i, [_vp, _sz, _sz, _vp, _sz]),
     "ullm_cuda_forward_greedy": (_i, [_vp, _vp, _i, C.c_uint32, _sz, _sz, _vp]),
     "ullm_cuda_forward_greedy_weight": (_i, [_vp, _vp, C.c_uint32, _sz, _sz, _vp]),
 }
@@ -938,6 +940,22 @@ class GpuForward:
         out = np.empty(self.params["vocab"], np.float32)
         self._ctx._check(self._ctx._lib.ullm_cuda_forward_batch(self._h, _ptr(e), s, _ptr(out)))
         return out
+
+    def verify(self, embeds, pos: int, parents=None) -> np.ndarray:
+        """A tree of drafted tokens in one pass: ``embeds`` [n, n_embd], ``parents[i]`` the index of the token that token ``i``
+        follows (-1: the one at ``pos - 1``; ``None``: a chain); returns the logits of every token [n, vocab]."""
+        e = _f32(embeds)
+        n = e.shape[0]
+        par = None if parents is None else np.ascontiguousarray(parents, np.int32)
+        out = np.empty((n, self.params["vocab"]), np.float32)
+        self._ctx._check(self._ctx._lib.ullm_cuda_forward_verify(self._h, _ptr(e), _ptr(par), n, pos, _ptr(out)))
+        return out
+
+    def accept(self, pos: int, n: int, path):
+        """Of the ``n`` tokens of the last :meth:`verify` at ``pos`` those with the increasing indices ``path`` stay, as positions
+        ``pos`` .. ``pos + len(path) - 1``."""
+        p = np.ascontiguousarray(path, np.int32)
+        self._ctx._check(self._ctx._lib.ullm_cuda_forward_accept(self._h, pos, n, _ptr(p), p.size))
 
     def supports_batched_prefill(self) -> bool:
         return bool(self._ctx._lib.ullm_cuda_forward_supports_batched_prefill(self._h))

@@ -1104,6 +1104,26 @@ int ullm_cuda_forward_batch(ullm_cuda_fwd *f, const float *embeds, size_t s, flo
     return fwd_status(f);
 }
 
+int ullm_cuda_forward_verify(ullm_cuda_fwd *f, const float *embeds, const int32_t *parents, size_t n, size_t pos, float *logits) {
+    if (!f || !embeds || !logits) return ULLM_ERR_INVALID;
+    if (n == 0 || n > Forward::MAX_VERIFY) return ctx_fail(f->ctx, ULLM_ERR_FORMAT, "a tree has 1 to %zu tokens, not %zu", Forward::MAX_VERIFY, n);
+    if (pos > f->f.P.n_ctx || n > f->f.P.n_ctx - pos) return ctx_fail(f->ctx, ULLM_ERR_FORMAT, "positions beyond the context");
+    for (size_t i = 0; parents && i < n; ++i)
+        if (parents[i] < -1 || parents[i] >= (int64_t)i) return ctx_fail(f->ctx, ULLM_ERR_FORMAT, "token %zu of the tree follows token %d", i, parents[i]);
+    const int rc = f->f.verify(f->ctx, embeds, parents, n, pos, logits);
+    return rc ? rc : fwd_status(f);
+}
+
+int ullm_cuda_forward_accept(ullm_cuda_fwd *f, size_t pos, size_t n, const int32_t *path, size_t kept) {
+    if (!f || (kept && !path)) return ULLM_ERR_INVALID;
+    if (n == 0 || n > Forward::MAX_VERIFY || kept > n) return ctx_fail(f->ctx, ULLM_ERR_FORMAT, "%zu of %zu tokens kept", kept, n);
+    if (pos > f->f.P.n_ctx || n > f->f.P.n_ctx - pos) return ctx_fail(f->ctx, ULLM_ERR_FORMAT, "positions beyond the context");
+    for (size_t j = 0; j < kept; ++j)
+        if (path[j] < (j ? path[j - 1] + 1 : 0) || (size_t)path[j] >= n) return ctx_fail(f->ctx, ULLM_ERR_FORMAT, "the kept tokens' indices must increase and be below %zu", n);
+    if (!kept) return ULLM_OK;
+    return f->f.accept(f->ctx, pos, n, path, kept);
+}
+
 int ullm_cuda_forward_greedy(ullm_cuda_fwd *f, const ullm_cuda_buf *embd, int embd_dtype, uint32_t first_token, size_t pos,
                              size_t n, uint32_t *tokens_out) {
     if (!f || !embd || (n && !tokens_out)) return ULLM_ERR_INVALID;

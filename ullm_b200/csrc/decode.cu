@@ -529,6 +529,8 @@ Forward::~Forward() {
     if (h_pin) cudaFreeHost(h_pin);
     if (h_x) cudaFreeHost(h_x);
     if (h_logits) cudaFreeHost(h_logits);
+    if (h_vints) cudaFreeHost(h_vints);
+    if (h_vx) cudaFreeHost(h_vx);
     if (h_status) cudaFreeHost((void *)h_status);
     if (stream) cudaStreamDestroy(stream);
 }

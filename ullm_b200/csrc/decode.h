@@ -1,6 +1,7 @@
 // Resident dense-Llama decode engine (see decode.cu).
 #pragma once
 
+#include "../../include/ullm_cuda.h"
 #include "common.cuh"
 #include "kernels.h"
 
@@ -109,6 +110,20 @@ struct Forward {
     // logits of the last token
     bool batch_supported() const;
     cudaError_t forward_batch(const float *embeds_host, size_t s, float *logits_host);
+    // A tree of up to MAX_VERIFY drafted tokens behind position `pos` through every layer in one pass: logits of every node [n][vocab]; the
+    // drafts' K and V lie in the cache at pos .. pos + n - 1 afterwards.  accept() moves those of `path` up behind pos.
+    // Return ULLM_* codes.  From VERIFY_GEMM_MIN tokens on the projections run as tensor-core GEMMs (bf16 operands) where
+    // forward_batch is available; below, and for other models, as the decode step's matvecs.
+    static constexpr size_t MAX_VERIFY = 64, VERIFY_GEMM_MIN = 8;
+    int verify(ullm_cuda_ctx *c, const float *embeds, const int32_t *parents, size_t n, size_t pos, float *logits_host);
+    int accept(ullm_cuda_ctx *c, size_t pos, size_t n, const int32_t *path, size_t kept);
+    ullm_kv_pages pages() const;
+    float *vx = nullptr, *vxn = nullptr, *vqkv = nullptr, *vattn = nullptr, *vlogits = nullptr, *vrouter = nullptr;
+    int32_t *vints = nullptr, *h_vints = nullptr;
+    float *h_vx = nullptr;
+    void *vwork = nullptr, *vtable = nullptr, *vscratch = nullptr;
+    size_t vwork_bytes = 0, vtable_bytes = 0;
+    bool vready = false;
     float *bx = nullptr, *bxn = nullptr, *bqk = nullptr, *bv = nullptr, *bh = nullptr;
     void *bscratch = nullptr;
     // mixture-of-experts step: router logits, experts' output, routing scratch; tmpn / tmpo serve the
@@ -119,6 +134,8 @@ struct Forward {
     MlxTables embd_mlx; // tables of the embedding matrix when greedy() is given an MLX 4-bit one (embd_dtype 1000)
 
   private:
+    cudaError_t batch_buffers();
+    cudaError_t verify_buffers(ullm_cuda_ctx *c);
     cudaError_t dev_alloc(void **out, size_t bytes);
     cudaError_t upload(const void *host, size_t bytes, void **out);
     cudaError_t upload_rows(const void *bytes, int fmt, size_t out_dim, size_t cols, Mat *out);

@@ -8,7 +8,11 @@
 // [gate|up] GEMM with silu(g)*u in its epilogue -> W_down GEMM + residual (epilogue).  Only the last token goes through
 // the final norm and the output projection (a matvec).  Prompts longer than PREFILL_CHUNK
 // tokens are processed in chunks; the attention reads earlier chunks from the cache.
+//
+// Below it: a tree of drafted tokens in one pass (the paged operators over the engine's cache), and the accepted rows kept.
 #include "decode.h"
+#include "engine.h"
+#include "paged.h"
 
 #include <cstring>
 
@@ -216,6 +220,27 @@ bool Forward::batch_supported() const {
     return P.head_dim == 64 || P.head_dim == 128;
 }
 
+// Activation buffers for one chunk, allocated on first use.
+cudaError_t Forward::batch_buffers() {
+    cudaError_t e;
+#define TRY(x) \
+    if ((e = (x)) != cudaSuccess) return e;
+    if (bscratch) return cudaSuccess;
+    const size_t hd = P.head_dim, qd = P.n_head * hd, kvd = P.n_kv_head * hd, E = P.n_embd, F = P.n_ff, B = PREFILL_CHUNK;
+    size_t scratch = 0;
+    for (const auto &d : {std::pair<size_t, size_t>{qd + kvd, E}, {kvd, E}, {E, qd}, {2 * F, E}, {E, F}})
+        for (size_t n = 1; n <= B; ++n) // the split-K factor, and with it the partial-sum area, depends on the token count
+            scratch = std::max(scratch, gemm_tc_scratch_bytes(d.first, d.second, n, dev.sm_count));
+    if (!bx) TRY(dev_alloc((void **)&bx, B * E * 4));
+    if (!bxn) TRY(dev_alloc((void **)&bxn, B * std::max(E, qd) * 4));
+    if (!bqk) TRY(dev_alloc((void **)&bqk, B * (qd + kvd) * 4));
+    if (!bv) TRY(dev_alloc((void **)&bv, B * kvd * 4));
+    if (!bh) TRY(dev_alloc((void **)&bh, B * F * 4));
+    TRY(dev_alloc(&bscratch, scratch));
+#undef TRY
+    return cudaSuccess;
+}
+
 cudaError_t Forward::forward_batch(const float *embeds_host, size_t s, float *logits_host) {
     cudaError_t e;
 #define TRY(x) \
@@ -223,20 +248,9 @@ cudaError_t Forward::forward_batch(const float *embeds_host, size_t s, float *lo
     TRY(cudaSetDevice(device));
     if (!batch_supported()) return cudaErrorNotSupported;
     if (s == 0 || s > P.n_ctx) return cudaErrorInvalidValue;
-    const size_t hd = P.head_dim, qd = P.n_head * hd, kvd = P.n_kv_head * hd, E = P.n_embd, F = P.n_ff, B = PREFILL_CHUNK;
+    const size_t hd = P.head_dim, qd = P.n_head * hd, kvd = P.n_kv_head * hd, E = P.n_embd, B = PREFILL_CHUNK;
     const size_t kvb = P.kv_f16 ? 2 : 4;
-    if (!bx) { // activation buffers for one chunk, allocated on first use
-        size_t scratch = 0;
-        for (const auto &d : {std::pair<size_t, size_t>{qd + kvd, E}, {kvd, E}, {E, qd}, {2 * F, E}, {E, F}})
-            for (size_t n = 1; n <= B; ++n) // the split-K factor, and with it the partial-sum area, depends on the token count
-                scratch = std::max(scratch, gemm_tc_scratch_bytes(d.first, d.second, n, dev.sm_count));
-        TRY(dev_alloc((void **)&bx, B * E * 4));
-        TRY(dev_alloc((void **)&bxn, B * std::max(E, qd) * 4));
-        TRY(dev_alloc((void **)&bqk, B * (qd + kvd) * 4));
-        TRY(dev_alloc((void **)&bv, B * kvd * 4));
-        TRY(dev_alloc((void **)&bh, B * F * 4));
-        TRY(dev_alloc(&bscratch, scratch));
-    }
+    TRY(batch_buffers());
     auto gemm = [&](const Mat &m, const float *in, float *out, size_t n, int epi = EPI_STORE, const float *res = nullptr) {
         ++launches;
         return launch_gemm_tc(m.fmt, m.w, in, out, bscratch, m.out, m.cols, n, dev.sm_count, d_status, stream, epi, res);
@@ -293,5 +307,200 @@ cudaError_t Forward::forward_batch(const float *embeds_host, size_t s, float *lo
     memcpy(logits_host, h_logits, P.vocab * 4);
     return cudaSuccess;
 }
+
+// ---------------------------------------------------------------------------------------------------------------
+// A tree of drafted tokens through every layer in one pass, against the cache (verify) and what is kept of it (accept)
+// ---------------------------------------------------------------------------------------------------------------
+// The engine's cache is the paged operators' pool with one page of n_ctx slots.
+ullm_kv_pages Forward::pages() const {
+    const size_t kvd = P.n_kv_head * P.head_dim;
+    ullm_kv_pages kv;
+    kv.dtype = P.kv_f16 ? ULLM_DTYPE_F16 : ULLM_DTYPE_F32, kv.n_layer = P.n_layer, kv.n_pages = 1, kv.page_size = P.n_ctx;
+    kv.n_kv_head = P.n_kv_head, kv.head_dim = P.head_dim, kv.d_k = kcache, kv.d_v = vcache;
+    kv.layer_stride = kv.page_stride = P.n_ctx * kvd, kv.slot_stride = kvd, kv.head_stride = P.head_dim;
+    return kv;
+}
+
+// Device and page-locked int32 arrays of a tree step: table {block 0, length, count, fault, row 0, drafts, kept}, rows' offsets, parents,
+// path, and per row sequence, slot, position and the bits of its ancestors.
+namespace {
+constexpr size_t VN = Forward::MAX_VERIFY, VW = VN / 32;
+enum : size_t { V_BLOCK = 0, V_LEN = 1, V_REFS = 2, V_FAULT = 3, V_ROW = 4, V_DRAFT = 5, V_KEPT = 6, V_CU = 8, V_PARENT = 16, V_PATH = V_PARENT + VN, V_IN = V_PATH + VN,
+               V_SEQ = V_IN, V_SLOT = V_SEQ + VN, V_POS = V_SLOT + VN, V_MASK = V_POS + VN, V_INTS = V_MASK + VN * VW };
+}
+
+cudaError_t Forward::verify_buffers(ullm_cuda_ctx *c) {
+    cudaError_t e;
+#define TRY(x) \
+    if ((e = (x)) != cudaSuccess) return e;
+    if (vready) return cudaSuccess;
+    const size_t qd = P.n_head * P.head_dim, kvd = P.n_kv_head * P.head_dim;
+    const ullm_kv_pages kv = pages();
+    vwork_bytes = ullm_cuda_tree_attn_work_bytes(c, &kv, ULLM_DTYPE_F32), vtable_bytes = ullm_cuda_kv_work_bytes(1, 1);
+    if (!vx) TRY(dev_alloc((void **)&vx, VN * P.n_embd * 4));
+    if (!vxn) TRY(dev_alloc((void **)&vxn, VN * P.n_embd * 4));
+    if (!vqkv) TRY(dev_alloc((void **)&vqkv, VN * (qd + 2 * kvd) * 4));
+    if (!vattn) TRY(dev_alloc((void **)&vattn, VN * qd * 4));
+    if (!vlogits) TRY(dev_alloc((void **)&vlogits, VN * P.vocab * 4));
+    if (P.n_experts && !vrouter) TRY(dev_alloc((void **)&vrouter, VN * P.n_experts * 4));
+    if (!vints) TRY(dev_alloc((void **)&vints, V_INTS * 4));
+    if (!vwork) TRY(dev_alloc(&vwork, vwork_bytes));
+    if (!vtable) TRY(dev_alloc(&vtable, vtable_bytes));
+    if (!h_vints) TRY(cudaHostAlloc((void **)&h_vints, V_IN * 4, cudaHostAllocDefault));
+    if (!h_vx) TRY(cudaHostAlloc((void **)&h_vx, VN * std::max(P.n_embd, P.vocab) * 4, cudaHostAllocDefault));
+    if (batch_supported()) {
+        TRY(batch_buffers());
+        if (gemm_tc_supported(output.fmt, output.out, output.cols, 1)) {
+            size_t bytes = 0;
+            for (size_t n = 1; n <= VN; ++n) bytes = std::max(bytes, gemm_tc_scratch_bytes(output.out, output.cols, n, dev.sm_count));
+            if (!vscratch) TRY(dev_alloc(&vscratch, bytes));
+        }
+    }
+    vready = true;
+#undef TRY
+    return cudaSuccess;
+}
+
+int Forward::verify(ullm_cuda_ctx *c, const float *embeds, const int32_t *parents, size_t n, size_t pos, float *logits_host) {
+    auto fail = [&](cudaError_t err) {
+        cudaGetLastError();
+        if (err == cudaErrorNotSupported) return ctx_fail(c, ULLM_ERR_UNSUPPORTED, "a layer shape is outside the fused decode path");
+        return ctx_fail(c, err == cudaErrorMemoryAllocation ? ULLM_ERR_OOM : ULLM_ERR_CUDA, "verifying a tree: %s", cudaGetErrorString(err));
+    };
+    cudaError_t e;
+    int rc;
+#define TRY(x) \
+    if ((e = (x)) != cudaSuccess) return fail(e);
+    TRY(cudaSetDevice(device));
+    TRY(verify_buffers(c));
+    const size_t hd = P.head_dim, qd = P.n_head * hd, kvd = P.n_kv_head * hd, E = P.n_embd;
+    const bool gemms = n >= VERIFY_GEMM_MIN && batch_supported();
+    memset(h_vints, 0, V_PARENT * 4);
+    h_vints[V_LEN] = (int)(pos + n), h_vints[V_CU + 1] = (int)n;
+    for (size_t i = 0; i < n; ++i) h_vints[V_PARENT + i] = parents ? parents[i] : (int)i - 1;
+    memcpy(h_vx, embeds, n * E * 4);
+    TRY(cudaMemcpyAsync(vints, h_vints, V_PATH * 4, cudaMemcpyHostToDevice, stream));
+    float *const xs = gemms ? bx : vx;
+    TRY(cudaMemcpyAsync(xs, h_vx, n * E * 4, cudaMemcpyHostToDevice, stream));
+    if ((rc = ullm_cuda_tree_plan_dev(c, n, 1, vints + V_CU, vints + V_LEN, nullptr, 1, vints + V_PARENT, vints + V_SEQ, vints + V_SLOT, vints + V_POS,
+                                      (uint32_t *)vints + V_MASK, VW, vints + V_FAULT, stream)))
+        return rc;
+    const ullm_kv_pages kv = pages();
+    ullm_qk_norm_rope ro;
+    memset(&ro, 0, sizeof ro);
+    ro.kv = &kv, ro.x_dtype = ro.q_dtype = ULLM_DTYPE_F32, ro.n_rows = n, ro.n_head = P.n_head, ro.eps = P.eps, ro.d_rope = (const float *)rope, ro.n_pos = P.n_ctx;
+    ro.neox = P.rope_neox, ro.d_row_seq = vints + V_SEQ, ro.d_row_slot = vints + V_SLOT, ro.d_row_pos = vints + V_POS, ro.d_blocks = vints + V_BLOCK;
+    ro.n_table = ro.max_blocks = 1, ro.d_fault = vints + V_FAULT;
+    ullm_tree_attn at;
+    memset(&at, 0, sizeof at);
+    at.kv = &kv, at.dtype = ULLM_DTYPE_F32, at.n_rows = n, at.n_seq = 1, at.n_head = P.n_head, at.d_cu = vints + V_CU, at.d_len = vints + V_LEN, at.d_blocks = vints + V_BLOCK;
+    at.n_table = at.max_blocks = 1, at.d_mask = (const uint32_t *)vints + V_MASK, at.mask_words = VW, at.d_work = vwork, at.work_bytes = vwork_bytes;
+    auto gemm = [&](const Mat &m, const float *in, float *out, int epi = EPI_STORE, const float *res = nullptr, void *scratch = nullptr) {
+        return launch_gemm_tc(m.fmt, m.w, in, out, scratch ? scratch : bscratch, m.out, m.cols, n, dev.sm_count, d_status, stream, epi, res);
+    };
+    for (size_t l = 0; l < P.n_layer; ++l) {
+        Layer &L = layers[l];
+        float *qkv = vqkv, *attn_out = vattn;
+        size_t ld = qd + 2 * kvd; // row of a token's projections
+        const float *vsrc = vqkv + qd + kvd;
+        size_t vld = ld;
+        if (gemms) {
+            rmsnorm_batch_kernel<<<(unsigned)n, 256, 0, stream>>>(bx, L.attn_norm, P.eps, (int)E, bxn);
+            TRY(gemm(L.wqk, bxn, bqk));
+            TRY(gemm(L.wv, bxn, bv));
+            qkv = bqk, ld = qd + kvd, vsrc = bv, vld = kvd, attn_out = bxn;
+        } else {
+            for (size_t t = 0; t < n; ++t) {
+                const float *x0 = vx + t * E;
+                float *q0 = vqkv + t * ld;
+                if (L.qkv_fused) {
+                    TRY(mv(L.wqk, x0, q0, L.attn_norm, EPI_STORE, nullptr));
+                    continue;
+                }
+                if (L.qk_fused) {
+                    TRY(mv(L.wqk, x0, q0, L.attn_norm, EPI_STORE, nullptr));
+                } else {
+                    TRY(mv(L.wq, x0, q0, L.attn_norm, EPI_STORE, nullptr));
+                    TRY(mv(L.wk, x0, q0 + qd, L.attn_norm, EPI_STORE, nullptr));
+                }
+                TRY(mv(L.wv, x0, q0 + qd + kvd, L.attn_norm, EPI_STORE, nullptr));
+            }
+        }
+        ro.layer = at.layer = l;
+        ro.d_q = ro.d_q_out = qkv, ro.d_k = qkv + qd, ro.d_v = vsrc, ro.q_stride = ro.k_stride = ro.q_out_stride = ld, ro.v_stride = vld;
+        ro.d_q_norm = L.q_norm, ro.d_k_norm = L.k_norm, ro.d_q_bias = L.q_bias, ro.d_k_bias = L.k_bias, ro.d_v_bias = L.v_bias;
+        if ((rc = ullm_cuda_qk_norm_rope_dev(c, &ro, stream))) return rc;
+        at.d_q = qkv, at.q_stride = ld, at.d_out = attn_out;
+        if ((rc = ullm_cuda_tree_attn_dev(c, &at, stream))) return rc;
+        if (gemms) {
+            TRY(gemm(L.wo, bxn, bx, EPI_RESIDUAL, bx));
+            rmsnorm_batch_kernel<<<(unsigned)n, 256, 0, stream>>>(bx, L.ffn_norm, P.eps, (int)E, bxn);
+            TRY(gemm(L.wgu, bxn, bh, EPI_SWIGLU));
+            TRY(gemm(L.wd, bh, bx, EPI_RESIDUAL, bx));
+            TRY(cudaGetLastError());
+            continue;
+        }
+        for (size_t t = 0; t < n; ++t) {
+            float *x0 = vx + t * E;
+            TRY(mv(L.wo, vattn + t * qd, x0, nullptr, EPI_RESIDUAL, x0));
+            if (L.moe) {
+                TRY(mv(L.moe_gate, x0, vrouter + t * P.n_experts, L.ffn_norm, EPI_STORE, nullptr));
+                continue;
+            }
+            if (!L.gu_fused) return fail(cudaErrorNotSupported);
+            TRY(mv(L.wgu, x0, hidden, L.ffn_norm, EPI_SWIGLU, nullptr));
+            TRY(mv(L.wd, hidden, x0, nullptr, EPI_RESIDUAL, x0));
+        }
+        if (L.moe) { // every expert that any of the tokens chose is read once
+            // (eight tokens at a time: what one call takes in one go, so that a refusal has changed nothing yet)
+            for (size_t t = 0; t < n; t += 8) {
+                const size_t nt = std::min((size_t)8, n - t);
+                float *x0 = vx + t * E;
+                const float *r0 = vrouter + t * P.n_experts;
+                e = launch_moe_ffn(dev, L.experts, x0, r0, nt, P.n_experts_used, x0, nullptr, nullptr, moe_scratch, d_status, stream, false, use_pdl, nullptr, x0, L.ffn_norm,
+                                   P.eps);
+                if (e == cudaErrorNotSupported) { // shapes outside the streamed kernels go through a normalised copy, as in the decode step
+                    cudaGetLastError();
+                    rmsnorm_batch_kernel<<<(unsigned)nt, 256, 0, stream>>>(x0, L.ffn_norm, P.eps, (int)E, vxn);
+                    TRY(cudaGetLastError());
+                    e = launch_moe_ffn(dev, L.experts, vxn, r0, nt, P.n_experts_used, x0, nullptr, nullptr, moe_scratch, d_status, stream, false, use_pdl, nullptr, x0);
+                }
+                TRY(e);
+            }
+        }
+    }
+    if (gemms && vscratch) {
+        rmsnorm_batch_kernel<<<(unsigned)n, 256, 0, stream>>>(bx, final_norm, P.eps, (int)E, bxn);
+        TRY(gemm(output, bxn, vlogits, EPI_STORE, nullptr, vscratch));
+    } else {
+        for (size_t t = 0; t < n; ++t) TRY(mv(output, xs + t * E, vlogits + t * P.vocab, final_norm, EPI_STORE, nullptr));
+    }
+    TRY(cudaMemcpyAsync(h_vx, vlogits, n * P.vocab * 4, cudaMemcpyDeviceToHost, stream)); // page-locked staging, as in forward()
+    TRY(cudaStreamSynchronize(stream));
+    memcpy(logits_host, h_vx, n * P.vocab * 4);
+    return ctx_check_status(c); // (the tree operators' waits report to the context)
+}
+
+int Forward::accept(ullm_cuda_ctx *c, size_t pos, size_t n, const int32_t *path, size_t kept) {
+    cudaError_t e;
+    DeviceGuard guard(c->device);
+    if ((e = verify_buffers(c)) != cudaSuccess) {
+        cudaGetLastError();
+        return ctx_fail(c, e == cudaErrorMemoryAllocation ? ULLM_ERR_OOM : ULLM_ERR_CUDA, "accept: %s", cudaGetErrorString(e));
+    }
+    memset(h_vints, 0, V_PARENT * 4);
+    h_vints[V_LEN] = (int)(pos + n), h_vints[V_REFS] = 1, h_vints[V_DRAFT] = (int)n, h_vints[V_KEPT] = (int)kept;
+    for (size_t j = 0; j < kept; ++j) h_vints[V_PATH + j] = path[j];
+    const ullm_kv_pages kv = pages();
+    ullm_kv_table t;
+    t.d_blocks = vints + V_BLOCK, t.d_len = vints + V_LEN, t.d_refs = vints + V_REFS, t.d_fault = vints + V_FAULT, t.n_seq = 1, t.max_blocks = 1;
+    t.d_work = vtable, t.work_bytes = vtable_bytes;
+    ULLM_CUDA_TRY(c, cudaMemcpyAsync(vints, h_vints, V_IN * 4, cudaMemcpyHostToDevice, stream));
+    int rc = ullm_cuda_kv_accept_dev(c, &kv, &t, vints + V_ROW, vints + V_DRAFT, vints + V_PATH, vints + V_KEPT, 1, VN, stream);
+    if (rc) return rc;
+    ULLM_CUDA_TRY(c, cudaStreamSynchronize(stream)); // (the staging array is free again)
+    return ULLM_OK;
+}
+#undef TRY
 
 } // namespace ullm

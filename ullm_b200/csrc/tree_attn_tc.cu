@@ -33,7 +33,7 @@ namespace ullm {
 namespace {
 
 constexpr int TM = 128, TK = 128, TT = 384;
-constexpr int T_COST = 2, T_MIN = 4; // places that a unit costs beside its blocks; places that a CTA takes at least
+constexpr int T_COST = 4, T_MIN = 2; // places that a unit costs beside its blocks; places that a CTA takes at least
 constexpr int SEGS = 4;
 template <int D> struct Cfg {
     static constexpr int ATOMS = D / 64;            // 64 values of a head: one 128-byte swizzle row
@@ -49,7 +49,9 @@ struct TcParams {
     int box;       // keys of a TMA box
     int slot_dim;  // coordinate (1 or 2) of the slot; the other one is the head
     int q_box;     // rows of the step in a TMA box of queries; 0: queries through cp.async
-    int lanes;     // CTAs of a team (Sched)
+    int team;      // logarithm of the CTAs of a team (Sched)
+    int page_log;  // logarithm of the page size where it is below a block's keys
+    int page_blocks; // blocks of a page where it is not
 };
 struct TcMaps {
     CUtensorMap k, v, q;
@@ -290,7 +292,7 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
         // ---- division of the work ----
         if (lane == 0) p.meta[blockIdx.x * TREE_META] = make_int4(-1, 0, 0, 0);
         __syncwarp();
-        Sched<ROWS, TK, T_COST, T_MIN> sched(p, prm.lanes);
+        Sched<ROWS, TK, T_COST, T_MIN> sched(p, prm.team);
         const bool some = sched.init();
         for (;; ++seg) {
             Seg next;
@@ -312,15 +314,16 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
             const Seg &w = segs[seg % SEGS];
             const int key_end = w.key_end, h = w.h, first = w.blk * TK + part * box;
             // entries of the page table, 32 at a time and one such load ahead: a block has 1 to 16 of them
-            const int per = p.page_size < TK ? parts : 1, e0 = p.page_size < TK ? w.blk * parts : w.blk * TK / p.page_size, e_end = (key_end + p.page_size - 1) / p.page_size;
+            const bool small = p.page_size < TK;
+            auto entry_of = [&](int block) { return small ? block << (7 - prm.page_log) : (int)((unsigned)block / (unsigned)prm.page_blocks); }; // of a block's first key
+            const int e0 = entry_of(w.blk), e_end = small ? (key_end + p.page_size - 1) >> prm.page_log : entry_of((key_end + TK - 1) / TK - 1) + 1;
             const int *const table = p.blocks + (size_t)w.id * p.max_blocks;
             auto entries = [&](int e) { return e + (int)lane < e_end ? table[e + lane] : 0; };
             int win = e0, now = entries(e0), ahead = entries(e0 + 32);
             auto page_of = [&](int j) { // page of this lane's box in block j of the segment
-                const int block_e = p.page_size < TK ? e0 + j * per : max(min((w.blk + j) * TK, key_end - 1), 0) / p.page_size; // the same in every lane
-                const int e = p.page_size < TK ? block_e + part : block_e;
-                if (block_e >= win + 32) win += 32, now = ahead, ahead = entries(win + 32);
-                return __shfl_sync(0xffffffffu, now, (e - win) & 31);
+                const int first_e = entry_of(w.blk + j); // the same in every lane
+                if (first_e >= win + 32) win += 32, now = ahead, ahead = entries(win + 32);
+                return __shfl_sync(0xffffffffu, now, (first_e - win + (small ? part : 0)) & 31);
             };
             auto load = [&](const CUtensorMap *map, int j, uint32_t tile, int page) {
                 const uint32_t st = tile % NST;
@@ -331,7 +334,7 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
                 if (lane == 0) mbar_arrive_expect_tx(&full[st], boxes * box * 128);
                 __syncwarp();
                 if (go) {
-                    const int slot = p.page_size <= TK ? 0 : token % p.page_size;
+                    const int slot = prm.page_blocks <= 1 ? 0 : (int)((unsigned)(token / TK) % (unsigned)prm.page_blocks) * TK;
                     tma_box(smem_u32(ring) + st * C::TILE + atom * (TK * 128) + part * box * 128, map, atom * 64, prm.slot_dim == 1 ? slot : h,
                             prm.slot_dim == 1 ? h : slot, page, smem_u32(&full[st]));
                 }
@@ -737,8 +740,10 @@ cudaError_t launch_tree_attn_tc(const DeviceInfo &dev, const PoolDev &pool, int 
     // Rows per sequence and key head on average (the lengths themselves are on the device; either way is right for any of them).
     const long long rows = ((long long)t.n_rows * t.group + t.n_seq - 1) / t.n_seq;
     const bool two = rows > TM;
-    prm.lanes = 1;
-    while (two && prm.lanes < 4 && rows > prm.lanes * 2 * TM * 5 / 4 && dev.sm_count / (prm.lanes * 2) > 0) prm.lanes *= 2;
+    prm.team = 0;
+    while (two && prm.team < 2 && rows > (2 * TM << prm.team) * 5 / 4 && dev.sm_count >> (prm.team + 1) > 0) ++prm.team;
+    prm.page_blocks = pool.page_size / TK, prm.page_log = 0;
+    while (1 << prm.page_log < pool.page_size && prm.page_log < 7) ++prm.page_log;
     // query boxes of about a sequence's rows
     prm.q_box = 0;
     if (TM % t.group == 0) {

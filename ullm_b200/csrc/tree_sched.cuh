@@ -68,7 +68,7 @@ template <int M, int KB, int COST, int MINS> struct Sched {
     static constexpr unsigned ALL = 0xffffffffu;
     const TreeDev &p;
     const int lane;
-    const int lanes, member, team; // CTAs of a team, this one's place in it, the team
+    const int shift, lanes, member, team; // CTAs of a team (a power of two), this one's place in it, the team
     unsigned total, active, each, more, lo, hi, cur; // share c begins at c * each + min(c, more)
     int b, h, t, nt;
     unsigned off; // place of `cur` in its unit
@@ -76,10 +76,10 @@ template <int M, int KB, int COST, int MINS> struct Sched {
     int wb;
     SeqView v;
 
-    __device__ __forceinline__ explicit Sched(const TreeDev &p_, int lanes_ = 1)
-        : p(p_), lane((int)(threadIdx.x & 31)), lanes(lanes_), member((int)blockIdx.x % lanes_), team((int)blockIdx.x / lanes_) {}
+    __device__ __forceinline__ explicit Sched(const TreeDev &p_, int shift_ = 0)
+        : p(p_), lane((int)(threadIdx.x & 31)), shift(shift_), lanes(1 << shift_), member((int)blockIdx.x & ((1 << shift_) - 1)), team((int)blockIdx.x >> shift_) {}
     // tiles that a team takes together, and their places: those of the one that sees most
-    __device__ __forceinline__ int groups(const SeqView &u) const { return (T::count(p, u) + lanes - 1) / lanes; }
+    __device__ __forceinline__ int groups(const SeqView &u) const { return (T::count(p, u) + lanes - 1) >> shift; }
     __device__ __forceinline__ int group_blocks(const SeqView &u, int g) const { return T::blocks(p, u, min((g + 1) * lanes, T::count(p, u)) - 1); }
 
     __device__ __forceinline__ unsigned share_at(unsigned c) const { return c * each + min(c, more); }
@@ -133,7 +133,7 @@ template <int M, int KB, int COST, int MINS> struct Sched {
             for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(ALL, x, o);
             total += x;
         }
-        active = max(1u, min(gridDim.x / lanes, (total + MINS - 1) / MINS));
+        active = max(1u, min(gridDim.x >> shift, (total + MINS - 1) / MINS));
         each = total / active, more = total - each * active;
         if ((unsigned)team >= active || total == 0) return false;
         lo = share_at(team), hi = share_at(team + 1), cur = lo;
@@ -278,7 +278,10 @@ template <typename O, int M> __global__ void __launch_bounds__(32 * JOIN_WARPS) 
         }
     }
     __syncthreads();
-    const int split = most > 8 ? 4 : 1, per = JOIN_WARPS / split, sub = warp % split, wide = D <= 128 ? 4 : 8;
+    // four warps to a row where that takes fewer round trips: passes over the rows times loads in turn per row
+    const int warps = gridDim.x * JOIN_WARPS;
+    const bool shared = (n_rows * 4 + warps - 1) / warps * ((most + 31) / 32) < (n_rows + warps - 1) / warps * ((most + 7) / 8);
+    const int split = shared ? 4 : 1, per = JOIN_WARPS / split, sub = warp % split, wide = D <= 128 ? 4 : 8;
     const bool on = lane * wide < D;
     for (int i0 = blockIdx.x * per; i0 < n_rows; i0 += gridDim.x * per) {
         const int i = i0 + warp / split;

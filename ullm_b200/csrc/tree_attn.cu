@@ -18,6 +18,7 @@ namespace ullm {
 
 constexpr int FT = 256;              // threads
 constexpr int F_COST = 1, F_MIN = 2; // places that a unit costs beside its blocks; places that a CTA takes at least
+constexpr int F_STATIC = 1280;       // bytes of static shared memory at most
 constexpr int F_PER_SM = 2;          // CTAs on an SM at most: 128 registers a thread
 constexpr int FSP = 4;               // floats behind a row of queries and of scores, for the same
 constexpr int F_PAD = 16;            // bytes behind a key's row: 128-bit reads one row apart hit distinct banks
@@ -39,6 +40,13 @@ __device__ __forceinline__ void copy16(void *dst, const void *src, bool on) { //
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
 
+// Two multiply-adds in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b), "l"(*(unsigned long long *)&c));
+    return *(float2 *)&r;
+}
+
 // bytes of shared memory: queries, two stages of keys (padded) and values, scores, three numbers per row
 inline size_t fma_smem(int dim, int kv_bytes, int rows) {
     const int keys = fma_keys(dim * kv_bytes);
@@ -47,12 +55,13 @@ inline size_t fma_smem(int dim, int kv_bytes, int rows) {
 
 template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bounds__(FT, F_PER_SM) tree_attn_fma_kernel(const TreeDev p) {
     extern __shared__ __align__(16) uint8_t fsm[];
-    constexpr int SP = KEYS + FSP, KS = KEYS / 32, RG = M / 4; // RG: groups of four rows
+    constexpr int SP = KEYS + FSP, KS = KEYS / 32, RG = M / 4, RW = M / (FT / 32); // RG: groups of four rows; RW: rows of a warp
     const int D = p.dim, QP = D + FSP, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row_b = D * (int)sizeof(KV), key_b = row_b + F_PAD;
     float *const qs = (float *)fsm, *const sc = qs + M * QP, *const ms = sc + M * SP, *const ls = ms + M, *const cs = ls + M;
     uint8_t *const stage0 = (uint8_t *)(cs + M);
     const int stage_b = KEYS * (key_b + row_b);
     __shared__ Seg seg;
+    __shared__ long long offs[2][KEYS]; // where the keys of a block lie: bytes behind p.k and p.v, -1 for none
     pdl_wait_prior();
     pdl_launch_dependents();
     Sched<M, KEYS, F_COST, F_MIN> sched(p);
@@ -65,6 +74,8 @@ template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bou
     // weighted sums of values: items (four rows, four values), spread over the threads, each for a part of the keys
     const int quads = D / 4, items = RG * quads, split = items <= FT / 4 ? 4 : (items <= FT / 2 ? 2 : 1), per = (items + FT - 1) / FT;
     const int part = split > 1 ? tid / items : 0;
+    // pieces of a row; a thread's first piece of a block, and how far it is to its next one
+    const int pieces = row_b / 16, step_j = FT / pieces, step_c = FT % pieces, first_j = tid / pieces, first_c = tid % pieces;
     for (;;) {
         __syncthreads();
         if (warp == 0) {
@@ -82,28 +93,31 @@ template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bou
         auto token_of = [&](int r) { return (w.row0 + r) / p.group; };
         auto head_of = [&](int r) { return w.h * p.group + (w.row0 + r) % p.group; };
         const int *const table = p.blocks + (size_t)v.id * p.max_blocks;
-        // 16-byte pieces of a block's keys and values; keys behind the last, and pages outside the pool, as zeros
-        const int pieces = row_b / 16, total = KEYS * pieces;
+        auto page_at = [&](int token) { return token < key_end ? table[token / p.page_size] : -1; };
+        auto place = [&](int page, int token) { // a key behind the last, or of a page outside the pool, has none
+            return (unsigned)page < (unsigned)p.n_pages ? (page * p.page_stride + token % p.page_size * p.slot_stride + w.h * p.head_stride) * (long long)sizeof(KV) : -1ll;
+        };
+        // 16-byte pieces of a block's keys and values; zeros for a key that has no place
         auto fetch = [&](int blk, uint8_t *stage) {
-            for (int i0 = tid; i0 < total; i0 += 4 * FT) { // four page numbers on their way at once
-                int page[4];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int token = blk * KEYS + (i0 + u * FT) / pieces;
-                    page[u] = i0 + u * FT < total && token < key_end ? table[token / p.page_size] : -1;
-                }
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int i = i0 + u * FT, j = i / pieces, c = (i - j * pieces) * 16, token = blk * KEYS + j;
-                    if (i >= total) break;
-                    const bool on = (unsigned)page[u] < (unsigned)p.n_pages;
-                    const long long at = on ? (page[u] * p.page_stride + token % p.page_size * p.slot_stride + w.h * p.head_stride) * (long long)sizeof(KV) + c : 0;
-                    copy16(stage + j * key_b + c, p.k + at, on);
-                    copy16(stage + KEYS * key_b + j * row_b + c, p.v + at, on);
-                }
+            const long long *const at = offs[(blk - w.blk) & 1];
+            int j = first_j, c = first_c;
+#pragma unroll 2
+            while (j < KEYS) {
+                const long long off = at[j];
+                const bool on = off >= 0;
+                const long long from = on ? off + c * 16 : 0;
+                copy16(stage + j * key_b + c * 16, p.k + from, on);
+                copy16(stage + KEYS * key_b + j * row_b + c * 16, p.v + from, on);
+                j += step_j, c += step_c;
+                if (c >= pieces) c -= pieces, ++j;
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
+        if (tid < 2 * KEYS) { // the first two blocks' keys, one per thread
+            const int token = w.blk * KEYS + tid;
+            offs[tid / KEYS][tid % KEYS] = place(page_at(token), token);
+        }
+        __syncthreads();
         fetch(w.blk, stage0);
         for (int i = tid; i < M * quads; i += FT) {
             const int r = i / quads, d = i % quads * 4;
@@ -111,14 +125,17 @@ template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bou
             if (r < rows) x = widen4((const Q *)p.q + (v.r0 + token_of(r)) * p.q_stride + (long long)head_of(r) * D + d);
             *(float4 *)(qs + r * QP + d) = x;
         }
-        if (tid < M) ms[tid] = -INFINITY, ls[tid] = 0.f;
-        float acc[2][4][4];
+        // a warp's rows are every eighth: the reference of each, and the lane's share of its sum
+        float m_r[RW], l_r[RW];
+#pragma unroll
+        for (int a = 0; a < RW; ++a) m_r[a] = -INFINITY, l_r[a] = 0.f;
+        float2 acc[2][4][2];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int a = 0; a < 4; ++a)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[u][a][e] = 0.f;
+                for (int e = 0; e < 2; ++e) acc[u][a][e] = make_float2(0.f, 0.f);
         for (int blk = w.blk; blk < blk_end; ++blk) {
             uint8_t *const stage = stage0 + ((blk - w.blk) & 1) * stage_b;
             const KV *const vs = (const KV *)(stage + KEYS * key_b);
@@ -130,28 +147,33 @@ template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bou
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
             }
             __syncthreads();
+            // the block after the next: its page numbers travel while the scores are made
+            const int ahead = (blk + 2) * KEYS + tid;
+            const bool more = tid < KEYS && blk + 2 < blk_end;
+            const int page = more ? page_at(ahead) : -1;
             if (k0 + KEYS > v.ctx) { // the rows' own tokens: some rows may not see them, and 0 * inf must not reach those
-                for (int i = tid; i < KEYS * D; i += FT) {
-                    KV *const at = (KV *)(stage + KEYS * key_b) + i;
-                    if (k0 + i / D >= v.ctx && !isfinite((float)*at)) *at = (KV)0.f, seg.odd = 1;
-                }
+                KV *const own = (KV *)(stage + KEYS * key_b);
+                for (int i = max(v.ctx - k0, 0) * D + tid; i < min(key_end - k0, KEYS) * D; i += FT)
+                    if (!isfinite((float)own[i])) own[i] = (KV)0.f, seg.odd = 1;
             }
             { // scores: warps (tile of 16 keys, tile of rows), lanes 8 x 4, a thread two keys eight apart and every fourth of its rows
                 constexpr int TILES = KEYS / 16, GROUPS = FT / 32 / TILES, R = M / GROUPS / 4;
                 const int j0 = warp % TILES * 16 + lane % 8, r0 = warp / TILES * (4 * R) + lane / 8;
                 if (warp / TILES * (4 * R) < rows) {
-                    float s[2][R];
+                    float2 s[2][R]; // sums over the even and the odd values of a head
 #pragma unroll
-                    for (int a = 0; a < R; ++a) s[0][a] = s[1][a] = 0.f;
+                    for (int a = 0; a < R; ++a) s[0][a] = s[1][a] = make_float2(0.f, 0.f);
                     const KV *const key0 = (const KV *)(stage + j0 * key_b), *const key1 = (const KV *)(stage + (j0 + 8) * key_b);
 #pragma unroll 4
                     for (int d = 0; d < D; d += 4) {
-                        const float4 k0 = widen4(key0 + d), k1 = widen4(key1 + d);
+                        const float4 x = widen4(key0 + d), y = widen4(key1 + d);
 #pragma unroll
                         for (int a = 0; a < R; ++a) {
                             const float4 q = *(const float4 *)(qs + (r0 + 4 * a) * QP + d);
-                            s[0][a] += q.x * k0.x + q.y * k0.y + q.z * k0.z + q.w * k0.w;
-                            s[1][a] += q.x * k1.x + q.y * k1.y + q.z * k1.z + q.w * k1.w;
+                            s[0][a] = fma2(make_float2(q.x, q.y), make_float2(x.x, x.y), s[0][a]);
+                            s[1][a] = fma2(make_float2(q.x, q.y), make_float2(y.x, y.y), s[1][a]);
+                            s[0][a] = fma2(make_float2(q.z, q.w), make_float2(x.z, x.w), s[0][a]);
+                            s[1][a] = fma2(make_float2(q.z, q.w), make_float2(y.z, y.w), s[1][a]);
                         }
                     }
 #pragma unroll
@@ -161,28 +183,41 @@ template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bou
                             const int r = r0 + 4 * a, j = j0 + 8 * b;
                             bool see = k0 + j < key_end && r < rows;
                             if (see && k0 + j >= v.ctx) see = sees(p, v, token_of(r), k0 + j - v.ctx);
-                            sc[r * SP + j] = see ? s[b][a] * p.scale_log2 : -INFINITY;
+                            sc[r * SP + j] = see ? (s[b][a].x + s[b][a].y) * p.scale_log2 : -INFINITY;
                         }
                 }
             }
             __syncthreads();
-            for (int r = warp; r < rows; r += FT / 32) {
-                float s[KS], mn = -INFINITY, sum = 0.f;
-                const float m = ms[r];
+            if (more) offs[(blk - w.blk) & 1][tid] = place(page, ahead);
+            float s[RW][KS], mn[RW];
 #pragma unroll
-                for (int k = 0; k < KS; ++k) s[k] = sc[r * SP + lane + 32 * k], mn = fmaxf(mn, s[k]);
-                mn = fmaxf(m, warp_max(mn));
+            for (int a = 0; a < RW; ++a) {
+                mn[a] = -INFINITY;
+                if (a * (FT / 32) < rows) {
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) s[a][k] = sc[(warp + a * (FT / 32)) * SP + lane + 32 * k], mn[a] = fmaxf(mn[a], s[a][k]);
+                }
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+                for (int a = 0; a < RW; ++a)
+                    if (a * (FT / 32) < rows) mn[a] = fmaxf(mn[a], __shfl_xor_sync(0xffffffffu, mn[a], o));
+#pragma unroll
+            for (int a = 0; a < RW; ++a) { // (what lies behind the last row is worked on and never written)
+                if (a * (FT / 32) >= rows) continue;
+                const int r = warp + a * (FT / 32);
+                mn[a] = fmaxf(m_r[a], mn[a]);
+                const float corr = m_r[a] == -INFINITY ? 0.f : exp2f(m_r[a] - mn[a]);
+                l_r[a] *= corr, m_r[a] = mn[a];
                 // nothing seen so far: all weights are zero.  (A score of +inf or NaN gives NaN, as the formula does.)
 #pragma unroll
                 for (int k = 0; k < KS; ++k) {
-                    s[k] = s[k] == -INFINITY ? 0.f : exp2f(s[k] - mn);
-                    sum += s[k];
-                    sc[r * SP + lane + 32 * k] = s[k];
+                    const float x = s[a][k] == -INFINITY ? 0.f : exp2f(s[a][k] - mn[a]);
+                    l_r[a] += x;
+                    sc[r * SP + lane + 32 * k] = x;
                 }
-                const float corr = m == -INFINITY ? 0.f : exp2f(m - mn);
-                sum = warp_sum(sum);
-                __syncwarp();
-                if (lane == 0) ms[r] = mn, ls[r] = ls[r] * corr + sum, cs[r] = corr;
+                if (lane == 0) cs[r] = corr;
             }
             __syncthreads();
 #pragma unroll
@@ -193,7 +228,7 @@ template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bou
                 for (int a = 0; a < 4; ++a) {
                     const float corr = rg * 4 + a < rows ? cs[rg * 4 + a] : 0.f;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[u][a][e] *= corr;
+                    for (int e = 0; e < 2; ++e) acc[u][a][e].x *= corr, acc[u][a][e].y *= corr;
                 }
                 const int j0 = part * (KEYS / split), j1 = j0 + KEYS / split;
 #pragma unroll 2
@@ -207,12 +242,18 @@ template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bou
 #pragma unroll
                         for (int a = 0; a < 4; ++a) {
                             const float wa = k == 0 ? q[a].x : (k == 1 ? q[a].y : (k == 2 ? q[a].z : q[a].w));
-                            acc[u][a][0] += wa * x.x, acc[u][a][1] += wa * x.y, acc[u][a][2] += wa * x.z, acc[u][a][3] += wa * x.w;
+                            acc[u][a][0] = fma2(make_float2(wa, wa), make_float2(x.x, x.y), acc[u][a][0]);
+                            acc[u][a][1] = fma2(make_float2(wa, wa), make_float2(x.z, x.w), acc[u][a][1]);
                         }
                     }
                 }
             }
             __syncthreads(); // the stage and the scores are free
+        }
+#pragma unroll
+        for (int a = 0; a < RW; ++a) {
+            const float l = warp_sum(l_r[a]);
+            if (lane == 0) ms[warp + a * (FT / 32)] = m_r[a], ls[warp + a * (FT / 32)] = l;
         }
         // sum the key parts in order, in the stages' memory
         float *const red = (float *)stage0;
@@ -222,7 +263,7 @@ template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bou
             if (u >= per || part >= split || item >= items) continue;
 #pragma unroll
             for (int a = 0; a < 4; ++a)
-                if (rg * 4 + a < rows) *(float4 *)(red + ((size_t)part * M + rg * 4 + a) * D + dq * 4) = make_float4(acc[u][a][0], acc[u][a][1], acc[u][a][2], acc[u][a][3]);
+                if (rg * 4 + a < rows) *(float4 *)(red + ((size_t)part * M + rg * 4 + a) * D + dq * 4) = make_float4(acc[u][a][0].x, acc[u][a][0].y, acc[u][a][1].x, acc[u][a][1].y);
         }
         __syncthreads();
         const bool whole = w.flags & 1, odd = seg.odd;
@@ -262,7 +303,7 @@ template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bou
 
 // CTAs of the f32 kernel: as many as the SMs hold at once
 static int fma_ctas(const DeviceInfo &dev, int dim, int kv_bytes, int rows) {
-    const size_t one = fma_smem(dim, kv_bytes, rows) + 1024 + 256; // what the system and the static variables take
+    const size_t one = fma_smem(dim, kv_bytes, rows) + 1024 + F_STATIC; // with what the system and the static variables take
     return dev.sm_count * (int)std::max((size_t)1, std::min((size_t)F_PER_SM, (size_t)dev.max_smem_sm / one));
 }
 static size_t meta_bytes(int ctas) { return ((size_t)ctas * TREE_META * sizeof(int4) + 255) / 256 * 256; }
@@ -270,7 +311,7 @@ constexpr int F_ROWS = 32; // rows of the larger tile
 
 template <typename Q, typename KV, int M, int KEYS> static cudaError_t launch_fma_as(const DeviceInfo &dev, const TreeDev &t, bool pdl, cudaStream_t st) {
     const size_t smem = fma_smem(t.dim, sizeof(KV), M);
-    cudaError_t e = cudaFuncSetAttribute(tree_attn_fma_kernel<Q, KV, M, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, dev.max_smem_optin - 1024);
+    cudaError_t e = cudaFuncSetAttribute(tree_attn_fma_kernel<Q, KV, M, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, dev.max_smem_optin - F_STATIC);
     if (e != cudaSuccess) return e;
     const int ctas = fma_ctas(dev, t.dim, sizeof(KV), M);
     e = launch_kernel(tree_attn_fma_kernel<Q, KV, M, KEYS>, dim3(ctas), dim3(FT), smem, st, pdl, t);

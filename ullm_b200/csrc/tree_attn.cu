@@ -5,9 +5,11 @@
 // over the keys that row i sees, in one pass with a running maximum m, sum l and weighted sum of values, all f32.
 //
 // tree_attn_fma_kernel: f32 arithmetic on the CUDA cores, for f32 queries and for whatever the tensor-core kernel (tree_attn_tc.cu) does not take.
-// A CTA of 256 threads holds 16 or 32 query rows in shared memory and walks blocks of keys; the next block's keys and values arrive by cp.async, as they lie
-// in the pages, while one is worked on.  A warp's scores form a tile of 16 keys x 16 (or 8) rows, a thread's one of two keys x four (two) rows, so that
-// lanes share what they read from shared memory: with a key per lane these reads took three times as long as the multiply-adds.
+// A CTA of 256 threads holds 8 to 64 query rows in shared memory and walks blocks of keys; the next block's keys and values arrive by cp.async, as they lie
+// in the pages, while one is worked on.  A warp's scores form a tile, a thread's one of up to 4 keys x 4 rows, so that lanes share what they read from
+// shared memory: with a key per lane these reads took three times as long as the multiply-adds, which go two to an instruction.
+// It is bound by the turns that scores, softmax and weighted sums take between barriers with 8 to 16 warps on an SM: 22 of the 72 TFLOP/s of the f32 units
+// with 64 rows and heads of 128, 2.7 TB/s with four rows per key head.
 #include "engine.h"
 #include "tree_sched.cuh"
 
@@ -22,8 +24,6 @@ constexpr int F_STATIC = 1280;       // bytes of static shared memory at most
 constexpr int F_PER_SM = 2;          // CTAs on an SM at most: 128 registers a thread
 constexpr int FSP = 4;               // floats behind a row of queries and of scores, for the same
 constexpr int F_PAD = 16;            // bytes behind a key's row: 128-bit reads one row apart hit distinct banks
-// keys of a block, by the bytes of a row
-__host__ __device__ constexpr int fma_keys(int row_bytes) { return row_bytes <= 512 ? 64 : 32; }
 
 // Four neighbouring values as f32
 __device__ __forceinline__ float4 widen4(const float *p) { return *(const float4 *)p; }
@@ -48,14 +48,16 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 }
 
 // bytes of shared memory: queries, two stages of keys (padded) and values, scores, three numbers per row
-inline size_t fma_smem(int dim, int kv_bytes, int rows) {
-    const int keys = fma_keys(dim * kv_bytes);
+inline size_t fma_smem(int dim, int kv_bytes, int rows, int keys) {
     return sizeof(float) * ((size_t)rows * (dim + FSP) + (size_t)rows * (keys + FSP) + 3 * rows) + 2 * (size_t)keys * (2 * dim * kv_bytes + F_PAD);
 }
 
-template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bounds__(FT, F_PER_SM) tree_attn_fma_kernel(const TreeDev p) {
+template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bounds__(FT, M == 64 ? 1 : F_PER_SM) tree_attn_fma_kernel(const TreeDev p) {
     extern __shared__ __align__(16) uint8_t fsm[];
-    constexpr int SP = KEYS + FSP, KS = KEYS / 32, RG = M / 4, RW = M / (FT / 32); // RG: groups of four rows; RW: rows of a warp
+    constexpr int SP = KEYS + FSP, KS = KEYS / 32, RW = M / (FT / 32); // RW: rows of a warp
+    // A thread's scores: KT keys x R rows; its weighted sums: PR rows x four values, U times
+    constexpr int KT = M == 8 ? 1 : (M == 64 ? 4 : 2), TILES = KEYS / (8 * KT), GROUPS = FT / 32 / TILES, R = M / GROUPS / 4;
+    constexpr int PR = M == 64 ? 8 : 4, U = M == 32 ? 2 : 1;
     const int D = p.dim, QP = D + FSP, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row_b = D * (int)sizeof(KV), key_b = row_b + F_PAD;
     float *const qs = (float *)fsm, *const sc = qs + M * QP, *const ms = sc + M * SP, *const ls = ms + M, *const cs = ls + M;
     uint8_t *const stage0 = (uint8_t *)(cs + M);
@@ -71,9 +73,7 @@ template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bou
         __syncwarp();
         some = sched.init();
     }
-    // weighted sums of values: items (four rows, four values), spread over the threads, each for a part of the keys
-    const int quads = D / 4, items = RG * quads, split = items <= FT / 4 ? 4 : (items <= FT / 2 ? 2 : 1), per = (items + FT - 1) / FT;
-    const int part = split > 1 ? tid / items : 0;
+    const int quads = D / 4;
     // pieces of a row; a thread's first piece of a block, and how far it is to its next one
     const int pieces = row_b / 16, step_j = FT / pieces, step_c = FT % pieces, first_j = tid / pieces, first_c = tid % pieces;
     for (;;) {
@@ -90,6 +90,11 @@ template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bou
         SeqView v;
         v.r0 = w.r0, v.n = w.n, v.id = w.id, v.ctx = w.ctx, v.kv = w.kv;
         const int rows = w.rows, key_end = w.key_end, blk_end = w.blk + w.count;
+        // weighted sums of values: items (PR rows, four values), spread over the threads, each for a part of the keys
+        const int items = (rows + PR - 1) / PR * quads;
+        int split = 1;
+        while (split * items * 2 <= FT && split * 8 <= KEYS && split * rows * D * (int)sizeof(float) <= stage_b) split *= 2; // (they meet in the stages' memory)
+        const int part = split > 1 ? tid / items : 0, item0 = split > 1 ? tid % items : tid;
         auto token_of = [&](int r) { return (w.row0 + r) / p.group; };
         auto head_of = [&](int r) { return w.h * p.group + (w.row0 + r) % p.group; };
         const int *const table = p.blocks + (size_t)v.id * p.max_blocks;
@@ -129,13 +134,11 @@ template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bou
         float m_r[RW], l_r[RW];
 #pragma unroll
         for (int a = 0; a < RW; ++a) m_r[a] = -INFINITY, l_r[a] = 0.f;
-        float2 acc[2][4][2];
+        float2 acc[U][PR][2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int a = 0; a < 4; ++a)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) acc[u][a][e] = make_float2(0.f, 0.f);
+            for (int a = 0; a < PR; ++a) acc[u][a][0] = acc[u][a][1] = make_float2(0.f, 0.f);
         for (int blk = w.blk; blk < blk_end; ++blk) {
             uint8_t *const stage = stage0 + ((blk - w.blk) & 1) * stage_b;
             const KV *const vs = (const KV *)(stage + KEYS * key_b);
@@ -156,30 +159,34 @@ template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bou
                 for (int i = max(v.ctx - k0, 0) * D + tid; i < min(key_end - k0, KEYS) * D; i += FT)
                     if (!isfinite((float)own[i])) own[i] = (KV)0.f, seg.odd = 1;
             }
-            { // scores: warps (tile of 16 keys, tile of rows), lanes 8 x 4, a thread two keys eight apart and every fourth of its rows
-                constexpr int TILES = KEYS / 16, GROUPS = FT / 32 / TILES, R = M / GROUPS / 4;
-                const int j0 = warp % TILES * 16 + lane % 8, r0 = warp / TILES * (4 * R) + lane / 8;
+            { // scores: warps (tile of keys, tile of rows), lanes 8 x 4, a thread every eighth of its keys and every fourth of its rows
+                const int j0 = warp % TILES * (8 * KT) + lane % 8, r0 = warp / TILES * (4 * R) + lane / 8;
                 if (warp / TILES * (4 * R) < rows) {
-                    float2 s[2][R]; // sums over the even and the odd values of a head
+                    float2 s[KT][R]; // sums over the even and the odd values of a head
 #pragma unroll
-                    for (int a = 0; a < R; ++a) s[0][a] = s[1][a] = make_float2(0.f, 0.f);
-                    const KV *const key0 = (const KV *)(stage + j0 * key_b), *const key1 = (const KV *)(stage + (j0 + 8) * key_b);
+                    for (int b = 0; b < KT; ++b)
+#pragma unroll
+                        for (int a = 0; a < R; ++a) s[b][a] = make_float2(0.f, 0.f);
+                    const uint8_t *const key = stage + j0 * key_b;
 #pragma unroll 4
                     for (int d = 0; d < D; d += 4) {
-                        const float4 x = widen4(key0 + d), y = widen4(key1 + d);
+                        float4 x[KT];
+#pragma unroll
+                        for (int b = 0; b < KT; ++b) x[b] = widen4((const KV *)(key + 8 * b * key_b) + d);
 #pragma unroll
                         for (int a = 0; a < R; ++a) {
                             const float4 q = *(const float4 *)(qs + (r0 + 4 * a) * QP + d);
-                            s[0][a] = fma2(make_float2(q.x, q.y), make_float2(x.x, x.y), s[0][a]);
-                            s[1][a] = fma2(make_float2(q.x, q.y), make_float2(y.x, y.y), s[1][a]);
-                            s[0][a] = fma2(make_float2(q.z, q.w), make_float2(x.z, x.w), s[0][a]);
-                            s[1][a] = fma2(make_float2(q.z, q.w), make_float2(y.z, y.w), s[1][a]);
+#pragma unroll
+                            for (int b = 0; b < KT; ++b) {
+                                s[b][a] = fma2(make_float2(q.x, q.y), make_float2(x[b].x, x[b].y), s[b][a]);
+                                s[b][a] = fma2(make_float2(q.z, q.w), make_float2(x[b].z, x[b].w), s[b][a]);
+                            }
                         }
                     }
 #pragma unroll
                     for (int a = 0; a < R; ++a)
 #pragma unroll
-                        for (int b = 0; b < 2; ++b) {
+                        for (int b = 0; b < KT; ++b) {
                             const int r = r0 + 4 * a, j = j0 + 8 * b;
                             bool see = k0 + j < key_end && r < rows;
                             if (see && k0 + j >= v.ctx) see = sees(p, v, token_of(r), k0 + j - v.ctx);
@@ -221,26 +228,26 @@ template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bou
             }
             __syncthreads();
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int item = split > 1 ? tid % items : tid + u * FT, rg = item / quads, dq = item % quads;
-                if (u >= per || part >= split || item >= items || rg * 4 >= rows) continue;
+            for (int u = 0; u < U; ++u) {
+                const int item = item0 + u * FT, rg = item / quads, dq = item % quads;
+                if (part >= split || item >= items) continue;
 #pragma unroll
-                for (int a = 0; a < 4; ++a) {
-                    const float corr = rg * 4 + a < rows ? cs[rg * 4 + a] : 0.f;
+                for (int a = 0; a < PR; ++a) {
+                    const float corr = rg * PR + a < rows ? cs[rg * PR + a] : 0.f;
 #pragma unroll
                     for (int e = 0; e < 2; ++e) acc[u][a][e].x *= corr, acc[u][a][e].y *= corr;
                 }
                 const int j0 = part * (KEYS / split), j1 = j0 + KEYS / split;
 #pragma unroll 2
                 for (int j = j0; j < j1; j += 4) {
-                    float4 q[4];
+                    float4 q[PR];
 #pragma unroll
-                    for (int a = 0; a < 4; ++a) q[a] = *(const float4 *)(sc + (rg * 4 + a) * SP + j);
+                    for (int a = 0; a < PR; ++a) q[a] = *(const float4 *)(sc + (rg * PR + a) * SP + j);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const float4 x = widen4(vs + (j + k) * D + dq * 4);
 #pragma unroll
-                        for (int a = 0; a < 4; ++a) {
+                        for (int a = 0; a < PR; ++a) {
                             const float wa = k == 0 ? q[a].x : (k == 1 ? q[a].y : (k == 2 ? q[a].z : q[a].w));
                             acc[u][a][0] = fma2(make_float2(wa, wa), make_float2(x.x, x.y), acc[u][a][0]);
                             acc[u][a][1] = fma2(make_float2(wa, wa), make_float2(x.z, x.w), acc[u][a][1]);
@@ -258,12 +265,12 @@ template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bou
         // sum the key parts in order, in the stages' memory
         float *const red = (float *)stage0;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int item = split > 1 ? tid % items : tid + u * FT, rg = item / quads, dq = item % quads;
-            if (u >= per || part >= split || item >= items) continue;
+        for (int u = 0; u < U; ++u) {
+            const int item = item0 + u * FT, rg = item / quads, dq = item % quads;
+            if (part >= split || item >= items) continue;
 #pragma unroll
-            for (int a = 0; a < 4; ++a)
-                if (rg * 4 + a < rows) *(float4 *)(red + ((size_t)part * M + rg * 4 + a) * D + dq * 4) = make_float4(acc[u][a][0].x, acc[u][a][0].y, acc[u][a][1].x, acc[u][a][1].y);
+            for (int a = 0; a < PR; ++a)
+                if (rg * PR + a < rows) *(float4 *)(red + ((size_t)part * rows + rg * PR + a) * D + dq * 4) = make_float4(acc[u][a][0].x, acc[u][a][0].y, acc[u][a][1].x, acc[u][a][1].y);
         }
         __syncthreads();
         const bool whole = w.flags & 1, odd = seg.odd;
@@ -272,7 +279,7 @@ template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bou
             const int r = i / quads, d = (i - r * quads) * 4;
             float4 o = *(const float4 *)(red + r * D + d);
             for (int s = 1; s < split; ++s) {
-                const float4 x = *(const float4 *)(red + ((size_t)s * M + r) * D + d);
+                const float4 x = *(const float4 *)(red + ((size_t)s * rows + r) * D + d);
                 o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
             }
             if (odd) { // infinities and NaN of the tokens that the row does see
@@ -302,26 +309,34 @@ template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bou
 }
 
 // CTAs of the f32 kernel: as many as the SMs hold at once
-static int fma_ctas(const DeviceInfo &dev, int dim, int kv_bytes, int rows) {
-    const size_t one = fma_smem(dim, kv_bytes, rows) + 1024 + F_STATIC; // with what the system and the static variables take
+static int fma_ctas(const DeviceInfo &dev, int dim, int kv_bytes, int rows, int keys) {
+    const size_t one = fma_smem(dim, kv_bytes, rows, keys) + 1024 + F_STATIC; // with what the system and the static variables take
     return dev.sm_count * (int)std::max((size_t)1, std::min((size_t)F_PER_SM, (size_t)dev.max_smem_sm / one));
 }
 static size_t meta_bytes(int ctas) { return ((size_t)ctas * TREE_META * sizeof(int4) + 255) / 256 * 256; }
-constexpr int F_ROWS = 32; // rows of the larger tile
+// Keys of a block: 64 while two CTAs with two stages of them fit an SM, else 32 (32 rows of 512 bytes: 303 us with 64 keys and one CTA, 268 with 32 and two).
+inline int fma_keys(int row_bytes) { return row_bytes <= 256 ? 64 : 32; }
+// 64 rows x 64 keys in one CTA per SM, with twice the sums per thread and no shared registers, for many rows over keys of 257 to 512 bytes in 32 bits: 232 us
+// where two CTAs of 32 x 32 take 268.  Over shorter keys two CTAs of 32 x 64 are faster: 242 us against 262.
+inline bool fma_64_rows(int dim, int kv_bytes) { return kv_bytes == 4 && dim > 64 && dim <= 128; }
 
 template <typename Q, typename KV, int M, int KEYS> static cudaError_t launch_fma_as(const DeviceInfo &dev, const TreeDev &t, bool pdl, cudaStream_t st) {
-    const size_t smem = fma_smem(t.dim, sizeof(KV), M);
+    const size_t smem = fma_smem(t.dim, sizeof(KV), M, KEYS);
     cudaError_t e = cudaFuncSetAttribute(tree_attn_fma_kernel<Q, KV, M, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, dev.max_smem_optin - F_STATIC);
     if (e != cudaSuccess) return e;
-    const int ctas = fma_ctas(dev, t.dim, sizeof(KV), M);
+    const int ctas = fma_ctas(dev, t.dim, sizeof(KV), M, KEYS);
     e = launch_kernel(tree_attn_fma_kernel<Q, KV, M, KEYS>, dim3(ctas), dim3(FT), smem, st, pdl, t);
     if (e != cudaSuccess) return e;
     return launch_kernel(tree_join_kernel<Q, M>, dim3(dev.sm_count * JOIN_PER_SM), dim3(32 * JOIN_WARPS), 0, st, pdl, t, ctas);
 }
 template <typename Q, typename KV> static cudaError_t launch_fma(const DeviceInfo &dev, const TreeDev &t, bool pdl, cudaStream_t st) {
-    const bool wide = ((long long)t.n_rows * t.group + t.n_seq - 1) / t.n_seq > 16; // rows per sequence and key head, on average
-    if (fma_keys(t.dim * (int)sizeof(KV)) == 64) return wide ? launch_fma_as<Q, KV, F_ROWS, 64>(dev, t, pdl, st) : launch_fma_as<Q, KV, 16, 64>(dev, t, pdl, st);
-    return wide ? launch_fma_as<Q, KV, F_ROWS, 32>(dev, t, pdl, st) : launch_fma_as<Q, KV, 16, 32>(dev, t, pdl, st);
+    const long long rows = ((long long)t.n_rows * t.group + t.n_seq - 1) / t.n_seq; // per sequence and key head, on average
+    const bool k64 = fma_keys(t.dim * (int)sizeof(KV)) == 64;
+    if constexpr (sizeof(KV) == 4)
+        if (rows > 32 && fma_64_rows(t.dim, sizeof(KV))) return launch_fma_as<Q, KV, 64, 64>(dev, t, pdl, st);
+    if (rows > 16) return k64 ? launch_fma_as<Q, KV, 32, 64>(dev, t, pdl, st) : launch_fma_as<Q, KV, 32, 32>(dev, t, pdl, st);
+    if (rows > 8) return k64 ? launch_fma_as<Q, KV, 16, 64>(dev, t, pdl, st) : launch_fma_as<Q, KV, 16, 32>(dev, t, pdl, st);
+    return k64 ? launch_fma_as<Q, KV, 8, 64>(dev, t, pdl, st) : launch_fma_as<Q, KV, 8, 32>(dev, t, pdl, st);
 }
 
 } // namespace ullm
@@ -329,15 +344,15 @@ template <typename Q, typename KV> static cudaError_t launch_fma(const DeviceInf
 using namespace ullm;
 
 // The work area begins with the CTAs' records (for the most CTAs of any kernel), then the partial results.
-static size_t tree_work_bytes(const DeviceInfo &dev, int dim, bool tc) {
-    const size_t fma = sizeof(float) * (size_t)dev.sm_count * F_PER_SM * 2 * F_ROWS * (dim + 2);
+static size_t tree_work_bytes(const DeviceInfo &dev, int dim, int kv_bytes, bool tc) {
+    const size_t fma = sizeof(float) * (size_t)dev.sm_count * F_PER_SM * 2 * (fma_64_rows(dim, kv_bytes) ? 64 : 32) * (dim + 2);
     return meta_bytes(dev.sm_count * F_PER_SM) + (tc ? std::max(fma, tree_attn_tc_work(dev.sm_count, dim)) : fma);
 }
 
 size_t ullm_cuda_tree_attn_work_bytes(const ullm_cuda_ctx *c, const ullm_kv_pages *kv, int dtype) {
     PoolDev pool;
     if (!c || !kv || pool_check(kv, &pool)) return 0;
-    return tree_work_bytes(c->dev, pool.head_dim, tree_attn_tc_supported(pool, dtype));
+    return tree_work_bytes(c->dev, pool.head_dim, pool.elem_bytes, tree_attn_tc_supported(pool, dtype));
 }
 
 int ullm_cuda_tree_attn_dev(ullm_cuda_ctx *c, const ullm_tree_attn *a, void *stream) {

@@ -43,6 +43,9 @@ struct TreeDev {
 };
 constexpr int TREE_META = 2; // int4 per CTA
 
+// f32 queries with heads of 64 or 128 values: the tensor cores on values split in two
+bool tree_attn_split_supported(int dim);
+cudaError_t launch_tree_attn_split(const DeviceInfo &dev, int kv_dtype, const TreeDev &t, bool pdl, cudaStream_t st);
 bool tree_attn_tc_supported(const PoolDev &pool, int dtype);
 size_t tree_attn_tc_work(int sm_count, int dim);
 cudaError_t launch_tree_attn_tc(const DeviceInfo &dev, const PoolDev &pool, int dtype, const TreeDev &t, int *d_status, bool pdl, cudaStream_t st);

@@ -25,21 +25,6 @@ constexpr int F_PER_SM = 2;          // CTAs on an SM at most: 128 registers a t
 constexpr int FSP = 4;               // floats behind a row of queries and of scores, for the same
 constexpr int F_PAD = 16;            // bytes behind a key's row: 128-bit reads one row apart hit distinct banks
 
-// Four neighbouring values as f32
-__device__ __forceinline__ float4 widen4(const float *p) { return *(const float4 *)p; }
-__device__ __forceinline__ float4 widen4(const __half *p) {
-    const uint2 v = *(const uint2 *)p;
-    const float2 a = __half22float2(*(const __half2 *)&v.x), b = __half22float2(*(const __half2 *)&v.y);
-    return make_float4(a.x, a.y, b.x, b.y);
-}
-__device__ __forceinline__ float4 widen4(const __nv_bfloat16 *p) {
-    const uint2 v = *(const uint2 *)p;
-    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
-}
-__device__ __forceinline__ void copy16(void *dst, const void *src, bool on) { // zeros where it is off
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(on ? 16 : 0) : "memory");
-}
-
 // Two multiply-adds in one instruction
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     unsigned long long r;
@@ -52,12 +37,12 @@ inline size_t fma_smem(int dim, int kv_bytes, int rows, int keys) {
     return sizeof(float) * ((size_t)rows * (dim + FSP) + (size_t)rows * (keys + FSP) + 3 * rows) + 2 * (size_t)keys * (2 * dim * kv_bytes + F_PAD);
 }
 
-template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bounds__(FT, M == 64 ? 1 : F_PER_SM) tree_attn_fma_kernel(const TreeDev p) {
+template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bounds__(FT, F_PER_SM) tree_attn_fma_kernel(const TreeDev p) {
     extern __shared__ __align__(16) uint8_t fsm[];
     constexpr int SP = KEYS + FSP, KS = KEYS / 32, RW = M / (FT / 32); // RW: rows of a warp
     // A thread's scores: KT keys x R rows; its weighted sums: PR rows x four values, U times
-    constexpr int KT = M == 8 ? 1 : (M == 64 ? 4 : 2), TILES = KEYS / (8 * KT), GROUPS = FT / 32 / TILES, R = M / GROUPS / 4;
-    constexpr int PR = M == 64 ? 8 : 4, U = M == 32 ? 2 : 1;
+    constexpr int KT = M == 8 ? 1 : 2, TILES = KEYS / (8 * KT), GROUPS = FT / 32 / TILES, R = M / GROUPS / 4;
+    constexpr int PR = 4, U = M == 32 ? 2 : 1;
     const int D = p.dim, QP = D + FSP, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row_b = D * (int)sizeof(KV), key_b = row_b + F_PAD;
     float *const qs = (float *)fsm, *const sc = qs + M * QP, *const ms = sc + M * SP, *const ls = ms + M, *const cs = ls + M;
     uint8_t *const stage0 = (uint8_t *)(cs + M);
@@ -316,10 +301,6 @@ static int fma_ctas(const DeviceInfo &dev, int dim, int kv_bytes, int rows, int 
 static size_t meta_bytes(int ctas) { return ((size_t)ctas * TREE_META * sizeof(int4) + 255) / 256 * 256; }
 // Keys of a block: 64 while two CTAs with two stages of them fit an SM, else 32 (32 rows of 512 bytes: 303 us with 64 keys and one CTA, 268 with 32 and two).
 inline int fma_keys(int row_bytes) { return row_bytes <= 256 ? 64 : 32; }
-// 64 rows x 64 keys in one CTA per SM, with twice the sums per thread and no shared registers, for many rows over keys of 257 to 512 bytes in 32 bits: 232 us
-// where two CTAs of 32 x 32 take 268.  Over shorter keys two CTAs of 32 x 64 are faster: 242 us against 262.
-inline bool fma_64_rows(int dim, int kv_bytes) { return kv_bytes == 4 && dim > 64 && dim <= 128; }
-
 template <typename Q, typename KV, int M, int KEYS> static cudaError_t launch_fma_as(const DeviceInfo &dev, const TreeDev &t, bool pdl, cudaStream_t st) {
     const size_t smem = fma_smem(t.dim, sizeof(KV), M, KEYS);
     cudaError_t e = cudaFuncSetAttribute(tree_attn_fma_kernel<Q, KV, M, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, dev.max_smem_optin - F_STATIC);
@@ -332,8 +313,6 @@ template <typename Q, typename KV, int M, int KEYS> static cudaError_t launch_fm
 template <typename Q, typename KV> static cudaError_t launch_fma(const DeviceInfo &dev, const TreeDev &t, bool pdl, cudaStream_t st) {
     const long long rows = ((long long)t.n_rows * t.group + t.n_seq - 1) / t.n_seq; // per sequence and key head, on average
     const bool k64 = fma_keys(t.dim * (int)sizeof(KV)) == 64;
-    if constexpr (sizeof(KV) == 4)
-        if (rows > 32 && fma_64_rows(t.dim, sizeof(KV))) return launch_fma_as<Q, KV, 64, 64>(dev, t, pdl, st);
     if (rows > 16) return k64 ? launch_fma_as<Q, KV, 32, 64>(dev, t, pdl, st) : launch_fma_as<Q, KV, 32, 32>(dev, t, pdl, st);
     if (rows > 8) return k64 ? launch_fma_as<Q, KV, 16, 64>(dev, t, pdl, st) : launch_fma_as<Q, KV, 16, 32>(dev, t, pdl, st);
     return k64 ? launch_fma_as<Q, KV, 8, 64>(dev, t, pdl, st) : launch_fma_as<Q, KV, 8, 32>(dev, t, pdl, st);
@@ -344,15 +323,15 @@ template <typename Q, typename KV> static cudaError_t launch_fma(const DeviceInf
 using namespace ullm;
 
 // The work area begins with the CTAs' records (for the most CTAs of any kernel), then the partial results.
-static size_t tree_work_bytes(const DeviceInfo &dev, int dim, int kv_bytes, bool tc) {
-    const size_t fma = sizeof(float) * (size_t)dev.sm_count * F_PER_SM * 2 * (fma_64_rows(dim, kv_bytes) ? 64 : 32) * (dim + 2);
+static size_t tree_work_bytes(const DeviceInfo &dev, int dim, bool f32, bool tc) {
+    const size_t rows = f32 && tree_attn_split_supported(dim) ? 64 : 32, fma = sizeof(float) * (size_t)dev.sm_count * F_PER_SM * 2 * rows * (dim + 2); // of the largest tile
     return meta_bytes(dev.sm_count * F_PER_SM) + (tc ? std::max(fma, tree_attn_tc_work(dev.sm_count, dim)) : fma);
 }
 
 size_t ullm_cuda_tree_attn_work_bytes(const ullm_cuda_ctx *c, const ullm_kv_pages *kv, int dtype) {
     PoolDev pool;
     if (!c || !kv || pool_check(kv, &pool)) return 0;
-    return tree_work_bytes(c->dev, pool.head_dim, pool.elem_bytes, tree_attn_tc_supported(pool, dtype));
+    return tree_work_bytes(c->dev, pool.head_dim, dtype == ULLM_DTYPE_F32, tree_attn_tc_supported(pool, dtype));
 }
 
 int ullm_cuda_tree_attn_dev(ullm_cuda_ctx *c, const ullm_tree_attn *a, void *stream) {
@@ -406,6 +385,10 @@ int ullm_cuda_tree_attn_dev(ullm_cuda_ctx *c, const ullm_tree_attn *a, void *str
     if (tree_attn_tc_supported(pool, a->dtype)) e = launch_tree_attn_tc(c->dev, pool, a->dtype, t, c->d_status, c->use_pdl, st);
     if (e != cudaErrorNotSupported) { // (strides that a tensor map cannot describe go to the f32 kernel)
         ULLM_CUDA_TRY(c, e);
+        return ULLM_OK;
+    }
+    if (a->dtype == ULLM_DTYPE_F32 && tree_attn_split_supported(t.dim)) {
+        ULLM_CUDA_TRY(c, launch_tree_attn_split(c->dev, a->kv->dtype, t, c->use_pdl, st));
         return ULLM_OK;
     }
     if (a->dtype == ULLM_DTYPE_F16) e = launch_fma<__half, __half>(c->dev, t, c->use_pdl, st);

@@ -1,0 +1,374 @@
+// Attention of drafted rows over a paged cache with f32 queries: 32-bit products on the tensor cores.
+//
+// The formula is that of tree_attn.cu.  The tensor cores multiply 11-bit significands (tf32) and add in f32; a 32-bit value x is taken as the sum
+// x = a + b of its 11 leading bits, rounded to nearest, and the next 11, so that
+//   x y = a a' + a b' + b a'  within  2^-21 + 2^-22 + 2^-21 of |x y|,
+// which is less than what a sum of 64 products loses to f32 rounding at worst.  Values of 16 bits fit in one part: two products instead of three.
+//
+// A CTA of eight warps takes 16, 32 or 64 query rows and walks blocks of 64 keys, whose keys and values arrive by cp.async, as they lie in the pages, while the
+// block before is worked on.  A warp has 16 rows and a fixed share of every block's keys (8, 16 or 32), keeps a maximum, a sum and weighted
+// values for these keys alone, and the warps of a row meet once, at the end of the segment: there is no barrier between scores, softmax and weighted sums.
+// The accumulators of the scores are in the place where the products with the values want the weights.  The order of a head's values, and of the keys, within a
+// product is free as long as both sides agree; it is chosen so that a lane reads 16 neighbouring bytes.
+// On the CUDA cores (tree_attn.cu) the reads of shared memory bound the same work: 32 lanes x 16 bytes take four cycles and feed 32 multiply-adds per lane.
+// Rows are few (a group's heads x drafted tokens), so that tcgen05's tile of 128 rows would be empty for the most part.
+#include "engine.h"
+#include "tree_sched.cuh"
+
+#include <algorithm>
+
+namespace ullm {
+namespace {
+
+constexpr int XT = 256, XK = 64;     // threads; keys of a block
+constexpr int X_COST = 2, X_MIN = 2; // places that a unit costs beside its blocks; places that a CTA takes at least
+
+template <typename KV, int D, int M> struct SplitCfg {
+    static constexpr int RT = M / 16, KG = 8 / RT, NT = XK / KG / 8;   // row tiles; groups of keys; tiles of eight keys of a warp
+    // bytes from key to key: lanes four apart read different banks
+    static constexpr int KP = D * (int)sizeof(KV) + (sizeof(KV) == 4 ? 16 : 64), VP = D * (int)sizeof(KV) + 16;
+    static constexpr int QF = M * D;                                   // floats of one part of the queries
+    static constexpr int STAGE = XK * (KP + VP), SMEM = 2 * QF * (int)sizeof(float) + 2 * STAGE;
+    static constexpr int PER_SM = D == 64 ? 2 : 1;                     // CTAs: 128 or 255 registers a thread
+    static_assert(8 * 16 * D * (int)sizeof(float) <= 2 * STAGE, "the warps' results meet in the stages' memory");
+};
+
+// D += A B on 16 rows x 8 columns x 8 products
+__device__ __forceinline__ void mma8(float (&d)[4], const float4 &a, float b0, float b1) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(__float_as_uint(a.x)), "r"(__float_as_uint(a.y)), "r"(__float_as_uint(a.z)), "r"(__float_as_uint(a.w)), "r"(__float_as_uint(b0)),
+                   "r"(__float_as_uint(b1)));
+}
+// The 11 leading bits, rounded; what is left of an infinity or a NaN is NaN
+__device__ __forceinline__ float lead(float x) { return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u); }
+__device__ __forceinline__ float tail(float x, float a) { return x - a; }
+__device__ __forceinline__ float cut11(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
+// Eight neighbouring values as f32
+__device__ __forceinline__ void widen8(float (&x)[8], const float *p) {
+    const float4 a = *(const float4 *)p, b = *(const float4 *)(p + 4);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+__device__ __forceinline__ void widen8(float (&x)[8], const __half *p) {
+    const uint4 v = *(const uint4 *)p;
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 a = __half22float2(*(const __half2 *)&w[i]);
+        x[2 * i] = a.x, x[2 * i + 1] = a.y;
+    }
+}
+__device__ __forceinline__ void widen8(float (&x)[8], const __nv_bfloat16 *p) {
+    const uint4 v = *(const uint4 *)p;
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+// acc += (a + b) y for a y of the cache; z collects NaN where y is not finite
+template <typename KV> __device__ __forceinline__ void product(float (&acc)[4], const float4 &a, const float4 &b, float y0, float y1, float &z) {
+    if constexpr (sizeof(KV) == 4) {
+        const float h0 = lead(y0), h1 = lead(y1), l0 = tail(y0, h0), l1 = tail(y1, h1);
+        z += l0 + l1;
+        mma8(acc, a, cut11(l0), cut11(l1));
+        mma8(acc, b, h0, h1);
+        mma8(acc, a, h0, h1);
+    } else {
+        z = fmaf(y0, 0.f, fmaf(y1, 0.f, z));
+        mma8(acc, b, y0, y1);
+        mma8(acc, a, y0, y1);
+    }
+}
+
+template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (SplitCfg<KV, D, M>::PER_SM)) tree_attn_split_kernel(const TreeDev p) {
+    using C = SplitCfg<KV, D, M>;
+    extern __shared__ __align__(16) uint8_t xsm[];
+    float *const qa = (float *)xsm, *const qb = qa + C::QF; // the parts of the queries, as the products want them: 16 bytes per row tile, step and lane
+    uint8_t *const stage0 = (uint8_t *)(qb + C::QF);
+    __shared__ Seg seg;
+    __shared__ long long offs[2][XK]; // where the keys of a block lie: bytes behind p.k and p.v, -1 for none
+    __shared__ float2 ml[8][16];      // maximum and sum of each warp's rows
+    pdl_wait_prior();
+    pdl_launch_dependents();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int rt = warp % C::RT, kg = warp / C::RT, kbase = kg * C::NT * 8;
+    Sched<M, XK, X_COST, X_MIN> sched(p);
+    bool some = false;
+    if (warp == 0) {
+        if (lane == 0) p.meta[blockIdx.x * TREE_META] = make_int4(-1, 0, 0, 0);
+        __syncwarp();
+        some = sched.init();
+    }
+    constexpr int PIECES = D * (int)sizeof(KV) / 16, STEP = XT / PIECES; // 16-byte pieces of a row; rows that the threads take at once
+    const int piece_j = tid / PIECES, piece_c = tid % PIECES * 16;
+    for (;;) {
+        __syncthreads();
+        if (warp == 0) {
+            Seg next;
+            next.count = 0;
+            if (some) next = sched.next(p.meta + blockIdx.x * TREE_META);
+            if (lane == 0) seg = next;
+        }
+        __syncthreads();
+        const Seg w = seg;
+        if (!w.count) break;
+        SeqView v;
+        v.r0 = w.r0, v.n = w.n, v.id = w.id, v.ctx = w.ctx, v.kv = w.kv;
+        const int rows = w.rows, key_end = w.key_end, blk_end = w.blk + w.count;
+        auto token_of = [&](int r) { return (w.row0 + r) / p.group; };
+        auto head_of = [&](int r) { return w.h * p.group + (w.row0 + r) % p.group; };
+        const int *const table = p.blocks + (size_t)v.id * p.max_blocks;
+        auto page_at = [&](int token) { return token < key_end ? table[token / p.page_size] : -1; };
+        auto place = [&](int page, int token) { // a key behind the last, or of a page outside the pool, has none
+            return (unsigned)page < (unsigned)p.n_pages ? (page * p.page_stride + token % p.page_size * p.slot_stride + w.h * p.head_stride) * (long long)sizeof(KV) : -1ll;
+        };
+        auto fetch = [&](int blk, uint8_t *stage) { // zeros for a key that has no place
+            const long long *const at = offs[(blk - w.blk) & 1];
+#pragma unroll
+            for (int j0 = 0; j0 < XK; j0 += STEP) {
+                const int j = j0 + piece_j;
+                const long long off = at[j];
+                const bool on = off >= 0;
+                const long long from = on ? off + piece_c : 0;
+                copy16(stage + j * C::KP + piece_c, p.k + from, on);
+                copy16(stage + XK * C::KP + j * C::VP + piece_c, p.v + from, on);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        if (tid < 2 * XK) { // the first two blocks' keys, one per thread
+            const int token = w.blk * XK + tid;
+            offs[tid / XK][tid % XK] = place(page_at(token), token);
+        }
+        __syncthreads();
+        fetch(w.blk, stage0);
+        for (int i = tid; i < M * (D / 4); i += XT) { // queries: value 8 t + e of 32 is product t (or t + 4, for e >= 4) of step e % 4
+            const int r = i / (D / 4), d = i % (D / 4) * 4;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < rows) x = *(const float4 *)((const float *)p.q + (v.r0 + token_of(r)) * p.q_stride + (long long)head_of(r) * D + d);
+            const float y[4] = {x.x, x.y, x.z, x.w};
+            const int step = d / 32 * 4, l = r % 8 * 4 + d % 32 / 8, at = (((r / 16) * (D / 8) + step) * 32 + l) * 4 + (r % 16 / 8 + d % 8 / 4 * 2);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float a = lead(y[e]);
+                qa[at + e * 128] = a, qb[at + e * 128] = tail(y[e], a);
+            }
+        }
+        const bool work = rt * 16 < rows;
+        const int row[2] = {rt * 16 + g, rt * 16 + g + 8}, token[2] = {token_of(row[0]), token_of(row[1])};
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}; // l: this lane's share
+        float o[D / 8][4]; // [4 c + i]: value 32 c + 8 t + i of rows 0 and 1 in 0 and 2, value 32 c + 8 t + 4 + i in 1 and 3
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+        for (int blk = w.blk; blk < blk_end; ++blk) {
+            uint8_t *const ks = stage0 + ((blk - w.blk) & 1) * C::STAGE, *const vs = ks + XK * C::KP;
+            const int k0 = blk * XK;
+            if (blk + 1 < blk_end) {
+                fetch(blk + 1, stage0 + ((blk + 1 - w.blk) & 1) * C::STAGE);
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+            } else {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+            }
+            __syncthreads();
+            // the block after the next: its page numbers travel while this one is worked on
+            const int ahead = (blk + 2) * XK + tid;
+            const bool more = tid < XK && blk + 2 < blk_end;
+            const int page = more ? page_at(ahead) : -1;
+            if (work && k0 + kbase < key_end) {
+                float s[C::NT][4], z = 0.f;
+#pragma unroll
+                for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) { // (unrolled, it held more than the registers of two CTAs)
+                    float y[C::NT][8];
+#pragma unroll
+                    for (int n = 0; n < C::NT; ++n) widen8(y[n], (const KV *)(ks + (kbase + n * 8 + g) * C::KP) + c * 32 + t * 8);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int at = ((rt * (D / 8) + c * 4 + i) * 32 + lane) * 4;
+                        const float4 a = *(const float4 *)(qa + at);
+                        float4 b = *(const float4 *)(qb + at);
+                        b.x = cut11(b.x), b.y = cut11(b.y), b.z = cut11(b.z), b.w = cut11(b.w);
+#pragma unroll
+                        for (int n = 0; n < C::NT; ++n) product<KV>(s[n], a, b, y[n][i], y[n][4 + i], z);
+                    }
+                }
+                if (__any_sync(0xffffffffu, z != z)) { // a key that is not finite: the products one by one, since b times an infinity is not what x times it is
+#pragma unroll
+                    for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const KV *const key = (const KV *)(ks + (kbase + n * 8 + 2 * t + (e & 1)) * C::KP);
+                            float sum = 0.f;
+                            for (int d = 0; d < D; ++d) {
+                                const int at = ((rt * (D / 8) + d / 32 * 4 + d % 4) * 32 + g * 4 + d % 32 / 8) * 4 + (e >> 1) + d % 8 / 4 * 2;
+                                sum = fmaf(qa[at] + qb[at], (float)key[d], sum);
+                            }
+                            s[n][e] = sum;
+                        }
+                }
+                const bool all = k0 + kbase + C::NT * 8 <= min(key_end, v.ctx); // every row sees all of them
+                float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[n][e] *= p.scale_log2;
+                        if (!all) {
+                            const int key = k0 + kbase + n * 8 + 2 * t + (e & 1);
+                            bool see = key < key_end && row[e >> 1] < rows;
+                            if (see && key >= v.ctx) see = sees(p, v, token[e >> 1], key - v.ctx);
+                            if (!see) s[n][e] = -INFINITY;
+                        }
+                        mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
+                    }
+                float corr[2];
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    mx[a] = fmaxf(mx[a], __shfl_xor_sync(0xffffffffu, mx[a], 1));
+                    mx[a] = fmaxf(fmaxf(mx[a], __shfl_xor_sync(0xffffffffu, mx[a], 2)), m[a]);
+                    corr[a] = m[a] == -INFINITY ? 0.f : exp2f(m[a] - mx[a]);
+                    m[a] = mx[a], l[a] *= corr[a];
+                }
+                // nothing seen so far: all weights are zero.  (A score of +inf or NaN gives NaN, as the formula does.)
+#pragma unroll
+                for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[n][e] = s[n][e] == -INFINITY ? 0.f : exp2f(s[n][e] - m[e >> 1]);
+                        l[e >> 1] += s[n][e];
+                    }
+                if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+#pragma unroll
+                    for (int n = 0; n < D / 8; ++n) o[n][0] *= corr[0], o[n][1] *= corr[0], o[n][2] *= corr[1], o[n][3] *= corr[1];
+                }
+                // Values that are not finite must not reach a row that does not see them (0 * inf), nor be split: they become zeros here and are added at the end.
+                {
+                    KV *const own = (KV *)(vs + kbase * C::VP);
+                    float bad = 0.f;
+#pragma unroll 2
+                    for (int i = lane; i < C::NT * 8 * (D / 8); i += 32) {
+                        float y[8];
+                        widen8(y, (const KV *)((uint8_t *)own + i / (D / 8) * C::VP) + i % (D / 8) * 8);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) bad = fmaf(y[e], 0.f, bad);
+                    }
+                    if (__any_sync(0xffffffffu, bad != bad)) {
+                        for (int i = lane; i < C::NT * 8 * D; i += 32) {
+                            KV *const at = (KV *)((uint8_t *)own + i / D * C::VP) + i % D;
+                            if (!isfinite((float)*at)) *at = (KV)0.f;
+                        }
+                        seg.odd = 1;
+                        __syncwarp();
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < C::NT; ++n) {
+                    const float4 x = make_float4(s[n][0], s[n][2], s[n][1], s[n][3]); // product t is key 2 t, product t + 4 key 2 t + 1
+                    const float4 a = make_float4(lead(x.x), lead(x.y), lead(x.z), lead(x.w));
+                    const float4 b = make_float4(cut11(tail(x.x, a.x)), cut11(tail(x.y, a.y)), cut11(tail(x.z, a.z)), cut11(tail(x.w, a.w)));
+                    const KV *const v0 = (const KV *)(vs + (kbase + n * 8 + 2 * t) * C::VP) + g * 4, *const v1 = (const KV *)((const uint8_t *)v0 + C::VP);
+                    float unused = 0.f;
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        const float4 y0 = widen4(v0 + c * 32), y1 = widen4(v1 + c * 32);
+                        product<KV>(o[c * 4], a, b, y0.x, y1.x, unused);
+                        product<KV>(o[c * 4 + 1], a, b, y0.y, y1.y, unused);
+                        product<KV>(o[c * 4 + 2], a, b, y0.z, y1.z, unused);
+                        product<KV>(o[c * 4 + 3], a, b, y0.w, y1.w, unused);
+                    }
+                }
+            }
+            if (more) offs[(blk - w.blk) & 1][tid] = place(page, ahead);
+            __syncthreads(); // the stage is free
+        }
+        // the warps' results meet in the stages' memory
+        float *const red = (float *)stage0;
+        if (work) {
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                float sum = l[a];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                if (t == 0) ml[warp][g + 8 * a] = make_float2(m[a], sum);
+                float *const to = red + (warp * 16 + g + 8 * a) * D + t * 8;
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    *(float4 *)(to + c * 32) = make_float4(o[4 * c][2 * a], o[4 * c + 1][2 * a], o[4 * c + 2][2 * a], o[4 * c + 3][2 * a]);
+                    *(float4 *)(to + c * 32 + 4) = make_float4(o[4 * c][2 * a + 1], o[4 * c + 1][2 * a + 1], o[4 * c + 2][2 * a + 1], o[4 * c + 3][2 * a + 1]);
+                }
+            }
+        }
+        __syncthreads();
+        const bool whole = w.flags & 1, odd = seg.odd;
+        float *const mine = whole ? nullptr : part_of<M>(p, blockIdx.x, w.flags >> 1);
+        for (int i = tid; i < rows * (D / 4); i += XT) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < C::KG; ++k) top = fmaxf(top, ml[k * C::RT + r / 16][r % 16].x);
+#pragma unroll
+            for (int k = 0; k < C::KG; ++k) {
+                const int wp = k * C::RT + r / 16;
+                const float2 a = ml[wp][r % 16];
+                const float c = a.x == -INFINITY ? 0.f : exp2f(a.x - top);
+                const float4 y = *(const float4 *)(red + (wp * 16 + r % 16) * D + d);
+                sum += a.y * c; // (NaN where a score was NaN)
+                x.x += c * y.x, x.y += c * y.y, x.z += c * y.z, x.w += c * y.w;
+            }
+            if (odd) { // infinities and NaN of the tokens that the row does see
+                const int last = min(key_end, blk_end * XK), me = token_of(r);
+                for (int key = w.blk * XK; key < last; ++key) {
+                    const int page = table[key / p.page_size];
+                    if ((unsigned)page >= (unsigned)p.n_pages || (key >= v.ctx && !sees(p, v, me, key - v.ctx))) continue;
+                    const float4 y = widen4((const KV *)p.v + page * p.page_stride + key % p.page_size * p.slot_stride + w.h * p.head_stride + d);
+                    if (!isfinite(y.x)) x.x += y.x;
+                    if (!isfinite(y.y)) x.y += y.y;
+                    if (!isfinite(y.z)) x.z += y.z;
+                    if (!isfinite(y.w)) x.w += y.w;
+                }
+            }
+            if (whole) {
+                const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+                const float4 y = sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+                *(float4 *)((float *)p.out + (v.r0 + token_of(r)) * p.out_stride + (long long)head_of(r) * D + d) = y;
+            } else {
+                *(float4 *)(mine + (size_t)r * D + d) = x;
+                if (d == 0) *(float2 *)(mine + (size_t)M * D + 2 * r) = make_float2(top, sum);
+            }
+        }
+    }
+}
+
+template <typename KV, int D, int M> cudaError_t launch_as(const DeviceInfo &dev, const TreeDev &t, bool pdl, cudaStream_t st) {
+    using C = SplitCfg<KV, D, M>;
+    cudaError_t e = cudaFuncSetAttribute(tree_attn_split_kernel<KV, D, M>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return e;
+    const int ctas = dev.sm_count * C::PER_SM;
+    e = launch_kernel(tree_attn_split_kernel<KV, D, M>, dim3(ctas), dim3(XT), (size_t)C::SMEM, st, pdl, t);
+    if (e != cudaSuccess) return e;
+    return launch_kernel(tree_join_kernel<float, M>, dim3(dev.sm_count * JOIN_PER_SM), dim3(32 * JOIN_WARPS), 0, st, pdl, t, ctas);
+}
+template <typename KV> cudaError_t launch_for(const DeviceInfo &dev, const TreeDev &t, bool pdl, cudaStream_t st) {
+    const long long rows = ((long long)t.n_rows * t.group + t.n_seq - 1) / t.n_seq; // per sequence and key head, on average
+    if (t.dim == 64) {
+        if (rows <= 16) return launch_as<KV, 64, 16>(dev, t, pdl, st);
+        return rows <= 32 ? launch_as<KV, 64, 32>(dev, t, pdl, st) : launch_as<KV, 64, 64>(dev, t, pdl, st);
+    }
+    if (rows <= 16) return launch_as<KV, 128, 16>(dev, t, pdl, st);
+    return rows <= 32 ? launch_as<KV, 128, 32>(dev, t, pdl, st) : launch_as<KV, 128, 64>(dev, t, pdl, st);
+}
+
+} // namespace
+
+bool tree_attn_split_supported(int dim) { return dim == 64 || dim == 128; }
+
+cudaError_t launch_tree_attn_split(const DeviceInfo &dev, int kv_dtype, const TreeDev &t, bool pdl, cudaStream_t st) {
+    if (kv_dtype == ULLM_DTYPE_F32) return launch_for<float>(dev, t, pdl, st);
+    return kv_dtype == ULLM_DTYPE_F16 ? launch_for<__half>(dev, t, pdl, st) : launch_for<__nv_bfloat16>(dev, t, pdl, st);
+}
+
+} // namespace ullm

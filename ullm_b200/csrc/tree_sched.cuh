@@ -224,6 +224,21 @@ template <int M> __device__ __forceinline__ float *part_of(const TreeDev &p, int
     return p.part + ((size_t)c * 2 + slot) * M * (p.dim + 2);
 }
 
+// Four neighbouring values as f32
+__device__ __forceinline__ float4 widen4(const float *p) { return *(const float4 *)p; }
+__device__ __forceinline__ float4 widen4(const __half *p) {
+    const uint2 v = *(const uint2 *)p;
+    const float2 a = __half22float2(*(const __half2 *)&v.x), b = __half22float2(*(const __half2 *)&v.y);
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ float4 widen4(const __nv_bfloat16 *p) {
+    const uint2 v = *(const uint2 *)p;
+    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+}
+__device__ __forceinline__ void copy16(void *dst, const void *src, bool on) { // zeros where it is off
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+
 template <typename T> __device__ __forceinline__ T out_from(float v);
 template <> __device__ __forceinline__ float out_from<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half out_from<__half>(float v) { return __float2half_rn(v); }

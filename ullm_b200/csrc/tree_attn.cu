@@ -4,12 +4,13 @@
 //
 // over the keys that row i sees, in one pass with a running maximum m, sum l and weighted sum of values, all f32.
 //
-// tree_attn_fma_kernel: f32 arithmetic on the CUDA cores, for f32 queries and for whatever the tensor-core kernel (tree_attn_tc.cu) does not take.
-// A CTA of 256 threads holds 8 to 64 query rows in shared memory and walks blocks of keys; the next block's keys and values arrive by cp.async, as they lie
-// in the pages, while one is worked on.  A warp's scores form a tile, a thread's one of up to 4 keys x 4 rows, so that lanes share what they read from
+// tree_attn_fma_kernel: f32 arithmetic on the CUDA cores, for the head sizes, page sizes and strides that the kernels on the tensor cores do not take
+// (tree_attn_tc.cu: 16-bit queries; tree_attn_split.cu: f32 queries, heads of 64 and 128).
+// A CTA of 256 threads holds 8 to 32 query rows in shared memory and walks blocks of keys; the next block's keys and values arrive by cp.async, as they lie
+// in the pages, while one is worked on.  A warp's scores form a tile, a thread's one of up to 2 keys x 4 rows, so that lanes share what they read from
 // shared memory: with a key per lane these reads took three times as long as the multiply-adds, which go two to an instruction.
-// It is bound by the turns that scores, softmax and weighted sums take between barriers with 8 to 16 warps on an SM: 22 of the 72 TFLOP/s of the f32 units
-// with 64 rows and heads of 128, 2.7 TB/s with four rows per key head.
+// Shared memory bounds it all the same: 32 lanes x 16 bytes take four cycles, six such reads feed a tile's 32 multiply-adds per lane, which need eight.
+// 90 rows of each of 16 sequences over heads of 64 in 32 bits: 16.5 TFLOP/s of the 72 of the f32 units.
 #include "engine.h"
 #include "tree_sched.cuh"
 
@@ -323,15 +324,15 @@ template <typename Q, typename KV> static cudaError_t launch_fma(const DeviceInf
 using namespace ullm;
 
 // The work area begins with the CTAs' records (for the most CTAs of any kernel), then the partial results.
-static size_t tree_work_bytes(const DeviceInfo &dev, int dim, bool f32, bool tc) {
-    const size_t rows = f32 && tree_attn_split_supported(dim) ? 64 : 32, fma = sizeof(float) * (size_t)dev.sm_count * F_PER_SM * 2 * rows * (dim + 2); // of the largest tile
+static size_t tree_work_bytes(const DeviceInfo &dev, int dim, bool tc) {
+    const size_t fma = sizeof(float) * (size_t)dev.sm_count * F_PER_SM * 2 * 32 * (dim + 2); // of 32 rows, the most that a tile of the f32 kernels has
     return meta_bytes(dev.sm_count * F_PER_SM) + (tc ? std::max(fma, tree_attn_tc_work(dev.sm_count, dim)) : fma);
 }
 
 size_t ullm_cuda_tree_attn_work_bytes(const ullm_cuda_ctx *c, const ullm_kv_pages *kv, int dtype) {
     PoolDev pool;
     if (!c || !kv || pool_check(kv, &pool)) return 0;
-    return tree_work_bytes(c->dev, pool.head_dim, dtype == ULLM_DTYPE_F32, tree_attn_tc_supported(pool, dtype));
+    return tree_work_bytes(c->dev, pool.head_dim, tree_attn_tc_supported(pool, dtype));
 }
 
 int ullm_cuda_tree_attn_dev(ullm_cuda_ctx *c, const ullm_tree_attn *a, void *stream) {

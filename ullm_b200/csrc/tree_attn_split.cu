@@ -5,9 +5,10 @@
 //   x y = a a' + a b' + b a'  within  2^-21 + 2^-22 + 2^-21 of |x y|,
 // which is less than what a sum of 64 products loses to f32 rounding at worst.  Values of 16 bits fit in one part: two products instead of three.
 //
-// A CTA of eight warps takes 16, 32 or 64 query rows and walks blocks of 64 keys, whose keys and values arrive by cp.async, as they lie in the pages, while the
-// block before is worked on.  A warp has 16 rows and a fixed share of every block's keys (8, 16 or 32), keeps a maximum, a sum and weighted
-// values for these keys alone, and the warps of a row meet once, at the end of the segment: there is no barrier between scores, softmax and weighted sums.
+// A CTA of eight warps takes 16 or 32 query rows and walks blocks of 64 keys, whose keys and values arrive by cp.async, as they lie in the pages, while the
+// block before is worked on.  A warp has 16 rows and a fixed share of every block's keys (8 or 16), keeps a maximum, a sum and weighted
+// values for these keys alone, and the warps of a row meet once, at the end of the segment: there is no barrier between scores, softmax and weighted sums,
+// and only the warps over the same keys wait for one another between blocks.
 // The accumulators of the scores are in the place where the products with the values want the weights.  The order of a head's values, and of the keys, within a
 // product is free as long as both sides agree; it is chosen so that a lane reads 16 neighbouring bytes.
 // On the CUDA cores (tree_attn.cu) the reads of shared memory bound the same work: 32 lanes x 16 bytes take four cycles and feed 32 multiply-adds per lane.
@@ -21,7 +22,7 @@ namespace ullm {
 namespace {
 
 constexpr int XT = 256, XK = 64;     // threads; keys of a block
-constexpr int X_COST = 2, X_MIN = 2; // places that a unit costs beside its blocks; places that a CTA takes at least
+constexpr int X_COST = 1, X_MIN = 2; // places that a unit costs beside its blocks; places that a CTA takes at least
 
 template <typename KV, int D, int M> struct SplitCfg {
     static constexpr int RT = M / 16, KG = 8 / RT, NT = XK / KG / 8;   // row tiles; groups of keys; tiles of eight keys of a warp
@@ -64,18 +65,29 @@ __device__ __forceinline__ void widen8(float (&x)[8], const __nv_bfloat16 *p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
 }
-// acc += (a + b) y for a y of the cache; z collects NaN where y is not finite
-template <typename KV> __device__ __forceinline__ void product(float (&acc)[4], const float4 &a, const float4 &b, float y0, float y1, float &z) {
+// acc[n] += (a + b) y[n] for several y of the cache, product by product, so that those into one place are apart; z collects NaN where a y is not finite.
+// SETS: places per sum, 1 to 3
+template <typename KV, int N, int SETS> __device__ __forceinline__ void products(float (&acc)[N][SETS][4], const float4 &a, const float4 &b, const float (&y0)[N], const float (&y1)[N], float &z) {
     if constexpr (sizeof(KV) == 4) {
-        const float h0 = lead(y0), h1 = lead(y1), l0 = tail(y0, h0), l1 = tail(y1, h1);
-        z += l0 + l1;
-        mma8(acc, a, cut11(l0), cut11(l1));
-        mma8(acc, b, h0, h1);
-        mma8(acc, a, h0, h1);
+        float h0[N], h1[N], l0[N], l1[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            h0[n] = lead(y0[n]), h1[n] = lead(y1[n]), l0[n] = tail(y0[n], h0[n]), l1[n] = tail(y1[n], h1[n]);
+            z += l0[n] + l1[n];
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) mma8(acc[n][SETS - 1], a, cut11(l0[n]), cut11(l1[n]));
+#pragma unroll
+        for (int n = 0; n < N; ++n) mma8(acc[n][SETS / 2], b, h0[n], h1[n]);
+#pragma unroll
+        for (int n = 0; n < N; ++n) mma8(acc[n][0], a, h0[n], h1[n]);
     } else {
-        z = fmaf(y0, 0.f, fmaf(y1, 0.f, z));
-        mma8(acc, b, y0, y1);
-        mma8(acc, a, y0, y1);
+#pragma unroll
+        for (int n = 0; n < N; ++n) z = fmaf(y0[n], 0.f, fmaf(y1[n], 0.f, z));
+#pragma unroll
+        for (int n = 0; n < N; ++n) mma8(acc[n][SETS - 1], b, y0[n], y1[n]);
+#pragma unroll
+        for (int n = 0; n < N; ++n) mma8(acc[n][0], a, y0[n], y1[n]);
     }
 }
 
@@ -98,8 +110,13 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
         __syncwarp();
         some = sched.init();
     }
-    constexpr int PIECES = D * (int)sizeof(KV) / 16, STEP = XT / PIECES; // 16-byte pieces of a row; rows that the threads take at once
-    const int piece_j = tid / PIECES, piece_c = tid % PIECES * 16;
+    // The warps over the same keys fetch them and wait for one another, and for no others.
+    constexpr int PIECES = D * (int)sizeof(KV) / 16, TG = 32 * C::RT, STEP = TG / PIECES; // 16-byte pieces of a row; threads of such a group; rows that they take at once
+    const int tg = rt * 32 + lane, piece_j = tg / PIECES, piece_c = tg % PIECES * 16;
+    auto meet = [&] {
+        if constexpr (C::RT == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(1 + kg), "n"(TG) : "memory");
+    };
     for (;;) {
         __syncthreads();
         if (warp == 0) {
@@ -124,8 +141,8 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
         auto fetch = [&](int blk, uint8_t *stage) { // zeros for a key that has no place
             const long long *const at = offs[(blk - w.blk) & 1];
 #pragma unroll
-            for (int j0 = 0; j0 < XK; j0 += STEP) {
-                const int j = j0 + piece_j;
+            for (int j0 = 0; j0 < C::NT * 8; j0 += STEP) {
+                const int j = kbase + j0 + piece_j;
                 const long long off = at[j];
                 const bool on = off >= 0;
                 const long long from = on ? off + piece_c : 0;
@@ -134,11 +151,12 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
-        if (tid < 2 * XK) { // the first two blocks' keys, one per thread
-            const int token = w.blk * XK + tid;
-            offs[tid / XK][tid % XK] = place(page_at(token), token);
+        const bool mine = tg < C::NT * 8; // threads that look up a key each
+        if (mine) {                       // of the first two blocks
+            const int key = w.blk * XK + kbase + tg, page0 = page_at(key), page1 = page_at(key + XK);
+            offs[0][kbase + tg] = place(page0, key), offs[1][kbase + tg] = place(page1, key + XK);
         }
-        __syncthreads();
+        meet();
         fetch(w.blk, stage0);
         for (int i = tid; i < M * (D / 4); i += XT) { // queries: value 8 t + e of 32 is product t (or t + 4, for e >= 4) of step e % 4
             const int r = i / (D / 4), d = i % (D / 4) * 4;
@@ -152,14 +170,13 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
                 qa[at + e * 128] = a, qb[at + e * 128] = tail(y[e], a);
             }
         }
+        __syncthreads();
         const bool work = rt * 16 < rows;
         const int row[2] = {rt * 16 + g, rt * 16 + g + 8}, token[2] = {token_of(row[0]), token_of(row[1])};
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}; // l: this lane's share
-        float o[D / 8][4]; // [4 c + i]: value 32 c + 8 t + i of rows 0 and 1 in 0 and 2, value 32 c + 8 t + 4 + i in 1 and 3
+        float o[D / 32][4][1][4]; // [c][i]: value 32 c + 8 t + i of rows 0 and 1 in 0 and 2, value 32 c + 8 t + 4 + i in 1 and 3
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+        for (int n = 0; n < D / 2; ++n) o[n / 16][n / 4 % 4][0][n % 4] = 0.f;
         for (int blk = w.blk; blk < blk_end; ++blk) {
             uint8_t *const ks = stage0 + ((blk - w.blk) & 1) * C::STAGE, *const vs = ks + XK * C::KP;
             const int k0 = blk * XK;
@@ -169,17 +186,18 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
             } else {
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
             }
-            __syncthreads();
+            meet();
             // the block after the next: its page numbers travel while this one is worked on
-            const int ahead = (blk + 2) * XK + tid;
-            const bool more = tid < XK && blk + 2 < blk_end;
+            const int ahead = (blk + 2) * XK + kbase + tg;
+            const bool more = mine && blk + 2 < blk_end;
             const int page = more ? page_at(ahead) : -1;
             if (work && k0 + kbase < key_end) {
-                float s[C::NT][4], z = 0.f;
+                constexpr int SETS = C::NT == 1 ? 3 : 2; // a product waits for the one before it in its place: three places at least
+                float parts[C::NT][SETS][4], s[C::NT][4], z = 0.f;
 #pragma unroll
                 for (int n = 0; n < C::NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+                    for (int e = 0; e < SETS * 4; ++e) parts[n][e / 4][e % 4] = 0.f;
 #pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) { // (unrolled, it held more than the registers of two CTAs)
                     float y[C::NT][8];
@@ -191,10 +209,20 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
                         const float4 a = *(const float4 *)(qa + at);
                         float4 b = *(const float4 *)(qb + at);
                         b.x = cut11(b.x), b.y = cut11(b.y), b.z = cut11(b.z), b.w = cut11(b.w);
+                        float y0[C::NT], y1[C::NT];
 #pragma unroll
-                        for (int n = 0; n < C::NT; ++n) product<KV>(s[n], a, b, y[n][i], y[n][4 + i], z);
+                        for (int n = 0; n < C::NT; ++n) y0[n] = y[n][i], y1[n] = y[n][4 + i];
+                        products<KV>(parts, a, b, y0, y1, z);
                     }
                 }
+#pragma unroll
+                for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[n][e] = parts[n][0][e];
+#pragma unroll
+                        for (int k = 1; k < SETS; ++k) s[n][e] += parts[n][k][e];
+                    }
                 if (__any_sync(0xffffffffu, z != z)) { // a key that is not finite: the products one by one, since b times an infinity is not what x times it is
 #pragma unroll
                     for (int n = 0; n < C::NT; ++n)
@@ -242,7 +270,7 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
                     }
                 if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
 #pragma unroll
-                    for (int n = 0; n < D / 8; ++n) o[n][0] *= corr[0], o[n][1] *= corr[0], o[n][2] *= corr[1], o[n][3] *= corr[1];
+                    for (int n = 0; n < D / 2; ++n) o[n / 16][n / 4 % 4][0][n % 4] *= corr[n % 4 / 2];
                 }
                 // Values that are not finite must not reach a row that does not see them (0 * inf), nor be split: they become zeros here and are added at the end.
                 {
@@ -274,16 +302,15 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
 #pragma unroll
                     for (int c = 0; c < D / 32; ++c) {
                         const float4 y0 = widen4(v0 + c * 32), y1 = widen4(v1 + c * 32);
-                        product<KV>(o[c * 4], a, b, y0.x, y1.x, unused);
-                        product<KV>(o[c * 4 + 1], a, b, y0.y, y1.y, unused);
-                        product<KV>(o[c * 4 + 2], a, b, y0.z, y1.z, unused);
-                        product<KV>(o[c * 4 + 3], a, b, y0.w, y1.w, unused);
+                        const float w0[4] = {y0.x, y0.y, y0.z, y0.w}, w1[4] = {y1.x, y1.y, y1.z, y1.w};
+                        products<KV>(o[c], a, b, w0, w1, unused);
                     }
                 }
             }
-            if (more) offs[(blk - w.blk) & 1][tid] = place(page, ahead);
-            __syncthreads(); // the stage is free
+            if (more) offs[(blk - w.blk) & 1][kbase + tg] = place(page, ahead);
+            meet(); // the stage is free
         }
+        __syncthreads();
         // the warps' results meet in the stages' memory
         float *const red = (float *)stage0;
         if (work) {
@@ -296,14 +323,14 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
                 float *const to = red + (warp * 16 + g + 8 * a) * D + t * 8;
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) {
-                    *(float4 *)(to + c * 32) = make_float4(o[4 * c][2 * a], o[4 * c + 1][2 * a], o[4 * c + 2][2 * a], o[4 * c + 3][2 * a]);
-                    *(float4 *)(to + c * 32 + 4) = make_float4(o[4 * c][2 * a + 1], o[4 * c + 1][2 * a + 1], o[4 * c + 2][2 * a + 1], o[4 * c + 3][2 * a + 1]);
+                    *(float4 *)(to + c * 32) = make_float4(o[c][0][0][2 * a], o[c][1][0][2 * a], o[c][2][0][2 * a], o[c][3][0][2 * a]);
+                    *(float4 *)(to + c * 32 + 4) = make_float4(o[c][0][0][2 * a + 1], o[c][1][0][2 * a + 1], o[c][2][0][2 * a + 1], o[c][3][0][2 * a + 1]);
                 }
             }
         }
         __syncthreads();
         const bool whole = w.flags & 1, odd = seg.odd;
-        float *const mine = whole ? nullptr : part_of<M>(p, blockIdx.x, w.flags >> 1);
+        float *const to = whole ? nullptr : part_of<M>(p, blockIdx.x, w.flags >> 1);
         for (int i = tid; i < rows * (D / 4); i += XT) {
             const int r = i / (D / 4), d = i % (D / 4) * 4;
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -336,8 +363,8 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
                 const float4 y = sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
                 *(float4 *)((float *)p.out + (v.r0 + token_of(r)) * p.out_stride + (long long)head_of(r) * D + d) = y;
             } else {
-                *(float4 *)(mine + (size_t)r * D + d) = x;
-                if (d == 0) *(float2 *)(mine + (size_t)M * D + 2 * r) = make_float2(top, sum);
+                *(float4 *)(to + (size_t)r * D + d) = x;
+                if (d == 0) *(float2 *)(to + (size_t)M * D + 2 * r) = make_float2(top, sum);
             }
         }
     }
@@ -352,14 +379,17 @@ template <typename KV, int D, int M> cudaError_t launch_as(const DeviceInfo &dev
     if (e != cudaSuccess) return e;
     return launch_kernel(tree_join_kernel<float, M>, dim3(dev.sm_count * JOIN_PER_SM), dim3(32 * JOIN_WARPS), 0, st, pdl, t, ctas);
 }
-template <typename KV> cudaError_t launch_for(const DeviceInfo &dev, const TreeDev &t, bool pdl, cudaStream_t st) {
-    const long long rows = ((long long)t.n_rows * t.group + t.n_seq - 1) / t.n_seq; // per sequence and key head, on average
-    if (t.dim == 64) {
-        if (rows <= 16) return launch_as<KV, 64, 16>(dev, t, pdl, st);
-        return rows <= 32 ? launch_as<KV, 64, 32>(dev, t, pdl, st) : launch_as<KV, 64, 64>(dev, t, pdl, st);
-    }
-    if (rows <= 16) return launch_as<KV, 128, 16>(dev, t, pdl, st);
-    return rows <= 32 ? launch_as<KV, 128, 32>(dev, t, pdl, st) : launch_as<KV, 128, 64>(dev, t, pdl, st);
+template <typename KV, int D> cudaError_t launch_for(const DeviceInfo &dev, const TreeDev &t, bool pdl, cudaStream_t st) {
+    // Rows per sequence and key head on average (the lengths themselves are on the device; either way is right for any of them).
+    const long long rows = ((long long)t.n_rows * t.group + t.n_seq - 1) / t.n_seq;
+    // Tiles of 32 rows split the keys half as often (90 rows: 149 us, with 16 rows 179; 64 rows take 160), but 16 rows spread a little work over more CTAs, where
+    // even tables in full use would give a CTA no more than four blocks (24 units of 28 rows and up to 2,000 keys: 21.8 us, with 32 rows 24.0).
+    const long long blocks = (rows + 31) / 32 * t.n_seq * t.n_kv * (((long long)t.max_blocks * t.page_size + XK - 1) / XK);
+    if (rows <= 16 || blocks <= 4 * dev.sm_count * SplitCfg<KV, D, 16>::PER_SM) return launch_as<KV, D, 16>(dev, t, pdl, st);
+    return launch_as<KV, D, 32>(dev, t, pdl, st);
+}
+template <typename KV> cudaError_t launch_dim(const DeviceInfo &dev, const TreeDev &t, bool pdl, cudaStream_t st) {
+    return t.dim == 64 ? launch_for<KV, 64>(dev, t, pdl, st) : launch_for<KV, 128>(dev, t, pdl, st);
 }
 
 } // namespace
@@ -367,8 +397,8 @@ template <typename KV> cudaError_t launch_for(const DeviceInfo &dev, const TreeD
 bool tree_attn_split_supported(int dim) { return dim == 64 || dim == 128; }
 
 cudaError_t launch_tree_attn_split(const DeviceInfo &dev, int kv_dtype, const TreeDev &t, bool pdl, cudaStream_t st) {
-    if (kv_dtype == ULLM_DTYPE_F32) return launch_for<float>(dev, t, pdl, st);
-    return kv_dtype == ULLM_DTYPE_F16 ? launch_for<__half>(dev, t, pdl, st) : launch_for<__nv_bfloat16>(dev, t, pdl, st);
+    if (kv_dtype == ULLM_DTYPE_F32) return launch_dim<float>(dev, t, pdl, st);
+    return kv_dtype == ULLM_DTYPE_F16 ? launch_dim<__half>(dev, t, pdl, st) : launch_dim<__nv_bfloat16>(dev, t, pdl, st);
 }
 
 } // namespace ullm

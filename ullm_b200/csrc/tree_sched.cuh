@@ -246,20 +246,102 @@ template <> __device__ __forceinline__ __nv_bfloat16 out_from<__nv_bfloat16>(flo
 
 // Joins the parts of the units that were cut, in the order of the CTAs:
 //   out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c.
-// A fixed number of CTAs share the rows of all cut units; every CTA reads the records.  Four warps take a row together (or one, where units have few
-// parts), each every fourth part, up to eight at a time; a row's values, references and sums are all on their way at once, because
-// the kernel is bound by round trips to memory: with weights first and values after them a row took 6,500 cycles.
-constexpr int JOIN_WARPS = 8, JOIN_MAX = 1024, JOIN_PER_SM = 4; // JOIN_MAX: CTAs of the attention kernel at most
-template <typename O, int M> __global__ void __launch_bounds__(32 * JOIN_WARPS) tree_join_kernel(const TreeDev p, int ctas) {
-    struct Duty {
-        int front;                // rows of the units in front of it
-        short c, c0;              // the CTAs in which it ends and begins ...
-        int r0, t;
-        unsigned short h, how;    // how: slot | lanes << 1
-    };
-    __shared__ Duty duty[JOIN_MAX];
-    __shared__ int s_found[JOIN_WARPS], s_rows[JOIN_WARPS], s_most[JOIN_WARPS];
-    __shared__ float red[JOIN_WARPS][256], red_l[JOIN_WARPS];
+// A fixed number of CTAs share the rows of all cut units; every CTA reads the records.  The kernel is bound by round trips to memory: a row's values, references
+// and sums are all on their way at once, since with weights first and values after them a row took 6,500 cycles.  Four warps take a row together (or one,
+// where that saves passes), each every fourth part, up to eight at a time.  Behind tiles of 256 rows there are many more rows than warps, of two or three parts
+// each: a warp then has eight parts of two or four rows on their way (join_rows; 12 sequences of 64 rows: 247 -> 230 us in all; it is no gain, and 1 to 3 us
+// slower, where rows are few).
+constexpr int JOIN_WARPS = 8, JOIN_MAX = 512, JOIN_PER_SM = 4; // JOIN_MAX: CTAs of the attention kernel at most
+struct Duty {                 // a unit that was cut
+    int front;                // rows of the units in front of it
+    short c, c0;              // the CTAs in which it ends and begins ...
+    int r0, t;
+    unsigned short h, how;    // how: slot | lanes << 1
+};
+struct JoinShared {
+    Duty duty[JOIN_MAX];
+    int found[JOIN_WARPS], rows[JOIN_WARPS], most[JOIN_WARPS];
+    float acc[JOIN_WARPS][256], l[JOIN_WARPS];
+};
+
+// K: parts of a row on their way at once, 8 / K rows per warp
+template <typename O, int M, int K> __device__ __forceinline__ void join_rows(const TreeDev &p, JoinShared &sm, int n_duty, int n_rows) {
+    constexpr int R = 8 / K, PER = JOIN_WARPS * R;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = p.dim;
+    for (int first = blockIdx.x * PER; first < n_rows; first += gridDim.x * PER) {
+        // lane L, L + 8, ... stand for part L % K of row L / K
+        const int i = first + warp * R + (lane & 7) / K, k = lane % K;
+        int parts = 0, at = 0, step = 0, at0 = 0, pair = 0, pair0 = 0; // places in floats: of part k * step behind at, of the first one at at0; and of the pairs
+        long long out = 0;
+        if (i < n_rows) {
+            int lo = 0, hi = n_duty; // the unit of row i
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (sm.duty[mid].front <= i) lo = mid;
+                else hi = mid;
+            }
+            const Duty u = sm.duty[lo];
+            const int r = i - u.front, lanes = u.how >> 1, size = M * (D + 2), row = u.t * M + r;
+            parts = (u.c - u.c0) / lanes + 1, step = lanes * 2 * size, at = u.c0 * 2 * size + r * D, at0 = at + (u.how & 1) * size;
+            pair = u.c0 * 2 * size + M * D + 2 * r, pair0 = pair + (u.how & 1) * size;
+            out = (u.r0 + row / p.group) * p.out_stride + ((long long)u.h * p.group + row % p.group) * D;
+        }
+        auto pair_of = [&](int j) { return j < parts ? *(const float2 *)(p.part + (j == 0 ? pair0 : pair + j * step)) : make_float2(-INFINITY, 0.f); };
+        for (int d0 = 0; d0 < D; d0 += 128) {
+            const int d = d0 + lane * 4;
+            float m = -INFINITY, l = 0.f;
+            float4 acc[R];
+#pragma unroll
+            for (int a = 0; a < R; ++a) acc[a] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int j0 = 0; K < 8 ? j0 == 0 : j0 < parts; j0 += K) {
+                const int j = j0 + k;
+                const int mine = j < parts ? (j == 0 ? at0 : at + j * step) : -1;
+                float4 x[8];
+#pragma unroll
+                for (int s = 0; s < 8; ++s) {
+                    const int from = __shfl_sync(0xffffffffu, mine, s);
+                    x[s] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (from >= 0 && d < D) x[s] = *(const float4 *)(p.part + from + d);
+                }
+                const float2 ml = pair_of(j);
+                if (j0 == 0) { // the row's reference, over all parts
+                    if (K == 8) {
+                        for (int q = lane; q < parts; q += 32) m = fmaxf(m, pair_of(q).x);
+                        m = warp_max(m);
+                    } else {
+                        m = ml.x;
+#pragma unroll
+                        for (int o = K / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                    }
+                }
+                const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
+                l += ml.y * w;
+#pragma unroll
+                for (int s = 0; s < 8; ++s) {
+                    const float ws = __shfl_sync(0xffffffffu, w, s);
+                    if (ws == 0.f) continue; // (an empty part's values were never written)
+                    acc[s / K].x += ws * x[s].x, acc[s / K].y += ws * x[s].y, acc[s / K].z += ws * x[s].z, acc[s / K].w += ws * x[s].w;
+                }
+            }
+#pragma unroll
+            for (int o = K / 2; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+#pragma unroll
+            for (int a = 0; a < R; ++a) {
+                const float la = __shfl_sync(0xffffffffu, l, a * K), inv = la == 0.f ? 0.f : 1.0f / la;
+                const long long to = __shfl_sync(0xffffffffu, out, a * K);
+                const bool there = __shfl_sync(0xffffffffu, parts, a * K) > 0;
+                if (!there || d >= D) continue;
+                O *const o = (O *)p.out + to + d;
+                const float y[4] = {acc[a].x, acc[a].y, acc[a].z, acc[a].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = out_from<O>(la == 0.f ? 0.f : y[e] * inv);
+            }
+        }
+    }
+}
+
+template <typename O, int M> __global__ void __launch_bounds__(32 * JOIN_WARPS, M >= 256 ? 3 : 2) tree_join_kernel(const TreeDev p, int ctas) {
+    __shared__ JoinShared sm;
     pdl_wait_prior();
     pdl_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = p.dim;
@@ -279,20 +361,26 @@ template <typename O, int M> __global__ void __launch_bounds__(32 * JOIN_WARPS) 
             parts = max(parts, __shfl_xor_sync(0xffffffffu, parts, o));
         }
         __syncthreads();
-        if (lane == 31) s_found[warp] = __popc(who), s_rows[warp] = incl, s_most[warp] = parts;
+        if (lane == 31) sm.found[warp] = __popc(who), sm.rows[warp] = incl, sm.most[warp] = parts;
         __syncthreads();
         int at = n_duty + __popc(who & ((1u << lane) - 1u)), front = n_rows + incl - r;
         for (int k = 0; k < JOIN_WARPS; ++k) {
-            if (k < warp) at += s_found[k], front += s_rows[k];
-            n_duty += s_found[k], n_rows += s_rows[k], most = max(most, s_most[k]);
+            if (k < warp) at += sm.found[k], front += sm.rows[k];
+            n_duty += sm.found[k], n_rows += sm.rows[k], most = max(most, sm.most[k]);
         }
         if (has) {
             Duty d;
             d.front = front, d.c = (short)c, d.c0 = (short)a.x, d.r0 = a.z, d.t = b.x, d.h = (unsigned short)b.y, d.how = (unsigned short)a.y;
-            duty[at] = d;
+            sm.duty[at] = d;
         }
     }
     __syncthreads();
+    if constexpr (M >= 256) {
+        if (most <= 2) join_rows<O, M, 2>(p, sm, n_duty, n_rows);
+        else if (most <= 4) join_rows<O, M, 4>(p, sm, n_duty, n_rows);
+        else join_rows<O, M, 8>(p, sm, n_duty, n_rows);
+        return;
+    }
     // four warps to a row where that takes fewer round trips: passes over the rows times loads in turn per row
     const int warps = gridDim.x * JOIN_WARPS;
     const bool shared = (n_rows * 4 + warps - 1) / warps * ((most + 31) / 32) < (n_rows + warps - 1) / warps * ((most + 7) / 8);
@@ -309,10 +397,10 @@ template <typename O, int M> __global__ void __launch_bounds__(32 * JOIN_WARPS) 
             int lo = 0, hi = n_duty; // the unit of row i
             while (hi - lo > 1) {
                 const int mid = (lo + hi) / 2;
-                if (duty[mid].front <= i) lo = mid;
+                if (sm.duty[mid].front <= i) lo = mid;
                 else hi = mid;
             }
-            u = duty[lo];
+            u = sm.duty[lo];
             r = i - u.front;
             const int lanes = u.how >> 1, parts = (u.c - u.c0) / lanes + 1;
             auto part = [&](int k) { return part_of<M>(p, u.c0 + k * lanes, k == 0 ? u.how & 1 : 0); };
@@ -356,17 +444,17 @@ template <typename O, int M> __global__ void __launch_bounds__(32 * JOIN_WARPS) 
             if (on)
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (e < wide) red[warp][lane * wide + e] = acc[e];
-            if (lane == 0) red_l[warp] = l;
+                    if (e < wide) sm.acc[warp][lane * wide + e] = acc[e];
+            if (lane == 0) sm.l[warp] = l;
             __syncthreads();
         }
         if (i >= n_rows || sub) continue;
         if (split > 1)
             for (int s = 1; s < split; ++s) {
-                l += red_l[warp + s];
+                l += sm.l[warp + s];
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (e < wide && on) acc[e] += red[warp + s][lane * wide + e];
+                    if (e < wide && on) acc[e] += sm.acc[warp + s][lane * wide + e];
             }
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         const int row = u.t * M + r;

@@ -15,6 +15,7 @@
 #include "tree_sched.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 namespace ullm {
@@ -323,10 +324,10 @@ template <typename Q, typename KV> static cudaError_t launch_fma(const DeviceInf
 
 using namespace ullm;
 
-// The work area begins with the CTAs' records (for the most CTAs of any kernel), then the partial results.
+// The work area begins with the CTAs' records and their counters (for the most CTAs of any kernel), then the partial results.
 static size_t tree_work_bytes(const DeviceInfo &dev, int dim, bool tc) {
     const size_t fma = sizeof(float) * (size_t)dev.sm_count * F_PER_SM * 2 * 32 * (dim + 2); // of 32 rows, the most that a tile of the f32 kernels has
-    return meta_bytes(dev.sm_count * F_PER_SM) + (tc ? std::max(fma, tree_attn_tc_work(dev.sm_count, dim)) : fma);
+    return 2 * meta_bytes(dev.sm_count * F_PER_SM) + (tc ? std::max(fma, tree_attn_tc_work(dev.sm_count, dim)) : fma);
 }
 
 size_t ullm_cuda_tree_attn_work_bytes(const ullm_cuda_ctx *c, const ullm_kv_pages *kv, int dtype) {
@@ -381,7 +382,10 @@ int ullm_cuda_tree_attn_dev(ullm_cuda_ctx *c, const ullm_tree_attn *a, void *str
     t.scale_log2 = (float)((a->scale == 0.f ? 1.0 / std::sqrt((double)dim) : (double)a->scale) * 1.4426950408889634);
     DeviceGuard guard(c->device);
     const cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
-    t.meta = (int4 *)a->d_work, t.part = (float *)((uint8_t *)a->d_work + meta_bytes(c->dev.sm_count * F_PER_SM));
+    const size_t records = meta_bytes(c->dev.sm_count * F_PER_SM);
+    static std::atomic<unsigned long long> calls{0};
+    t.meta = (int4 *)a->d_work, t.count = (unsigned long long *)((uint8_t *)a->d_work + records), t.part = (float *)((uint8_t *)a->d_work + 2 * records);
+    t.call = ++calls;
     cudaError_t e = cudaErrorNotSupported;
     if (tree_attn_tc_supported(pool, a->dtype)) e = launch_tree_attn_tc(c->dev, pool, a->dtype, t, c->d_status, c->use_pdl, st);
     if (e != cudaErrorNotSupported) { // (strides that a tensor map cannot describe go to the f32 kernel)

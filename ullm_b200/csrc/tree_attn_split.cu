@@ -97,6 +97,7 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
     float *const qa = (float *)xsm, *const qb = qa + C::QF; // the parts of the queries, as the products want them: 16 bytes per row tile, step and lane
     uint8_t *const stage0 = (uint8_t *)(qb + C::QF);
     __shared__ Seg seg;
+    __shared__ int last;
     __shared__ long long offs[2][XK]; // where the keys of a block lie: bytes behind p.k and p.v, -1 for none
     __shared__ float2 ml[8][16];      // maximum and sum of each warp's rows
     pdl_wait_prior();
@@ -104,12 +105,7 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int rt = warp % C::RT, kg = warp / C::RT, kbase = kg * C::NT * 8;
     Sched<M, XK, X_COST, X_MIN> sched(p);
-    bool some = false;
-    if (warp == 0) {
-        if (lane == 0) p.meta[blockIdx.x * TREE_META] = make_int4(-1, 0, 0, 0);
-        __syncwarp();
-        some = sched.init();
-    }
+    const bool some = warp == 0 && sched.init();
     // The warps over the same keys fetch them and wait for one another, and for no others.
     constexpr int PIECES = D * (int)sizeof(KV) / 16, TG = 32 * C::RT, STEP = TG / PIECES; // 16-byte pieces of a row; threads of such a group; rows that they take at once
     const int tg = rt * 32 + lane, piece_j = tg / PIECES, piece_c = tg % PIECES * 16;
@@ -122,7 +118,7 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
         if (warp == 0) {
             Seg next;
             next.count = 0;
-            if (some) next = sched.next(p.meta + blockIdx.x * TREE_META);
+            if (some) next = sched.next(nullptr);
             if (lane == 0) seg = next;
         }
         __syncthreads();
@@ -367,6 +363,7 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
                 if (d == 0) *(float2 *)(to + (size_t)M * D + 2 * r) = make_float2(top, sum);
             }
         }
+        if (!whole) join_last<float, M, D>(p, w, &last);
     }
 }
 
@@ -375,9 +372,7 @@ template <typename KV, int D, int M> cudaError_t launch_as(const DeviceInfo &dev
     cudaError_t e = cudaFuncSetAttribute(tree_attn_split_kernel<KV, D, M>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return e;
     const int ctas = dev.sm_count * C::PER_SM;
-    e = launch_kernel(tree_attn_split_kernel<KV, D, M>, dim3(ctas), dim3(XT), (size_t)C::SMEM, st, pdl, t);
-    if (e != cudaSuccess) return e;
-    return launch_kernel(tree_join_kernel<float, M>, dim3(dev.sm_count * JOIN_PER_SM), dim3(32 * JOIN_WARPS), 0, st, pdl, t, ctas);
+    return launch_kernel(tree_attn_split_kernel<KV, D, M>, dim3(ctas), dim3(XT), (size_t)C::SMEM, st, pdl, t);
 }
 template <typename KV, int D> cudaError_t launch_for(const DeviceInfo &dev, const TreeDev &t, bool pdl, cudaStream_t st) {
     // Rows per sequence and key head on average (the lengths themselves are on the device; either way is right for any of them).

@@ -60,7 +60,7 @@ struct __align__(16) Seg {
     int blk, count;               // first key block, blocks (0: no more segments)
     int flags;                    // 1: the whole unit; 2: its partial result goes to slot 1
     int odd;                      // set by who finds values that are not finite among the rows' own tokens
-    int pad[3];
+    int first, parts, end;        // of a unit that was cut: the CTA that begins it (<< 1 | its slot there), the CTAs that have a part of it, the one that ends it
 };
 
 template <int M, int KB, int COST, int MINS> struct Sched {
@@ -180,7 +180,7 @@ template <int M, int KB, int COST, int MINS> struct Sched {
         }
         return true;
     }
-    // The next segment; count 0 when the share is used up.  meta: where the joining kernel's record goes.
+    // The next segment; count 0 when the share is used up.  meta: where the joining kernel's record goes; null: the segment says who joins (join_last).
     __device__ __forceinline__ Seg next(int4 *meta) {
         Seg s;
         s.count = 0, s.odd = 0;
@@ -196,7 +196,10 @@ template <int M, int KB, int COST, int MINS> struct Sched {
                 s.blk = b0, s.count = b1 - b0;
                 const bool whole = b0 == 0 && b1 == mine;
                 s.flags = (whole ? 1 : 0) | (cur == lo ? 0 : 2); // slot 0: the unit with which the share begins
-                if (!whole && b1 == mine && lane == 0) {
+                if (!whole && !meta) {
+                    const unsigned unit = cur - off, c0 = share_of(unit + COST), c1 = share_of(unit + COST + mine - 1); // the teams that hold its first and its last block
+                    s.first = (int)(c0 * lanes + member) << 1 | (share_at(c0) >= unit ? 0 : 1), s.parts = (int)(c1 - c0) + 1, s.end = (int)c1 * lanes + member;
+                } else if (!whole && b1 == mine && lane == 0) {
                     const unsigned unit = cur - off, c0 = share_of(unit + COST); // the team that holds its first block
                     meta[0] = make_int4((int)c0 * lanes + member, (share_at(c0) >= unit ? 0 : 1) | lanes << 1, v.r0, v.n);
                     meta[1] = make_int4(tile, h, 0, 0);
@@ -243,6 +246,63 @@ template <typename T> __device__ __forceinline__ T out_from(float v);
 template <> __device__ __forceinline__ float out_from<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half out_from<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 out_from<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Joins a unit's parts without a second launch: the CTAs that have a part of it count, and the last one to arrive joins them all, in the order of the CTAs.
+// A count is kept in 64 bits beside the number of the call, and any other number there counts as none: the memory needs no preparation, and
+// what an abandoned call leaves does no harm.  Every thread calls it, behind its stores of the CTA's own part.
+template <typename O, int M, int D> __device__ __forceinline__ void join_last(const TreeDev &p, const Seg &w, int *flag) {
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        unsigned long long *const count = p.count + w.end, call = p.call << 16;
+        unsigned long long old = *(volatile unsigned long long *)count, seen;
+        for (;; old = seen) {
+            const unsigned long long n = (old & ~0xffffull) == call ? (old & 0xffff) + 1 : 1;
+            seen = atomicCAS(count, old, n == (unsigned long long)w.parts ? 0 : call | n);
+            if (seen == old) {
+                *flag = n == (unsigned long long)w.parts;
+                break;
+            }
+        }
+    }
+    __syncthreads();
+    if (!*flag) return;
+    __threadfence();
+    const int size = M * (D + 2), c0 = w.first >> 1;
+    for (int i = threadIdx.x; i < w.rows * (D / 4); i += blockDim.x) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float m = -INFINITY, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k0 = 0; k0 < w.parts; k0 += 8) { // eight parts on their way at once
+            float4 x[8];
+            float2 ml[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float *const part = p.part + ((c0 + k0 + k) * 2 + (k0 + k == 0 ? w.first & 1 : 0)) * size;
+                ml[k] = make_float2(-INFINITY, 0.f), x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (k0 + k < w.parts) ml[k] = __ldcg((const float2 *)(part + M * D + 2 * r)), x[k] = __ldcg((const float4 *)(part + r * D + d));
+            }
+            float top = m;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
+            const float corr = m == -INFINITY ? 0.f : exp2f(m - top);
+            if (m != -INFINITY) l *= corr, acc.x *= corr, acc.y *= corr, acc.z *= corr, acc.w *= corr;
+            m = top;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float c = ml[k].x == -INFINITY ? 0.f : exp2f(ml[k].x - m);
+                l += ml[k].y * c; // (NaN where a score was NaN)
+                acc.x += c * x[k].x, acc.y += c * x[k].y, acc.z += c * x[k].z, acc.w += c * x[k].w;
+            }
+        }
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        const int row = w.row0 + r;
+        O *const out = (O *)p.out + (w.r0 + row / p.group) * p.out_stride + ((long long)w.h * p.group + row % p.group) * D + d;
+        const float y[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[e] = out_from<O>(l == 0.f ? 0.f : y[e] * inv);
+    }
+}
 
 // Joins the parts of the units that were cut, in the order of the CTAs:
 //   out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c.

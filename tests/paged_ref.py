@@ -187,7 +187,7 @@ def rope_rows(x, heads, norm, eps, cs, rot, neox):
 
 def attention(q, k, v, see, scale):
     """One sequence: q [n, heads, dim], k and v [keys, kv_heads, dim] in float64, see [n, keys] -> out, sum of p |v| and
-    the largest sum of |q| |k| * scale of each row and head."""
+    the largest (finite) sum of |q| |k| * scale of each row and head."""
     n, heads, dim = q.shape
     g = heads // k.shape[1]
     out, weight, size = np.zeros(q.shape), np.zeros(q.shape), np.zeros((n, heads))
@@ -203,7 +203,8 @@ def attention(q, k, v, see, scale):
                 p = p / p.sum()
                 out[i, h] = (p[:, None] * vv[j]).sum(0)
                 weight[i, h] = (p[:, None] * np.abs(vv[j])).sum(0)
-            size[i, h] = (np.abs(kk[j]) @ np.abs(q[i, h])).max() * scale
+            terms = np.abs(kk[j]) @ np.abs(q[i, h])
+            size[i, h] = terms[np.isfinite(terms)].max(initial=0) * scale
     return out, weight, size
 
 

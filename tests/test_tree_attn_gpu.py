@@ -379,3 +379,62 @@ def test_a_step_of_speculative_decoding(ctx):
     t.trim_dev(ids.data_ptr(), None, 2, stream=st)
     torch.cuda.synchronize()
     assert int(refs.abs().sum()) == 0 and int(fault[0]) == 0
+
+
+@pytest.mark.parametrize("dtype,dim", [("f32", 64), ("f32", 128), ("f16", 128), ("bf16", 64), ("f32", 96)])
+@pytest.mark.parametrize("ctx_len,n", [(0, 1), (7, 1), (8, 1), (63, 1), (64, 1), (61, 6), (130, 40), (1000, 1), (700, 33), (4000, 9)])
+def test_32_bit_queries_around_the_blocks(ctx, dtype, dim, ctx_len, n):
+    """One row to many over pages of every type: tiles of 16 and of 32 rows (the table's size decides for few rows), whole units and units in many parts."""
+    for heads, kv_heads, blocks in ((8, 2, 1), (3, 3, 3000)):
+        c = Case([ctx_len, 5], [n, 2], heads, kv_heads, dim, dtype, 16, mask="any", seed=ctx_len + n + dim, q32=True, extra_blocks=blocks)
+        c.run(ctx)
+        c.check()
+
+
+@pytest.mark.parametrize("dtype,q32,dim", [("f32", True, 64), ("f16", True, 128), ("bf16", True, 64), ("bf16", False, 128), ("f16", False, 40), ("f32", True, 40)])
+def test_infinite_keys_and_values_of_the_context(ctx, dtype, q32, dim):
+    """A key whose score is -inf has no weight, one whose score is +inf or NaN makes its rows NaN; an infinite value that a row sees makes it infinite."""
+    c = Case([300, 90], [5, 3], 4, 2, dim, dtype, 16, mask="tree", seed=4, q32=q32)
+    c.q[:, :4 * dim] = c.q[:, :4 * dim].abs()
+    at = lambda b, tok: (c.layer, int(c.blocks[b, tok // 16]), tok % 16)
+    c.k[at(0, 17)][:, 3] = -float("inf")
+    c.k[at(0, 250)][:, dim - 1] = -float("inf")
+    c.v[at(0, 100)][0, 5] = float("inf")
+    c.v[at(0, 200)][1, 6] = -float("inf")
+    c.k[at(1, 40)][1, 2] = float("inf")
+    c.run(ctx)
+    c.check()
+
+
+def test_the_largest_32_bit_values(ctx):
+    """Keys, values and queries at the end of the range stay what they are: products of them are finite where the formula's are."""
+    big = torch.finfo(torch.float32).max
+    for dim in (64, 128, 40):
+        c = Case([100], [4], 2, 1, dim, "f32", 16, mask="tree", seed=dim)
+        c.q[:, :2 * dim] *= 0.01
+        c.q[1, 3], c.q[2, dim + 4] = big, -big
+        for tok in range(104):
+            page, slot = int(c.blocks[0, tok // 16]), tok % 16
+            c.k[c.layer, page, slot, 0, 3:5] = 0
+            c.k[c.layer, page, slot, 0, 4] = 1e-38 if tok % 2 else 0
+            c.v[c.layer, page, slot, 0, 7] = big if tok == 50 else 0  # (a sum of several would pass the range before it is divided)
+        c.run(ctx)
+        c.check()
+
+
+def test_a_work_area_needs_no_preparation(ctx):
+    """Whatever the work area held, and whichever calls used it before, a call's result is the same bit by bit."""
+    for dtype, dim in (("f32", 64), ("f16", 128), ("f32", 80)):
+        c = Case([2500, 300, 0], [7, 40, 1], 8, 2, dim, dtype, 16, mask="tree", q32=dtype == "f32", seed=3)
+        op = c.run(ctx)
+        c.check()
+        first = c.out.clone()
+        work = torch.empty(op._a.work_bytes // 4 + 1, dtype=torch.int32, device="cuda")
+        op._a.d_work = work.data_ptr()
+        for fill in (0, -1, 1, 0x7FC00000):
+            work.fill_(fill)
+            for _ in range(2):
+                c.out.fill_(7)
+                c.run(ctx, op)
+                torch.cuda.synchronize()
+                assert torch.equal(c.out, first)

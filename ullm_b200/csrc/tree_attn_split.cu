@@ -1,9 +1,11 @@
 // Attention of drafted rows over a paged cache with f32 queries: 32-bit products on the tensor cores.
 //
 // The formula is that of tree_attn.cu.  The tensor cores multiply 11-bit significands (tf32) and add in f32; a 32-bit value x is taken as the sum
-// x = a + b of its 11 leading bits, rounded to nearest, and the next 11, so that
-//   x y = a a' + a b' + b a'  within  2^-21 + 2^-22 + 2^-21 of |x y|,
-// which is less than what a sum of 64 products loses to f32 rounding at worst.  Values of 16 bits fit in one part: two products instead of three.
+// x = a + b of its 11 leading bits and the next 11, so that
+//   x y = a a' + a b' + b a'  within  2^-21 + 2^-20 + 2^-21 of |x y|
+// (what b of a query or a weight, b' of a key or value, and b b' leave out: the leading bits of the former are rounded, the rest is cut off, so that the largest
+// values stay finite), which is less than what a sum of 64 products loses to f32 rounding at worst.  Below 2^-126 the parts have fewer bits; a block
+// with a query or key beyond 2^60, where that could count, forms its products one by one.  Values of 16 bits fit in one part: two products instead of three.
 //
 // A CTA of eight warps takes 16 or 32 query rows and walks blocks of 64 keys, whose keys and values arrive by cp.async, as they lie in the pages, while the
 // block before is worked on.  A warp has 16 rows and a fixed share of every block's keys (8 or 16), keeps a maximum, a sum and weighted
@@ -22,6 +24,7 @@ namespace ullm {
 namespace {
 
 constexpr int XT = 256, XK = 64;     // threads; keys of a block
+constexpr float BIG = 1.152921504606847e18f; // 2^60
 constexpr int X_COST = 1, X_MIN = 2; // places that a unit costs beside its blocks; places that a CTA takes at least
 
 template <typename KV, int D, int M> struct SplitCfg {
@@ -41,9 +44,8 @@ __device__ __forceinline__ void mma8(float (&d)[4], const float4 &a, float b0, f
                  : "r"(__float_as_uint(a.x)), "r"(__float_as_uint(a.y)), "r"(__float_as_uint(a.z)), "r"(__float_as_uint(a.w)), "r"(__float_as_uint(b0)),
                    "r"(__float_as_uint(b1)));
 }
-// The 11 leading bits, rounded; what is left of an infinity or a NaN is NaN
-__device__ __forceinline__ float lead(float x) { return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u); }
-__device__ __forceinline__ float tail(float x, float a) { return x - a; }
+// The 11 leading bits, rounded (the largest values become infinite) or cut off; x - cut11(x) is NaN for an infinity or a NaN
+__device__ __forceinline__ float round11(float x) { return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u); }
 __device__ __forceinline__ float cut11(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
 // Eight neighbouring values as f32
 __device__ __forceinline__ void widen8(float (&x)[8], const float *p) {
@@ -65,15 +67,15 @@ __device__ __forceinline__ void widen8(float (&x)[8], const __nv_bfloat16 *p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
 }
-// acc[n] += (a + b) y[n] for several y of the cache, product by product, so that those into one place are apart; z collects NaN where a y is not finite.
+// acc[n] += (a + b) y[n] for several y of the cache, product by product, so that those into one place are apart; z: the sum of their squares.
 // SETS: places per sum, 1 to 3
 template <typename KV, int N, int SETS> __device__ __forceinline__ void products(float (&acc)[N][SETS][4], const float4 &a, const float4 &b, const float (&y0)[N], const float (&y1)[N], float &z) {
     if constexpr (sizeof(KV) == 4) {
         float h0[N], h1[N], l0[N], l1[N];
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            h0[n] = lead(y0[n]), h1[n] = lead(y1[n]), l0[n] = tail(y0[n], h0[n]), l1[n] = tail(y1[n], h1[n]);
-            z += l0[n] + l1[n];
+            h0[n] = cut11(y0[n]), h1[n] = cut11(y1[n]), l0[n] = y0[n] - h0[n], l1[n] = y1[n] - h1[n];
+            z = fmaf(y0[n], y0[n], fmaf(y1[n], y1[n], z));
         }
 #pragma unroll
         for (int n = 0; n < N; ++n) mma8(acc[n][SETS - 1], a, cut11(l0[n]), cut11(l1[n]));
@@ -83,7 +85,7 @@ template <typename KV, int N, int SETS> __device__ __forceinline__ void products
         for (int n = 0; n < N; ++n) mma8(acc[n][0], a, h0[n], h1[n]);
     } else {
 #pragma unroll
-        for (int n = 0; n < N; ++n) z = fmaf(y0[n], 0.f, fmaf(y1[n], 0.f, z));
+        for (int n = 0; n < N; ++n) z = fmaf(y0[n], y0[n], fmaf(y1[n], y1[n], z));
 #pragma unroll
         for (int n = 0; n < N; ++n) mma8(acc[n][SETS - 1], b, y0[n], y1[n]);
 #pragma unroll
@@ -162,12 +164,13 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
             const int step = d / 32 * 4, l = r % 8 * 4 + d % 32 / 8, at = (((r / 16) * (D / 8) + step) * 32 + l) * 4 + (r % 16 / 8 + d % 8 / 4 * 2);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float a = lead(y[e]);
-                qa[at + e * 128] = a, qb[at + e * 128] = tail(y[e], a);
+                float a = round11(y[e]), b = round11(y[e] - a);
+                if (!(fabsf(y[e]) <= BIG)) seg.big = 1, a = y[e], b = 0.f; // infinities and NaN too
+                qa[at + e * 128] = a, qb[at + e * 128] = b;
             }
         }
         __syncthreads();
-        const bool work = rt * 16 < rows;
+        const bool work = rt * 16 < rows, big = seg.big;
         const int row[2] = {rt * 16 + g, rt * 16 + g + 8}, token[2] = {token_of(row[0]), token_of(row[1])};
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}; // l: this lane's share
         float o[D / 32][4][1][4]; // [c][i]: value 32 c + 8 t + i of rows 0 and 1 in 0 and 2, value 32 c + 8 t + 4 + i in 1 and 3
@@ -203,8 +206,7 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
                     for (int i = 0; i < 4; ++i) {
                         const int at = ((rt * (D / 8) + c * 4 + i) * 32 + lane) * 4;
                         const float4 a = *(const float4 *)(qa + at);
-                        float4 b = *(const float4 *)(qb + at);
-                        b.x = cut11(b.x), b.y = cut11(b.y), b.z = cut11(b.z), b.w = cut11(b.w);
+                        const float4 b = *(const float4 *)(qb + at);
                         float y0[C::NT], y1[C::NT];
 #pragma unroll
                         for (int n = 0; n < C::NT; ++n) y0[n] = y[n][i], y1[n] = y[n][4 + i];
@@ -219,7 +221,7 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
 #pragma unroll
                         for (int k = 1; k < SETS; ++k) s[n][e] += parts[n][k][e];
                     }
-                if (__any_sync(0xffffffffu, z != z)) { // a key that is not finite: the products one by one, since b times an infinity is not what x times it is
+                if (__any_sync(0xffffffffu, !(z < BIG * BIG)) || big) { // (b times an infinity is not what x times it is, either)
 #pragma unroll
                     for (int n = 0; n < C::NT; ++n)
 #pragma unroll
@@ -291,8 +293,8 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
 #pragma unroll
                 for (int n = 0; n < C::NT; ++n) {
                     const float4 x = make_float4(s[n][0], s[n][2], s[n][1], s[n][3]); // product t is key 2 t, product t + 4 key 2 t + 1
-                    const float4 a = make_float4(lead(x.x), lead(x.y), lead(x.z), lead(x.w));
-                    const float4 b = make_float4(cut11(tail(x.x, a.x)), cut11(tail(x.y, a.y)), cut11(tail(x.z, a.z)), cut11(tail(x.w, a.w)));
+                    const float4 a = make_float4(round11(x.x), round11(x.y), round11(x.z), round11(x.w));
+                    const float4 b = make_float4(cut11(x.x - a.x), cut11(x.y - a.y), cut11(x.z - a.z), cut11(x.w - a.w));
                     const KV *const v0 = (const KV *)(vs + (kbase + n * 8 + 2 * t) * C::VP) + g * 4, *const v1 = (const KV *)((const uint8_t *)v0 + C::VP);
                     float unused = 0.f;
 #pragma unroll

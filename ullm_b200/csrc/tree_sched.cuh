@@ -59,7 +59,7 @@ struct __align__(16) Seg {
     int h, row0, rows;            // key head; first row of the tile among the sequence's query rows, and how many there are
     int blk, count;               // first key block, blocks (0: no more segments)
     int flags;                    // 1: the whole unit; 2: its partial result goes to slot 1
-    int odd;                      // set by who finds values that are not finite among the rows' own tokens
+    short odd, big;               // set by who finds values that are not finite, or queries beyond what a kernel's quick way takes
     int first, parts, end;        // of a unit that was cut: the CTA that begins it (<< 1 | its slot there), the CTAs that have a part of it, the one that ends it
 };
 
@@ -183,7 +183,7 @@ template <int M, int KB, int COST, int MINS> struct Sched {
     // The next segment; count 0 when the share is used up.  meta: where the joining kernel's record goes; null: the segment says who joins (join_last).
     __device__ __forceinline__ Seg next(int4 *meta) {
         Seg s;
-        s.count = 0, s.odd = 0;
+        s.count = 0, s.odd = s.big = 0;
         while (cur < hi) {
             const int nb = group_blocks(v, t), tile = t * lanes + member;
             const unsigned len = nb + COST, take = min(len - off, hi - cur);

@@ -310,7 +310,7 @@ template <typename Q, typename KV, int M, int KEYS> static cudaError_t launch_fm
     const int ctas = fma_ctas(dev, t.dim, sizeof(KV), M, KEYS);
     e = launch_kernel(tree_attn_fma_kernel<Q, KV, M, KEYS>, dim3(ctas), dim3(FT), smem, st, pdl, t);
     if (e != cudaSuccess) return e;
-    return launch_kernel(tree_join_kernel<Q, M>, dim3(dev.sm_count * JOIN_PER_SM), dim3(32 * JOIN_WARPS), 0, st, pdl, t, ctas);
+    return launch_kernel(tree_join_kernel<Q, M>, dim3(dev.sm_count * JOIN_PER_SM<M>), dim3(32 * JOIN_WARPS), 0, st, pdl, t, ctas);
 }
 template <typename Q, typename KV> static cudaError_t launch_fma(const DeviceInfo &dev, const TreeDev &t, bool pdl, cudaStream_t st) {
     const long long rows = ((long long)t.n_rows * t.group + t.n_seq - 1) / t.n_seq; // per sequence and key head, on average

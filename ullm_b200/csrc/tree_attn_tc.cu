@@ -715,7 +715,7 @@ template <typename T, int D, bool TWO> cudaError_t launch(const DeviceInfo &dev,
     cudaError_t e = cudaFuncSetAttribute(tree_attn_tc_kernel<T, D, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
     if (e != cudaSuccess) return e;
     if ((e = launch_kernel(tree_attn_tc_kernel<T, D, TWO>, dim3(dev.sm_count), dim3(TT), Cfg<D>::SMEM, st, pdl, prm, maps)) != cudaSuccess) return e;
-    return launch_kernel(tree_join_kernel<T, TWO ? 2 * TM : TM>, dim3(dev.sm_count * JOIN_PER_SM), dim3(32 * JOIN_WARPS), 0, st, pdl, prm.t, dev.sm_count);
+    return launch_kernel(tree_join_kernel<T, TWO ? 2 * TM : TM>, dim3(dev.sm_count * JOIN_PER_SM<TWO ? 2 * TM : TM>), dim3(32 * JOIN_WARPS), 0, st, pdl, prm.t, dev.sm_count);
 }
 template <typename T> cudaError_t launch_any(const DeviceInfo &dev, int dim, bool two, const TcParams &prm, const TcMaps &maps, bool pdl, cudaStream_t st) {
     if (dim == 64) return two ? launch<T, 64, true>(dev, prm, maps, pdl, st) : launch<T, 64, false>(dev, prm, maps, pdl, st);

@@ -311,7 +311,10 @@ template <typename O, int M, int D> __device__ __forceinline__ void join_last(co
 // where that saves passes), each every fourth part, up to eight at a time.  Behind tiles of 256 rows there are many more rows than warps, of two or three parts
 // each: a warp then has eight parts of two or four rows on their way (join_rows; 12 sequences of 64 rows: 247 -> 230 us in all; it is no gain, and 1 to 3 us
 // slower, where rows are few).
-constexpr int JOIN_WARPS = 8, JOIN_MAX = 512, JOIN_PER_SM = 4; // JOIN_MAX: CTAs of the attention kernel at most
+constexpr int JOIN_WARPS = 8, JOIN_MAX = 512; // JOIN_MAX: CTAs of the attention kernel at most
+// CTAs on an SM, as many as are launched: registers for the loads on their way count for more than warps (general form: 2 for 12.2 us on a one-token call,
+// 4 for 15.7)
+template <int M> constexpr int JOIN_PER_SM = M >= 256 ? 3 : 2;
 struct Duty {                 // a unit that was cut
     int front;                // rows of the units in front of it
     short c, c0;              // the CTAs in which it ends and begins ...
@@ -400,7 +403,7 @@ template <typename O, int M, int K> __device__ __forceinline__ void join_rows(co
     }
 }
 
-template <typename O, int M> __global__ void __launch_bounds__(32 * JOIN_WARPS, M >= 256 ? 3 : 2) tree_join_kernel(const TreeDev p, int ctas) {
+template <typename O, int M> __global__ void __launch_bounds__(32 * JOIN_WARPS, JOIN_PER_SM<M>) tree_join_kernel(const TreeDev p, int ctas) {
     __shared__ JoinShared sm;
     pdl_wait_prior();
     pdl_launch_dependents();

@@ -233,8 +233,9 @@ __host__ __device__ constexpr size_t grow_work_ints(size_t n_pages, size_t n_seq
 
 // One CTA: lengths -> needs -> the lowest free pages -> tables.  Reads before writes throughout: needs and copies are
 // decided on the counts as they were before the call.
+constexpr int FIRST_MAX = 2048; // entries whose places are searched in shared memory
 __global__ void __launch_bounds__(1024) kv_grow_plan_kernel(const TableDev t, int page_size, int n_pages, const int *seq, const int *add, int n) {
-    __shared__ int sums[32];
+    __shared__ int sums[32], s_first[FIRST_MAX];
     pdl_wait_prior();
     pdl_launch_dependents();
     const int tid = threadIdx.x;
@@ -276,7 +277,11 @@ __global__ void __launch_bounds__(1024) kv_grow_plan_kernel(const TableDev t, in
         }
         int excl;
         const int sum = cta_scan1024(want > 0 ? want : 0, &excl, sums);
-        if (i < n) first[i] = (int)min(total + excl, (long long)INT32_MAX / 2), need[i] = want < 0 ? -1 : want | flag;
+        if (i < n) {
+            const int f = (int)min(total + excl, (long long)INT32_MAX / 2);
+            need[i] = want < 0 ? -1 : want | flag, first[i] = f;
+            if (i < FIRST_MAX) s_first[i] = f;
+        }
         total += sum;
     }
     // the lowest `total` pages that nobody uses, in order: 8 counts per thread and sweep
@@ -308,10 +313,10 @@ __global__ void __launch_bounds__(1024) kv_grow_plan_kernel(const TableDev t, in
         int lo = 0, hi = n;
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
-            if (first[mid] <= u) lo = mid;
+            if ((mid < FIRST_MAX ? s_first[mid] : first[mid]) <= u) lo = mid;
             else hi = mid;
         }
-        const int i = lo, s = seq[i], len = t.len[s], k = u - first[i];
+        const int i = lo, s = seq[i], len = t.len[s], k = u - (i < FIRST_MAX ? s_first[i] : first[i]);
         const bool cow = (need[i] & COW) != 0;
         const int b = cdiv(len, page_size) - (cow ? 1 : 0) + k, page = picked[u];
         int *const e = t.blocks + (size_t)s * t.max_blocks + b;
@@ -329,24 +334,35 @@ __global__ void __launch_bounds__(1024) kv_grow_plan_kernel(const TableDev t, in
 }
 
 // ---- copies of whole pages ------------------------------------------------------------------------------------------
-// Slots [0, slots) of page `from` to page `to` in one layer of K or V, by the CTA.
-__device__ __forceinline__ void copy_slots(const PoolDev &pool, int y, int from, int to, int slots) {
-    uint8_t *const mem = (y & 1 ? pool.v : pool.k) + (y >> 1) * pool.layer_stride * pool.elem_bytes;
-    const uint8_t *const a = mem + from * pool.page_stride * pool.elem_bytes;
-    uint8_t *const b = mem + to * pool.page_stride * pool.elem_bytes;
-    const int pieces = pool.head_dim * pool.elem_bytes / 16, per_slot = pieces * pool.n_kv_head, total = per_slot * slots;
-    auto at = [&](int c) {
-        const int slot = c / per_slot, r = c % per_slot;
-        return (slot * pool.slot_stride + (long long)(r / pieces) * pool.head_stride) * pool.elem_bytes + (r % pieces) * 16;
-    };
-    for (int c = threadIdx.x; c < total; c += 4 * blockDim.x) { // four loads in flight per thread
-        uint4 v[4];
+// Slots [0, slots) of page `from` to page `to` in the CTA's share of the layers' K and V (blockIdx.y of gridDim.y).  A thread's 16-byte pieces are
+// 256 apart; their places (slot, head, piece) are counted on, not divided out, and a piece goes as far as every other one (192 half pages in 24
+// matrices, a CTA each and a division for every digit: 34 us, 76 % of the issue slots; nine CTAs per entry, places
+// counted on: 21 us).
+__device__ __forceinline__ void copy_slots(const PoolDev &pool, int from, int to, int slots) {
+    const int pieces = pool.head_dim * pool.elem_bytes / 16, heads = pool.n_kv_head, mats = 2 * pool.n_layer;
+    const int m0 = (int)((long long)mats * blockIdx.y / gridDim.y), m1 = (int)((long long)mats * (blockIdx.y + 1) / gridDim.y);
+    const long long slot_b = pool.slot_stride * pool.elem_bytes, head_b = pool.head_stride * pool.elem_bytes;
+    const long long start = from * pool.page_stride * pool.elem_bytes, way = (to - from) * pool.page_stride * pool.elem_bytes;
+    const int step_p = 256 % pieces, step_h = 256 / pieces % heads, step_s = 256 / pieces / heads, tid = threadIdx.x;
+    const int p0 = tid % pieces, h0 = tid / pieces % heads, s0 = tid / pieces / heads;
+    for (int m = m0; m < m1; ++m) {
+        uint8_t *const mem = (m & 1 ? pool.v : pool.k) + (m >> 1) * pool.layer_stride * pool.elem_bytes + start;
+        int p = p0, h = h0, s = s0;
+        while (s < slots) { // eight loads in flight per thread
+            uint4 v[8];
+            uint8_t *at[8];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (c + u * (int)blockDim.x < total) v[u] = *(const uint4 *)(a + at(c + u * blockDim.x));
+            for (int u = 0; u < 8; ++u) {
+                at[u] = s < slots ? mem + s * slot_b + h * head_b + p * 16 : nullptr;
+                p += step_p, h += step_h, s += step_s;
+                if (p >= pieces) p -= pieces, ++h;
+                if (h >= heads) h -= heads, ++s;
+                if (at[u]) v[u] = *(const uint4 *)at[u];
+            }
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (c + u * (int)blockDim.x < total) *(uint4 *)(b + at(c + u * blockDim.x)) = v[u];
+            for (int u = 0; u < 8; ++u)
+                if (at[u]) *(uint4 *)(at[u] + way) = v[u];
+        }
     }
 }
 __global__ void __launch_bounds__(256) kv_grow_copy_kernel(const TableDev t, const PoolDev pool) {
@@ -354,7 +370,7 @@ __global__ void __launch_bounds__(256) kv_grow_copy_kernel(const TableDev t, con
     pdl_launch_dependents();
     const int *const e = t.work + 2 * t.n_seq + 3 * blockIdx.x;
     const int from = e[0];
-    if (from >= 0) copy_slots(pool, blockIdx.y, from, e[1], e[2]);
+    if (from >= 0) copy_slots(pool, from, e[1], e[2]);
 }
 __global__ void __launch_bounds__(256) kv_copy_pages_kernel(const PoolDev pool, const int *src, const int *dst, int n, int *fault) {
     pdl_wait_prior();
@@ -367,7 +383,7 @@ __global__ void __launch_bounds__(256) kv_copy_pages_kernel(const PoolDev pool, 
         if (threadIdx.x == 0) set_fault(fault, ULLM_KV_FAULT_PAGE);
         return;
     }
-    copy_slots(pool, blockIdx.y, s, d, pool.page_size);
+    copy_slots(pool, s, d, pool.page_size);
 }
 
 // ---- plan of a step of trees ----------------------------------------------------------------------------------------
@@ -679,7 +695,7 @@ int ullm_cuda_kv_grow_dev(ullm_cuda_ctx *c, const ullm_kv_pages *kv, const ullm_
     DeviceGuard guard(c->device);
     const cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
     ULLM_CUDA_TRY(c, launch_kernel(kv_grow_plan_kernel, dim3(1), dim3(1024), 0, st, c->use_pdl, td, pool.page_size, pool.n_pages, d_seq, d_add, (int)n));
-    ULLM_CUDA_TRY(c, launch_kernel(kv_grow_copy_kernel, dim3((unsigned)n, (unsigned)pool.n_layer * 2), dim3(256), 0, st, c->use_pdl, td, pool));
+    ULLM_CUDA_TRY(c, launch_kernel(kv_grow_copy_kernel, dim3((unsigned)n, mats_per_wave(c, pool, n)), dim3(256), 0, st, c->use_pdl, td, pool));
     return ULLM_OK;
 }
 
@@ -720,7 +736,7 @@ int ullm_cuda_kv_copy_pages_dev(ullm_cuda_ctx *c, const ullm_kv_pages *kv, const
     if (n > kv->n_pages) return ctx_fail(c, ULLM_ERR_FORMAT, "%zu copies in a pool of %zu pages", n, kv->n_pages);
     if (!n) return ULLM_OK;
     DeviceGuard guard(c->device);
-    ULLM_CUDA_TRY(c, launch_kernel(kv_copy_pages_kernel, dim3((unsigned)n, (unsigned)pool.n_layer * 2), dim3(256), 0, stream ? (cudaStream_t)stream : c->stream,
+    ULLM_CUDA_TRY(c, launch_kernel(kv_copy_pages_kernel, dim3((unsigned)n, mats_per_wave(c, pool, n)), dim3(256), 0, stream ? (cudaStream_t)stream : c->stream,
                                    c->use_pdl, pool, d_src, d_dst, (int)n, d_fault));
     return ULLM_OK;
 }

@@ -365,7 +365,7 @@ int ullm_cuda_moe_ffn_noalloc(int device, const ullm_moe_experts_input *dev_expe
  * Where K and V lie: element (layer, page, slot, head, d) is at layer * layer_stride + page * page_stride +
  * slot * slot_stride + head * head_stride + d, counted in elements, from d_k and from d_v.  Any order of the axes
  * may be nearest to d; head_dim values are contiguous.  d_k and d_v are 16-byte aligned and the strides multiples of
- * 16 bytes; head_dim is a multiple of 8, at most 256.  dtype is F32, F16 or BF16. */
+ * 16 bytes; head_dim is a multiple of 8, at most 256; a page has at most 65,536 slots.  dtype is F32, F16 or BF16. */
 typedef struct ullm_kv_pages {
     int dtype;
     size_t n_layer, n_pages, page_size, n_kv_head, head_dim;

@@ -363,9 +363,14 @@ cudaError_t Forward::verify_buffers(ullm_cuda_ctx *c) {
 
 int Forward::verify(ullm_cuda_ctx *c, const float *embeds, const int32_t *parents, size_t n, size_t pos, float *logits_host) {
     auto fail = [&](cudaError_t err) {
+        cudaStreamSynchronize(stream); // (what was enqueued still reads the staging arrays)
         cudaGetLastError();
         if (err == cudaErrorNotSupported) return ctx_fail(c, ULLM_ERR_UNSUPPORTED, "a layer shape is outside the fused decode path");
         return ctx_fail(c, err == cudaErrorMemoryAllocation ? ULLM_ERR_OOM : ULLM_ERR_CUDA, "verifying a tree: %s", cudaGetErrorString(err));
+    };
+    auto drop = [&](int status) {
+        cudaStreamSynchronize(stream);
+        return status;
     };
     cudaError_t e;
     int rc;
@@ -384,7 +389,7 @@ int Forward::verify(ullm_cuda_ctx *c, const float *embeds, const int32_t *parent
     TRY(cudaMemcpyAsync(xs, h_vx, n * E * 4, cudaMemcpyHostToDevice, stream));
     if ((rc = ullm_cuda_tree_plan_dev(c, n, 1, vints + V_CU, vints + V_LEN, nullptr, 1, vints + V_PARENT, vints + V_SEQ, vints + V_SLOT, vints + V_POS,
                                       (uint32_t *)vints + V_MASK, VW, vints + V_FAULT, stream)))
-        return rc;
+        return drop(rc);
     const ullm_kv_pages kv = pages();
     ullm_qk_norm_rope ro;
     memset(&ro, 0, sizeof ro);
@@ -429,9 +434,9 @@ int Forward::verify(ullm_cuda_ctx *c, const float *embeds, const int32_t *parent
         ro.layer = at.layer = l;
         ro.d_q = ro.d_q_out = qkv, ro.d_k = qkv + qd, ro.d_v = vsrc, ro.q_stride = ro.k_stride = ro.q_out_stride = ld, ro.v_stride = vld;
         ro.d_q_norm = L.q_norm, ro.d_k_norm = L.k_norm, ro.d_q_bias = L.q_bias, ro.d_k_bias = L.k_bias, ro.d_v_bias = L.v_bias;
-        if ((rc = ullm_cuda_qk_norm_rope_dev(c, &ro, stream))) return rc;
+        if ((rc = ullm_cuda_qk_norm_rope_dev(c, &ro, stream))) return drop(rc);
         at.d_q = qkv, at.q_stride = ld, at.d_out = attn_out;
-        if ((rc = ullm_cuda_tree_attn_dev(c, &at, stream))) return rc;
+        if ((rc = ullm_cuda_tree_attn_dev(c, &at, stream))) return drop(rc);
         if (gemms) {
             TRY(gemm(L.wo, bxn, bx, EPI_RESIDUAL, bx));
             rmsnorm_batch_kernel<<<(unsigned)n, 256, 0, stream>>>(bx, L.ffn_norm, P.eps, (int)E, bxn);
@@ -497,8 +502,9 @@ int Forward::accept(ullm_cuda_ctx *c, size_t pos, size_t n, const int32_t *path,
     t.d_work = vtable, t.work_bytes = vtable_bytes;
     ULLM_CUDA_TRY(c, cudaMemcpyAsync(vints, h_vints, V_IN * 4, cudaMemcpyHostToDevice, stream));
     int rc = ullm_cuda_kv_accept_dev(c, &kv, &t, vints + V_ROW, vints + V_DRAFT, vints + V_PATH, vints + V_KEPT, 1, VN, stream);
+    const cudaError_t done = cudaStreamSynchronize(stream); // (the staging array is free again)
     if (rc) return rc;
-    ULLM_CUDA_TRY(c, cudaStreamSynchronize(stream)); // (the staging array is free again)
+    ULLM_CUDA_TRY(c, done);
     return ULLM_OK;
 }
 #undef TRY

@@ -362,7 +362,7 @@ int ullm_cuda_tree_attn_dev(ullm_cuda_ctx *c, const ullm_tree_attn *a, void *str
     if (!std::isfinite(a->scale) || a->scale < 0.f || (a->scale > 0.f && a->scale < 1e-30f))
         return ctx_fail(c, ULLM_ERR_FORMAT, "scale must be finite, at least 1e-30 or 0 for the default");
     { // the line of all blocks is counted in 32 bits (with what the smaller tiles of the f32 kernel would need)
-        const double units = ((double)a->n_rows * (a->n_head / a->kv->n_kv_head) / 16 + (double)a->n_seq) * a->kv->n_kv_head;
+        const double units = ((double)a->n_rows * (a->n_head / a->kv->n_kv_head) / 8 + (double)a->n_seq) * a->kv->n_kv_head;
         if (units * ((double)a->max_blocks * a->kv->page_size / 32 + 4) > 2147483000.0)
             return ctx_fail(c, ULLM_ERR_FORMAT, "rows times table size too large for one call: split the rows");
     }

@@ -438,3 +438,20 @@ def test_a_work_area_needs_no_preparation(ctx):
                 c.run(ctx, op)
                 torch.cuda.synchronize()
                 assert torch.equal(c.out, first)
+
+
+@pytest.mark.parametrize("dtype,ps", [("f16", 384), ("bf16", 512), ("f16", 128), ("f32", 512)])
+def test_sequences_without_keys_beside_large_pages(ctx, dtype, ps):
+    """Rows of a sequence whose length is inconsistent see nothing and read no page; the table's last row is one of them."""
+    c = Case([40, 700, 0], [3, 9, 2], 4, 2, 64, dtype, ps, mask="tree", q32=dtype == "f32", extra_blocks=0)
+    c.lens[0], c.lens[2] = 1, 0
+    c.run(ctx)
+    torch.cuda.synchronize()
+    assert bool((c.out[:3, :256] == 0).all()) and bool((c.out[12:14, :256] == 0).all())
+    c.ids, c.ctxs, c.counts, c.cu = c.ids[1:2], c.ctxs[1:2], c.counts[1:2], c.cu[1:3]
+    c.mask, keep = None if c.mask is None else c.mask, c.rows
+    c.rows = c.cu[-1]
+    k = c.out[c.rows:keep].clone()
+    c.out[c.rows:keep] = 7
+    c.check()
+    assert bool((k[:, :256] == 0).all())

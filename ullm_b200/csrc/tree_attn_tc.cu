@@ -316,7 +316,7 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
             // entries of the page table, 32 at a time and one such load ahead: a block has 1 to 16 of them
             const bool small = p.page_size < TK;
             auto entry_of = [&](int block) { return small ? block << (7 - prm.page_log) : (int)((unsigned)block / (unsigned)prm.page_blocks); }; // of a block's first key
-            const int e0 = entry_of(w.blk), e_end = small ? (key_end + p.page_size - 1) >> prm.page_log : entry_of((key_end + TK - 1) / TK - 1) + 1;
+            const int e0 = entry_of(w.blk), e_end = key_end <= 0 ? 0 : small ? (key_end + p.page_size - 1) >> prm.page_log : entry_of((key_end - 1) / TK) + 1;
             const int *const table = p.blocks + (size_t)w.id * p.max_blocks;
             auto entries = [&](int e) { return e + (int)lane < e_end ? table[e + lane] : 0; };
             int win = e0, now = entries(e0), ahead = entries(e0 + 32);

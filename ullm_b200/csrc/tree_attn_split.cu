@@ -25,7 +25,7 @@ namespace {
 
 constexpr int XT = 256, XK = 64;     // threads; keys of a block
 constexpr float BIG = 1.152921504606847e18f; // 2^60
-constexpr int X_COST = 1, X_MIN = 2; // places that a unit costs beside its blocks; places that a CTA takes at least
+constexpr int X_COST = 1, X_MIN = 2; // places that a unit costs beside its blocks (144 rows, heads of 128: 1 for 166 us, 2 for 173, 3 for 175); that a CTA takes at least
 
 template <typename KV, int D, int M> struct SplitCfg {
     static constexpr int RT = M / 16, KG = 8 / RT, NT = XK / KG / 8;   // row tiles; groups of keys; tiles of eight keys of a warp

@@ -24,8 +24,8 @@ constexpr int FT = 256;              // threads
 constexpr int F_COST = 1, F_MIN = 2; // places that a unit costs beside its blocks; places that a CTA takes at least
 constexpr int F_STATIC = 1280;       // bytes of static shared memory at most
 constexpr int F_PER_SM = 2;          // CTAs on an SM at most: 128 registers a thread
-constexpr int FSP = 4;               // floats behind a row of queries and of scores, for the same
 constexpr int F_PAD = 16;            // bytes behind a key's row: 128-bit reads one row apart hit distinct banks
+constexpr int FSP = 4;               // floats behind a row of queries and of scores, for the same
 
 // Two multiply-adds in one instruction
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {

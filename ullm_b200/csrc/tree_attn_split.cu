@@ -150,12 +150,16 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
         const bool mine = tg < C::NT * 8; // threads that look up a key each
-        if (mine) {                       // of the first two blocks
-            const int key = w.blk * XK + kbase + tg, page0 = page_at(key), page1 = page_at(key + XK);
-            offs[0][kbase + tg] = place(page0, key), offs[1][kbase + tg] = place(page1, key + XK);
-        }
-        meet();
-        fetch(w.blk, stage0);
+        auto begin = [&] {
+            if (mine) { // keys of the first two blocks
+                const int key = w.blk * XK + kbase + tg, page0 = page_at(key), page1 = page_at(key + XK);
+                offs[0][kbase + tg] = place(page0, key), offs[1][kbase + tg] = place(page1, key + XK);
+            }
+            meet();
+            fetch(w.blk, stage0);
+        };
+        begin();
+        const bool work = rt * 16 < rows;
         for (int i = tid; i < M * (D / 4); i += XT) { // queries: value 8 t + e of 32 is product t (or t + 4, for e >= 4) of step e % 4
             const int r = i / (D / 4), d = i % (D / 4) * 4;
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -170,145 +174,156 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
             }
         }
         __syncthreads();
-        const bool work = rt * 16 < rows, big = seg.big;
+        const bool big = seg.big;
         const int row[2] = {rt * 16 + g, rt * 16 + g + 8}, token[2] = {token_of(row[0]), token_of(row[1])};
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}; // l: this lane's share
+        float m[2], l[2]; // l: this lane's share
         float o[D / 32][4][1][4]; // [c][i]: value 32 c + 8 t + i of rows 0 and 1 in 0 and 2, value 32 c + 8 t + 4 + i in 1 and 3
+        // Values that are not finite must not reach a row that does not see them (0 * inf), nor be split.  They show in the sums, and the segment is
+        // worked through again with a look at every value: looking the first time cost 5 % (90 rows).
+        for (bool careful = false;;) {
+            m[0] = m[1] = -INFINITY, l[0] = l[1] = 0.f;
 #pragma unroll
-        for (int n = 0; n < D / 2; ++n) o[n / 16][n / 4 % 4][0][n % 4] = 0.f;
-        for (int blk = w.blk; blk < blk_end; ++blk) {
-            uint8_t *const ks = stage0 + ((blk - w.blk) & 1) * C::STAGE, *const vs = ks + XK * C::KP;
-            const int k0 = blk * XK;
-            if (blk + 1 < blk_end) {
-                fetch(blk + 1, stage0 + ((blk + 1 - w.blk) & 1) * C::STAGE);
-                asm volatile("cp.async.wait_group 1;" ::: "memory");
-            } else {
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
-            }
-            meet();
-            // the block after the next: its page numbers travel while this one is worked on
-            const int ahead = (blk + 2) * XK + kbase + tg;
-            const bool more = mine && blk + 2 < blk_end;
-            const int page = more ? page_at(ahead) : -1;
-            if (work && k0 + kbase < key_end) {
-                constexpr int SETS = C::NT == 1 ? 3 : 2; // a product waits for the one before it in its place: three places at least
-                float parts[C::NT][SETS][4], s[C::NT][4], z = 0.f;
-#pragma unroll
-                for (int n = 0; n < C::NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < SETS * 4; ++e) parts[n][e / 4][e % 4] = 0.f;
-#pragma unroll 1
-                for (int c = 0; c < D / 32; ++c) { // (unrolled, it held more than the registers of two CTAs)
-                    float y[C::NT][8];
-#pragma unroll
-                    for (int n = 0; n < C::NT; ++n) widen8(y[n], (const KV *)(ks + (kbase + n * 8 + g) * C::KP) + c * 32 + t * 8);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int at = ((rt * (D / 8) + c * 4 + i) * 32 + lane) * 4;
-                        const float4 a = *(const float4 *)(qa + at);
-                        const float4 b = *(const float4 *)(qb + at);
-                        float y0[C::NT], y1[C::NT];
-#pragma unroll
-                        for (int n = 0; n < C::NT; ++n) y0[n] = y[n][i], y1[n] = y[n][4 + i];
-                        products<KV>(parts, a, b, y0, y1, z);
-                    }
+            for (int n = 0; n < D / 2; ++n) o[n / 16][n / 4 % 4][0][n % 4] = 0.f;
+            for (int blk = w.blk; blk < blk_end; ++blk) {
+                uint8_t *const ks = stage0 + ((blk - w.blk) & 1) * C::STAGE, *const vs = ks + XK * C::KP;
+                const int k0 = blk * XK;
+                if (blk + 1 < blk_end) {
+                    fetch(blk + 1, stage0 + ((blk + 1 - w.blk) & 1) * C::STAGE);
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                } else {
+                    asm volatile("cp.async.wait_group 0;" ::: "memory");
                 }
+                meet();
+                // the block after the next: its page numbers travel while this one is worked on
+                const int ahead = (blk + 2) * XK + kbase + tg;
+                const bool more = mine && blk + 2 < blk_end;
+                const int page = more ? page_at(ahead) : -1;
+                if (work && k0 + kbase < key_end) {
+                    constexpr int SETS = C::NT == 1 ? 3 : 2; // a product waits for the one before it in its place: three places at least
+                    float parts[C::NT][SETS][4], s[C::NT][4], z = 0.f;
 #pragma unroll
-                for (int n = 0; n < C::NT; ++n)
+                    for (int n = 0; n < C::NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[n][e] = parts[n][0][e];
+                        for (int e = 0; e < SETS * 4; ++e) parts[n][e / 4][e % 4] = 0.f;
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; ++c) { // (unrolled, it held more than the registers of two CTAs)
+                        float y[C::NT][8];
 #pragma unroll
-                        for (int k = 1; k < SETS; ++k) s[n][e] += parts[n][k][e];
+                        for (int n = 0; n < C::NT; ++n) widen8(y[n], (const KV *)(ks + (kbase + n * 8 + g) * C::KP) + c * 32 + t * 8);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int at = ((rt * (D / 8) + c * 4 + i) * 32 + lane) * 4;
+                            const float4 a = *(const float4 *)(qa + at);
+                            const float4 b = *(const float4 *)(qb + at);
+                            float y0[C::NT], y1[C::NT];
+#pragma unroll
+                            for (int n = 0; n < C::NT; ++n) y0[n] = y[n][i], y1[n] = y[n][4 + i];
+                            products<KV>(parts, a, b, y0, y1, z);
+                        }
                     }
-                if (__any_sync(0xffffffffu, !(z < BIG * BIG)) || big) { // (b times an infinity is not what x times it is, either)
 #pragma unroll
                     for (int n = 0; n < C::NT; ++n)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const KV *const key = (const KV *)(ks + (kbase + n * 8 + 2 * t + (e & 1)) * C::KP);
-                            float sum = 0.f;
-                            for (int d = 0; d < D; ++d) {
-                                const int at = ((rt * (D / 8) + d / 32 * 4 + d % 4) * 32 + g * 4 + d % 32 / 8) * 4 + (e >> 1) + d % 8 / 4 * 2;
-                                sum = fmaf(qa[at] + qb[at], (float)key[d], sum);
+                            s[n][e] = parts[n][0][e];
+#pragma unroll
+                            for (int k = 1; k < SETS; ++k) s[n][e] += parts[n][k][e];
+                        }
+                    if (__any_sync(0xffffffffu, !(z < BIG * BIG)) || big) { // (b times an infinity is not what x times it is, either)
+#pragma unroll
+                        for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const KV *const key = (const KV *)(ks + (kbase + n * 8 + 2 * t + (e & 1)) * C::KP);
+                                float sum = 0.f;
+                                for (int d = 0; d < D; ++d) {
+                                    const int at = ((rt * (D / 8) + d / 32 * 4 + d % 4) * 32 + g * 4 + d % 32 / 8) * 4 + (e >> 1) + d % 8 / 4 * 2;
+                                    sum = fmaf(qa[at] + qb[at], (float)key[d], sum);
+                                }
+                                s[n][e] = sum;
                             }
-                            s[n][e] = sum;
-                        }
-                }
-                const bool all = k0 + kbase + C::NT * 8 <= min(key_end, v.ctx); // every row sees all of them
-                float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-                for (int n = 0; n < C::NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[n][e] *= p.scale_log2;
-                        if (!all) {
-                            const int key = k0 + kbase + n * 8 + 2 * t + (e & 1);
-                            bool see = key < key_end && row[e >> 1] < rows;
-                            if (see && key >= v.ctx) see = sees(p, v, token[e >> 1], key - v.ctx);
-                            if (!see) s[n][e] = -INFINITY;
-                        }
-                        mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
                     }
-                float corr[2];
+                    const bool all = k0 + kbase + C::NT * 8 <= min(key_end, v.ctx); // every row sees all of them
+                    float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    mx[a] = fmaxf(mx[a], __shfl_xor_sync(0xffffffffu, mx[a], 1));
-                    mx[a] = fmaxf(fmaxf(mx[a], __shfl_xor_sync(0xffffffffu, mx[a], 2)), m[a]);
-                    corr[a] = m[a] == -INFINITY ? 0.f : exp2f(m[a] - mx[a]);
-                    m[a] = mx[a], l[a] *= corr[a];
-                }
-                // nothing seen so far: all weights are zero.  (A score of +inf or NaN gives NaN, as the formula does.)
+                    for (int n = 0; n < C::NT; ++n)
 #pragma unroll
-                for (int n = 0; n < C::NT; ++n)
+                        for (int e = 0; e < 4; ++e) {
+                            s[n][e] *= p.scale_log2;
+                            if (!all) {
+                                const int key = k0 + kbase + n * 8 + 2 * t + (e & 1);
+                                bool see = key < key_end && row[e >> 1] < rows;
+                                if (see && key >= v.ctx) see = sees(p, v, token[e >> 1], key - v.ctx);
+                                if (!see) s[n][e] = -INFINITY;
+                            }
+                            mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
+                        }
+                    float corr[2];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[n][e] = s[n][e] == -INFINITY ? 0.f : exp2f(s[n][e] - m[e >> 1]);
-                        l[e >> 1] += s[n][e];
+                    for (int a = 0; a < 2; ++a) {
+                        mx[a] = fmaxf(mx[a], __shfl_xor_sync(0xffffffffu, mx[a], 1));
+                        mx[a] = fmaxf(fmaxf(mx[a], __shfl_xor_sync(0xffffffffu, mx[a], 2)), m[a]);
+                        corr[a] = m[a] == -INFINITY ? 0.f : exp2f(m[a] - mx[a]);
+                        m[a] = mx[a], l[a] *= corr[a];
                     }
-                if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+                    // nothing seen so far: all weights are zero.  (A score of +inf or NaN gives NaN, as the formula does.)
 #pragma unroll
-                    for (int n = 0; n < D / 2; ++n) o[n / 16][n / 4 % 4][0][n % 4] *= corr[n % 4 / 2];
-                }
-                // Values that are not finite must not reach a row that does not see them (0 * inf), nor be split: they become zeros here and are added at the end.
-                {
-                    KV *const own = (KV *)(vs + kbase * C::VP);
-                    float bad = 0.f;
+                    for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            s[n][e] = s[n][e] == -INFINITY ? 0.f : exp2f(s[n][e] - m[e >> 1]);
+                            l[e >> 1] += s[n][e];
+                        }
+                    if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+#pragma unroll
+                        for (int n = 0; n < D / 2; ++n) o[n / 16][n / 4 % 4][0][n % 4] *= corr[n % 4 / 2];
+                    }
+                    // Values that are not finite become zeros here and are added at the end.
+                    if (careful) {
+                        KV *const own = (KV *)(vs + kbase * C::VP);
+                        float bad = 0.f;
 #pragma unroll 2
-                    for (int i = lane; i < C::NT * 8 * (D / 8); i += 32) {
-                        float y[8];
-                        widen8(y, (const KV *)((uint8_t *)own + i / (D / 8) * C::VP) + i % (D / 8) * 8);
+                        for (int i = lane; i < C::NT * 8 * (D / 8); i += 32) {
+                            float y[8];
+                            widen8(y, (const KV *)((uint8_t *)own + i / (D / 8) * C::VP) + i % (D / 8) * 8);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) bad = fmaf(y[e], 0.f, bad);
-                    }
-                    if (__any_sync(0xffffffffu, bad != bad)) {
-                        for (int i = lane; i < C::NT * 8 * D; i += 32) {
-                            KV *const at = (KV *)((uint8_t *)own + i / D * C::VP) + i % D;
-                            if (!isfinite((float)*at)) *at = (KV)0.f;
+                            for (int e = 0; e < 8; ++e) bad = fmaf(y[e], 0.f, bad);
                         }
-                        seg.odd = 1;
-                        __syncwarp();
+                        if (__any_sync(0xffffffffu, bad != bad)) {
+                            for (int i = lane; i < C::NT * 8 * D; i += 32) {
+                                KV *const at = (KV *)((uint8_t *)own + i / D * C::VP) + i % D;
+                                if (!isfinite((float)*at)) *at = (KV)0.f;
+                            }
+                            seg.odd = 1;
+                            __syncwarp();
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < C::NT; ++n) {
+                        const float4 x = make_float4(s[n][0], s[n][2], s[n][1], s[n][3]); // product t is key 2 t, product t + 4 key 2 t + 1
+                        const float4 a = make_float4(round11(x.x), round11(x.y), round11(x.z), round11(x.w));
+                        const float4 b = make_float4(cut11(x.x - a.x), cut11(x.y - a.y), cut11(x.z - a.z), cut11(x.w - a.w));
+                        const KV *const v0 = (const KV *)(vs + (kbase + n * 8 + 2 * t) * C::VP) + g * 4, *const v1 = (const KV *)((const uint8_t *)v0 + C::VP);
+                        float unused = 0.f;
+#pragma unroll
+                        for (int c = 0; c < D / 32; ++c) {
+                            const float4 y0 = widen4(v0 + c * 32), y1 = widen4(v1 + c * 32);
+                            const float w0[4] = {y0.x, y0.y, y0.z, y0.w}, w1[4] = {y1.x, y1.y, y1.z, y1.w};
+                            products<KV>(o[c], a, b, w0, w1, unused);
+                        }
                     }
                 }
-#pragma unroll
-                for (int n = 0; n < C::NT; ++n) {
-                    const float4 x = make_float4(s[n][0], s[n][2], s[n][1], s[n][3]); // product t is key 2 t, product t + 4 key 2 t + 1
-                    const float4 a = make_float4(round11(x.x), round11(x.y), round11(x.z), round11(x.w));
-                    const float4 b = make_float4(cut11(x.x - a.x), cut11(x.y - a.y), cut11(x.z - a.z), cut11(x.w - a.w));
-                    const KV *const v0 = (const KV *)(vs + (kbase + n * 8 + 2 * t) * C::VP) + g * 4, *const v1 = (const KV *)((const uint8_t *)v0 + C::VP);
-                    float unused = 0.f;
-#pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        const float4 y0 = widen4(v0 + c * 32), y1 = widen4(v1 + c * 32);
-                        const float w0[4] = {y0.x, y0.y, y0.z, y0.w}, w1[4] = {y1.x, y1.y, y1.z, y1.w};
-                        products<KV>(o[c], a, b, w0, w1, unused);
-                    }
-                }
+                if (more) offs[(blk - w.blk) & 1][kbase + tg] = place(page, ahead);
+                meet(); // the stage is free
             }
-            if (more) offs[(blk - w.blk) & 1][kbase + tg] = place(page, ahead);
-            meet(); // the stage is free
+            bool odd = false;
+            if (work && !careful)
+#pragma unroll
+                for (int n = 0; n < D / 2; ++n) odd |= !(fabsf(o[n / 16][n / 4 % 4][0][n % 4]) < INFINITY);
+            if (!__syncthreads_or(odd)) break;
+            careful = true;
+            begin();
         }
-        __syncthreads();
         // the warps' results meet in the stages' memory
         float *const red = (float *)stage0;
         if (work) {

@@ -132,9 +132,10 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
         auto token_of = [&](int r) { return (w.row0 + r) / p.group; };
         auto head_of = [&](int r) { return w.h * p.group + (w.row0 + r) % p.group; };
         const int *const table = p.blocks + (size_t)v.id * p.max_blocks;
-        auto page_at = [&](int token) { return token < key_end ? table[token / p.page_size] : -1; };
+        auto entry = [&](int token) { return p.page_log >= 0 ? token >> p.page_log : token / p.page_size; };
+        auto page_at = [&](int token) { return token < key_end ? table[entry(token)] : -1; };
         auto place = [&](int page, int token) { // a key behind the last, or of a page outside the pool, has none
-            return (unsigned)page < (unsigned)p.n_pages ? (page * p.page_stride + token % p.page_size * p.slot_stride + w.h * p.head_stride) * (long long)sizeof(KV) : -1ll;
+            return (unsigned)page < (unsigned)p.n_pages ? (page * p.page_stride + (token - entry(token) * p.page_size) * p.slot_stride + w.h * p.head_stride) * (long long)sizeof(KV) : -1ll;
         };
         auto fetch = [&](int blk, uint8_t *stage) { // zeros for a key that has no place
             const long long *const at = offs[(blk - w.blk) & 1];
@@ -205,8 +206,8 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
                     for (int n = 0; n < C::NT; ++n)
 #pragma unroll
                         for (int e = 0; e < SETS * 4; ++e) parts[n][e / 4][e % 4] = 0.f;
-#pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) { // (unrolled, it held more than the registers of two CTAs)
+#pragma unroll(D == 64 ? 2 : 1)
+                    for (int c = 0; c < D / 32; ++c) { // (90 rows over heads of 64: 132 us, 135 with a loop; over heads of 128: 166 us, 164 with one)
                         float y[C::NT][8];
 #pragma unroll
                         for (int n = 0; n < C::NT; ++n) widen8(y[n], (const KV *)(ks + (kbase + n * 8 + g) * C::KP) + c * 32 + t * 8);

@@ -15,6 +15,8 @@
 // product is free as long as both sides agree; it is chosen so that a lane reads 16 neighbouring bytes.
 // On the CUDA cores (tree_attn.cu) the reads of shared memory bound the same work: 32 lanes x 16 bytes take four cycles and feed 32 multiply-adds per lane.
 // Rows are few (a group's heads x drafted tokens), so that tcgen05's tile of 128 rows would be empty for the most part.
+// It is bound by chains of dependent instructions, eight or sixteen warps on an SM: issue slots 42 % and the tensor pipe 26 to 35 % busy; 32 sequences of one row
+// and 1,500 keys (174 MB) 2.9 TB/s, 90 rows over heads of 64 27 TFLOP/s of 32-bit results, where the CUDA cores gave 2.6 TB/s and 14 to 16.
 #include "engine.h"
 #include "tree_sched.cuh"
 
@@ -25,7 +27,7 @@ namespace {
 
 constexpr int XT = 256, XK = 64;     // threads; keys of a block
 constexpr float BIG = 1.152921504606847e18f; // 2^60
-constexpr int X_COST = 1, X_MIN = 2; // places that a unit costs beside its blocks (144 rows, heads of 128: 1 for 166 us, 2 for 173, 3 for 175); that a CTA takes at least
+constexpr int X_COST = 2, X_MIN = 2; // places that a unit costs beside its blocks (32 sequences of one row: 1 for 59.5 us, 2 for 58.5, 3 for 59.4); that a CTA takes at least
 
 template <typename KV, int D, int M> struct SplitCfg {
     static constexpr int RT = M / 16, KG = 8 / RT, NT = XK / KG / 8;   // row tiles; groups of keys; tiles of eight keys of a warp
@@ -395,8 +397,8 @@ template <typename KV, int D, int M> cudaError_t launch_as(const DeviceInfo &dev
 template <typename KV, int D> cudaError_t launch_for(const DeviceInfo &dev, const TreeDev &t, bool pdl, cudaStream_t st) {
     // Rows per sequence and key head on average (the lengths themselves are on the device; either way is right for any of them).
     const long long rows = ((long long)t.n_rows * t.group + t.n_seq - 1) / t.n_seq;
-    // Tiles of 32 rows split the keys half as often (90 rows: 149 us, with 16 rows 179; 64 rows take 160), but 16 rows spread a little work over more CTAs, where
-    // even tables in full use would give a CTA no more than four blocks (24 units of 28 rows and up to 2,000 keys: 21.8 us, with 32 rows 24.0).
+    // Tiles of 32 rows split the keys half as often (90 rows: 129 us, with 16 rows 158; 64 rows took 7 % longer than 32), but 16 rows spread a little work over more CTAs, where
+    // even tables in full use would give a CTA no more than four blocks (24 units of 28 rows and up to 2,000 keys: 21.2 us, with 32 rows 25.9).
     const long long blocks = (rows + 31) / 32 * t.n_seq * t.n_kv * (((long long)t.max_blocks * t.page_size + XK - 1) / XK);
     if (rows <= 16 || blocks <= 4 * dev.sm_count * SplitCfg<KV, D, 16>::PER_SM) return launch_as<KV, D, 16>(dev, t, pdl, st);
     return launch_as<KV, D, 32>(dev, t, pdl, st);

@@ -455,3 +455,15 @@ def test_sequences_without_keys_beside_large_pages(ctx, dtype, ps):
     c.out[c.rows:keep] = 7
     c.check()
     assert bool((k[:, :256] == 0).all())
+
+
+@pytest.mark.parametrize("dtype,q32,dim,n", [("f16", False, 64, 2), ("bf16", False, 128, 2), ("f16", False, 128, 70), ("f32", True, 64, 2), ("f32", True, 128, 9), ("f32", True, 40, 2)])
+def test_an_infinite_value_of_next_to_no_weight(ctx, dtype, q32, dim, n):
+    """The parts that hold the rows' own tokens have weights below 2^-149 when they are joined; an infinite value there still shows, as in the formula."""
+    c = Case([3000], [n], 4, 1, dim, dtype, 16, mask="chain", q32=q32, seed=8)
+    c.q[:, :4 * dim] = c.q[:, :4 * dim].abs() + 1
+    for tok in range(2000, 3000 + n):
+        c.k[c.layer, int(c.blocks[0, tok // 16]), tok % 16] = -20
+    c.v[c.layer, int(c.blocks[0, 3000 // 16]), 3000 % 16, :, 5] = float("inf")
+    c.run(ctx)
+    c.check()

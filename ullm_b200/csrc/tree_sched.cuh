@@ -247,6 +247,9 @@ template <> __device__ __forceinline__ float out_from<float>(float v) { return v
 template <> __device__ __forceinline__ __half out_from<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 out_from<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// Weight of a part: 0 where nothing was seen, else at least the smallest number, so that an infinite value in it stays infinite.
+__device__ __forceinline__ float part_weight(float m_part, float m) { return m_part == -INFINITY ? 0.f : fmaxf(exp2f(m_part - m), 1.4e-45f); }
+
 // Joins a unit's parts without a second launch: the CTAs that have a part of it count, and the last one to arrive joins them all, in the order of the CTAs.
 // A count is kept in 64 bits beside the number of the call, and any other number there counts as none: the memory needs no preparation, and
 // what an abandoned call leaves does no harm.  Every thread calls it, behind its stores of the CTA's own part.
@@ -290,7 +293,7 @@ template <typename O, int M, int D> __device__ __forceinline__ void join_last(co
             m = top;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const float c = ml[k].x == -INFINITY ? 0.f : exp2f(ml[k].x - m);
+                const float c = part_weight(ml[k].x, m);
                 l += ml[k].y * c; // (NaN where a score was NaN)
                 acc.x += c * x[k].x, acc.y += c * x[k].y, acc.z += c * x[k].z, acc.w += c * x[k].w;
             }
@@ -377,7 +380,7 @@ template <typename O, int M, int K> __device__ __forceinline__ void join_rows(co
                         for (int o = K / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
                     }
                 }
-                const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
+                const float w = part_weight(ml.x, m);
                 l += ml.y * w;
 #pragma unroll
                 for (int s = 0; s < 8; ++s) {
@@ -483,7 +486,7 @@ template <typename O, int M> __global__ void __launch_bounds__(32 * JOIN_WARPS, 
                 float w = 0.f; // weight of this warp's part number `lane` of the eight
                 if (lane < n) {
                     const float2 ml = pair(j0 + lane * split);
-                    w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
+                    w = part_weight(ml.x, m);
                     l += ml.y * w;
                 }
 #pragma unroll

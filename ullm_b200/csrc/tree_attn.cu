@@ -313,7 +313,9 @@ template <typename Q, typename KV, int M, int KEYS> static cudaError_t launch_fm
     return launch_kernel(tree_join_kernel<Q, M>, dim3(dev.sm_count * JOIN_PER_SM<M>), dim3(32 * JOIN_WARPS), 0, st, pdl, t, ctas);
 }
 template <typename Q, typename KV> static cudaError_t launch_fma(const DeviceInfo &dev, const TreeDev &t, bool pdl, cudaStream_t st) {
-    const long long rows = ((long long)t.n_rows * t.group + t.n_seq - 1) / t.n_seq; // per sequence and key head, on average
+    // Rows per sequence and key head, on average.  A tile with room for many more rows than there are leaves threads idle (four rows over heads of 64: 65 us with
+    // tiles of 8 rows, 78 with 16), a smaller one reads the keys more often.
+    const long long rows = ((long long)t.n_rows * t.group + t.n_seq - 1) / t.n_seq;
     const bool k64 = fma_keys(t.dim * (int)sizeof(KV)) == 64;
     if (rows > 16) return k64 ? launch_fma_as<Q, KV, 32, 64>(dev, t, pdl, st) : launch_fma_as<Q, KV, 32, 32>(dev, t, pdl, st);
     if (rows > 8) return k64 ? launch_fma_as<Q, KV, 16, 64>(dev, t, pdl, st) : launch_fma_as<Q, KV, 16, 32>(dev, t, pdl, st);

@@ -467,3 +467,45 @@ def test_an_infinite_value_of_next_to_no_weight(ctx, dtype, q32, dim, n):
     c.v[c.layer, int(c.blocks[0, 3000 // 16]), 3000 % 16, :, 5] = float("inf")
     c.run(ctx)
     c.check()
+
+
+def test_32_bit_calls_on_two_streams_and_two_graphs_of_one_work_area(ctx):
+    """Units are joined by whoever arrives last: objects of their own at the same time, and graphs that share one object one after the other."""
+    cases = [Case([4000, 900], [7, 3], 8, 2, 128, "f32", 16, mask="tree", seed=1, q32=True), Case([2500, 1900], [5, 30], 8, 2, 64, "f16", 16, mask="tree", seed=2, q32=True)]
+    s, ops, first = [torch.cuda.Stream(), torch.cuda.Stream()], [None, None], []
+    torch.cuda.synchronize()
+    for rnd in range(6):
+        for c in cases:
+            c.out.fill_(7)
+        torch.cuda.synchronize()
+        for i, c in enumerate(cases):
+            ops[i] = c.run(ctx, ops[i], s=s[i].cuda_stream)
+        torch.cuda.synchronize()
+        if rnd == 0:
+            first = [c.out.clone() for c in cases]
+            for c in cases:
+                c.check()
+        assert all(torch.equal(c.out, f) for c, f in zip(cases, first))
+    # two calls of different shapes through one work area, each in a graph
+    c, d = cases[0], Case([700, 60], [40, 1], 8, 2, 128, "f32", 16, mask="any", seed=5, q32=True)
+    op = backend.TreeAttention(ctx, c.kv, 8)
+    other = backend.TreeAttention(ctx, d.kv, 8)
+    other._a.d_work = op._a.d_work
+    graphs = []
+    for x, o in ((c, op), (d, other)):
+        x.run(ctx, o, s=s[0].cuda_stream)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s[0]):
+            o.run_dev(x.layer, x.q.data_ptr(), x.out.data_ptr(), x.rows + x.pad, 2, x.d[0].data_ptr(), x.d[1].data_ptr(), x.d[2].data_ptr(), x.max_blocks,
+                      d_mask=x.d[4].data_ptr(), mask_words=x.words, d_ids=x.d[3].data_ptr(), n_table=2, q_stride=x.qs, out_stride=x.os, stream=s[0].cuda_stream)
+        graphs.append(g)
+    for _ in range(4):
+        c.out.fill_(7), d.out.fill_(7)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s[0]):
+            graphs[0].replay()
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(c.out, first[0])
+        d.check()

@@ -298,3 +298,33 @@ def test_rope_in_place_and_rows_outside_are_left_out(ctx):
     assert (err <= 2.0 ** -11 * np.abs(ref) + 4 * 2.0 ** -24 * mag + 6e-8).all()
     k0[0, 0, 0], v0[0, 0, 0] = k[0, 0, 0], v[0, 0, 0]
     assert torch.equal(k, k0) and torch.equal(v, v0)
+
+
+def test_lengths_at_the_ends_of_the_range_are_refused(ctx):
+    """Counting such a length in pages would pass 32 bits; every call refuses it before it looks into the table."""
+    for ps in (16, 5):
+        b = Both(ctx, 6, 8, 10, ps)
+        b.call("grow", [0], [ps + 3])
+        top, low = 2 ** 31 - 1, -(2 ** 31)
+        b.put(length=[ps + 3, top, top - 1, low, low + 1, 0])
+        for s in (1, 2, 3, 4):
+            for name, lists in (("fork", ([s], [5])), ("trim", ([s], [0])), ("trim", ([s], None)), ("accept", ([s], [4], [[1, 3]], [2])), ("accept", ([s], [top], [[top - 1]], [1])),
+                                ("grow", ([s], [1]))):
+                b.call(name, *lists)
+                assert b.ref.fault == backend.KV_FAULT_LEN
+                b.clear()
+        b.call("accept", [0], [3], [[0, 2]], [2])
+        assert b.ref.fault == 0
+
+
+def test_plan_refuses_lengths_at_the_ends_of_the_range(ctx):
+    lens = [2 ** 31 - 1, -(2 ** 31), -(2 ** 31) + 3, 9]
+    cu, rows = [0, 3, 7, 9, 11], 12
+    want = paged_ref.plan(cu, lens, None, rows, 1)
+    d = [ints(a) for a in (cu, lens)]
+    seq, slot, pos = (ints(np.full(rows, -9)) for _ in range(3))
+    mask, fault = torch.full((rows, 1), -286331154, dtype=torch.int32, device="cuda"), ints([0])
+    ctx.tree_plan_dev(rows, 4, d[0].data_ptr(), d[1].data_ptr(), None, seq.data_ptr(), slot.data_ptr(), pos.data_ptr(), mask.data_ptr(), 1, fault.data_ptr(), stream=stream())
+    torch.cuda.synchronize()
+    assert seq.tolist() == [0] * 3 + [-1] * 6 + [3] * 2 + [-1] and int(fault[0]) == want[4] == backend.KV_FAULT_LEN
+    assert np.array_equal(slot.cpu().numpy(), want[1]) and np.array_equal(pos.cpu().numpy(), want[2]) and np.array_equal(mask.cpu().numpy().view(np.uint32), want[3])

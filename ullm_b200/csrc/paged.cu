@@ -43,6 +43,9 @@ __device__ __forceinline__ void set_fault(int *fault, int bits) {
     if (fault && bits) atomicOr(fault, bits);
 }
 
+// Whether a row of the table can hold `len` tokens.  (Asked before `len` is counted in pages: near the end of the range that sum would pass 32 bits.)
+__device__ __forceinline__ bool len_fits(const TableDev &t, int page_size, int len) { return len >= 0 && len <= (long long)t.max_blocks * page_size; }
+
 // Whether `v` occurs in list[0 .. n) at another place than `self`; every thread of the CTA calls it with the same arguments.
 __device__ __forceinline__ bool cta_listed_elsewhere(const int *list, int n, int v, int self) {
     bool hit = false;
@@ -61,9 +64,9 @@ __global__ void __launch_bounds__(128) kv_fork_kernel(const TableDev t, int page
     if (cta_listed_elsewhere(dst, n, d, i) || cta_listed_elsewhere(src, n, d, -1)) bad |= ULLM_KV_FAULT_SEQ;
     if (!bad) {
         len = t.len[s];
-        blocks = len > 0 ? cdiv(len, page_size) : 0;
-        if (len < 0 || blocks > t.max_blocks) bad = ULLM_KV_FAULT_LEN;
+        if (!len_fits(t, page_size, len)) bad = ULLM_KV_FAULT_LEN;
         else if (t.len[d] != 0) bad = ULLM_KV_FAULT_SEQ;
+        else blocks = cdiv(len, page_size);
     }
     const int *from = t.blocks + (size_t)(bad ? 0 : s) * t.max_blocks;
     bool out = false;
@@ -109,7 +112,7 @@ __global__ void __launch_bounds__(128) kv_trim_kernel(const TableDev t, int page
     int len = 0, want = 0;
     if (!bad) {
         len = t.len[s], want = new_len ? new_len[i] : 0;
-        if (want < 0 || want > len || cdiv(len, page_size) > t.max_blocks) bad = ULLM_KV_FAULT_LEN;
+        if (want < 0 || want > len || !len_fits(t, page_size, len)) bad = ULLM_KV_FAULT_LEN;
     }
     __syncthreads(); // every thread has read the length before it changes
     if (bad) {
@@ -142,7 +145,7 @@ __global__ void __launch_bounds__(128) kv_accept_move_kernel(const TableDev t, c
     int len = 0;
     if (!bad) {
         len = t.len[s];
-        if (nd < 0 || nd > len || nk < 0 || nk > nd || nk > max_path || cdiv(len, ps) > t.max_blocks) bad = ULLM_KV_FAULT_LEN;
+        if (nd < 0 || nd > len || nk < 0 || nk > nd || nk > max_path || !len_fits(t, ps, len)) bad = ULLM_KV_FAULT_LEN;
     }
     const int base = len - nd;
     const int *row = t.blocks + (size_t)(bad ? 0 : s) * t.max_blocks;
@@ -410,8 +413,8 @@ __global__ void __launch_bounds__(128) tree_plan_kernel(int n_rows, int n_seq, c
     }
     const int n = r1 - r0, id = ids ? ids[b] : b;
     int bad = id < 0 || id >= n_table ? ULLM_KV_FAULT_SEQ : 0;
-    const int ctx = bad ? 0 : len[id] - n;
-    if (ctx < 0 || (mask && n > 32 * words) || (parent && n > PLAN_MAX)) bad |= ULLM_KV_FAULT_LEN;
+    const int held = bad ? n : len[id], ctx = held - n; // (n is not negative: only a length below it could leave the range)
+    if (held < n || (mask && n > 32 * words) || (parent && n > PLAN_MAX)) bad |= ULLM_KV_FAULT_LEN;
     if (bad) {
         if (tid == 0) set_fault(fault, bad);
         for (int i = tid; i < n; i += 128) row_seq[r0 + i] = -1;

@@ -328,3 +328,24 @@ def test_plan_refuses_lengths_at_the_ends_of_the_range(ctx):
     torch.cuda.synchronize()
     assert seq.tolist() == [0] * 3 + [-1] * 6 + [3] * 2 + [-1] and int(fault[0]) == want[4] == backend.KV_FAULT_LEN
     assert np.array_equal(slot.cpu().numpy(), want[1]) and np.array_equal(pos.cpu().numpy(), want[2]) and np.array_equal(mask.cpu().numpy().view(np.uint32), want[3])
+
+
+def test_wants_beyond_32_bits_are_refused_as_a_whole(ctx):
+    """512 rows that ask for 2^22 pages each: the sum is 2^31 pages."""
+    n, blocks, pages = 512, 1 << 22, 64
+    k, v, kv = make_pool(1, pages, 1, 1, 8, "f16", "slot", 1)
+    table = torch.empty((n, blocks), dtype=torch.int32, device="cuda")
+    lens, refs, fault = ints(np.zeros(n)), ints(np.zeros(pages)), ints([0])
+    t = backend.KvTable(ctx, kv, table.data_ptr(), lens.data_ptr(), refs.data_ptr(), fault.data_ptr(), n, blocks)
+    seq = ints(np.arange(n))
+    for add in (blocks, blocks - 1, 1 << 20):
+        adds = ints(np.full(n, add))
+        fault.zero_()
+        t.grow_dev(seq.data_ptr(), adds.data_ptr(), n, stream=stream())
+        torch.cuda.synchronize()
+        assert int(fault[0]) == backend.KV_FAULT_NO_PAGES and int(lens.abs().sum()) == 0 and int(refs.sum()) == 0
+    adds = ints(np.arange(n) < 60)
+    fault.zero_()
+    t.grow_dev(seq.data_ptr(), adds.data_ptr(), n, stream=stream())
+    torch.cuda.synchronize()
+    assert int(fault[0]) == 0 and int(lens.sum()) == 60 and torch.equal(table[:60, 0], torch.arange(60, dtype=torch.int32, device="cuda"))

@@ -204,29 +204,32 @@ __global__ void __launch_bounds__(128) kv_accept_end_kernel(const TableDev t, in
 }
 
 // ---- grow -----------------------------------------------------------------------------------------------------------
-// Exclusive prefix sum over the CTA's 1024 threads; returns the sum of all.
+// Exclusive prefix sum over the CTA's 1024 threads; returns the sum of all.  Sums stop at SCAN_MAX, more than any pool has pages: what many long
+// rows ask for together passes 32 bits.
+constexpr unsigned SCAN_MAX = 1u << 30;
 __device__ __forceinline__ int cta_scan1024(int v, int *excl, int *warp_sums) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int x = v;
+    auto add = [](unsigned a, unsigned b) { return min(a + b, SCAN_MAX); };
+    unsigned x = min((unsigned)v, SCAN_MAX);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
+        const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x = add(x, y);
     }
     __syncthreads();
-    if (lane == 31) warp_sums[warp] = x;
+    if (lane == 31) warp_sums[warp] = (int)x;
     __syncthreads();
     if (warp == 0) {
-        int w = warp_sums[lane];
+        unsigned w = (unsigned)warp_sums[lane];
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += y;
+            const unsigned y = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w = add(w, y);
         }
-        warp_sums[lane] = w;
+        warp_sums[lane] = (int)w;
     }
     __syncthreads();
-    *excl = x - v + (warp ? warp_sums[warp - 1] : 0);
+    *excl = (int)x - v + (warp ? warp_sums[warp - 1] : 0); // (of no use once the sum has stopped)
     return warp_sums[31];
 }
 

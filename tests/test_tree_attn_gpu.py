@@ -509,3 +509,28 @@ def test_32_bit_calls_on_two_streams_and_two_graphs_of_one_work_area(ctx):
         torch.cuda.synchronize()
         assert torch.equal(c.out, first[0])
         d.check()
+
+
+@pytest.mark.parametrize("dtype,dim,heads,kv_heads,n", [("f16", 64, 4, 1, 2), ("bf16", 128, 8, 2, 70), ("f16", 128, 6, 2, 9)])
+def test_a_wait_that_runs_out_ends_the_call_with_a_status(ctx, dtype, dim, heads, kv_heads, n):
+    """With a limit of no time at all the warps that enqueue loads and products give up where they would wait, with some of them under way, and the others
+    after their second: the call ends, the host learns of it, and the next call gives what the one before gave."""
+    c = Case([4000, 900, 20], [n, 3, 1], heads, kv_heads, dim, dtype, 16, mask="tree", seed=1)
+    op = c.run(ctx)
+    c.check()
+    first = c.out.clone()
+    for _ in range(2):
+        ctx.debug_set("tree_wait_cycles", 0)
+        try:
+            c.run(ctx, op)
+            torch.cuda.synchronize()
+            with pytest.raises(backend.UllmError) as e:
+                ctx.synchronize()
+            assert e.value.code == backend.ERR_TIMEOUT
+        finally:
+            ctx.debug_set("tree_wait_cycles", -1)
+        c.out.fill_(7)
+        c.run(ctx, op)
+        torch.cuda.synchronize()
+        ctx.synchronize()
+        assert torch.equal(c.out, first)

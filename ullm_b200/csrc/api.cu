@@ -724,6 +724,7 @@ extern "C" int ullm_cuda_debug_set(ullm_cuda_ctx *c, const char *key, int value)
     if (!strcmp(key, "force_generic")) c->force_generic = value != 0;
     else if (!strcmp(key, "no_prepare")) c->no_prepare = value != 0;
     else if (!strcmp(key, "gemm_min_s")) c->gemm_min_s = value;
+    else if (!strcmp(key, "tree_wait_cycles")) c->tree_wait_cycles = value < 0 ? TREE_WAIT_CYCLES : value;
     else if (!strcmp(key, "no_chain")) c->no_chain = value != 0;
     else if (!strcmp(key, "shard_no_tagged")) c->shard_no_tagged = value != 0;
     else if (!strcmp(key, "shard_gemm_exchange")) c->shard_gemm_exchange = value;

@@ -84,6 +84,8 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t *bar, uint32_t parity
         if (mbar_try_wait(bar, parity)) return true;
     return false;
 }
+constexpr long long TREE_WAIT_CYCLES = 1ll << 31; // limit of a wait in tree_attn_tc.cu: about a second
+
 // Global -> shared bulk copy, completion counted in bytes on `bar`.  Source,
 // destination and size must all be multiples of 16 bytes.
 __device__ __forceinline__ void bulk_g2s(void *smem_dst, const void *gsrc, uint32_t bytes, uint64_t *bar) {

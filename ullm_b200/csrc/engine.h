@@ -37,6 +37,7 @@ struct ullm_cuda_ctx {
     int shard_timeout_ms = 2000; // ULLM_OPT_SHARD_TIMEOUT_MS
     int shard_gemm_exchange = 0; // prefill form's block transfer: 0 chosen per block, 1 copy engines, 2 copy kernel (comparisons)
     bool shard_no_tagged = false; // sharded matvec steps through the flag protocol only (tests, comparisons)
+    long long tree_wait_cycles = ullm::TREE_WAIT_CYCLES; // limit of a wait in the attention of drafted rows (tests shorten it)
     int gemm_min_s = 32; // batches below this many tokens use per-token matvecs
     ullm::MatvecPlan last_plan;
 };

@@ -50,7 +50,8 @@ bool tree_attn_split_supported(int dim);
 cudaError_t launch_tree_attn_split(const DeviceInfo &dev, int kv_dtype, const TreeDev &t, bool pdl, cudaStream_t st);
 bool tree_attn_tc_supported(const PoolDev &pool, int dtype);
 size_t tree_attn_tc_work(int sm_count, int dim);
-cudaError_t launch_tree_attn_tc(const DeviceInfo &dev, const PoolDev &pool, int dtype, const TreeDev &t, int *d_status, bool pdl, cudaStream_t st);
+cudaError_t launch_tree_attn_tc(const DeviceInfo &dev, const PoolDev &pool, int dtype, const TreeDev &t, int *d_status, long long wait_cycles, bool pdl,
+                                cudaStream_t st);
 
 // Puts the caller's current device back when a call ends.
 struct DeviceGuard {

@@ -391,7 +391,7 @@ int ullm_cuda_tree_attn_dev(ullm_cuda_ctx *c, const ullm_tree_attn *a, void *str
     t.meta = (int4 *)a->d_work, t.count = (unsigned long long *)((uint8_t *)a->d_work + records), t.part = (float *)((uint8_t *)a->d_work + 2 * records);
     t.call = ++calls;
     cudaError_t e = cudaErrorNotSupported;
-    if (tree_attn_tc_supported(pool, a->dtype)) e = launch_tree_attn_tc(c->dev, pool, a->dtype, t, c->d_status, c->use_pdl, st);
+    if (tree_attn_tc_supported(pool, a->dtype)) e = launch_tree_attn_tc(c->dev, pool, a->dtype, t, c->d_status, c->tree_wait_cycles, c->use_pdl, st);
     if (e != cudaErrorNotSupported) { // (strides that a tensor map cannot describe go to the f32 kernel)
         ULLM_CUDA_TRY(c, e);
         return ULLM_OK;

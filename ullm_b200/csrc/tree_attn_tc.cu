@@ -22,8 +22,8 @@
 // first: rows behind the last key become zeros and values that are not finite are set aside (0 * inf would reach
 // rows that do not see the token); the epilogue adds them for the rows that do.
 //
-// Every wait is bounded (about a second); on expiry a role records DEV_TIMEOUT and leaves, all threads meet at the end and
-// the tensor memory is freed.
+// Every wait is bounded (about a second); on expiry a role leaves, waits (again with that limit) for the copies and products that it has in flight -
+// they write the CTA's shared and tensor memory - and records DEV_TIMEOUT; all threads meet at the end and the tensor memory is freed.
 #include "engine.h"
 #include "tree_sched.cuh"
 
@@ -54,21 +54,32 @@ struct TcParams {
     int team;      // logarithm of the CTAs of a team (Sched)
     int page_log;  // logarithm of the page size where it is below a block's keys
     int page_blocks; // blocks of a page where it is not
+    long long wait;  // clock cycles after which a wait of the warps that enqueue loads and products gives up (the others: TREE_WAIT_CYCLES)
 };
 struct TcMaps {
     CUtensorMap k, v, q;
 };
 
-// A converged warp waits; every lane gets the same answer, so that no lane leaves alone.
-__device__ __forceinline__ bool wait_bounded(uint64_t *bar, uint32_t parity) {
-    bool done = mbar_try_wait(bar, parity);
+__device__ __forceinline__ bool mbar_test_wait(uint64_t *bar, uint32_t parity) { // (does not wait at all)
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
+// A converged warp waits; every lane gets the same answer, so that no lane leaves alone.  A limit of 0 only looks.
+__device__ __forceinline__ bool wait_bounded(uint64_t *bar, uint32_t parity, long long limit = TREE_WAIT_CYCLES) {
+    bool done = limit ? mbar_try_wait(bar, parity) : mbar_test_wait(bar, parity);
     const long long t0 = clock64();
     while (!__all_sync(0xffffffffu, done)) {
+        if (!limit) return false;
 #pragma unroll 1
         for (int i = 0; i < 64 && !done; ++i) done = mbar_try_wait(bar, parity);
-        if (__any_sync(0xffffffffu, clock64() - t0 > (1ll << 31))) return __all_sync(0xffffffffu, done);
+        if (__any_sync(0xffffffffu, clock64() - t0 > limit)) return __all_sync(0xffffffffu, done);
     }
     return true;
+}
+// Waits for the last uses of a ring of barriers, `count` uses in all (uses i, i + stages, ... of barrier i).  Only where a role has given up.
+__device__ __noinline__ void wait_for_last(uint64_t *bars, uint32_t count, uint32_t stages) {
+    for (uint32_t i = count > stages ? count - stages : 0; i < count; ++i) wait_bounded(bars + i % stages, i / stages & 1);
 }
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap *map, int x, int c1, int c2, int page, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
@@ -245,7 +256,7 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
     constexpr int NST = C::STAGES, ROWS = TWO ? 2 * TM : TM, STEP = TWO ? 1 : 2; // STEP: a stream takes every so many blocks
     extern __shared__ __align__(1024) uint8_t gsm[];
     uint8_t *const q_sm = (uint8_t *)(((uintptr_t)gsm + 1023) & ~(uintptr_t)1023), *const ring = q_sm + 2 * C::TILE;
-    __shared__ uint64_t full[NST], empty[NST], s_full[2], p_full[2], o_done[2], h_full[2], q_full[2], q_empty[2], seg_full[SEGS], seg_empty[SEGS], x_full, epi_done;
+    __shared__ uint64_t full[NST], empty[NST], s_full[2], p_full[2], o_done[2], h_full[2], q_full[2], q_empty[2], seg_full[SEGS], seg_empty[SEGS], x_full, epi_done, mma_done;
     __shared__ Seg segs[SEGS];
     __shared__ uint32_t tmem_s;
     const TreeDev &p = prm.t;
@@ -259,7 +270,7 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
                 mbar_init(&q_full[s], 1), mbar_init(&q_empty[s], 8);
             }
             for (int i = 0; i < SEGS; ++i) mbar_init(&seg_full[i], 1), mbar_init(&seg_empty[i], 11);
-            mbar_init(&x_full, 8), mbar_init(&epi_done, 8);
+            mbar_init(&x_full, 8), mbar_init(&epi_done, 8), mbar_init(&mma_done, 1);
             mbar_fence_init();
         }
         __syncwarp();
@@ -278,6 +289,7 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
     pdl_launch_dependents();
     const uint32_t tmem = warp == 3 ? 0 : __shfl_sync(0xffffffffu, tmem_s, 0);
     bool ok = true;
+    auto wait = [&](uint64_t *bar, uint32_t parity) { return wait_bounded(bar, parity, prm.wait); };
     // the next segment of the ring; 0: no more
     uint32_t seg = 0;
     auto take = [&]() -> int {
@@ -311,7 +323,7 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
         // ---- TMA: lane -> (64 values, box of keys) ----
         const int atom = lane % C::ATOMS, part = lane / C::ATOMS, box = prm.box, parts = TK / box;
         const bool mine = part < parts;
-        uint32_t tile0 = 0;
+        uint32_t tile0 = 0, asked = 0; // asked: tiles whose boxes are under way or there
         for (int n; (n = take()) != 0 && ok; give()) {
             const Seg &w = segs[seg % SEGS];
             const int key_end = w.key_end, h = w.h, first = w.blk * TK + part * box;
@@ -329,7 +341,7 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
             };
             auto load = [&](const CUtensorMap *map, int j, uint32_t tile, int page) {
                 const uint32_t st = tile % NST;
-                if (tile >= NST && !wait_bounded(&empty[st], (tile / NST - 1) & 1)) return false;
+                if (tile >= NST && !wait(&empty[st], (tile / NST - 1) & 1)) return false;
                 const int token = first + j * TK;
                 const bool go = mine && token < key_end;
                 const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, go));
@@ -340,6 +352,7 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
                     tma_box(smem_u32(ring) + st * C::TILE + atom * (TK * 128) + part * box * 128, map, atom * 64, prm.slot_dim == 1 ? slot : h,
                             prm.slot_dim == 1 ? h : slot, page, smem_u32(&full[st]));
                 }
+                asked = tile + 1;
                 return true;
             };
             if (TWO) {
@@ -359,8 +372,10 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
             if (!ok) break;
             tile0 += 2 * n;
         }
+        if (!ok) wait_for_last(full, asked, NST);
     } else if (warp == 2) {
         // ---- queries, as rows of the swizzled tile(s): a stream's 128 rows, or those that the streams share ----
+        uint32_t asked = 0; // segments whose boxes are under way or there
         for (int n; (n = take()) != 0 && ok; give()) {
             const uint32_t b = TWO ? 0 : seg & 1, use = TWO ? seg : seg / 2; // TWO: both buffers in one go
             if (use && !(ok = wait_bounded(&q_empty[b], (use - 1) & 1))) break;
@@ -375,6 +390,7 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
                     tma_box(smem_u32(q_sm) + (b + r / TM) * C::TILE + atom * (TM * 128) + r % TM * 128, &maps.q, atom * 64, 0, w.h, token0 + part * prm.q_box,
                             smem_u32(&q_full[b]));
                 }
+                asked = seg + 1;
             } else {
                 constexpr int PIECES = D / 8, STRIDE = 32 / PIECES;
                 const int piece = lane % PIECES, jump = STRIDE / group, left = STRIDE % group;
@@ -394,13 +410,14 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
                 if (lane == 0) mbar_arrive(&q_full[b]);
             }
         }
+        if (!ok) wait_for_last(q_full, asked, TWO ? 1 : 2);
     } else if (warp == 1) {
         // ---- MMA issue: the whole warp with uniform control flow, one elected lane issues ----
         uint32_t tile0 = 0, done[2] = {0, 0};
         const uint32_t q0 = smem_u32(q_sm), r0 = smem_u32(ring);
         for (uint32_t n; (n = (uint32_t)take()) != 0 && ok; give()) {
             const uint64_t qd = desc_k_major(q0 + (TWO ? 0 : seg & 1) * C::TILE);
-            if (!(ok = TWO ? wait_bounded(&q_full[0], seg & 1) : wait_bounded(&q_full[seg & 1], seg / 2 & 1))) break;
+            if (!(ok = TWO ? wait(&q_full[0], seg & 1) : wait(&q_full[seg & 1], seg / 2 & 1))) break;
             // scores of block i for stream s; (the score tile's last user, P V of the stream's block before, was issued earlier and runs before)
             auto scores = [&](uint32_t s, uint32_t st) {
                 const uint64_t kd = desc_k_major(r0 + st * C::TILE), q = qd + (TWO ? s : 0) * (C::TILE >> 4);
@@ -411,11 +428,11 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
             // 4,000-16,000 tokens); where they alternate the second barrier costs more than it saves (64 decoded tokens: 125 -> 130 us).
             auto values = [&](uint32_t s, uint32_t st, bool add) {
                 const uint64_t vd = desc_mn_major(r0 + st * C::TILE);
-                if (!wait_bounded(TWO ? &h_full[s] : &p_full[s], done[s] & 1)) return false;
+                if (!wait(TWO ? &h_full[s] : &p_full[s], done[s] & 1)) return false;
                 fence_after();
                 mma4_ts(tmem + C::O_COL + s * D, tmem + s * 128, vd, idesc<T>(D, true), add);
                 if (TWO) {
-                    if (!wait_bounded(&p_full[s], done[s] & 1)) return false;
+                    if (!wait(&p_full[s], done[s] & 1)) return false;
                     fence_after();
                 }
                 ++done[s];
@@ -424,9 +441,9 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
             };
             for (uint32_t i = 0; i <= n && ok; ++i) {
                 const uint32_t kt = tile0 + k_tile<TWO>(i), ks = kt % NST, vt = tile0 + v_tile<TWO>(i - 1, n), vs = vt % NST; // (values of the block before)
-                if (i == 1 && seg && !(ok = wait_bounded(&epi_done, (seg - 1) & 1))) break; // the accumulators have been read
+                if (i == 1 && seg && !(ok = wait(&epi_done, (seg - 1) & 1))) break; // the accumulators have been read
                 if (TWO) {
-                    if (i > 0 && !(ok = wait_bounded(&full[vs], vt / NST & 1))) break;
+                    if (i > 0 && !(ok = wait(&full[vs], vt / NST & 1))) break;
 #pragma unroll
                     for (uint32_t s = 0; s < 2; ++s) {
                         if (i > 0) {
@@ -435,7 +452,7 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
                             else commit1(&o_done[s]);
                         }
                         if (i < n) {
-                            if (s == 0 && !(ok = wait_bounded(&full[ks], kt / NST & 1))) break;
+                            if (s == 0 && !(ok = wait(&full[ks], kt / NST & 1))) break;
                             fence_after();
                             scores(s, ks);
                             if (s == 1) commit2(&empty[ks], &s_full[s]);
@@ -444,20 +461,24 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
                     }
                 } else {
                     if (i < n) {
-                        if (!(ok = wait_bounded(&full[ks], kt / NST & 1))) break;
+                        if (!(ok = wait(&full[ks], kt / NST & 1))) break;
                         fence_after();
                         scores(i & 1, ks);
                         commit2(&empty[ks], &s_full[i & 1]);
                     }
                     if (i > 0) {
                         const uint32_t s = (i - 1) & 1;
-                        if (!(ok = wait_bounded(&full[vs], vt / NST & 1) && values(s, vs, i > 2))) break;
+                        if (!(ok = wait(&full[vs], vt / NST & 1) && values(s, vs, i > 2))) break;
                         commit2(&empty[vs], &o_done[s]);
                     }
                 }
             }
             if (!ok) break;
             tile0 += 2 * n;
+        }
+        if (!ok) { // the products issued so far
+            commit1(&mma_done);
+            wait_for_last(&mma_done, 1, 1);
         }
     } else {
         // ---- the streams ----
@@ -665,7 +686,11 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
             tile0 += 2 * n;
         }
     }
-    if (!ok) *(volatile int *)prm.status = DEV_TIMEOUT;
+    if (!ok) {
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); // (a stream may have left between a load and its use)
+        wait_st();
+        *(volatile int *)prm.status = DEV_TIMEOUT;
+    }
     __syncwarp();
     fence_before();
     __syncthreads();
@@ -733,10 +758,10 @@ bool tree_attn_tc_supported(const PoolDev &pool, int dtype) {
 }
 size_t tree_attn_tc_work(int sm_count, int dim) { return sizeof(float) * (size_t)sm_count * 2 * (2 * TM) * (dim + 2); }
 
-cudaError_t launch_tree_attn_tc(const DeviceInfo &dev, const PoolDev &pool, int dtype, const TreeDev &t, int *d_status, bool pdl, cudaStream_t st) {
+cudaError_t launch_tree_attn_tc(const DeviceInfo &dev, const PoolDev &pool, int dtype, const TreeDev &t, int *d_status, long long wait_cycles, bool pdl, cudaStream_t st) {
     TcParams prm;
     TcMaps maps;
-    prm.t = t, prm.status = d_status, prm.box = pool.page_size < TK ? pool.page_size : TK, prm.slot_dim = 1;
+    prm.t = t, prm.status = d_status, prm.wait = wait_cycles, prm.box = pool.page_size < TK ? pool.page_size : TK, prm.slot_dim = 1;
     if (!encode_pool(pool, dtype, t.k, prm.box, &prm.slot_dim, &maps.k) || !encode_pool(pool, dtype, t.v, prm.box, &prm.slot_dim, &maps.v))
         return cudaErrorNotSupported;
     // Rows per sequence and key head on average (the lengths themselves are on the device; either way is right for any of them).

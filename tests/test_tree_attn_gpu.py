@@ -1,4 +1,8 @@
 """GPU tests of the attention over a paged cache against the formula in 64 bits (paged_ref.attention)."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -534,3 +538,33 @@ def test_a_wait_that_runs_out_ends_the_call_with_a_status(ctx, dtype, dim, heads
         torch.cuda.synchronize()
         ctx.synchronize()
         assert torch.equal(c.out, first)
+
+
+STALE = """
+import torch
+import test_tree_attn_gpu as t
+from ullm_b200 import backend
+ctx = backend.CudaContext(0)
+c = t.Case([2500, 300, 0], [7, 40, 1], 8, 2, 64, "f32", 16, mask="tree", q32=True, seed=3)
+op = backend.TreeAttention(ctx, c.kv, c.heads, dtype=c.qd)
+work = torch.empty(op._a.work_bytes // 8 + 1, dtype=torch.int64, device="cuda")
+op._a.d_work = work.data_ptr()
+first = None
+for i in range(1, 9):
+    for n in (1, 2):
+        work.fill_((2 * i - 2 + n) << 16 | n)
+        c.out.fill_(7)
+        c.run(ctx, op)
+        c.check()
+        first = c.out.clone() if first is None else first
+        assert torch.equal(c.out, first), (i, n)
+print("equal")
+"""
+
+
+def test_numbers_left_in_a_work_area_are_no_counts(ctx):
+    """64-bit numbers of the size of token ids and slots, over the first calls of a process: a count beside the number of a call looked like that once."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([os.path.dirname(here), here, os.environ.get("PYTHONPATH", "")]))
+    r = subprocess.run([sys.executable, "-c", STALE], capture_output=True, text=True, env=env, timeout=300)
+    assert r.returncode == 0 and "equal" in r.stdout, r.stdout + r.stderr[-2000:]

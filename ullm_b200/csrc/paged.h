@@ -41,7 +41,7 @@ struct TreeDev {
     // work area: per CTA one record and two partial results (rows x (dim + 2) floats each)
     int4 *meta;
     float *part;
-    unsigned long long *count, call; // for kernels that join units themselves: a counter per CTA, the number of this call
+    int *count; // for kernels that join units themselves: a counter per CTA
 };
 constexpr int TREE_META = 2; // int4 per CTA
 

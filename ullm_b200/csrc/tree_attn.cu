@@ -15,7 +15,6 @@
 #include "tree_sched.cuh"
 
 #include <algorithm>
-#include <atomic>
 #include <cmath>
 
 namespace ullm {
@@ -387,9 +386,7 @@ int ullm_cuda_tree_attn_dev(ullm_cuda_ctx *c, const ullm_tree_attn *a, void *str
     DeviceGuard guard(c->device);
     const cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
     const size_t records = meta_bytes(c->dev.sm_count * F_PER_SM);
-    static std::atomic<unsigned long long> calls{0};
-    t.meta = (int4 *)a->d_work, t.count = (unsigned long long *)((uint8_t *)a->d_work + records), t.part = (float *)((uint8_t *)a->d_work + 2 * records);
-    t.call = ++calls;
+    t.meta = (int4 *)a->d_work, t.count = (int *)((uint8_t *)a->d_work + records), t.part = (float *)((uint8_t *)a->d_work + 2 * records);
     cudaError_t e = cudaErrorNotSupported;
     if (tree_attn_tc_supported(pool, a->dtype)) e = launch_tree_attn_tc(c->dev, pool, a->dtype, t, c->d_status, c->tree_wait_cycles, c->use_pdl, st);
     if (e != cudaErrorNotSupported) { // (strides that a tensor map cannot describe go to the f32 kernel)

@@ -250,24 +250,12 @@ template <> __device__ __forceinline__ __nv_bfloat16 out_from<__nv_bfloat16>(flo
 // Weight of a part: 0 where nothing was seen, else at least the smallest number, so that an infinite value in it stays infinite.
 __device__ __forceinline__ float part_weight(float m_part, float m) { return m_part == -INFINITY ? 0.f : fmaxf(exp2f(m_part - m), 1.4e-45f); }
 
-// Joins a unit's parts without a second launch: the CTAs that have a part of it count, and the last one to arrive joins them all, in the order of the CTAs.
-// A count is kept in 64 bits beside the number of the call, and any other number there counts as none: the memory needs no preparation, and
-// what an abandoned call leaves does no harm.  Every thread calls it, behind its stores of the CTA's own part.
+// Joins a unit's parts in the kernel that made them: the CTAs that have a part of it count, and the last one to arrive joins them all, in the order of the CTAs.
+// The counts are zeros when the kernel starts (tree_count_kernel).  Every thread calls it, behind its stores of the CTA's own part.
 template <typename O, int M, int D> __device__ __forceinline__ void join_last(const TreeDev &p, const Seg &w, int *flag) {
     __threadfence();
     __syncthreads();
-    if (threadIdx.x == 0) {
-        unsigned long long *const count = p.count + w.end, call = p.call << 16;
-        unsigned long long old = *(volatile unsigned long long *)count, seen;
-        for (;; old = seen) {
-            const unsigned long long n = (old & ~0xffffull) == call ? (old & 0xffff) + 1 : 1;
-            seen = atomicCAS(count, old, n == (unsigned long long)w.parts ? 0 : call | n);
-            if (seen == old) {
-                *flag = n == (unsigned long long)w.parts;
-                break;
-            }
-        }
-    }
+    if (threadIdx.x == 0) *flag = atomicAdd(p.count + w.end, 1) + 1 == w.parts;
     __syncthreads();
     if (!*flag) return;
     __threadfence();

@@ -568,3 +568,45 @@ def test_numbers_left_in_a_work_area_are_no_counts(ctx):
     env = dict(os.environ, PYTHONPATH=os.pathsep.join([os.path.dirname(here), here, os.environ.get("PYTHONPATH", "")]))
     r = subprocess.run([sys.executable, "-c", STALE], capture_output=True, text=True, env=env, timeout=300)
     assert r.returncode == 0 and "equal" in r.stdout, r.stdout + r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("dtype,dim,rows", [("f32", 64, 1), ("f32", 64, 5), ("f32", 128, 1), ("f32", 128, 9), ("f16", 64, 1), ("bf16", 128, 5), ("f32", 80, 2)])
+def test_32_bit_sums_over_long_contexts_do_not_drift(ctx, dtype, dim, rows):
+    """Sums of positive values over 32,000 tokens: each is off by no more than its roundings, and all of them together are not off to one side, as they are where
+    every addition cuts off instead of rounding (with 100 blocks to a CTA that was 3 to 7e-6, always too small)."""
+    n_seq, heads, kv_heads, ps, length = 8, 16, 8, 64, 32000
+    per = -(-(length + rows) // ps)
+    n_pages = n_seq * per
+    g = torch.Generator(device="cuda").manual_seed(dim + rows)
+    shape = (1, n_pages, ps, kv_heads, dim)
+    k = torch.randn(shape, generator=g, device="cuda").mul(0.2).to(DT[dtype][1])
+    v = torch.rand(shape, generator=g, device="cuda").add(0.5).to(DT[dtype][1])
+    kv = backend.KvPages(DT[dtype][0], 1, n_pages, ps, kv_heads, dim, k.data_ptr(), v.data_ptr())
+    total = n_seq * rows
+    q = torch.randn((total, heads, dim), generator=g, device="cuda")
+    out = torch.empty_like(q)
+    blocks = torch.randperm(n_pages, generator=g, device="cuda").to(torch.int32).view(n_seq, per)
+    cu, lens = ints(np.arange(n_seq + 1) * rows), ints(np.full(n_seq, length + rows))
+    op = backend.TreeAttention(ctx, kv, heads, dtype=backend.F32)
+    op.run_dev(0, q.data_ptr(), out.data_ptr(), total, n_seq, cu.data_ptr(), lens.data_ptr(), blocks.data_ptr(), per, stream=stream())
+    torch.cuda.synchronize()
+    apart = []
+    worst = 0.0
+    for b in range(n_seq):
+        kk, vv = (p[0, blocks[b].long()].reshape(per * ps, kv_heads, dim)[:length + rows].double() for p in (k, v))
+        qq = q[b * rows:(b + 1) * rows].double().view(rows, kv_heads, heads // kv_heads, dim)
+        s = torch.einsum("rhgd,khd->hgrk", qq, kk) * paged_ref.default_scale(dim)
+        keys, me = torch.arange(length + rows, device="cuda"), torch.arange(rows, device="cuda")
+        s = s.masked_fill(keys[None] > length + me[:, None], -float("inf"))
+        ref = torch.einsum("hgrk,khd->rhgd", torch.softmax(s, -1), vv).reshape(rows, heads, dim)
+        rel = (out[b * rows:(b + 1) * rows].double() - ref) / ref
+        apart.append(rel.flatten())
+        worst = max(worst, float(rel.abs().max()))
+    # One value: a score (below 2.5 in magnitude, dim products) and its power of two, 2 (dim + 4) 2.5 + 8 half steps of 2^-23 for numerator and sum; the blocks of a
+    # segment one after the other, its warps and the parts of a unit, at most 32000 / 32 + 8 + 296 additions, again twice.
+    assert worst <= (5 * (dim + 4) + 8 + 2 * (32000 / 32 + 8 + 296)) * 2.0 ** -24
+    # All values: additions that round to nearest are off to either side, and so are scores and weights, on which the values do not depend: over
+    # `total * heads * dim` values (8,192 at least) nothing is left of them.  What is cut off always has one sign: within a block four sums of its size at most (two
+    # tiles of keys, three products each, of which the first two come before there is a sum), a step of 2^-23 each; and where the two parts of a value end, on average half a unit of the lower part's
+    # 11 bits, below 2^-21 of the value.
+    assert abs(float(torch.cat(apart).mean())) <= 6 * 2.0 ** -23 + 2.0 ** -22

@@ -610,3 +610,27 @@ def test_32_bit_sums_over_long_contexts_do_not_drift(ctx, dtype, dim, rows):
     # tiles of keys, three products each, of which the first two come before there is a sum), a step of 2^-23 each; and where the two parts of a value end, on average half a unit of the lower part's
     # 11 bits, below 2^-21 of the value.
     assert abs(float(torch.cat(apart).mean())) <= 6 * 2.0 ** -23 + 2.0 ** -22
+
+
+@pytest.mark.parametrize("dtype,q32,dim,n", [("f16", False, 64, 3), ("f16", False, 128, 70), ("bf16", False, 128, 3), ("bf16", False, 64, 150), ("f16", False, 40, 3), ("bf16", False, 96, 9),
+                                             ("f32", True, 40, 3), ("f32", True, 64, 3), ("f32", True, 128, 40), ("f16", True, 64, 3)])
+def test_infinite_values_of_committed_tokens_under_any_weight(ctx, dtype, q32, dim, n):
+    """Committed tokens whose weights are 2^-50 and 2^-170 of the largest (zeros in 16 or 32 bits) hold infinities and a NaN: the row has them all the same.
+    A key whose score is -inf has no weight at all, and 0 * inf is NaN."""
+    c = Case([600, 4000, 3], [n, 2, 1], 4, 2, dim, dtype, 16, mask="any", seed=9, q32=q32)
+    c.q[:, :4 * dim] = 1
+    at = lambda b, tok: (c.layer, int(c.blocks[b, tok // 16]), tok % 16)
+    for b, total in ((0, 600 + n), (1, 4002)):
+        for tok in range(total):
+            c.k[at(b, tok)] = 0
+    low = lambda power: power / (1.4427 * dim ** 0.5)  # key whose score is 2^power of the others'
+    for b, tok, power, col, value in ((0, 100, -50, 1, "inf"), (0, 200, -170, 2, "-inf"), (0, 301, -170, 3, "nan"), (0, 302, -50, 4, "inf"), (0, 450, -50, 4, "-inf"), (1, 17, -170, 5, "inf"),
+                                      (1, 3999, -50, 6, "-inf"), (1, 2200, -170, 33, "inf")):
+        c.k[at(b, tok)] = low(power)
+        c.v[at(b, tok)][:, col] = float(value)
+    for tok in range(0, 1500):  # the first blocks of a long context weigh next to nothing
+        c.k[at(1, tok)] = low(-170)
+    c.k[at(1, 2300)][1, 0] = -float("inf")
+    c.v[at(1, 2300)][:, 7] = float("inf")
+    c.run(ctx)
+    c.check()

@@ -268,17 +268,27 @@ template <typename Q, typename KV, int M, int KEYS> __global__ void __launch_bou
                 const float4 x = *(const float4 *)(red + ((size_t)s * rows + r) * D + d);
                 o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
             }
-            if (odd) { // infinities and NaN of the tokens that the row does see
-                const int first = max(v.ctx, w.blk * KEYS), last = min(key_end, blk_end * KEYS), me = token_of(r);
+            // values that are not finite: of the rows' own tokens they were set aside, of those in front they show in the sums (where the sum of weights is NaN, every value is)
+            const bool bad = !(isfinite(o.x) && isfinite(o.y) && isfinite(o.z) && isfinite(o.w)) && ls[r] == ls[r];
+            if (odd || bad) {
+                const int first = bad ? w.blk * KEYS : max(v.ctx, w.blk * KEYS), last = min(key_end, blk_end * KEYS), me = token_of(r);
+                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
                 for (int token = first; token < last; ++token) {
                     const int page = table[token / p.page_size];
-                    if ((unsigned)page >= (unsigned)p.n_pages || !sees(p, v, me, token - v.ctx)) continue;
-                    const float4 x = widen4((const KV *)p.v + page * p.page_stride + token % p.page_size * p.slot_stride + w.h * p.head_stride + d);
-                    if (!isfinite(x.x)) o.x += x.x;
-                    if (!isfinite(x.y)) o.y += x.y;
-                    if (!isfinite(x.z)) o.z += x.z;
-                    if (!isfinite(x.w)) o.w += x.w;
+                    if ((unsigned)page >= (unsigned)p.n_pages || (token >= v.ctx && !sees(p, v, me, token - v.ctx))) continue;
+                    const long long at = page * p.page_stride + token % p.page_size * p.slot_stride + w.h * p.head_stride;
+                    const float4 x = widen4((const KV *)p.v + at + d);
+                    if (isfinite(x.x) && isfinite(x.y) && isfinite(x.z) && isfinite(x.w)) continue;
+                    const bool none = has_no_weight((const Q *)p.q + (v.r0 + me) * p.q_stride + (long long)head_of(r) * D, (const KV *)p.k + at, D, p.scale_log2);
+                    if (!isfinite(x.x)) sum.x += none ? NAN : x.x;
+                    if (!isfinite(x.y)) sum.y += none ? NAN : x.y;
+                    if (!isfinite(x.z)) sum.z += none ? NAN : x.z;
+                    if (!isfinite(x.w)) sum.w += none ? NAN : x.w;
                 }
+                if (sum.x != 0.f) o.x = sum.x;
+                if (sum.y != 0.f) o.y = sum.y;
+                if (sum.z != 0.f) o.z = sum.z;
+                if (sum.w != 0.f) o.w = sum.w;
             }
             if (whole) {
                 const float l = ls[r], inv = l == 0.f ? 0.f : 1.0f / l;

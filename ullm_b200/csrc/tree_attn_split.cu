@@ -380,11 +380,14 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
                 for (int key = w.blk * XK; key < last; ++key) {
                     const int page = table[key / p.page_size];
                     if ((unsigned)page >= (unsigned)p.n_pages || (key >= v.ctx && !sees(p, v, me, key - v.ctx))) continue;
-                    const float4 y = widen4((const KV *)p.v + page * p.page_stride + key % p.page_size * p.slot_stride + w.h * p.head_stride + d);
-                    if (!isfinite(y.x)) x.x += y.x;
-                    if (!isfinite(y.y)) x.y += y.y;
-                    if (!isfinite(y.z)) x.z += y.z;
-                    if (!isfinite(y.w)) x.w += y.w;
+                    const long long at = page * p.page_stride + key % p.page_size * p.slot_stride + w.h * p.head_stride;
+                    const float4 y = widen4((const KV *)p.v + at + d);
+                    if (isfinite(y.x) && isfinite(y.y) && isfinite(y.z) && isfinite(y.w)) continue;
+                    const bool none = has_no_weight((const float *)p.q + (v.r0 + me) * p.q_stride + (long long)head_of(r) * D, (const KV *)p.k + at, D, p.scale_log2);
+                    if (!isfinite(y.x)) x.x += none ? NAN : y.x;
+                    if (!isfinite(y.y)) x.y += none ? NAN : y.y;
+                    if (!isfinite(y.z)) x.z += none ? NAN : y.z;
+                    if (!isfinite(y.w)) x.w += none ? NAN : y.w;
                 }
             }
             if (whole) {

@@ -20,7 +20,7 @@
 // score products of the next one begin while the last one's results are stored.  Warps of a stream whose rows are all padding only keep step.
 // Blocks that hold the rows' own tokens, or keys behind the last one, are masked, and their values in shared memory are cleaned
 // first: rows behind the last key become zeros and values that are not finite are set aside (0 * inf would reach
-// rows that do not see the token); the epilogue adds them for the rows that do.
+// rows that do not see the token); the epilogue puts them in for the rows that do (put_odd).
 //
 // Every wait is bounded (about a second); on expiry a role leaves, waits (again with that limit) for the copies and products that it has in flight -
 // they write the CTA's shared and tensor memory - and records DEV_TIMEOUT; all threads meet at the end and the tensor memory is freed.
@@ -229,24 +229,37 @@ __device__ __forceinline__ uint32_t view_bits(const TreeDev &p, const SeqView &v
 template <bool TWO> __device__ __forceinline__ uint32_t k_tile(uint32_t j) { return TWO ? 2 * j : (j ? 2 * j - 1 : 0); }
 template <bool TWO> __device__ __forceinline__ uint32_t v_tile(uint32_t j, uint32_t n) { return TWO ? 2 * j + 1 : (j + 1 == n ? 2 * n - 1 : 2 * j + 2); }
 
-// Infinities and NaN among the values [c, c + 32) of tokens [first, last) that row `me` sees, added to the row's sums.  Rare, and out of the way.
-template <typename T> __device__ __noinline__ void add_odd_at(const TreeDev &p, const SeqView &v, int head, int me, int first, int last, int c, float *o) {
+// Infinities and NaN among the values [c, c + 32) of tokens [first, last) that row `me` sees, in the place of the row's sums.  Rare, and out of the way.
+template <typename T> __device__ __noinline__ void put_odd_at(const TreeDev &p, const SeqView &v, const T *q, int head, int me, int first, int last, int c, float *o) {
     const int *const table = p.blocks + (size_t)v.id * p.max_blocks;
+    float sum[32];
+    for (int e = 0; e < 32; ++e) sum[e] = 0.f;
     for (int token = first; token < last; ++token) {
         const int page = table[token / p.page_size];
-        if ((unsigned)page >= (unsigned)p.n_pages || !sees(p, v, me, token - v.ctx)) continue;
-        const T *const at = (const T *)p.v + page * p.page_stride + token % p.page_size * p.slot_stride + head * p.head_stride + c;
+        if ((unsigned)page >= (unsigned)p.n_pages || (token >= v.ctx && !sees(p, v, me, token - v.ctx))) continue;
+        const long long at = page * p.page_stride + token % p.page_size * p.slot_stride + head * p.head_stride;
+        const uint4 *const values = (const uint4 *)((const T *)p.v + at + c);
+        uint32_t odd = 0;
+        for (int i = 0; i < 4; ++i) {
+            const uint4 x = values[i];
+            odd |= odd_halves<T>(x.x) | odd_halves<T>(x.y) | odd_halves<T>(x.z) | odd_halves<T>(x.w);
+        }
+        if (!odd) continue;
+        const bool none = has_no_weight(q, (const T *)p.k + at, p.dim, p.scale_log2);
         for (int e = 0; e < 32; ++e) {
-            const float y = (float)at[e];
-            if (!isfinite(y)) o[e] += y;
+            const float y = (float)((const T *)values)[e];
+            if (!isfinite(y)) sum[e] += none ? NAN : y;
         }
     }
+    for (int e = 0; e < 32; ++e)
+        if (sum[e] != 0.f) o[e] = sum[e];
 }
-template <typename T> __device__ __forceinline__ void add_odd(const TreeDev &p, const SeqView &v, int head, int me, int first, int last, int c, float (&o)[32]) {
-    float copy[32]; // (a register array cannot be indexed by the loop above)
+template <typename T>
+__device__ __forceinline__ void put_odd(const TreeDev &p, const SeqView &v, const T *q, int head, int me, int first, int last, int c, float (&o)[32]) {
+    float copy[32]; // (a register array cannot be indexed by the loops above)
 #pragma unroll
     for (int e = 0; e < 32; ++e) copy[e] = o[e];
-    add_odd_at<T>(p, v, head, me, first, last, c, copy);
+    put_odd_at<T>(p, v, q, head, me, first, last, c, copy);
 #pragma unroll
     for (int e = 0; e < 32; ++e) o[e] = copy[e];
 }
@@ -663,8 +676,17 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
                     float o[32];
 #pragma unroll
                     for (int e = 0; e < 32; ++e) o[e] = TWO ? __uint_as_float(o0[e]) : __uint_as_float(o0[e]) * wa + (n < 2 ? 0.f : __uint_as_float(o1[e]) * wb);
-                    if (odd && live) add_odd<T>(p, v, head, me, max(v.ctx, blk * TK), min(key_end, (int)(blk + n) * TK), c, o);
                     if (!live) continue;
+                    float2 all[4]; // infinite or NaN where any of the values is (or where they pass the range together: then nothing is found below)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) all[e] = make_float2(o[2 * e], o[2 * e + 1]);
+#pragma unroll
+                    for (int e = 4; e < 16; ++e) all[e & 3] = add2(all[e & 3], make_float2(o[2 * e], o[2 * e + 1]));
+                    all[0] = add2(add2(all[0], all[1]), add2(all[2], all[3]));
+                    const bool bad = !(fabsf(all[0].x + all[0].y) < INFINITY) && ll == ll; // of tokens in front of the rows'; with a sum of weights that is NaN every value is
+                    if (odd || bad)
+                        put_odd<T>(p, v, (const T *)p.q + (v.r0 + me) * p.q_stride + (head * p.group + (row0 + row) % p.group) * (long long)D, head, me,
+                                   bad ? blk * TK : max(v.ctx, blk * TK), min(key_end, (int)(blk + n) * TK), c, o);
                     if (whole) {
 #pragma unroll
                         for (int e = 0; e < 32; e += 8) {

@@ -242,6 +242,15 @@ __device__ __forceinline__ void copy16(void *dst, const void *src, bool on) { //
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
 
+// Values that are not finite, of keys that a row sees, decide what becomes of the row, however small their weights: products of a weight that has become
+// zero in 32 bits or fewer with an infinity would be NaN where the formula has an infinity.  The kernels add up such values alone and put the sum in
+// the place of what the products gave.  A key whose score is -inf does have no weight: an infinite value of it makes NaN, as in the formula.
+template <typename Q, typename KV> __device__ __noinline__ bool has_no_weight(const Q *q, const KV *k, int dim, float scale) {
+    float s = 0.f;
+    for (int d = 0; d < dim; ++d) s = fmaf((float)q[d], (float)k[d], s);
+    return s * scale == -INFINITY;
+}
+
 template <typename T> __device__ __forceinline__ T out_from(float v);
 template <> __device__ __forceinline__ float out_from<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half out_from<__half>(float v) { return __float2half_rn(v); }
@@ -276,7 +285,7 @@ template <typename O, int M, int D> __device__ __forceinline__ void join_last(co
             float top = m;
 #pragma unroll
             for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
-            const float corr = m == -INFINITY ? 0.f : exp2f(m - top);
+            const float corr = part_weight(m, top);
             if (m != -INFINITY) l *= corr, acc.x *= corr, acc.y *= corr, acc.z *= corr, acc.w *= corr;
             m = top;
 #pragma unroll

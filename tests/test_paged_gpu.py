@@ -349,3 +349,21 @@ def test_wants_beyond_32_bits_are_refused_as_a_whole(ctx):
     t.grow_dev(seq.data_ptr(), adds.data_ptr(), n, stream=stream())
     torch.cuda.synchronize()
     assert int(fault[0]) == 0 and int(lens.sum()) == 60 and torch.equal(table[:60, 0], torch.arange(60, dtype=torch.int32, device="cuda"))
+
+
+@pytest.mark.parametrize("cu,good", [([0, 5, 3, 8], False), ([0, 3, -1], False), ([-2, 3, 6], False), ([0, 4, 13], False), ([9, 4, 2], False), ([0, 2 ** 31 - 1, 5], False),
+                                     ([-(2 ** 31), 2, 5], False), ([3, 5, 5, 9], True), ([12, 12], True), ([0, 0], True)])
+def test_plan_leaves_no_row_stale(ctx, cu, good):
+    """Rows that no sequence owns get -1, whatever the array held: a later cache write skips them.  Offsets out of order refuse all rows."""
+    rows, n = 12, len(cu) - 1
+    d_cu, d_len = ints(cu), ints([40] * n)
+    seq, slot, pos = (ints(np.full(rows, 1)) for _ in range(3))
+    fault = ints([0])
+    ctx.tree_plan_dev(rows, n, d_cu.data_ptr(), d_len.data_ptr(), None, seq.data_ptr(), slot.data_ptr(), pos.data_ptr(), None, 0, fault.data_ptr(), stream=stream())
+    torch.cuda.synchronize()
+    want = np.full(rows, -1)
+    if good:
+        for b in range(n):
+            want[cu[b]:cu[b + 1]] = b
+    assert seq.tolist() == want.tolist() and int(fault[0]) == (0 if good else backend.KV_FAULT_LEN)
+    assert slot[np.nonzero(want < 0)[0].tolist()].eq(1).all() and pos[np.nonzero(want < 0)[0].tolist()].eq(1).all()

@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(256) kv_copy_pages_kernel(const PoolDev pool, 
 }
 
 // ---- plan of a step of trees ----------------------------------------------------------------------------------------
-// CTA b < n_seq: the rows of sequence b; the CTAs behind them mark the rows behind the last sequence.  A row walks
+// CTA b < n_seq: the rows of sequence b; the CTAs behind them mark the rows in front of the first sequence and behind the last.  A row walks
 // up its ancestors (parents in shared memory), which meet descending indices, so each mask word is complete when the walk leaves it.
 constexpr int PLAN_MAX = 4096;
 constexpr int PLAN_PAD_CTAS = 4;
@@ -404,16 +404,20 @@ __global__ void __launch_bounds__(128) tree_plan_kernel(int n_rows, int n_seq, c
     pdl_wait_prior();
     pdl_launch_dependents();
     const int tid = threadIdx.x, b = blockIdx.x;
+    bool wild = false; // offsets that decrease or leave the rows: two sequences could own a row, or nobody
+    for (int j = tid; n_seq && j <= n_seq; j += 128) wild |= cu[j] < 0 || cu[j] > n_rows || (j < n_seq && cu[j + 1] < cu[j]);
+    if (__syncthreads_or(wild)) {
+        if (b == 0 && tid == 0) set_fault(fault, ULLM_KV_FAULT_LEN);
+        for (int r = b * 128 + tid; r < n_rows; r += gridDim.x * 128) row_seq[r] = -1;
+        return;
+    }
     if (b >= n_seq) {
-        const int end = min(max(n_seq ? cu[n_seq] : 0, 0), n_rows);
-        for (int r = end + (b - n_seq) * 128 + tid; r < n_rows; r += PLAN_PAD_CTAS * 128) row_seq[r] = -1;
+        const int first = n_seq ? cu[0] : 0, end = n_seq ? cu[n_seq] : 0, at = (b - n_seq) * 128 + tid;
+        for (int r = at; r < first; r += PLAN_PAD_CTAS * 128) row_seq[r] = -1;
+        for (int r = end + at; r < n_rows; r += PLAN_PAD_CTAS * 128) row_seq[r] = -1;
         return;
     }
     const int r0 = cu[b], r1 = cu[b + 1];
-    if (r0 < 0 || r1 < r0 || r1 > n_rows) {
-        if (tid == 0) set_fault(fault, ULLM_KV_FAULT_LEN);
-        return;
-    }
     const int n = r1 - r0, id = ids ? ids[b] : b;
     int bad = id < 0 || id >= n_table ? ULLM_KV_FAULT_SEQ : 0;
     const int held = bad ? n : len[id], ctx = held - n; // (n is not negative: only a length below it could leave the range)

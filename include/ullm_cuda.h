@@ -429,7 +429,8 @@ int ullm_cuda_kv_copy_pages_dev(ullm_cuda_ctx *ctx, const ullm_kv_pages *kv, con
  * d_mask [n_rows][mask_words] = the bits of itself and its ancestors (d_mask may be NULL).  Rows in front of d_cu[0] and behind
  * d_cu[n_seq] get d_row_seq = -1, which the other calls skip; their other entries are left alone.  Offsets that decrease or leave 0 .. n_rows refuse
  * the whole call (d_fault; every row gets -1).  With d_mask a sequence has at most
- * 32 * mask_words rows, with d_parent at most 4096: one that has more is refused (d_fault, may be NULL) and its rows get -1. */
+ * 32 * mask_words rows, with d_parent at most 4096: one that has more is refused (d_fault, may be NULL) and its rows get -1.  So are sequences with
+ * rows that name the same table row (they would be the same tokens); one without rows may name any. */
 int ullm_cuda_tree_plan_dev(ullm_cuda_ctx *ctx, size_t n_rows, size_t n_seq, const int32_t *d_cu, const int32_t *d_len,
                             const int32_t *d_ids, size_t n_table, const int32_t *d_parent, int32_t *d_row_seq,
                             int32_t *d_row_slot, int32_t *d_row_pos, uint32_t *d_mask, size_t mask_words, int32_t *d_fault,

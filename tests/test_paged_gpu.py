@@ -367,3 +367,18 @@ def test_plan_leaves_no_row_stale(ctx, cu, good):
             want[cu[b]:cu[b + 1]] = b
     assert seq.tolist() == want.tolist() and int(fault[0]) == (0 if good else backend.KV_FAULT_LEN)
     assert slot[np.nonzero(want < 0)[0].tolist()].eq(1).all() and pos[np.nonzero(want < 0)[0].tolist()].eq(1).all()
+
+
+@pytest.mark.parametrize("cu,ids,want", [
+    ([0, 3, 5], [2, 2], [-1] * 5), ([0, 3, 5, 8], [1, 0, 1], [-1] * 3 + [0] * 2 + [-1] * 3), ([0, 3, 5, 5, 5], [1, 0, 0, 1], [1] * 3 + [0] * 2), ([0, 0, 4, 4], [1, 1, 1], [1] * 4),
+    ([0] + [200] * 300, [2] * 300, [2] * 200),
+])
+def test_plan_refuses_a_table_row_that_is_named_twice(ctx, cu, ids, want):
+    """Two sequences cannot both be a row's last tokens.  Entries without rows (a padded batch) may name any row."""
+    rows, n = cu[-1], len(ids)
+    d_cu, d_len, d_ids = ints(cu), ints([400] * 3), ints(ids)
+    seq, slot, pos = (ints(np.full(rows, -9)) for _ in range(3))
+    fault = ints([0])
+    ctx.tree_plan_dev(rows, n, d_cu.data_ptr(), d_len.data_ptr(), None, seq.data_ptr(), slot.data_ptr(), pos.data_ptr(), None, 0, fault.data_ptr(), d_ids.data_ptr(), 3, stream())
+    torch.cuda.synchronize()
+    assert seq.tolist() == want and int(fault[0]) == (backend.KV_FAULT_SEQ if -1 in want else 0)

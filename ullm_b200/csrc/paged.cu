@@ -420,6 +420,11 @@ __global__ void __launch_bounds__(128) tree_plan_kernel(int n_rows, int n_seq, c
     const int r0 = cu[b], r1 = cu[b + 1];
     const int n = r1 - r0, id = ids ? ids[b] : b;
     int bad = id < 0 || id >= n_table ? ULLM_KV_FAULT_SEQ : 0;
+    if (ids && n) { // (entries without rows are padding and may name any row of the table)
+        bool twice = false;
+        for (int j = tid; j < n_seq; j += 128) twice |= j != b && ids[j] == id && cu[j + 1] != cu[j];
+        if (__syncthreads_or(twice)) bad |= ULLM_KV_FAULT_SEQ;
+    }
     const int held = bad ? n : len[id], ctx = held - n; // (n is not negative: only a length below it could leave the range)
     if (held < n || (mask && n > 32 * words) || (parent && n > PLAN_MAX)) bad |= ULLM_KV_FAULT_LEN;
     if (bad) {

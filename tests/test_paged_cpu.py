@@ -205,3 +205,22 @@ def test_reference_plan_of_a_small_tree():
     seq, slot, pos, mask, fault = paged_ref.plan([0, 4, 5], [10, 1], [-1, 0, 0, 2, -1], 7, words=1)
     assert seq.tolist() == [0, 0, 0, 0, 1, -1, -1] and slot[:5].tolist() == [6, 7, 8, 9, 0] and pos[:5].tolist() == [6, 7, 7, 8, 0]
     assert mask[:5, 0].tolist() == [0b1, 0b11, 0b101, 0b1101, 0b1] and fault == 0
+
+
+class NoCalls:
+    """A context whose library must not be reached."""
+
+    def _check(self, code):
+        raise AssertionError("called")
+
+    def __getattr__(self, name):
+        raise AssertionError(name)
+
+
+@pytest.mark.parametrize("embeds,parents", [((3, 255), None), ((3, 257), None), ((256,), None), ((1, 3, 256), None), ((3, 256), [-1, 0]), ((3, 256), [-1, 0, 1, 2]), ((3, 256), []),
+                                            ((3, 256), [[-1, 0, 1]])])
+def test_verify_does_not_read_behind_its_arrays(embeds, parents):
+    f = backend.GpuForward.__new__(backend.GpuForward)
+    f._ctx, f._h, f.params = NoCalls(), None, dict(n_embd=256, vocab=8)
+    with pytest.raises(backend.FormatError):
+        f.verify(np.zeros(embeds, np.float32), 0, parents)

@@ -945,8 +945,12 @@ class GpuForward:
         """A tree of drafted tokens in one pass: ``embeds`` [n, n_embd], ``parents[i]`` the index of the token that token ``i``
         follows (-1: the one at ``pos - 1``; ``None``: a chain); returns the logits of every token [n, vocab]."""
         e = _f32(embeds)
+        if e.ndim != 2 or e.shape[1] != self.params["n_embd"]:
+            raise FormatError(ERR_FORMAT, f"embeddings of shape {e.shape} for a model of width {self.params['n_embd']}")
         n = e.shape[0]
         par = None if parents is None else np.ascontiguousarray(parents, np.int32)
+        if par is not None and par.shape != (n,):
+            raise FormatError(ERR_FORMAT, f"parents of shape {par.shape} for {n} tokens")
         out = np.empty((n, self.params["vocab"]), np.float32)
         self._ctx._check(self._ctx._lib.ullm_cuda_forward_verify(self._h, _ptr(e), _ptr(par), n, pos, _ptr(out)))
         return out

@@ -224,3 +224,22 @@ def test_verify_does_not_read_behind_its_arrays(embeds, parents):
     f._ctx, f._h, f.params = NoCalls(), None, dict(n_embd=256, vocab=8)
     with pytest.raises(backend.FormatError):
         f.verify(np.zeros(embeds, np.float32), 0, parents)
+
+
+class Plain:
+    """The library with a context that nothing is launched on (calls without rows)."""
+
+    _lib, _h = LIB, CTX
+
+    def _check(self, code):
+        assert code == backend.OK
+
+
+def test_a_layers_weights_are_given_with_its_calls():
+    kv = pages()
+    names = ("d_q_norm", "d_k_norm", "d_q_bias", "d_k_bias", "d_v_bias")
+    op = backend.QkNormRope(Plain(), kv, 4, backend.F32, P, 8, d_q_norm=P, d_k_norm=P + 16, d_v_bias=P + 32)
+    rows = dict(layer=0, d_q=P, d_k=P, d_v=P, d_q_out=P, n_rows=0, d_row_pos=P, d_row_seq=P, d_row_slot=P, d_blocks=P, n_table=2, max_blocks=4)
+    for given in ({}, dict(d_q_norm=P + 64, d_k_norm=P + 80), dict(d_q_bias=P + 96, d_k_bias=P + 112, d_v_bias=P + 128), {}):
+        op.run_dev(**rows, **given)
+        assert [getattr(op._a, n) for n in names] == [given.get(n, w) for n, w in zip(names, (P, P + 16, None, None, P + 32))]

@@ -737,7 +737,7 @@ class QkNormRopeC(C.Structure):
 
 class QkNormRope:
     """Bias, per-head norm and rotation of a step's projections, K and V into their pages (``ullm_cuda_qk_norm_rope_dev``).
-    What the layers share is given once; weights of one layer may be given again with every call."""
+    What the layers share is given once; norm weights and biases of one layer may be given with its calls (``run_dev``), where they stand in for the constructor's."""
 
     def __init__(self, ctx: CudaContext, pages: KvPages, n_head: int, x_dtype: int, d_rope: int, n_pos: int, q_dtype: int | None = None, rot_dim: int = 0,
                  neox: bool = False, d_q_norm: int | None = None, d_k_norm: int | None = None, eps: float = 1e-6, d_q_bias: int | None = None,
@@ -746,13 +746,16 @@ class QkNormRope:
         a = self._a = QkNormRopeC()
         a.kv, a.x_dtype, a.q_dtype, a.n_head = C.addressof(pages), x_dtype, pages.dtype if q_dtype is None else q_dtype, n_head
         a.d_rope, a.n_pos, a.rot_dim, a.neox, a.eps = d_rope, n_pos, rot_dim, 1 if neox else 0, eps
-        a.d_q_norm, a.d_k_norm, a.d_q_bias, a.d_k_bias, a.d_v_bias = d_q_norm, d_k_norm, d_q_bias, d_k_bias, d_v_bias
+        self._weights = (d_q_norm, d_k_norm, d_q_bias, d_k_bias, d_v_bias)
         self._ref = C.byref(a)
 
     def run_dev(self, layer: int, d_q: int, d_k: int, d_v: int, d_q_out: int, n_rows: int, d_row_pos: int, d_row_seq: int, d_row_slot: int, d_blocks: int,
-                n_table: int, max_blocks: int, x_stride: int = 0, q_out_stride: int = 0, d_fault: int | None = None, stream=None):
-        """``x_stride``: elements between two rows of q, of k and of v (0: each packed)."""
+                n_table: int, max_blocks: int, x_stride: int = 0, q_out_stride: int = 0, d_fault: int | None = None, stream=None, d_q_norm: int | None = None,
+                d_k_norm: int | None = None, d_q_bias: int | None = None, d_k_bias: int | None = None, d_v_bias: int | None = None):
+        """``x_stride``: elements between two rows of q, of k and of v (0: each packed).  A norm weight or bias that is ``None`` is the constructor's."""
         a, c = self._a, self._ctx
+        given = (d_q_norm, d_k_norm, d_q_bias, d_k_bias, d_v_bias)
+        a.d_q_norm, a.d_k_norm, a.d_q_bias, a.d_k_bias, a.d_v_bias = (w if g is None else g for g, w in zip(given, self._weights))
         a.layer, a.n_rows, a.d_q, a.d_k, a.d_v, a.d_q_out, a.q_out_stride = layer, n_rows, d_q, d_k, d_v, d_q_out, q_out_stride
         a.q_stride = a.k_stride = a.v_stride = x_stride
         a.d_row_pos, a.d_row_seq, a.d_row_slot, a.d_blocks = d_row_pos, d_row_seq, d_row_slot, d_blocks

@@ -243,3 +243,24 @@ def test_a_layers_weights_are_given_with_its_calls():
     for given in ({}, dict(d_q_norm=P + 64, d_k_norm=P + 80), dict(d_q_bias=P + 96, d_k_bias=P + 112, d_v_bias=P + 128), {}):
         op.run_dev(**rows, **given)
         assert [getattr(op._a, n) for n in names] == [given.get(n, w) for n, w in zip(names, (P, P + 16, None, None, P + 32))]
+
+
+def test_lists_off_their_alignment_are_refused():
+    """A 32-bit number off its boundary would end in a fault on the device."""
+    kv = pages()
+    t = table(kv)
+    k, tt = C.byref(kv), C.byref(t)
+    calls = [
+        (lambda *p: LIB.ullm_cuda_kv_fork_dev(CTX, k, tt, *p, 1, None), 2), (lambda *p: LIB.ullm_cuda_kv_grow_dev(CTX, k, tt, *p, 1, None), 2),
+        (lambda *p: LIB.ullm_cuda_kv_accept_dev(CTX, k, tt, *p, 1, 4, None), 4), (lambda *p: LIB.ullm_cuda_kv_trim_dev(CTX, k, tt, *p, 1, None), 2),
+        (lambda s, d, f: LIB.ullm_cuda_kv_copy_pages_dev(CTX, k, s, d, 1, f, None), 3),
+        (lambda cu, ln, ids, par, seq, slot, pos, mask, fault: LIB.ullm_cuda_tree_plan_dev(CTX, 4, 2, cu, ln, ids, 2, par, seq, slot, pos, mask, 1, fault, None), 9),
+    ]
+    for call, n in calls:
+        for i in range(n):
+            for off in (1, 2, 3):
+                assert call(*[P + off if j == i else P for j in range(n)]) == backend.ERR_FORMAT
+    for name in ("d_row_seq", "d_row_slot", "d_row_pos", "d_blocks", "d_fault"):
+        assert LIB.ullm_cuda_qk_norm_rope_dev(CTX, C.byref(rope(**{name: P + 2})), None) == backend.ERR_FORMAT
+    for name in ("d_cu", "d_len", "d_ids", "d_blocks", "d_mask"):
+        assert LIB.ullm_cuda_tree_attn_dev(CTX, C.byref(attn(**{name: P + 2})), None) == backend.ERR_FORMAT

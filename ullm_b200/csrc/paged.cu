@@ -694,6 +694,7 @@ int ullm_cuda_kv_fork_dev(ullm_cuda_ctx *c, const ullm_kv_pages *kv, const ullm_
     PoolDev pool;
     TableDev td;
     if (int rc = table_check(c, kv, t, n, &pool, &td)) return rc;
+    if (!ints_aligned(d_src, d_dst)) return ctx_fail(c, ULLM_ERR_FORMAT, "lists must be 4-byte aligned");
     if (!n) return ULLM_OK;
     DeviceGuard guard(c->device);
     ULLM_CUDA_TRY(c, launch_kernel(kv_fork_kernel, dim3((unsigned)n), dim3(128), 0, stream ? (cudaStream_t)stream : c->stream, c->use_pdl, td, pool.page_size,
@@ -707,6 +708,7 @@ int ullm_cuda_kv_grow_dev(ullm_cuda_ctx *c, const ullm_kv_pages *kv, const ullm_
     PoolDev pool;
     TableDev td;
     if (int rc = table_check(c, kv, t, n, &pool, &td)) return rc;
+    if (!ints_aligned(d_seq, d_add)) return ctx_fail(c, ULLM_ERR_FORMAT, "lists must be 4-byte aligned");
     if (!n) return ULLM_OK;
     DeviceGuard guard(c->device);
     const cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
@@ -721,6 +723,7 @@ int ullm_cuda_kv_accept_dev(ullm_cuda_ctx *c, const ullm_kv_pages *kv, const ull
     PoolDev pool;
     TableDev td;
     if (int rc = table_check(c, kv, t, n, &pool, &td)) return rc;
+    if (!ints_aligned(d_seq, d_draft, d_path, d_kept)) return ctx_fail(c, ULLM_ERR_FORMAT, "lists must be 4-byte aligned");
     if (max_path > INT32_MAX / 2) return ctx_fail(c, ULLM_ERR_FORMAT, "max_path is too large");
     if (!n) return ULLM_OK;
     DeviceGuard guard(c->device);
@@ -737,6 +740,7 @@ int ullm_cuda_kv_trim_dev(ullm_cuda_ctx *c, const ullm_kv_pages *kv, const ullm_
     PoolDev pool;
     TableDev td;
     if (int rc = table_check(c, kv, t, n, &pool, &td)) return rc;
+    if (!ints_aligned(d_seq, d_new_len)) return ctx_fail(c, ULLM_ERR_FORMAT, "lists must be 4-byte aligned");
     if (!n) return ULLM_OK;
     DeviceGuard guard(c->device);
     ULLM_CUDA_TRY(c, launch_kernel(kv_trim_kernel, dim3((unsigned)n), dim3(128), 0, stream ? (cudaStream_t)stream : c->stream, c->use_pdl, td, pool.page_size,
@@ -749,6 +753,7 @@ int ullm_cuda_kv_copy_pages_dev(ullm_cuda_ctx *c, const ullm_kv_pages *kv, const
     if (!c || !kv || !kv->d_k || !kv->d_v || (n && (!d_src || !d_dst))) return ULLM_ERR_INVALID;
     PoolDev pool;
     if (const char *m = pool_check(kv, &pool)) return ctx_fail(c, ULLM_ERR_FORMAT, "%s", m);
+    if (!ints_aligned(d_src, d_dst, d_fault)) return ctx_fail(c, ULLM_ERR_FORMAT, "lists must be 4-byte aligned");
     if (n > kv->n_pages) return ctx_fail(c, ULLM_ERR_FORMAT, "%zu copies in a pool of %zu pages", n, kv->n_pages);
     if (!n) return ULLM_OK;
     DeviceGuard guard(c->device);
@@ -763,6 +768,7 @@ int ullm_cuda_tree_plan_dev(ullm_cuda_ctx *c, size_t n_rows, size_t n_seq, const
     if (!c || (n_seq && (!d_cu || !d_len)) || (n_rows && (!d_row_seq || !d_row_slot || !d_row_pos))) return ULLM_ERR_INVALID;
     if (n_rows > INT32_MAX / 2 || n_seq > INT32_MAX / 2 || n_table > INT32_MAX / 2) return ctx_fail(c, ULLM_ERR_FORMAT, "too many rows or sequences");
     if (d_mask && (mask_words == 0 || mask_words > 65536)) return ctx_fail(c, ULLM_ERR_FORMAT, "a mask has 1 to 65536 words per row");
+    if (!ints_aligned(d_cu, d_len, d_ids, d_parent, d_row_seq, d_row_slot, d_row_pos, d_mask, d_fault)) return ctx_fail(c, ULLM_ERR_FORMAT, "lists must be 4-byte aligned");
     if (!n_rows) return ULLM_OK;
     DeviceGuard guard(c->device);
     ULLM_CUDA_TRY(c, launch_kernel(tree_plan_kernel, dim3((unsigned)(n_seq + PLAN_PAD_CTAS)), dim3(128), 0, stream ? (cudaStream_t)stream : c->stream, c->use_pdl,
@@ -797,6 +803,7 @@ int ullm_cuda_qk_norm_rope_dev(ullm_cuda_ctx *c, const ullm_qk_norm_rope *a, voi
     const void *aligned[6] = {a->d_q_norm, a->d_k_norm, a->d_q_bias, a->d_k_bias, a->d_v_bias, a->d_rope};
     for (const void *p : aligned)
         if ((uintptr_t)p % 16) return ctx_fail(c, ULLM_ERR_FORMAT, "norm weights, biases and the rotation table must be 16-byte aligned");
+    if (!ints_aligned(a->d_row_seq, a->d_row_slot, a->d_row_pos, a->d_blocks, a->d_fault)) return ctx_fail(c, ULLM_ERR_FORMAT, "lists must be 4-byte aligned");
     const size_t items = a->n_rows * (a->n_head + 2 * a->kv->n_kv_head);
     if (items >= (size_t)INT32_MAX) return ctx_fail(c, ULLM_ERR_FORMAT, "too many rows for one call");
     if (!a->n_rows) return ULLM_OK;

@@ -23,6 +23,8 @@ struct TableDev {
 };
 
 inline size_t dtype_bytes(int dtype) { return dtype == ULLM_DTYPE_F32 ? 4 : 2; }
+// Whether every one of these arrays of 32-bit numbers (null: absent) can be read as such.
+template <typename... P> bool ints_aligned(const P *...p) { return (((uintptr_t)p | ...) & 3) == 0; }
 // A message when the description cannot be used, else null; fills `out`.
 const char *pool_check(const ullm_kv_pages *kv, PoolDev *out);
 

@@ -370,6 +370,7 @@ int ullm_cuda_tree_attn_dev(ullm_cuda_ctx *c, const ullm_tree_attn *a, void *str
     if (qs < qd || os < qd) return ctx_fail(c, ULLM_ERR_FORMAT, "row strides must cover all heads");
     if (qs * qb % 16 || os * qb % 16 || (uintptr_t)a->d_q % 16 || (uintptr_t)a->d_out % 16)
         return ctx_fail(c, ULLM_ERR_FORMAT, "rows must start on 16-byte boundaries");
+    if (!ints_aligned(a->d_cu, a->d_len, a->d_ids, a->d_blocks, a->d_mask)) return ctx_fail(c, ULLM_ERR_FORMAT, "lists must be 4-byte aligned");
     if (!std::isfinite(a->scale) || a->scale < 0.f || (a->scale > 0.f && a->scale < 1e-30f))
         return ctx_fail(c, ULLM_ERR_FORMAT, "scale must be finite, at least 1e-30 or 0 for the default");
     { // the line of all blocks is counted in 32 bits (with what the smaller tiles of the f32 kernel would need)

@@ -478,7 +478,7 @@ int ullm_cuda_qk_norm_rope_dev(ullm_cuda_ctx *ctx, const ullm_qk_norm_rope *a, v
  * causal chain).  A row that sees nothing becomes zeros.  Rows, d_cu, d_len, d_ids as in ullm_cuda_tree_plan_dev; a sequence whose
  * length is smaller than its row count gets zeros, rows behind d_cu[n_seq] are left alone.  dtype (of d_q and d_out) is
  * the pages' type, or F32 with pages of any type.  Query head h reads key head h / (n_head / n_kv_head).  Row strides are in elements,
- * multiples of 16 bytes, 0 = n_head * head_dim.  scale 0 = 1 / sqrt(head_dim).  A page number outside the pool reads as zeros.  d_work: ullm_cuda_tree_attn_work_bytes
+ * multiples of 16 bytes, 0 = n_head * head_dim.  scale is 1e-30 to 2e38, 0 = 1 / sqrt(head_dim).  A page number outside the pool reads as zeros.  d_work: ullm_cuda_tree_attn_work_bytes
  * bytes, not shared by calls that may run at the same time. */
 typedef struct ullm_tree_attn {
     const ullm_kv_pages *kv;

@@ -264,3 +264,9 @@ def test_lists_off_their_alignment_are_refused():
         assert LIB.ullm_cuda_qk_norm_rope_dev(CTX, C.byref(rope(**{name: P + 2})), None) == backend.ERR_FORMAT
     for name in ("d_cu", "d_len", "d_ids", "d_blocks", "d_mask"):
         assert LIB.ullm_cuda_tree_attn_dev(CTX, C.byref(attn(**{name: P + 2})), None) == backend.ERR_FORMAT
+
+
+@pytest.mark.parametrize("scale", [2.5e38, 3.4e38, float("inf"), -float("inf"), 9e-31, -0.5])
+def test_scales_that_are_no_number_in_powers_of_two_are_refused(scale):
+    """The kernels work with scale * log2(e), which passes 32 bits from 2.36e38 on: every score of zero would become NaN."""
+    assert LIB.ullm_cuda_tree_attn_dev(CTX, C.byref(attn(scale=scale)), None) == backend.ERR_FORMAT

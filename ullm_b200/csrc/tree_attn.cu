@@ -371,8 +371,8 @@ int ullm_cuda_tree_attn_dev(ullm_cuda_ctx *c, const ullm_tree_attn *a, void *str
     if (qs * qb % 16 || os * qb % 16 || (uintptr_t)a->d_q % 16 || (uintptr_t)a->d_out % 16)
         return ctx_fail(c, ULLM_ERR_FORMAT, "rows must start on 16-byte boundaries");
     if (!ints_aligned(a->d_cu, a->d_len, a->d_ids, a->d_blocks, a->d_mask)) return ctx_fail(c, ULLM_ERR_FORMAT, "lists must be 4-byte aligned");
-    if (!std::isfinite(a->scale) || a->scale < 0.f || (a->scale > 0.f && a->scale < 1e-30f))
-        return ctx_fail(c, ULLM_ERR_FORMAT, "scale must be finite, at least 1e-30 or 0 for the default");
+    if (!std::isfinite(a->scale) || a->scale < 0.f || (a->scale > 0.f && a->scale < 1e-30f) || a->scale > 2e38f) // (times log2(e) it is a 32-bit number too)
+        return ctx_fail(c, ULLM_ERR_FORMAT, "scale must be 1e-30 to 2e38, or 0 for the default");
     { // the line of all blocks is counted in 32 bits (with what the smaller tiles of the f32 kernel would need)
         const double units = ((double)a->n_rows * (a->n_head / a->kv->n_kv_head) / 8 + (double)a->n_seq) * a->kv->n_kv_head;
         if (units * ((double)a->max_blocks * a->kv->page_size / 32 + 4) > 2147483000.0)

@@ -634,3 +634,21 @@ def test_infinite_values_of_committed_tokens_under_any_weight(ctx, dtype, q32, d
     c.v[at(1, 2300)][:, 7] = float("inf")
     c.run(ctx)
     c.check()
+
+
+@pytest.mark.parametrize("dim,n", [(64, 2), (128, 3), (128, 70), (96, 2)])
+def test_the_largest_bf16_values(ctx, dim, n):
+    """A value at the end of the range under a weight of nearly one, in a block behind those whose scores are a few powers of two lower: the result is finite."""
+    n_seq = 60
+    c = Case([900] * n_seq, [n] * n_seq, 8, 4, dim, "bf16", 16, mask="tree", seed=dim)
+    big = torch.finfo(torch.bfloat16).max
+    c.q[:, :8 * dim] = 1
+    for pool in (c.k, c.v):  # (what no sequence uses stays NaN)
+        pool[c.layer] = pool[c.layer] * 0
+    for b in range(n_seq):
+        for tok, power, value in ((100, 0.0, -big), (600, 7.5, big)):  # the second one's score is 2^7.5 of the others'
+            page, slot = int(c.blocks[b, tok // 16]), tok % 16
+            c.k[c.layer, page, slot] = power / (1.4427 * dim ** 0.5)
+            c.v[c.layer, page, slot, b % 4, 7 + (tok == 100)] = value
+    c.run(ctx)
+    c.check()

@@ -11,7 +11,7 @@
 //   O_s += P_s V_j         tcgen05.mma, P from tensor memory, V from shared memory as it lies there (keys are the rows)
 //
 // and, where they shared the rows, the two accumulators are joined when the CTA leaves the unit.  A row's reference m_s follows its running maximum
-// only when that has grown by more than 2^8 (weights then stay below 2^8 and the accumulator is rarely rescaled: the
+// only when that has grown by more than 2^8 (weights then stay below 2^8 of the reference's and the accumulator is rarely rescaled: the
 // result is the same quotient).  Sums, references and accumulators are f32; the weights are rounded once, to the type
 // the tensor cores take.
 //
@@ -204,8 +204,9 @@ template <typename T> __device__ __forceinline__ uint32_t odd_halves(uint32_t w)
     constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
     return ((w & E) == E ? 0xffffu : 0u) | ((w >> 16 & E) == E ? 0xffff0000u : 0u);
 }
-// f16 weights are held 2^6 larger, which keeps small ones out of the subnormals; at most 2^(6 + 8) < 65504
-template <typename T> constexpr float lift() { return std::is_same<T, __half>::value ? 6.f : 0.f; }
+// f16 weights are held 2^6 larger, which keeps small ones out of the subnormals; at most 2^(6 + 8) < 65504.  bf16 values reach the end of the 32-bit range: weights
+// 2^8 smaller are at most 1 however far the reference lags, so that a product is no larger than its value.
+template <typename T> constexpr float lift() { return std::is_same<T, __half>::value ? 6.f : -8.f; }
 
 // The part of a row's view that falls on keys key0 .. key0 + 31, as bits.
 __device__ __forceinline__ uint32_t view_bits(const TreeDev &p, const SeqView &v, int i, int key0) {

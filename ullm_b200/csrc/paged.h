@@ -37,7 +37,7 @@ struct TreeDev {
     const uint32_t *mask;
     const uint8_t *k, *v; // this layer's
     long long page_stride, slot_stride, head_stride;
-    int n_rows, n_seq, n_head, n_kv, group, dim, n_table, max_blocks, n_pages, page_size, mask_words, layer;
+    int n_rows, n_seq, n_kv, group, dim, n_table, max_blocks, n_pages, page_size, mask_words;
     int page_log; // logarithm of the page size, -1 where that is no power of two (then by division: 2 to 4 % of a call in 32 bits)
     float scale_log2; // scale * log2(e): the kernels work with powers of two
     // work area: per CTA one record and two partial results (rows x (dim + 2) floats each)

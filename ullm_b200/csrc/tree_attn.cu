@@ -388,9 +388,9 @@ int ullm_cuda_tree_attn_dev(ullm_cuda_ctx *c, const ullm_tree_attn *a, void *str
     const long long layer = (long long)a->layer * pool.layer_stride * pool.elem_bytes;
     t.k = pool.k + layer, t.v = pool.v + layer;
     t.page_stride = pool.page_stride, t.slot_stride = pool.slot_stride, t.head_stride = pool.head_stride;
-    t.n_rows = (int)a->n_rows, t.n_seq = (int)a->n_seq, t.n_head = (int)a->n_head, t.n_kv = pool.n_kv_head, t.group = t.n_head / t.n_kv;
+    t.n_rows = (int)a->n_rows, t.n_seq = (int)a->n_seq, t.n_kv = pool.n_kv_head, t.group = (int)a->n_head / t.n_kv;
     t.dim = pool.head_dim, t.n_table = (int)a->n_table, t.max_blocks = (int)a->max_blocks, t.n_pages = pool.n_pages, t.page_size = pool.page_size;
-    t.mask_words = (int)a->mask_words, t.layer = (int)a->layer, t.page_log = -1;
+    t.mask_words = (int)a->mask_words, t.page_log = -1;
     for (int l = 0; l < 31; ++l)
         if (t.page_size == 1 << l) t.page_log = l;
     t.scale_log2 = (float)((a->scale == 0.f ? 1.0 / std::sqrt((double)dim) : (double)a->scale) * 1.4426950408889634);

@@ -652,3 +652,17 @@ def test_the_largest_bf16_values(ctx, dim, n):
             c.v[c.layer, page, slot, b % 4, 7 + (tok == 100)] = value
     c.run(ctx)
     c.check()
+
+
+@pytest.mark.parametrize("dtype,q32", [("f16", False), ("bf16", False), ("f32", True)])
+def test_many_chains_of_any_length(ctx, dtype, q32):
+    """More than a window of 32 sequences without a mask, prompts of hundreds of rows in the later windows among single rows and empty entries."""
+    rng = np.random.default_rng(12)
+    counts = [int(x) for x in rng.integers(0, 3, 75)]
+    ctxs = [int(x) for x in rng.integers(0, 200, 75)]
+    for b, n in ((3, 150), (31, 40), (32, 290), (33, 0), (50, 131), (74, 270)):
+        counts[b] = n
+    for heads, kv_heads in ((4, 1), (4, 2)):
+        c = Case(ctxs, counts, heads, kv_heads, 64, dtype, 16, mask="chain", seed=3, q32=q32)
+        c.run(ctx)
+        c.check()

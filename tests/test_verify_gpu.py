@@ -127,3 +127,27 @@ def test_refusals(ctx):
     assert lib.ullm_cuda_forward_accept(gf._h, 0, 3, None, 1) == backend.ERR_INVALID
     gf.verify(e[:4], 60)  # the last four positions
     gf.free()
+
+
+@pytest.mark.parametrize("kv_f16,n", [(False, 6), (True, 6), (False, 1)])
+def test_a_tree_behind_a_long_context(ctx, kv_f16, n):
+    """Two thousand cached positions: the attention's units are cut into parts."""
+    p = dict(synth.LLAMA_TINY, n_ctx=2100)
+    m = variant_model(p, 31, False, False)
+    a, b = backend.GpuForward(ctx, m, kv_f16=kv_f16), backend.GpuForward(ctx, m, kv_f16=kv_f16)
+    rng = np.random.default_rng(8)
+    pos, width = 2000, p["n_kv_head"] * p["head_dim"]
+    k, v = (rng.standard_normal((p["n_layer"], pos, width)).astype(np.float32) for _ in range(2))
+    e = rng.standard_normal((n, p["n_embd"])).astype(np.float32)
+    parents = paged_ref.tree_parents(n, rng, 0.3)
+    for f in (a, b):
+        f.set_kv(0, k, v)
+    got = a.verify(e, pos, parents)
+    for i in range(n):
+        path = path_to(parents, i)
+        assert synth.rel_err(got[i], [b.forward(e[j], pos + d) for d, j in enumerate(path)][-1]) < SAME
+    path = path_to(parents, n - 1)
+    a.accept(pos, n, path)
+    x = rng.standard_normal(p["n_embd"]).astype(np.float32)
+    assert synth.rel_err(a.forward(x, pos + len(path)), b.forward(x, pos + len(path))) < SAME
+    a.free(), b.free()

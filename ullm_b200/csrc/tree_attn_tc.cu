@@ -670,6 +670,7 @@ template <typename T, int D, bool TWO> __global__ void __launch_bounds__(TT, 1) 
 #pragma unroll 1
                 for (int c = TWO ? 0 : (int)s * (D / 2); c < (TWO ? D : (int)(s + 1) * (D / 2)); c += 32) {
                     uint32_t o0[32], o1[32];
+                    __syncwarp(); // (rows part ways below)
                     tmem_ld32(TWO ? t_o + c : t_lane + C::O_COL + c, o0);
                     if (!TWO) tmem_ld32(t_lane + C::O_COL + D + c, o1);
                     wait_ld32(o0);

@@ -10,7 +10,7 @@
 // in the pages, while one is worked on.  A warp's scores form a tile, a thread's one of up to 2 keys x 4 rows, so that lanes share what they read from
 // shared memory: with a key per lane these reads took three times as long as the multiply-adds, which go two to an instruction.
 // Shared memory bounds it all the same: 32 lanes x 16 bytes take four cycles, six such reads feed a tile's 32 multiply-adds per lane, which need eight.
-// 90 rows of each of 16 sequences over heads of 64 in 32 bits: 16.5 TFLOP/s of the 72 of the f32 units.
+// 90 rows of each of 16 sequences over heads of 96 in 32 bits: 402 us, 16.6 TFLOP/s of the 72 of the f32 units.
 #include "engine.h"
 #include "tree_sched.cuh"
 
@@ -310,7 +310,7 @@ static int fma_ctas(const DeviceInfo &dev, int dim, int kv_bytes, int rows, int 
     return dev.sm_count * (int)std::max((size_t)1, std::min((size_t)F_PER_SM, (size_t)dev.max_smem_sm / one));
 }
 static size_t meta_bytes(int ctas) { return ((size_t)ctas * TREE_META * sizeof(int4) + 255) / 256 * 256; }
-// Keys of a block: 64 while two CTAs with two stages of them fit an SM, else 32 (32 rows of 512 bytes: 303 us with 64 keys and one CTA, 268 with 32 and two).
+// Keys of a block: 64 while two CTAs with two stages of them fit an SM, else 32 (32 rows over 16-bit heads of 256, 512 bytes: 194 us with 64 keys and one CTA, 180 with 32 and two).
 inline int fma_keys(int row_bytes) { return row_bytes <= 256 ? 64 : 32; }
 template <typename Q, typename KV, int M, int KEYS> static cudaError_t launch_fma_as(const DeviceInfo &dev, const TreeDev &t, bool pdl, cudaStream_t st) {
     const size_t smem = fma_smem(t.dim, sizeof(KV), M, KEYS);
@@ -322,8 +322,8 @@ template <typename Q, typename KV, int M, int KEYS> static cudaError_t launch_fm
     return launch_kernel(tree_join_kernel<Q, M>, dim3(dev.sm_count * JOIN_PER_SM<M>), dim3(32 * JOIN_WARPS), 0, st, pdl, t, ctas);
 }
 template <typename Q, typename KV> static cudaError_t launch_fma(const DeviceInfo &dev, const TreeDev &t, bool pdl, cudaStream_t st) {
-    // Rows per sequence and key head, on average.  A tile with room for many more rows than there are leaves threads idle (four rows over heads of 64: 65 us with
-    // tiles of 8 rows, 78 with 16), a smaller one reads the keys more often.
+    // Rows per sequence and key head, on average.  A tile with room for many more rows than there are leaves threads idle (four rows over heads of 96 in 32 bits: 37.5 us
+    // with tiles of 8 rows, 39.6 with 16; in 16 bits 31.2 and 32.7), a smaller one reads the keys more often.
     const long long rows = ((long long)t.n_rows * t.group + t.n_seq - 1) / t.n_seq;
     const bool k64 = fma_keys(t.dim * (int)sizeof(KV)) == 64;
     if (rows > 16) return k64 ? launch_fma_as<Q, KV, 32, 64>(dev, t, pdl, st) : launch_fma_as<Q, KV, 32, 32>(dev, t, pdl, st);

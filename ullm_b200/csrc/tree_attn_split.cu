@@ -8,7 +8,7 @@
 // products one by one.  Values of 16 bits fit in one part: two products instead of three.
 // The tensor cores cut off what does not fit when they add, always towards zero, so that long sums come out too small: with a segment's weighted values left in their
 // accumulators 1 to 4e-5 over 32,000 to 100,000 tokens.  They hold one block's sums only, which ordinary additions join to those of the blocks before (90 rows
-// over heads of 64: 128 -> 133 us).  Errors against 64 bits, as a share of the values' mean: 1.4e-7 (root mean square) over 100,000 positive values, 9.4e-7 over such of either sign;
+// over heads of 64: 129 -> 132 us).  Errors against 64 bits, as a share of the values' mean: 1.4e-7 (root mean square) over 100,000 positive values, 9.4e-7 over such of either sign;
 // the same formula in f32 with a matrix library: 1.4e-7 and 7.0e-7.
 //
 // A CTA of eight warps takes 16 or 32 query rows and walks blocks of 64 keys, whose keys and values arrive by cp.async, as they lie in the pages, while the
@@ -19,8 +19,9 @@
 // product is free as long as both sides agree; it is chosen so that a lane reads 16 neighbouring bytes.
 // On the CUDA cores (tree_attn.cu) the reads of shared memory bound the same work: 32 lanes x 16 bytes take four cycles and feed 32 multiply-adds per lane.
 // Rows are few (a group's heads x drafted tokens), so that tcgen05's tile of 128 rows would be empty for the most part.
-// It is bound by chains of dependent instructions, eight or sixteen warps on an SM: issue slots 42 % and the tensor pipe 26 to 35 % busy; 32 sequences of one row
-// and 1,500 keys (174 MB) 2.9 TB/s, 90 rows over heads of 64 27 TFLOP/s of 32-bit results, where the CUDA cores gave 2.6 TB/s and 14 to 16.
+// It is bound by chains of dependent instructions, eight or sixteen warps on an SM: issue slots 34 % and the tensor pipe 10 % busy for 24 units of 28 rows, 42 and 26 to 35 %
+// for 90 rows; 32 sequences of one row and 1,500 keys (174 MB) 2.9 TB/s, 90 rows over heads of 64 29 TFLOP/s of 32-bit results, where the CUDA cores gave 2.6 TB/s
+// and 14 to 16.
 #include "engine.h"
 #include "tree_sched.cuh"
 
@@ -31,7 +32,8 @@ namespace {
 
 constexpr int XT = 256, XK = 64;     // threads; keys of a block
 constexpr float BIG = 1.152921504606847e18f; // 2^60
-constexpr int X_COST = 2, X_MIN = 2; // places that a unit costs beside its blocks (32 sequences of one row: 1 for 59.5 us, 2 for 58.5, 3 for 59.4); that a CTA takes at least
+// places that a unit costs beside its blocks (90 rows over heads of 64: 1 and 3 for 135 us, 2 for 132; 32 sequences of one row: 60.5, 62.5 and 60.8); that a CTA takes at least
+constexpr int X_COST = 2, X_MIN = 2;
 
 template <typename KV, int D, int M> struct SplitCfg {
     static constexpr int RT = M / 16, KG = 8 / RT, NT = XK / KG / 8;   // row tiles; groups of keys; tiles of eight keys of a warp
@@ -212,8 +214,8 @@ template <typename KV, int D, int M> __global__ void __launch_bounds__(XT, (Spli
                     for (int n = 0; n < C::NT; ++n)
 #pragma unroll
                         for (int e = 0; e < SETS * 4; ++e) parts[n][e / 4][e % 4] = 0.f;
-#pragma unroll(D == 64 ? 2 : 1)
-                    for (int c = 0; c < D / 32; ++c) { // (90 rows over heads of 64: 132 us, 135 with a loop; over heads of 128: 166 us, 164 with one)
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) { // (90 rows over heads of 64: 132 us, 136 with a loop; over heads of 128: 159 us, 164 with one)
                         float y[C::NT][8];
 #pragma unroll
                         for (int n = 0; n < C::NT; ++n) widen8(y[n], (const KV *)(ks + (kbase + n * 8 + g) * C::KP) + c * 32 + t * 8);
@@ -422,8 +424,8 @@ template <typename KV, int D, int M> cudaError_t launch_as(const DeviceInfo &dev
 template <typename KV, int D> cudaError_t launch_for(const DeviceInfo &dev, const TreeDev &t, bool pdl, cudaStream_t st) {
     // Rows per sequence and key head on average (the lengths themselves are on the device; either way is right for any of them).
     const long long rows = ((long long)t.n_rows * t.group + t.n_seq - 1) / t.n_seq;
-    // Tiles of 32 rows split the keys half as often (90 rows: 129 us, with 16 rows 158; 64 rows took 7 % longer than 32), but 16 rows spread a little work over more CTAs, where
-    // even tables in full use would give a CTA no more than four blocks (24 units of 28 rows and up to 2,000 keys: 21.2 us, with 32 rows 25.9).
+    // Tiles of 32 rows split the keys half as often (90 rows over heads of 64: 132 us, with 16 rows 162; 64 rows took 7 % longer than 32), but 16 rows spread a little work over more CTAs, where
+    // even tables in full use would give a CTA no more than four blocks (24 units of 28 rows and up to 2,000 keys: 19.5 us, with 32 rows 22.1; 32 sequences of one row: 60.7 and 67.9).
     const long long blocks = (rows + 31) / 32 * t.n_seq * t.n_kv * (((long long)t.max_blocks * t.page_size + XK - 1) / XK);
     if (rows <= 16 || blocks <= 4 * dev.sm_count * SplitCfg<KV, D, 16>::PER_SM) return launch_as<KV, D, 16>(dev, t, pdl, st);
     return launch_as<KV, D, 32>(dev, t, pdl, st);

@@ -666,3 +666,18 @@ def test_many_chains_of_any_length(ctx, dtype, q32):
         c = Case(ctxs, counts, heads, kv_heads, 64, dtype, 16, mask="chain", seed=3, q32=q32)
         c.run(ctx)
         c.check()
+
+
+@pytest.mark.parametrize("dtype,q32,dim", [("f16", False, 64), ("bf16", False, 128), ("f32", True, 64), ("f16", True, 128), ("f32", True, 40)])
+def test_a_row_of_infinitely_low_scores_becomes_zeros(ctx, dtype, q32, dim):
+    """As a row that sees nothing; the other sequences are what they were."""
+    c = Case([300, 50], [5, 3], 4, 2, dim, dtype, 16, mask="tree", seed=4, q32=q32)
+    c.q[:, :4 * dim] = c.q[:, :4 * dim].abs() + 0.1
+    c.run(ctx)
+    torch.cuda.synchronize()
+    before = c.out.clone()
+    for tok in range(305):
+        c.k[c.layer, int(c.blocks[0, tok // 16]), tok % 16, :, 1] = -float("inf")
+    c.run(ctx)
+    torch.cuda.synchronize()
+    assert bool((c.out[:5, :4 * dim] == 0).all()) and torch.equal(c.out[5:], before[5:])

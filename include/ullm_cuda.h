@@ -412,7 +412,8 @@ int ullm_cuda_kv_grow_dev(ullm_cuda_ctx *ctx, const ullm_kv_pages *kv, const ull
 int ullm_cuda_kv_accept_dev(ullm_cuda_ctx *ctx, const ullm_kv_pages *kv, const ullm_kv_table *t, const int32_t *d_seq,
                             const int32_t *d_draft, const int32_t *d_path, const int32_t *d_kept, size_t n, size_t max_path,
                             void *stream);
-/* Sequence d_seq[i] keeps its first d_new_len[i] tokens (NULL: none, the row becomes unused); pages behind them are freed. */
+/* Sequence d_seq[i] keeps its first d_new_len[i] tokens (NULL: none, the row becomes unused); pages behind them are freed.  (A table entry to be freed,
+ * here and in kv_accept, that is no page or one that nobody uses is passed over, with ULLM_KV_FAULT_PAGE; the rest of the entry is carried out.) */
 int ullm_cuda_kv_trim_dev(ullm_cuda_ctx *ctx, const ullm_kv_pages *kv, const ullm_kv_table *t, const int32_t *d_seq,
                           const int32_t *d_new_len, size_t n, void *stream);
 /* Page d_src[i] is copied to page d_dst[i], all layers and slots.  An entry whose destination is also
@@ -443,7 +444,7 @@ int ullm_cuda_tree_plan_dev(ullm_cuda_ctx *ctx, size_t n_rows, size_t n_seq, con
  * d_rope [n_pos][rot_dim / 2][2] f32: cosine and sine of a position's angles; rot_dim (a multiple of 16, at most
  * head_dim, 0 = head_dim) leading values of a head are rotated, as pairs (2i, 2i + 1) or, with neox, (i, i + rot_dim / 2).  Rows
  * with d_row_seq < 0 are skipped.  d_q_out may be d_q when types and strides agree.  d_fault (may be NULL) tells of rows whose position or page
- * is outside: nothing of such a row is written. */
+ * is outside: nothing of such a row is written.  No two rows of a call have the same sequence and slot. */
 typedef struct ullm_qk_norm_rope {
     const ullm_kv_pages *kv;
     size_t layer;
@@ -475,11 +476,13 @@ int ullm_cuda_qk_norm_rope_dev(ullm_cuda_ctx *ctx, const ullm_qk_norm_rope *a, v
 
 /* Attention of a step's rows over their sequences' pages: out = softmax(scale * q . K) V over all tokens in front of the
  * sequence's rows and, among the rows themselves, those whose bit is set in the row's mask (NULL: itself and those in front of it, a
- * causal chain).  A row that sees nothing becomes zeros.  Rows, d_cu, d_len, d_ids as in ullm_cuda_tree_plan_dev; a sequence whose
+ * causal chain).  A row that sees nothing, or only keys whose scores are -inf, becomes zeros; keys and values that are not finite reach the rows that
+ * see them and no others.  Rows, d_cu, d_len, d_ids as in ullm_cuda_tree_plan_dev; a sequence whose
  * length is smaller than its row count gets zeros, rows behind d_cu[n_seq] are left alone.  dtype (of d_q and d_out) is
  * the pages' type, or F32 with pages of any type.  Query head h reads key head h / (n_head / n_kv_head).  Row strides are in elements,
  * multiples of 16 bytes, 0 = n_head * head_dim.  scale is 1e-30 to 2e38, 0 = 1 / sqrt(head_dim).  A page number outside the pool reads as zeros.  d_work: ullm_cuda_tree_attn_work_bytes
- * bytes, not shared by calls that may run at the same time. */
+ * bytes, not shared by calls that may run at the same time, contents free between calls.  Rows times the table's size is limited (2^31
+ * places of 32 keys for tiles of 8 query rows): a call beyond that is refused, and takes its rows in several calls. */
 typedef struct ullm_tree_attn {
     const ullm_kv_pages *kv;
     size_t layer;
